@@ -80,6 +80,8 @@ int mi_version(void);
  *                       instead of whole rows through LDS
  *   "attn_simd_waves"   "2" | "3": fp16 attention build of 2 or 3 waves per
  *                       SIMD (fp16-precision, non-causal, 4-wave launches)
+ *   "gemm_bwd_cfg"      "<build 0..2>[:<N parts>]" (input-gradient GEMM tile
+ *                       build; the parts apply to calls with a workspace)
  * MI_ERR_INVALID_ARG for an unknown name or a malformed value. Not
  * synchronised with calls in flight on other threads.                      */
 int mi_tuning_set(const char* name, const char* value);
@@ -459,6 +461,69 @@ int mi_block_ctx_kv(const mi_block_weights* w, const mi_block_dims* dims, const 
 int mi_sdxl_block_forward_kv(const mi_block_weights* w, const mi_block_dims* dims, float* x,
                              const float* kv, uint64_t kv_bytes, const int32_t* ctx_len, void* workspace,
                              uint64_t workspace_bytes, void* stream);
+
+/* ----------------------------------------------------- backward passes -- *
+ * What fine-tuning on frozen Q8_0 weights needs of the operators above: the
+ * gradients of their activations and of the LayerNorm parameters (the linears'
+ * weights stay as they are). (Extension: the reference's SDXL path only runs
+ * forward.) Contract as for every entry: nothing is allocated, work is ordered
+ * on the stream, results repeat bit for bit, an entry may be captured into a
+ * HIP graph. A workspace is used in stream order; calls that may overlap in time
+ * (streams, captured graphs) need one each. Gradients are held in fp32 inside and
+ * rounded once.                                                              */
+
+/* Input gradient of mi_gemm_nt_q8_0 (C = A . deq(W)^T):
+ *   dA[M,K] (=|+=) dC[M,N] . deq(W[N,K])
+ * dC and dA of one dtype (MI_F32 / MI_F16), row strides ldc (0 -> N) and lda
+ * (0 -> K) in elements; mode 0 stores, 1 adds to dA. W: 34-byte blocks, 16-byte
+ * aligned, below 2 GiB, K % 32 == 0; N any. dC and dA aligned to their element;
+ * 16-byte aligned rows of dC (and N * element size % 16 == 0) take the wide loads,
+ * 4-element aligned rows of dA the wide stores. dA must not overlap dC or W.
+ * MI_F16: weights rounded to fp16, fp32 sums, one rounding. MI_F32: both operands
+ * carried as fp16 hi + lo (weights below 1023 in magnitude; a row of dC of any
+ * size, by an exponent of its own): the accuracy of an fp32 product. N == 0 stores
+ * zeros in mode 0.
+ * workspace (or NULL): grids too small to fill the GPU split N into parts, fp32,
+ * added in order, when it holds mi_gemm_nt_q8_0_bwd_ws_bytes(M, N, K, dtype) bytes
+ * (16-byte aligned, disjoint from the operands); with less the call runs unsplit.
+ * A row of M is computed alike in every call of one plan.                    */
+uint64_t mi_gemm_nt_q8_0_bwd_ws_bytes(uint32_t M, uint32_t N, uint32_t K, int dtype);
+int mi_gemm_nt_q8_0_bwd(const void* dC, const void* W, void* dA, int dtype, uint32_t M, uint32_t N, uint32_t K,
+                        uint32_t mode, uint32_t ldc, uint32_t lda, void* workspace, uint64_t workspace_bytes,
+                        void* stream);
+
+/* Gradient of mi_gemm_nt_q8_0_geglu_f16 with respect to its projection h = A . deq(W)^T
+ * + bias (value columns 0..F-1, gate columns F..2F-1), which is recomputed from A, in
+ * one GEMM:
+ *   dH[m, j] = dG[m, j] gelu(h[m, F + j]),  dH[m, F + j] = dG[m, j] h[m, j] gelu'(h[m, F + j])
+ * A, dG, dH fp16 with row strides lda (0 -> K), lddg (0 -> F), lddh (0 -> 2F); dA is
+ * then mi_gemm_nt_q8_0_bwd(dH, W). A and W as for mi_gemm_nt_q8_0_geglu_f16; dG 2-byte
+ * and dH 4-byte aligned (8-byte with strides and F multiples of 4 for the wide accesses);
+ * dH must not overlap an input.                                                 */
+int mi_gemm_nt_q8_0_geglu_bwd(const void* A, const void* W, const float* bias, const void* dG, void* dH, uint32_t M,
+                              uint32_t F, uint32_t K, uint32_t lda, uint32_t lddg, uint32_t lddh, void* stream);
+
+/* Gradient of mi_geglu / mi_geglu_f16 from a kept h = [rows, 2F], fp32: dh[r, j] =
+ * dy[r, j] gelu(h[r, F + j]), dh[r, F + j] = dy[r, j] h[r, j] gelu'(h[r, F + j]). dy
+ * [rows, F] and dh [rows, 2F] of one dtype (MI_F32 / MI_F16). Any F, any alignment of
+ * elements; F % 4 == 0 with 16-byte aligned rows (8-byte for fp16) is the fast path. An
+ * fp32 dh may be h itself; no other overlap.                                 */
+int mi_geglu_bwd(const float* h, const void* dy, void* dh, int dtype, uint32_t rows, uint32_t F, void* stream);
+
+/* Gradients of mi_layernorm / mi_layernorm_f16 (y = xh gamma + beta) from x and dy:
+ *   dx = inv (dy gamma - mean(dy gamma) - xh mean(dy gamma xh)) (+ res)
+ *   dgamma = sum_rows dy xh,  dbeta = sum_rows dy
+ * gamma NULL: no affine (1). dy MI_F32 or MI_F16 (dy_dtype); the rest fp32. res (or
+ * NULL) is added to dx: the gradient that reaches x past the norm, on the residual
+ * stream; dx may be res itself, and overlaps nothing else. dgamma and dbeta both NULL
+ * or both set; set, they need `workspace` of mi_layernorm_bwd_ws_bytes(rows, d) bytes,
+ * 16-byte aligned, disjoint from the tensors (rows added in a fixed order). rows <=
+ * 2^31; any d; d % 4 == 0, d <= 4096 and 16-byte aligned tensors (8-byte for an fp16
+ * dy) is the fast path. rows == 0 stores zeros in dgamma and dbeta.          */
+uint64_t mi_layernorm_bwd_ws_bytes(uint32_t rows, uint32_t d);
+int mi_layernorm_bwd(const float* x, const float* gamma, const void* dy, int dy_dtype, const float* res, float* dx,
+                     float* dgamma, float* dbeta, uint32_t rows, uint32_t d, float eps, void* workspace,
+                     uint64_t workspace_bytes, void* stream);
 
 /* ---------------------------------------------------------------- GGUF -- *
  * Checkpoint access: the container reader and the upload of its tensors into

@@ -115,6 +115,13 @@ SIGNATURES = {
                                        _vp]),
     "mi_sdxl_block_forward_kv": (ctypes.c_int, [ctypes.POINTER(MiBlockWeights), ctypes.POINTER(MiBlockDims), _vp,
                                                 _vp, _u64, _vp, _vp, _u64, _vp]),
+    "mi_gemm_nt_q8_0_bwd_ws_bytes": (_u64, [_u32, _u32, _u32, ctypes.c_int]),
+    "mi_gemm_nt_q8_0_bwd": (ctypes.c_int, [_vp, _vp, _vp, ctypes.c_int, _u32, _u32, _u32, _u32, _u32, _u32, _vp, _u64, _vp]),
+    "mi_gemm_nt_q8_0_geglu_bwd": (ctypes.c_int, [_vp, _vp, _vp, _vp, _vp, _u32, _u32, _u32, _u32, _u32, _u32, _vp]),
+    "mi_geglu_bwd": (ctypes.c_int, [_vp, _vp, _vp, ctypes.c_int, _u32, _u32, _vp]),
+    "mi_layernorm_bwd_ws_bytes": (_u64, [_u32, _u32]),
+    "mi_layernorm_bwd": (ctypes.c_int, [_vp, _vp, _vp, ctypes.c_int, _vp, _vp, _vp, _vp, _u32, _u32, ctypes.c_float, _vp,
+                                        _u64, _vp]),
     "mi_gguf_open": (ctypes.c_int, [ctypes.c_char_p, ctypes.c_char_p, ctypes.POINTER(_vp)]),
     "mi_gguf_close": (None, [_vp]),
     "mi_gguf_info": (ctypes.c_int, [_vp, ctypes.POINTER(_u32), ctypes.POINTER(_u64), ctypes.POINTER(_u64),

@@ -124,14 +124,6 @@ __device__ __forceinline__ void lds_dma16(__amdgpu_buffer_rsrc_t r, void* lds, u
     __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (__attribute__((address_space(3))) void*)lds, 16, voffset, 0, 0, 0);
 }
 
-// Transposing LDS read: within each 16-lane group, lane i returns element i % 4
-// of the 8-byte pieces addressed by lanes i/4, i/4 + 4, i/4 + 8, i/4 + 12.
-__device__ __forceinline__ half4 lds_read_tr16(const _Float16* p) {
-    typedef __fp16 fp16x4 __attribute__((ext_vector_type(4)));
-    return __builtin_bit_cast(
-        half4, __builtin_amdgcn_ds_read_tr16_b64_v4f16((__attribute__((address_space(3))) fp16x4*)(const_cast<_Float16*>(p))));
-}
-
 __device__ __forceinline__ void wait_vmcnt0() { __builtin_amdgcn_s_waitcnt(0x0F70); }
 
 // Writes one wave's O^T accumulators (32 queries x 64 d, times inv) as output

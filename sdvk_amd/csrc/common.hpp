@@ -32,6 +32,7 @@ int check_launch(const char* what);
 // sizes only: no override changes an operator's arithmetic beyond the
 // summation order of a different plan.
 constexpr int kGemmBuilds = 7;  // tile builds of gemm_q8.hip (kNumCfg)
+constexpr int kGemmBwdBuilds = 3;  // tile builds of gemm_q8_bwd.hip
 struct Tuning {
     std::atomic<int> gemm_cfg{-1};          // tile build, or -1
     std::atomic<int> gemm_splits{1};        // K splits with gemm_cfg (workspace entries)
@@ -42,6 +43,8 @@ struct Tuning {
     std::atomic<int> attn_split_pieces{2};  // key split: pieces per rest block
     std::atomic<int> attn_direct_store{0};  // 1: attention outputs stored from the MFMA layout
     std::atomic<int> attn_simd_waves{0};    // fp16 attention build: 2 or 3 waves per SIMD, or 0
+    std::atomic<int> gemm_bwd_cfg{-1};      // input-gradient GEMM tile build, or -1
+    std::atomic<int> gemm_bwd_splits{1};    // N parts with gemm_bwd_cfg (with a workspace)
 };
 Tuning& tuning();
 
@@ -112,6 +115,44 @@ __device__ __forceinline__ float gelu_erf(float v) {
     return 0.5f * v * (1.0f + erf);
 }
 
+// GEGLU's gradient: y = v * gelu(x), gelu(x) = x cdf(x), gelu'(x) = cdf(x) + x pdf(x) with the normal
+// distribution's cdf and pdf:
+//   dv = dy * x * cdf(x),   dx = dy * v * (cdf(x) + x * pdf(x)).
+// The cdf's tail q = (1 - erf(|x| / sqrt 2)) / 2 is half the rational approximation of gelu_erf (7.1.26,
+// |error| <= 0.75e-7 of the cdf) times exp(-x^2 / 2), and that exponential is the pdf's too, so the two
+// derivatives cost one v_exp_f32 and one v_rcp_f32. Taking the tail itself (cdf = q for x < 0, 1 - q for
+// x >= 0) avoids the cancellation of 1 + erf at negative x. Contraction is off: every kernel that inlines
+// this computes the same bits.
+__device__ __forceinline__ void geglu_grad(float v, float x, float dy, float& dv, float& dx) {
+#pragma clang fp contract(off)
+    const float ax = fabsf(x) * 0.70710678118654752440f;
+    const float t = __builtin_amdgcn_rcpf(1.0f + 0.3275911f * ax);
+    const float poly = ((((1.061405429f * t - 1.453152027f) * t + 1.421413741f) * t - 0.284496736f) * t + 0.254829592f) * t;
+    const float e = __builtin_amdgcn_exp2f(-ax * ax * 1.44269504088896341f);
+    const float q = 0.5f * poly * e;
+    const float cdf = x >= 0.0f ? 1.0f - q : q;
+    dv = dy * (x * cdf);
+    dx = dy * (v * (cdf + x * (0.39894228040143267794f * e)));
+}
+
+// Eight Q8_0 weights, fp16(d * q), of the q dwords lo and hi.
+// fp16 bits of (1024 + u) for each byte u of x ^ 0x80808080: subtracting 1152
+// leaves the signed byte value exactly (|q| <= 128 < 2^11).
+__device__ __forceinline__ half8 dequant8_f16(uint32_t lo, uint32_t hi, _Float16 d) {
+    const uint32_t xl = lo ^ 0x80808080u, xh = hi ^ 0x80808080u;
+    const half2 bias = {static_cast<_Float16>(1152.0f), static_cast<_Float16>(1152.0f)};
+    const half2 dd = {d, d};
+    half2 h0 = __builtin_bit_cast(half2, __builtin_amdgcn_perm(0x64646464u, xl, 0x04010400u));
+    half2 h1 = __builtin_bit_cast(half2, __builtin_amdgcn_perm(0x64646464u, xl, 0x04030402u));
+    half2 h2 = __builtin_bit_cast(half2, __builtin_amdgcn_perm(0x64646464u, xh, 0x04010400u));
+    half2 h3 = __builtin_bit_cast(half2, __builtin_amdgcn_perm(0x64646464u, xh, 0x04030402u));
+    h0 = (h0 - bias) * dd;  // one rounding of the exact product q * d
+    h1 = (h1 - bias) * dd;
+    h2 = (h2 - bias) * dd;
+    h3 = (h3 - bias) * dd;
+    return half8{h0[0], h0[1], h1[0], h1[1], h2[0], h2[1], h3[0], h3[1]};
+}
+
 // Scheduling groups for one K step (instruction-class masks of
 // __builtin_amdgcn_sched_group_barrier: 0x008 MFMA, 0x002 VALU, 0x100 LDS read,
 // 0x200 LDS write). The step's first fragment reads go first; then every MFMA
@@ -128,6 +169,14 @@ __device__ __forceinline__ void interleave_step() {
         __builtin_amdgcn_sched_group_barrier(0x002, (NVALU + NMFMA - 1) / NMFMA, 0);
         __builtin_amdgcn_sched_group_barrier(0x200, (NWRITE + NMFMA - 1) / NMFMA, 0);
     }
+}
+
+// Transposing LDS read: within each 16-lane group, lane i returns element i % 4
+// of the 8-byte pieces addressed by lanes i/4, i/4 + 4, i/4 + 8, i/4 + 12.
+__device__ __forceinline__ half4 lds_read_tr16(const _Float16* p) {
+    typedef __fp16 fp16x4 __attribute__((ext_vector_type(4)));
+    return __builtin_bit_cast(
+        half4, __builtin_amdgcn_ds_read_tr16_b64_v4f16((__attribute__((address_space(3))) fp16x4*)(const_cast<_Float16*>(p))));
 }
 
 // Remaps a linear workgroup id so that consecutive logical tiles land on the

@@ -56,6 +56,9 @@ struct GemmArgs {
     // (gemm_q8_0_shared_a), else 0 and the batch strides. (Offsets, not pointers to
     // choose from: those would make every C access a flat one.)
     int64_t w1, w2, c1, c2;
+    const _Float16* dG;     // GEGLU gradient epilogue: the gradient of GEGLU's output, row stride lddg
+    uint64_t lddg;
+    uint32_t gvec;          // dG's and C's rows 8-byte aligned (F % 4 == 0 for C's gate half)
 };
 
 // This workgroup's weights and output.
@@ -76,7 +79,11 @@ __device__ __forceinline__ float* output_of(const GemmArgs& a) {
 // products v, g of output column j: each 32-wide MFMA column tile holds 16
 // value columns and the 16 gate columns that pair with them, so the
 // epilogue combines them in registers and only F columns reach memory.
-enum Epi { kEpiPlain = 0, kEpiGeglu = 1, kEpiResidual = 2 };
+// kEpiGegluBwd: the same tiles; v + bias[j] and g + bias[F + j] are what the forward pass had, and
+// with dG[m, j] the epilogue stores the projection's gradient, fp16: C[m, j] = dG gelu(g) and
+// C[m, F + j] = dG v gelu'(g) (geglu_grad). The [M, 2F] projection is recomputed instead of kept.
+enum Epi { kEpiPlain = 0, kEpiGeglu = 1, kEpiResidual = 2, kEpiGegluBwd = 3 };
+constexpr bool pairs_gates(int epi) { return epi == kEpiGeglu || epi == kEpiGegluBwd; }
 
 // W row of tile column c (0 <= c < BN) for an output tile starting at column
 // o0: the first 16 columns of every 32 are value rows, the next 16 the gate
@@ -113,23 +120,6 @@ GemmArgs make_args(const float* A, const uint8_t* W, const float* scales, const 
 }
 
 enum WKind { kBlocks34 = 0, kSplit = 1 };
-
-// fp16 bits of (1024 + u) for each byte u of x ^ 0x80808080: subtracting 1152
-// leaves the signed byte value exactly (|q| <= 128 < 2^11).
-__device__ __forceinline__ half8 dequant8_f16(uint32_t lo, uint32_t hi, _Float16 d) {
-    const uint32_t xl = lo ^ 0x80808080u, xh = hi ^ 0x80808080u;
-    const half2 bias = {static_cast<_Float16>(1152.0f), static_cast<_Float16>(1152.0f)};
-    const half2 dd = {d, d};
-    half2 h0 = __builtin_bit_cast(half2, __builtin_amdgcn_perm(0x64646464u, xl, 0x04010400u));
-    half2 h1 = __builtin_bit_cast(half2, __builtin_amdgcn_perm(0x64646464u, xl, 0x04030402u));
-    half2 h2 = __builtin_bit_cast(half2, __builtin_amdgcn_perm(0x64646464u, xh, 0x04010400u));
-    half2 h3 = __builtin_bit_cast(half2, __builtin_amdgcn_perm(0x64646464u, xh, 0x04030402u));
-    h0 = (h0 - bias) * dd;  // one rounding of the exact product q * d
-    h1 = (h1 - bias) * dd;
-    h2 = (h2 - bias) * dd;
-    h3 = (h3 - bias) * dd;
-    return half8{h0[0], h0[1], h1[0], h1[1], h2[0], h2[1], h3[0], h3[1]};
-}
 
 // fp32 scales (split layout, arbitrary fp32): w = fp16(fp32(q) * s).
 __device__ __forceinline__ half8 dequant8_f32(uint32_t lo, uint32_t hi, float s0, float s1) {
@@ -201,7 +191,8 @@ constexpr int kStageFloats = 32 * kStageLd;        // per wave
 template <int FM, int FN, bool SPLITK, int EPI = kEpiPlain>
 __device__ __forceinline__ void store_tiles(const GemmArgs& a, float* C, float* stage, uint32_t mw, uint32_t nw,
                                             const floatx16 (&acc)[FM][FN], int lane) {
-    static_assert(!(SPLITK && EPI == kEpiGeglu), "the GEGLU epilogue needs the whole K sum");
+    constexpr bool kPairs = pairs_gates(EPI);
+    static_assert(!(SPLITK && kPairs), "the GEGLU epilogues need the whole K sum");
     const int l32 = lane & 31, g = lane >> 5;
     const bool vec = a.cvec != 0;
     const bool use_bias = !SPLITK && (EPI == kEpiResidual ? true : a.mode == 0) && a.bias != nullptr;
@@ -227,9 +218,9 @@ __device__ __forceinline__ void store_tiles(const GemmArgs& a, float* C, float* 
     // waits out a memory round trip -- and every store issued before it -- per
     // tile. GEGLU: value and gate biases of output columns nw + 16 fn + 4 (lane
     // % 4) + e; 16-byte path: columns nw + 32 fn + 4 (lane % 8) + e.
-    float gbv[EPI == kEpiGeglu ? FN : 1][4], gbg[EPI == kEpiGeglu ? FN : 1][4];
-    floatx4 bias4[EPI == kEpiGeglu ? 1 : FN];
-    if constexpr (EPI == kEpiGeglu) {
+    float gbv[kPairs ? FN : 1][4], gbg[kPairs ? FN : 1][4];
+    floatx4 bias4[kPairs ? 1 : FN];
+    if constexpr (kPairs) {
 #pragma unroll
         for (int fn = 0; fn < FN; ++fn)
 #pragma unroll
@@ -246,6 +237,29 @@ __device__ __forceinline__ void store_tiles(const GemmArgs& a, float* C, float* 
             if (use_bias && vec && vec_bias && n + 3 < a.N) bias4[fn] = *reinterpret_cast<const floatx4*>(a.bias + n);
         }
     }
+    // kEpiGegluBwd: this lane's dG of every tile, loaded ahead of the tile loop (elements past
+    // M or F are never used)
+    half4 dy[EPI == kEpiGegluBwd ? FM * FN : 1][2];
+    if constexpr (EPI == kEpiGegluBwd) {
+#pragma unroll
+        for (int b = 0; b < FM * FN; ++b)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const int u = lane + 64 * i;
+                const uint32_t m = mw + 32 * (b / FN) + (u >> 2), n = nw + 16 * (b % FN) + (u & 3) * 4;
+                dy[b][i] = half4{0, 0, 0, 0};
+                if (m < a.M && n < a.F) {
+                    const _Float16* p = a.dG + static_cast<uint64_t>(m) * a.lddg + n;
+                    if (a.gvec) {
+                        dy[b][i] = *reinterpret_cast<const half4*>(p);
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < 4; ++e)
+                            if (n + e < a.F) dy[b][i][e] = p[e];
+                    }
+                }
+            }
+    }
     for (int b = 0; b < FM * FN; ++b) {
 #pragma unroll
         for (int fm = 0; fm < FM; ++fm)
@@ -261,6 +275,55 @@ __device__ __forceinline__ void store_tiles(const GemmArgs& a, float* C, float* 
         // the staged tile is read back by other lanes of the wave: keep every
         // write of the wave ahead of every read (no instruction is emitted)
         __builtin_amdgcn_wave_barrier();
+        if constexpr (EPI == kEpiGegluBwd) {
+            const uint32_t mb = mw + 32 * (b / FN), ob = nw + 16 * (b % FN);
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const int u = lane + 64 * i;
+                const int row = u >> 2, col = (u & 3) * 4;
+                const floatx4 v = *reinterpret_cast<const floatx4*>(&stage[row * kStageLd + col]);
+                const floatx4 gt = *reinterpret_cast<const floatx4*>(&stage[row * kStageLd + 16 + col]);
+                const uint32_t m = mb + row, n = ob + col;
+                if (m >= a.M || n >= a.F) continue;
+                float bv[4], bg[4];
+                half4 y = dy[0][i];
+#pragma unroll
+                for (int fn = 0; fn < FN; ++fn)
+                    if (b % FN == fn) {
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            bv[e] = gbv[fn][e];
+                            bg[e] = gbg[fn][e];
+                        }
+                    }
+#pragma unroll
+                for (int t = 1; t < FM * FN; ++t)
+                    if (b == t) y = dy[t][i];
+                half4 dv, dx;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    float p, q;
+                    geglu_grad(v[e] + bv[e], gt[e] + bg[e], static_cast<float>(y[e]), p, q);
+                    asm volatile("" : "+v"(p), "+v"(q));  // the fp32 values, rounded once
+                    dv[e] = static_cast<_Float16>(p);
+                    dx[e] = static_cast<_Float16>(q);
+                }
+                _Float16* ch = reinterpret_cast<_Float16*>(C) + static_cast<uint64_t>(m) * a.ldc + n;
+                if (a.gvec) {
+                    *reinterpret_cast<half4*>(ch) = dv;
+                    *reinterpret_cast<half4*>(ch + a.F) = dx;
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        if (n + e < a.F) {
+                            ch[e] = dv[e];
+                            ch[a.F + e] = dx[e];
+                        }
+                }
+            }
+            __builtin_amdgcn_wave_barrier();
+            continue;
+        }
         if constexpr (EPI == kEpiGeglu) {
             // 32 rows x 4 groups of 4 output columns: value at column 4 c4, gate at 16 + 4 c4
             const uint32_t mb = mw + 32 * (b / FN), ob = nw + 16 * (b % FN);
@@ -460,7 +523,7 @@ __global__ __launch_bounds__(WM * WN * 64) void gemm_q8_kernel(GemmArgs a) {
     const uint32_t rows_in = min(a.group_m, a.tiles_m - grp * a.group_m);
     const uint32_t m0 = __builtin_amdgcn_readfirstlane((grp * a.group_m + rem % rows_in) * BM);
     // GEGLU: n0 is the tile's first output column (BN / 2 outputs per tile)
-    const uint32_t n0 = __builtin_amdgcn_readfirstlane((rem / rows_in) * (EPI == kEpiGeglu ? BN / 2 : BN));
+    const uint32_t n0 = __builtin_amdgcn_readfirstlane((rem / rows_in) * (pairs_gates(EPI) ? BN / 2 : BN));
     const uint32_t s_begin = SPLITK ? blockIdx.y * a.steps_per_split : 0;
     const uint32_t s_end = SPLITK ? min(a.ksteps, s_begin + a.steps_per_split) : a.ksteps;
 
@@ -492,7 +555,7 @@ __global__ __launch_bounds__(WM * WN * 64) void gemm_q8_kernel(GemmArgs a) {
 #pragma unroll
     for (int i = 0; i < W_IT; ++i) {
         const int u = tid + i * NT;
-        const uint32_t n = EPI == kEpiGeglu ? geglu_wrow(n0, u / (BK / 8), a.F) : min(n0 + u / (BK / 8), a.N - 1);
+        const uint32_t n = pairs_gates(EPI) ? geglu_wrow(n0, u / (BK / 8), a.F) : min(n0 + u / (BK / 8), a.N - 1);
         w_k[i] = (u % (BK / 8)) * 8;
         if constexpr (WK == kBlocks34) {
             w_aux[i] = n * a.rowbytes + (w_k[i] / 32) * 34;
@@ -530,7 +593,7 @@ __global__ __launch_bounds__(WM * WN * 64) void gemm_q8_kernel(GemmArgs a) {
 #pragma unroll
     for (int i = 0; i < WB_IT; ++i) {
         const int wb = (tid + i * NT) % W_BLOCKS;
-        const uint32_t n = EPI == kEpiGeglu ? geglu_wrow(n0, wb / KB, a.F) : min(n0 + wb / KB, a.N - 1);
+        const uint32_t n = pairs_gates(EPI) ? geglu_wrow(n0, wb / KB, a.F) : min(n0 + wb / KB, a.N - 1);
         const uint32_t byte = WK == kBlocks34 ? n * a.rowbytes + (wb % KB) * 34 : n * a.K + (wb % KB) * 32;
         // past the step's blocks: out of range, so the load returns zeros and touches no memory
         wb_off[i] = (!WHALF && W_BLOCKS % NT != 0 && tid + i * NT >= W_BLOCKS) ? 0xffffff00u : byte & ~3u;
@@ -834,7 +897,7 @@ __global__ __launch_bounds__(WM * WN * 64) void gemm_q8_kernel(GemmArgs a) {
     __syncthreads();  // every wave is done with the operand tiles before LDS is reused
     const int wm_s = kFreshLane ? wave_s % WM : wm, wn_s = kFreshLane ? wave_s / WM : wn;
     store_tiles<FM, FN, SPLITK, EPI>(a, C, reinterpret_cast<float*>(smem) + wave_s * kStageFloats, m0 + wm_s * TM,
-                                     EPI == kEpiGeglu ? n0 + wn_s * TN / 2 : n0 + wn_s * TN, acc,
+                                     pairs_gates(EPI) ? n0 + wn_s * TN / 2 : n0 + wn_s * TN, acc,
                                      kFreshLane ? lane_id() : lane);
 }
 
@@ -873,7 +936,7 @@ __global__ __launch_bounds__(512) void gemm_q8_rows_kernel(GemmArgs a) {
     constexpr int LPR = 128 * AE / 16;                      // lanes per A row piece
     constexpr int LDA = 136;                                // halves per staged A row (16-byte pad)
     constexpr int kRed = 20;                                // floats per partial row (16-byte pad)
-    constexpr int kCols = EPI == kEpiGeglu ? 8 : 16;        // outputs per row of a workgroup
+    constexpr int kCols = pairs_gates(EPI) ? 8 : 16;        // outputs per row of a workgroup
     constexpr uint32_t kPast = 0x80000000u;                 // an offset past every record (few_rows)
     static_assert(AL >= 1, "a load covers at least one whole row");
     __shared__ __attribute__((aligned(16))) _Float16 As[NWV][kFewRows * LDA];
@@ -883,8 +946,8 @@ __global__ __launch_bounds__(512) void gemm_q8_rows_kernel(GemmArgs a) {
     const uint32_t l16 = lane & 15, c = lane >> 4;
     const uint32_t n0 = blockIdx.x * kCols;
     // GEGLU: eight value rows, then the gate rows of the same outputs
-    const uint32_t o = EPI == kEpiGeglu ? min(n0 + (l16 & 7u), a.F - 1u) : 0u;
-    const uint32_t n = EPI == kEpiGeglu ? ((l16 & 8u) ? a.F + o : o) : min(n0 + l16, a.N - 1);
+    const uint32_t o = pairs_gates(EPI) ? min(n0 + (l16 & 7u), a.F - 1u) : 0u;
+    const uint32_t n = pairs_gates(EPI) ? ((l16 & 8u) ? a.F + o : o) : min(n0 + l16, a.N - 1);
     const uint32_t nblk = a.K / 32, nsteps = (nblk + 3) / 4;
 
     const __amdgpu_buffer_rsrc_t rA = __builtin_amdgcn_make_buffer_rsrc(
@@ -973,7 +1036,7 @@ __global__ __launch_bounds__(512) void gemm_q8_rows_kernel(GemmArgs a) {
     if (l16 < a.M) *reinterpret_cast<floatx4*>(&red[wave][l16][4 * c]) = acc;
     __syncthreads();
     const uint32_t m = tid / kCols, col = tid % kCols, out = n0 + col;
-    if (m >= a.M || out >= (EPI == kEpiGeglu ? a.F : a.N)) return;
+    if (m >= a.M || out >= (pairs_gates(EPI) ? a.F : a.N)) return;
     auto total = [&](uint32_t i) {
         float v = red[0][m][i];
 #pragma unroll
@@ -981,6 +1044,16 @@ __global__ __launch_bounds__(512) void gemm_q8_rows_kernel(GemmArgs a) {
         return v;
     };
     float v = total(col);
+    if constexpr (EPI == kEpiGegluBwd) {
+        const float bv = a.bias ? a.bias[out] : 0.0f, bg = a.bias ? a.bias[a.F + out] : 0.0f;
+        float p, q;
+        geglu_grad(v + bv, total(8 + col) + bg, static_cast<float>(a.dG[m * a.lddg + out]), p, q);
+        asm volatile("" : "+v"(p), "+v"(q));
+        _Float16* c = reinterpret_cast<_Float16*>(a.C) + static_cast<uint64_t>(m) * a.ldc + out;
+        c[0] = static_cast<_Float16>(p);
+        c[a.F] = static_cast<_Float16>(q);
+        return;
+    }
     if constexpr (EPI == kEpiGeglu) {
         const float bv = a.bias ? a.bias[out] : 0.0f, bg = a.bias ? a.bias[a.F + out] : 0.0f;
         v = (v + bv) * gelu_erf(total(8 + col) + bg);
@@ -1207,8 +1280,8 @@ template <int BM, int BN, int WM, int WN, int KB, int WK, bool KTAIL, int PF = 2
 void launch_cfg(const GemmArgs& a0, uint32_t batch, uint32_t splits, float* ws, hipStream_t s) {
     GemmArgs a = a0;
     // GEGLU: BN / 2 outputs per tile, and the epilogue needs the whole K sum
-    a.tiles_n = EPI == kEpiGeglu ? ceil_div(a.F, BN / 2) : ceil_div(a.N, BN);
-    if (EPI == kEpiGeglu || !SPLIT || !ws) splits = 1;
+    a.tiles_n = pairs_gates(EPI) ? ceil_div(a.F, BN / 2) : ceil_div(a.N, BN);
+    if (pairs_gates(EPI) || !SPLIT || !ws) splits = 1;
     a.tiles_m = ceil_div(a.M, BM);
     a.group_m = pick_group(a.tiles_m, a.tiles_n, BM, BN, a.K);
     a.ksteps = ceil_div(a.K, 32 * KB);
@@ -1218,7 +1291,7 @@ void launch_cfg(const GemmArgs& a0, uint32_t batch, uint32_t splits, float* ws, 
         splits = ceil_div(a.ksteps, a.steps_per_split);
     }
     if (splits > 1) {
-        if constexpr (EPI != kEpiGeglu && SPLIT) {
+        if constexpr (!pairs_gates(EPI) && SPLIT) {
             const GemmArgs p = partial_args(a, splits, ws);
             gemm_q8_kernel<BM, BN, WM, WN, KB, WK, true, KTAIL, PF, kEpiPlain, AH, PP>
                 <<<dim3(tiles, splits, batch), WM * WN * 64, 0, s>>>(p);
@@ -1278,7 +1351,7 @@ void launch(int cfg, const GemmArgs& a, uint32_t batch, uint32_t splits, float* 
             // compiler spills LDS addresses inside the K loop, and every
             // scratch reload waits for all global loads in flight. They run
             // 256x128 tiles instead.
-            if constexpr (WK == kSplit || EPI == kEpiGeglu)
+            if constexpr (WK == kSplit || pairs_gates(EPI))
                 launch_cfg<256, 128, 4, 2, 2, WK, false, 2, EPI, true, AH>(a, batch, splits, ws, s);
             else
                 launch_cfg<256, 256, 4, 2, 2, WK, false, 1, EPI, true, AH>(a, batch, splits, ws, s);
@@ -1463,7 +1536,7 @@ Plan plan_for(uint32_t M, uint32_t N, uint32_t K, uint32_t batch, const void* ws
 template <int WK, int EPI = kEpiPlain, bool AH = false>
 void dispatch(const GemmArgs& a, uint32_t batch, const Plan& p, float* ws, hipStream_t s) {
     if (few_rows(a.M, a.N, a.K)) {
-        const dim3 grid(EPI == kEpiGeglu ? ceil_div(a.F, 8) : ceil_div(a.N, 16), 1, batch);
+        const dim3 grid(pairs_gates(EPI) ? ceil_div(a.F, 8) : ceil_div(a.N, 16), 1, batch);
         if (a.M <= 4) gemm_q8_rows_kernel<WK, EPI, AH, 4><<<grid, 512, 0, s>>>(a);
         else gemm_q8_rows_kernel<WK, EPI, AH, 16><<<grid, 512, 0, s>>>(a);
         return;
@@ -1808,6 +1881,40 @@ extern "C" int mi_gemm_nt_q8_0_geglu_f16(const void* A, const void* W, const flo
                                          uint32_t F, uint32_t K, uint32_t lda, uint32_t ldg, void* stream) {
     return gemm_geglu("mi_gemm_nt_q8_0_geglu_f16", A, W, bias, G, M, F, K, lda, ldg,
                       static_cast<hipStream_t>(stream), true, true);
+}
+
+extern "C" int mi_gemm_nt_q8_0_geglu_bwd(const void* A, const void* W, const float* bias, const void* dG, void* dH,
+                                         uint32_t M, uint32_t F, uint32_t K, uint32_t lda, uint32_t lddg, uint32_t lddh,
+                                         void* stream) {
+    const char* fn = "mi_gemm_nt_q8_0_geglu_bwd";
+    if (M == 0 || F == 0) return MI_OK;
+    if (!dG) return fail(MI_ERR_INVALID_ARG, "%s: null pointer", fn);
+    if (K == 0 || K % 32) return fail(MI_ERR_UNSUPPORTED, "%s: K=%u must be a positive multiple of 32", fn, K);
+    if (F > (1u << 30)) return fail(MI_ERR_UNSUPPORTED, "%s: F=%u too large", fn, F);
+    const uint32_t N = 2 * F;
+    int st = validate(fn, A, W, dH, M, N, K, 0, lda, lddh, 1, 0, 0, true, true);
+    if (st) return st;
+    if (lddg == 0) lddg = F;
+    if (lddg < F) return fail(MI_ERR_INVALID_ARG, "%s: lddg %u < F %u", fn, lddg, F);
+    if (!aligned(W, 16)) return fail(MI_ERR_ALIGNMENT, "%s: W must be 16-byte aligned", fn);
+    if (!aligned(dG, 2)) return fail(MI_ERR_ALIGNMENT, "%s: dG must be 2-byte aligned", fn);
+    const uint64_t wbytes = static_cast<uint64_t>(N) * (K / 32) * 34;
+    if (wbytes + 16 >= (uint64_t(1) << 32)) return fail(MI_ERR_UNSUPPORTED, "%s: weight >= 4 GiB", fn);
+    const uint64_t hbytes = (static_cast<uint64_t>(M - 1) * lddh + N) * 2, gbytes = (static_cast<uint64_t>(M - 1) * lddg + F) * 2;
+    const uint64_t abytes = (static_cast<uint64_t>(M - 1) * lda + K) * 2;
+    if (overlaps(dH, hbytes, A, abytes) || overlaps(dH, hbytes, W, wbytes) || overlaps(dH, hbytes, bias, uint64_t(N) * 4) ||
+        overlaps(dH, hbytes, dG, gbytes))
+        return fail(MI_ERR_ALIASING, "%s: dH overlaps an input", fn);
+    GemmArgs a = make_args(static_cast<const float*>(A), static_cast<const uint8_t*>(W), nullptr, bias,
+                           static_cast<float*>(dH), M, N, K, 0, lda, lddh, 0, 0, (K / 32) * 34);
+    a.F = F;
+    a.dG = static_cast<const _Float16*>(dG);
+    a.lddg = lddg;
+    a.gvec = aligned(dG, 8) && aligned(dH, 8) && lddg % 4 == 0 && lddh % 4 == 0 && F % 4 == 0 ? 1u : 0u;
+    // the epilogue needs the whole K sum: never split
+    const Plan p = plan_for(M, N, K, 1, nullptr, 0);
+    dispatch<kBlocks34, kEpiGegluBwd, true>(a, 1, p, nullptr, static_cast<hipStream_t>(stream));
+    return check_launch(fn);
 }
 
 namespace mi {

@@ -1,0 +1,546 @@
+// gemm_q8_bwd.hip -- the input gradient of a frozen Q8_0 linear for gfx950:
+//   dA[M,K] (=|+=) dC[M,N] . deq(W[N,K])
+// for the forward product C = A . deq(W)^T of gemm_q8.hip (the weights are frozen, so there is no dW).
+//
+// A workgroup computes a BM x BN tile of dA (BN columns k, whole 32-wide blocks) in steps of NS rows n of W:
+//   * dC's rows are staged row-major in LDS, 128 bytes of a row per step;
+//   * a step's BN / 32 blocks of each of NS weight rows are dequantised once per workgroup and staged row-major
+//     [n][k]; the sum runs over n, so a weight fragment has to be k-major: ds_read_b64_tr_b16 transposes on the way
+//     out of LDS (row stride BN + 32 halves, so that the four rows of a 32-lane read cover all banks);
+//   * v_mfma_f32_32x32x16_f16 of the transposed product (a lane holds one row of dA and runs of four columns).
+//
+// fp16: dC as it is, w = fp16(d * q), fp32 sums, dA rounded once.
+// fp32: both operands as fp16 pairs x = hi + lo and three products (hi hi + hi lo + lo hi): what is dropped is
+//   2^-22 of a product, the accuracy of an fp32 product summed in fp32. fp16's range is kept by powers of two, which
+//   are exact: the weights times 2^6 (|w| < 1023; the pair's absolute error 2^-31 is then 2^-25 of a weight of 0.02);
+//   each row of dC by its own exponent, which follows the row's largest element seen so far (gradients of 1e-8 and
+//   of 1e4 keep all their bits). A row's exponent falls by a step only when an element would pass 2^14 (its first
+//   elements are taken to 2^9 .. 2^10), and the row's sums are then brought down with it.
+//
+// Grids too small to fill the GPU split N when the caller gives a workspace: each part stores its sums, fp32, and a
+// second kernel adds them in order (results repeat bit for bit).
+#include "common.hpp"
+
+#include <algorithm>
+#include <type_traits>
+
+namespace mi {
+namespace {
+
+constexpr uint32_t kPast = 0x80000000u;  // a buffer offset past every record: the load returns zeros
+constexpr int kWExp = 6;                 // fp32: the weights' power of two
+constexpr float kRowMax = 16384.0f;      // fp32: a row's exponent falls when an element passes this
+constexpr int kRowExp = 9;               // ... and takes the row's largest element to [2^9, 2^10)
+
+struct BwdArgs {
+    const void* dC;
+    const uint8_t* W;
+    void* dA;
+    float* part;         // N parts: [splits][M][K] fp32, else NULL
+    uint32_t M, N, K, ldc, lda, mode;
+    uint32_t rowbytes;   // of a weight row
+    uint32_t tiles_m, tiles_k, group_m;
+    uint32_t steps, steps_per_split;
+    uint32_t vec;        // dA's rows (or the parts') take 4-element stores
+};
+
+// dA from one 32 x 32 accumulator tile at a time, through a wave-private LDS region (row stride 36 floats): eight
+// lanes store a row's 32 columns. e: the lane's row exponents (fp32).
+constexpr int kStageLd = 36;
+constexpr int kStageFloats = 32 * kStageLd;
+
+template <typename T, int FM, int FN>
+__device__ __forceinline__ void store_tiles(const BwdArgs& a, float* stage, uint32_t mw, uint32_t kw, const floatx16 (&acc)[FM][FN],
+                                            const int (&e)[FM], int lane, float* part) {
+    const int l32 = lane & 31, g = lane >> 5;
+    typedef T T4 __attribute__((ext_vector_type(4)));
+    T* const out = static_cast<T*>(a.dA);
+    for (int b = 0; b < FM * FN; ++b) {
+#pragma unroll
+        for (int i = 0; i < FM; ++i)
+#pragma unroll
+            for (int j = 0; j < FN; ++j)
+                if (b == i * FN + j) {
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) {
+                        floatx4 v = {acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]};
+                        if constexpr (sizeof(T) == 4) {
+#pragma unroll
+                            for (int x = 0; x < 4; ++x) v[x] = ldexpf(v[x], -(e[i] + kWExp));
+                        }
+                        *reinterpret_cast<floatx4*>(&stage[l32 * kStageLd + 8 * q + 4 * g]) = v;
+                    }
+                }
+        __builtin_amdgcn_wave_barrier();
+        const uint32_t mb = mw + 32 * (b / FN), k = kw + 32 * (b % FN) + (lane & 7) * 4;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int row = (lane >> 3) + 8 * i;
+            const uint32_t m = mb + row;
+            floatx4 v = *reinterpret_cast<const floatx4*>(&stage[row * kStageLd + (lane & 7) * 4]);
+            if (m >= a.M || k >= a.K) continue;  // K is a multiple of 32: a tile is inside or past it
+            if (part) {
+                *reinterpret_cast<floatx4*>(part + static_cast<uint64_t>(m) * a.K + k) = v;
+                continue;
+            }
+            T* p = out + static_cast<uint64_t>(m) * a.lda + k;
+            if (a.vec) {
+                if (a.mode) {
+                    const T4 old = *reinterpret_cast<const T4*>(p);
+#pragma unroll
+                    for (int x = 0; x < 4; ++x) v[x] += static_cast<float>(old[x]);
+                }
+                *reinterpret_cast<T4*>(p) = T4{static_cast<T>(v[0]), static_cast<T>(v[1]), static_cast<T>(v[2]), static_cast<T>(v[3])};
+            } else {
+#pragma unroll
+                for (int x = 0; x < 4; ++x) p[x] = static_cast<T>(a.mode ? static_cast<float>(p[x]) + v[x] : v[x]);
+            }
+        }
+        __builtin_amdgcn_wave_barrier();  // every read of this tile precedes the next tile's writes
+    }
+}
+
+template <int CTRL>
+__device__ __forceinline__ float dpp_max(float v) {
+    return fmaxf(v, __builtin_bit_cast(float, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, v), CTRL, 0xf, 0xf, false)));
+}
+
+// ANY: dC's rows or its N do not allow 16-byte loads (element-wise ones instead).
+template <typename T, int BM, int BN, int WM, int WN, bool ANY>
+__global__ __launch_bounds__(WM * WN * 64) void gemm_q8_bwd_kernel(BwdArgs a) {
+    constexpr bool kPair = sizeof(T) == 4;
+    constexpr int NP = kPair ? 2 : 1;
+    constexpr int NT = WM * WN * 64;
+    constexpr int NS = 128 / static_cast<int>(sizeof(T));    // n per step: 128 bytes of a dC row
+    constexpr int AV = 16 / static_cast<int>(sizeof(T));     // dC elements per 16-byte unit
+    constexpr int LDA = NS + 8, LDW = BN + 32;               // LDS row strides in halves
+    constexpr int TM = BM / WM, TN = BN / WN, FM = TM / 32, FN = TN / 32;
+    constexpr int A_IT = BM * 8 / NT;
+    constexpr int KB = BN / 32, W_BLOCKS = NS * KB;          // blocks of a step
+    constexpr int PARTS = W_BLOCKS >= NT ? 1 : NT / W_BLOCKS >= 4 ? 4 : NT / W_BLOCKS;  // threads per block
+    constexpr int QD = 8 / PARTS;                            // q dwords per thread
+    constexpr int W_IT = (W_BLOCKS * PARTS + NT - 1) / NT;
+    static_assert(BM * 8 % NT == 0 && W_BLOCKS * PARTS % NT == 0, "staging must divide evenly");
+    constexpr int kAPlane = BM * LDA, kWPlane = NS * LDW;
+    constexpr int kStage = NP * (kAPlane + kWPlane);
+    constexpr int kHalves = 2 * kStage > 2 * NT / 64 * kStageFloats ? 2 * kStage : 2 * NT / 64 * kStageFloats;
+    __shared__ __attribute__((aligned(16))) _Float16 smem[kHalves];
+    __shared__ int rowexp[kPair ? 2 * BM : 1];
+
+    const int tid = threadIdx.x, lane = tid & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int l32 = lane & 31, g = lane >> 5;
+    const int wm = wave % WM, wn = wave / WM;
+
+    // tile order: groups of group_m row panels, column-major inside a group, one contiguous chunk per XCD
+    const unsigned lin = xcd_swizzle(blockIdx.x, gridDim.x);
+    const uint32_t gsz = a.group_m * a.tiles_k;
+    const uint32_t grp = lin / gsz, rem = lin % gsz;
+    const uint32_t rows_in = min(a.group_m, a.tiles_m - grp * a.group_m);
+    const uint32_t m0 = __builtin_amdgcn_readfirstlane((grp * a.group_m + rem % rows_in) * BM);
+    const uint32_t k0 = __builtin_amdgcn_readfirstlane((rem / rows_in) * BN);
+    const uint32_t s_begin = blockIdx.y * a.steps_per_split;
+    const uint32_t s_end = min(a.steps, s_begin + a.steps_per_split);
+
+    const T* const panel = static_cast<const T*>(a.dC) + static_cast<uint64_t>(m0) * a.ldc;
+    const uint32_t rows = min(a.M - m0, static_cast<uint32_t>(BM));
+    const __amdgpu_buffer_rsrc_t rA = __builtin_amdgcn_make_buffer_rsrc(
+        const_cast<T*>(panel), 0, static_cast<int>(((rows - 1) * a.ldc + a.N) * sizeof(T)), 0x00020000);
+    const __amdgpu_buffer_rsrc_t rW = __builtin_amdgcn_make_buffer_rsrc(
+        const_cast<uint8_t*>(a.W), 0, static_cast<int>((a.N * a.rowbytes + 15u) & ~15u), 0x00020000);
+
+    // dC: unit f of the step is row f / 8, elements AV (f % 8) .. of the step's NS
+    uint32_t a_off[A_IT];
+#pragma unroll
+    for (int i = 0; i < A_IT; ++i) {
+        const uint32_t row = (tid + i * NT) >> 3;
+        a_off[i] = row < rows ? row * a.ldc * sizeof(T) : kPast;
+    }
+    // W: thread u handles part u / W_BLOCKS of block u % W_BLOCKS: row n = block / KB, column block % KB. 64 (32) rows
+    // of 34 * K / 32 bytes are a multiple of 4 bytes, so a thread's place in its dwords is the same every step.
+    uint32_t w_off[W_IT], w_n[W_IT], w_sel[W_IT], w_d[W_IT];
+#pragma unroll
+    for (int i = 0; i < W_IT; ++i) {
+        const uint32_t u = tid + i * NT, blk = u % W_BLOCKS, pt = u / W_BLOCKS;
+        w_n[i] = blk / KB;
+        const uint32_t byte = w_n[i] * a.rowbytes + min(k0 / 32 + blk % KB, a.K / 32 - 1) * 34;
+        const uint32_t q = byte + 2 + pt * (QD * 4);
+        w_d[i] = byte;
+        w_off[i] = q & ~3u;
+        w_sel[i] = (q & 2u) ? 0x05040302u : 0x03020100u;  // bytes 2..5 or 0..3 of (x[j+1]:x[j])
+    }
+
+    typedef T Unit __attribute__((ext_vector_type(AV)));
+    Unit areg[2][A_IT];
+    uint32_t wq[2][W_IT][QD + 1], wd[2][W_IT];
+    auto load_step = [&](uint32_t step, auto RS) {
+        constexpr int rs = decltype(RS)::value;
+        const uint32_t n0 = __builtin_amdgcn_readfirstlane(step * NS);
+#pragma unroll
+        for (int i = 0; i < A_IT; ++i) {
+            const uint32_t n = n0 + ((tid + i * NT) & 7) * AV;
+            if constexpr (ANY) {
+                const uint32_t row = (tid + i * NT) >> 3;
+#pragma unroll
+                for (int e = 0; e < AV; ++e)
+                    areg[rs][i][e] = row < rows && n + e < a.N ? panel[static_cast<uint64_t>(row) * a.ldc + n + e] : static_cast<T>(0.0f);
+            } else {
+                const uint32_t off = n < a.N && a_off[i] != kPast ? a_off[i] + n * static_cast<uint32_t>(sizeof(T)) : kPast;
+                areg[rs][i] = __builtin_bit_cast(Unit, __builtin_amdgcn_raw_buffer_load_b128(rA, off, 0, 0));
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < W_IT; ++i) {
+            const bool in = n0 + w_n[i] < a.N;  // rows past N read as zeros
+            const uint32_t o = in ? w_off[i] + n0 * a.rowbytes : kPast;
+            if constexpr (QD == 8) {
+                const auto x0 = __builtin_amdgcn_raw_buffer_load_b128(rW, o, 0, 0);
+                const auto x1 = __builtin_amdgcn_raw_buffer_load_b128(rW, o + 16, 0, 0);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    wq[rs][i][e] = x0[e];
+                    wq[rs][i][QD / 2 + e] = x1[e];
+                }
+            } else if constexpr (QD == 4) {
+                const auto x0 = __builtin_amdgcn_raw_buffer_load_b128(rW, o, 0, 0);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) wq[rs][i][e] = x0[e];
+            } else {
+                const auto x0 = __builtin_amdgcn_raw_buffer_load_b64(rW, o, 0, 0);
+                wq[rs][i][0] = x0[0];
+                wq[rs][i][1] = x0[1];
+            }
+            wq[rs][i][QD] = __builtin_amdgcn_raw_buffer_load_b32(rW, o + 4 * QD, 0, 0);
+            wd[rs][i] = __builtin_amdgcn_raw_buffer_load_b16(rW, in ? w_d[i] + n0 * a.rowbytes : kPast, 0, 0);
+        }
+    };
+
+    int re[A_IT];  // fp32: the exponents of this thread's rows (the same in the eight threads of a row)
+#pragma unroll
+    for (int i = 0; i < A_IT; ++i) re[i] = 127;
+    auto store_step = [&](auto RS, auto ST) {
+        constexpr int rs = decltype(RS)::value, st = decltype(ST)::value;
+        _Float16* const As = smem + st * kStage;
+        _Float16* const Ws = As + NP * kAPlane;
+#pragma unroll
+        for (int i = 0; i < A_IT; ++i) {
+            const int f = tid + i * NT;
+            _Float16* dst = As + (f >> 3) * LDA + (f & 7) * AV;
+            if constexpr (kPair) {
+                const floatx4 x = areg[rs][i];
+                float mx = fmaxf(fmaxf(fabsf(x[0]), fabsf(x[1])), fmaxf(fabsf(x[2]), fabsf(x[3])));
+                mx = dpp_max<0xb1>(mx);   // quad_perm [1, 0, 3, 2]
+                mx = dpp_max<0x4e>(mx);   // quad_perm [2, 3, 0, 1]
+                mx = dpp_max<0x141>(mx);  // row_half_mirror: the row's eight lanes
+                if (ldexpf(mx, re[i]) > kRowMax)
+                    re[i] = min(re[i], kRowExp + 127 - static_cast<int>(__float_as_uint(mx) >> 23));
+                half4 hi, lo;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const float v = ldexpf(x[e], re[i]);
+                    hi[e] = static_cast<_Float16>(v);
+                    lo[e] = static_cast<_Float16>(v - static_cast<float>(hi[e]));
+                }
+                *reinterpret_cast<half4*>(dst) = hi;
+                *reinterpret_cast<half4*>(dst + kAPlane) = lo;
+                if ((f & 7) == 0) rowexp[st * BM + (f >> 3)] = re[i];
+            } else {
+                *reinterpret_cast<half8*>(dst) = __builtin_bit_cast(half8, areg[rs][i]);
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < W_IT; ++i) {
+            const int u = tid + i * NT, blk = u % W_BLOCKS, pt = u / W_BLOCKS;
+            _Float16* dst = Ws + (blk / KB) * LDW + (blk % KB) * 32 + pt * (QD * 4);
+            const _Float16 d = __builtin_bit_cast(_Float16, static_cast<uint16_t>(wd[rs][i]));
+            uint32_t q[QD];
+#pragma unroll
+            for (int j = 0; j < QD; ++j) q[j] = __builtin_amdgcn_perm(wq[rs][i][j + 1], wq[rs][i][j], w_sel[i]);
+#pragma unroll
+            for (int j = 0; j < QD; j += 2) {
+                if constexpr (kPair) {
+                    // 64 d q is exact in fp32 (19 bits), and so is each step to it
+                    const float s = static_cast<float>(d) * (1 << kWExp), s128 = -128.0f * s;
+                    half8 hi, lo;
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        const uint32_t byte = ((q[j + e / 4] ^ 0x80808080u) >> (8 * (e % 4))) & 0xffu;
+                        const float w = __builtin_fmaf(static_cast<float>(byte), s, s128);
+                        hi[e] = static_cast<_Float16>(w);
+                        lo[e] = static_cast<_Float16>(w - static_cast<float>(hi[e]));
+                    }
+                    *reinterpret_cast<half8*>(dst + 4 * j) = hi;
+                    *reinterpret_cast<half8*>(dst + 4 * j + kWPlane) = lo;
+                } else {
+                    *reinterpret_cast<half8*>(dst + 4 * j) = dequant8_f16(q[j], q[j + 1], d);
+                }
+            }
+        }
+    };
+
+    floatx16 acc[FM][FN];
+    int ce[FM];  // fp32: the exponents that the sums of this lane's rows carry
+#pragma unroll
+    for (int i = 0; i < FM; ++i) {
+        ce[i] = 127;
+#pragma unroll
+        for (int j = 0; j < FN; ++j)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.0f;
+    }
+    // W^T fragment: lane (k = l32, g) takes n = 16 s + 8 g + 0..7 as two transposing reads of four rows; lane i of a
+    // 16-lane group supplies row i / 4, columns 4 (i % 4) .. + 3 of the group's 16
+    const int w_rd = (8 * g + ((lane >> 2) & 3)) * LDW + wn * TN + 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
+    const int a_rd = (wm * TM + l32) * LDA + 8 * g;
+    auto compute = [&](auto ST) {
+        constexpr int st = decltype(ST)::value;
+        const _Float16* const As = smem + st * kStage;
+        const _Float16* const Ws = As + NP * kAPlane;
+        if constexpr (kPair) {
+            int ne[FM];
+            bool moved = false;
+#pragma unroll
+            for (int i = 0; i < FM; ++i) {
+                ne[i] = rowexp[st * BM + wm * TM + 32 * i + l32];
+                moved |= ne[i] != ce[i];
+            }
+            if (__any(moved)) {
+#pragma unroll
+                for (int i = 0; i < FM; ++i) {
+#pragma unroll
+                    for (int j = 0; j < FN; ++j)
+#pragma unroll
+                        for (int r = 0; r < 16; ++r) acc[i][j][r] = ldexpf(acc[i][j][r], ne[i] - ce[i]);
+                    ce[i] = ne[i];
+                }
+            }
+        }
+#pragma unroll
+        for (int s = 0; s < NS / 16; ++s) {
+            half8 af[NP][FM], wf[NP][FN];
+#pragma unroll
+            for (int pl = 0; pl < NP; ++pl) {
+#pragma unroll
+                for (int i = 0; i < FM; ++i)
+                    af[pl][i] = *reinterpret_cast<const half8*>(&As[pl * kAPlane + a_rd + 32 * i * LDA + 16 * s]);
+#pragma unroll
+                for (int j = 0; j < FN; ++j) {
+                    const _Float16* p = &Ws[pl * kWPlane + w_rd + 16 * s * LDW + 32 * j];
+                    const half4 x = lds_read_tr16(p), y = lds_read_tr16(p + 4 * LDW);
+                    wf[pl][j] = half8{x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]};
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < FM; ++i)
+#pragma unroll
+                for (int j = 0; j < FN; ++j) {
+                    if constexpr (kPair) {
+                        acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(wf[NP - 1][j], af[0][i], acc[i][j], 0, 0, 0);
+                        acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(wf[0][j], af[NP - 1][i], acc[i][j], 0, 0, 0);
+                    }
+                    acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(wf[0][j], af[0][i], acc[i][j], 0, 0, 0);
+                }
+        }
+    };
+    using S0 = std::integral_constant<int, 0>;
+    using S1 = std::integral_constant<int, 1>;
+
+    // Step j computes from LDS stage j & 1 while the loads of step j + 2 are in flight; those of step j + 1 are then
+    // stored into the other stage. Loads past the last step re-read it and are not used.
+    const uint32_t n_steps = s_end - s_begin, last = s_end - 1;
+    load_step(s_begin, S0{});
+    store_step(S0{}, S0{});
+    load_step(min(s_begin + 1, last), S1{});
+    __syncthreads();
+    uint32_t j = 0;
+    for (; j + 2 <= n_steps; j += 2) {
+        load_step(min(s_begin + j + 2, last), S0{});
+        __builtin_amdgcn_sched_barrier(0);
+        compute(S0{});
+        store_step(S1{}, S1{});
+        __syncthreads();
+        load_step(min(s_begin + j + 3, last), S1{});
+        __builtin_amdgcn_sched_barrier(0);
+        compute(S1{});
+        // an odd last step is the one just stored; an even one needs nothing more, and storing the last step again
+        // would not change the sums, but would count its rows' exponents twice: the same exponents
+        store_step(S0{}, S0{});
+        __syncthreads();
+    }
+    if (j < n_steps) compute(S0{});
+    __syncthreads();  // every wave is done with the operand tiles before LDS is reused
+    store_tiles<T, FM, FN>(a, reinterpret_cast<float*>(smem) + wave * kStageFloats, m0 + wm * TM, k0 + wn * TN, acc, ce, lane,
+                           a.part ? a.part + static_cast<uint64_t>(blockIdx.y) * a.M * a.K : nullptr);
+}
+
+// The N parts' sums in order: dA = P0 + P1 + ... (+ dA).
+template <typename T>
+__global__ __launch_bounds__(256) void gemm_q8_bwd_sum_kernel(const float* P, uint32_t splits, T* dA, uint32_t M, uint32_t K,
+                                                              uint32_t lda, uint32_t mode, uint32_t vec) {
+    typedef T T4 __attribute__((ext_vector_type(4)));
+    const uint64_t plane = static_cast<uint64_t>(M) * K, total = plane / 4;
+    for (uint64_t i = blockIdx.x * 256ull + threadIdx.x; i < total; i += static_cast<uint64_t>(gridDim.x) * 256) {
+        const float* p = P + 4 * i;
+        floatx4 v = *reinterpret_cast<const floatx4*>(p);
+        uint32_t s = 1;
+        for (; s + 3 < splits; s += 4) {
+            const floatx4 x0 = *reinterpret_cast<const floatx4*>(p + s * plane), x1 = *reinterpret_cast<const floatx4*>(p + (s + 1) * plane),
+                          x2 = *reinterpret_cast<const floatx4*>(p + (s + 2) * plane), x3 = *reinterpret_cast<const floatx4*>(p + (s + 3) * plane);
+            v += x0;
+            v += x1;
+            v += x2;
+            v += x3;
+        }
+        for (; s < splits; ++s) v += *reinterpret_cast<const floatx4*>(p + s * plane);
+        const uint32_t m = static_cast<uint32_t>(4 * i / K), k = static_cast<uint32_t>(4 * i % K);
+        T* o = dA + static_cast<uint64_t>(m) * lda + k;
+        T4 old = {0, 0, 0, 0};
+        if (mode) {
+            if (vec) old = *reinterpret_cast<const T4*>(o);
+            else
+#pragma unroll
+                for (int x = 0; x < 4; ++x) old[x] = o[x];
+        }
+        T4 r;
+#pragma unroll
+        for (int x = 0; x < 4; ++x) r[x] = static_cast<T>(mode ? v[x] + static_cast<float>(old[x]) : v[x]);
+        if (vec) *reinterpret_cast<T4*>(o) = r;
+        else
+#pragma unroll
+            for (int x = 0; x < 4; ++x) o[x] = r[x];
+    }
+}
+
+// N == 0: a sum over nothing.
+template <typename T>
+__global__ __launch_bounds__(256) void gemm_q8_bwd_zero_kernel(T* dA, uint32_t M, uint32_t K, uint32_t lda) {
+    const uint64_t total = static_cast<uint64_t>(M) * K;
+    for (uint64_t i = blockIdx.x * 256ull + threadIdx.x; i < total; i += static_cast<uint64_t>(gridDim.x) * 256)
+        dA[i / K * lda + i % K] = static_cast<T>(0.0f);
+}
+
+constexpr uint32_t kCUs = 256;
+
+enum BuildId { k256x128 = 0, k128x128 = 1, k64x64 = 2 };
+static_assert(k64x64 + 1 == kGemmBwdBuilds, "mi_tuning_set bounds gemm_bwd_cfg by kGemmBwdBuilds");
+
+struct Plan {
+    int build;
+    uint32_t splits;
+};
+
+uint32_t n_step(bool f32) { return f32 ? 32 : 64; }
+
+// The parts that whole steps make of N when `splits` are asked for: none empty.
+uint32_t launched_splits(uint32_t N, bool f32, uint32_t splits) {
+    const uint32_t steps = ceil_div(N, n_step(f32));
+    return ceil_div(steps, ceil_div(steps, splits));
+}
+
+Plan choose(uint32_t M, uint32_t N, uint32_t K, bool f32, bool allow_split) {
+    const int forced = tuning().gemm_bwd_cfg.load(std::memory_order_relaxed);
+    if (forced >= 0) {
+        const uint32_t s = static_cast<uint32_t>(tuning().gemm_bwd_splits.load(std::memory_order_relaxed));
+        return Plan{forced, allow_split ? launched_splits(N, f32, s) : 1u};
+    }
+    auto tiles = [&](uint32_t bm, uint32_t bk) { return static_cast<uint64_t>(ceil_div(M, bm)) * ceil_div(K, bk); };
+    const uint64_t t256 = tiles(256, 128), t128 = tiles(128, 128), t64 = tiles(64, 64);
+    Plan p{t256 >= kCUs ? k256x128 : t128 > kCUs / 2 ? k128x128 : k64x64, 1};
+    if (!allow_split) return p;
+    const uint64_t t = p.build == k256x128 ? t256 : p.build == k128x128 ? t128 : t64;
+    if (p.build == k64x64 && t <= kCUs / 2)
+        p.splits = launched_splits(N, f32, static_cast<uint32_t>(std::min<uint64_t>(kCUs / t, std::max<uint32_t>(N / 128, 1))));
+    return p;
+}
+
+uint64_t part_bytes(uint32_t M, uint32_t K, uint32_t splits) { return splits > 1 ? static_cast<uint64_t>(splits) * M * K * 4 : 0; }
+
+template <typename T, int BM, int BN, int WM, int WN, bool ANY>
+void launch_build(BwdArgs a, uint32_t splits, hipStream_t s) {
+    a.tiles_m = ceil_div(a.M, BM);
+    a.tiles_k = ceil_div(a.K, BN);
+    a.group_m = std::min(a.tiles_m, 4u);
+    a.steps = ceil_div(a.N, 128 / sizeof(T));
+    a.steps_per_split = ceil_div(a.steps, splits);
+    gemm_q8_bwd_kernel<T, BM, BN, WM, WN, ANY><<<dim3(a.tiles_m * a.tiles_k, splits), WM * WN * 64, 0, s>>>(a);
+}
+
+template <typename T>
+void launch(const BwdArgs& a, const Plan& p, bool any, hipStream_t s) {
+    if (any) launch_build<T, 64, 64, 2, 2, true>(a, p.splits, s);
+    else if (p.build == k256x128) launch_build<T, 256, 128, 4, 2, false>(a, p.splits, s);
+    else if (p.build == k128x128) launch_build<T, 128, 128, 4, 2, false>(a, p.splits, s);
+    else launch_build<T, 64, 64, 2, 2, false>(a, p.splits, s);
+    if (!a.part) return;
+    const uint64_t units = static_cast<uint64_t>(a.M) * a.K / 4;
+    gemm_q8_bwd_sum_kernel<T><<<static_cast<unsigned>(std::min<uint64_t>(ceil_div(units, 256), 2048)), 256, 0, s>>>(
+        a.part, p.splits, static_cast<T*>(a.dA), a.M, a.K, a.lda, a.mode, a.vec);
+}
+
+}  // namespace
+}  // namespace mi
+
+using namespace mi;
+
+extern "C" uint64_t mi_gemm_nt_q8_0_bwd_ws_bytes(uint32_t M, uint32_t N, uint32_t K, int dtype) {
+    if (M == 0 || N == 0 || K == 0 || K % 32 || (dtype != MI_F32 && dtype != MI_F16)) return 0;
+    return part_bytes(M, K, choose(M, N, K, dtype == MI_F32, true).splits);
+}
+
+extern "C" int mi_gemm_nt_q8_0_bwd(const void* dC, const void* W, void* dA, int dtype, uint32_t M, uint32_t N, uint32_t K,
+                                   uint32_t mode, uint32_t ldc, uint32_t lda, void* workspace, uint64_t workspace_bytes,
+                                   void* stream) {
+    const char* fn = "mi_gemm_nt_q8_0_bwd";
+    if (M == 0 || K == 0) return MI_OK;
+    if (dtype != MI_F32 && dtype != MI_F16) return fail(MI_ERR_INVALID_ARG, "%s: dtype %d", fn, dtype);
+    if (!dA || (N && (!dC || !W))) return fail(MI_ERR_INVALID_ARG, "%s: null pointer", fn);
+    if (mode > 1) return fail(MI_ERR_INVALID_ARG, "%s: mode %u (0 = store, 1 = accumulate)", fn, mode);
+    if (K % 32) return fail(MI_ERR_UNSUPPORTED, "%s: K=%u is not a multiple of 32 (Q8_0 block)", fn, K);
+    if (ldc == 0) ldc = N;
+    if (lda == 0) lda = K;
+    if (ldc < N || lda < K) return fail(MI_ERR_INVALID_ARG, "%s: ldc %u < N %u or lda %u < K %u", fn, ldc, N, lda, K);
+    const uint64_t e = dtype == MI_F16 ? 2 : 4;
+    if (!aligned(W, 16)) return fail(MI_ERR_ALIGNMENT, "%s: W must be 16-byte aligned", fn);
+    if (!aligned(dC, e) || !aligned(dA, e)) return fail(MI_ERR_ALIGNMENT, "%s: dC and dA must be aligned to their element size", fn);
+    const uint64_t wbytes = static_cast<uint64_t>(N) * (K / 32) * 34;
+    // 32-bit buffer offsets, the upper half of which reads as zeros
+    if (wbytes + 16 >= kPast) return fail(MI_ERR_UNSUPPORTED, "%s: weight >= 2 GiB", fn);
+    if (static_cast<uint64_t>(ldc) * e * 256 >= kPast) return fail(MI_ERR_UNSUPPORTED, "%s: ldc=%u too large", fn, ldc);
+    if (static_cast<uint64_t>(ceil_div(M, 64)) * ceil_div(K, 64) >= (1u << 23)) return fail(MI_ERR_UNSUPPORTED, "%s: M=%u K=%u too large", fn, M, K);
+    const uint64_t cbytes = N ? (static_cast<uint64_t>(M - 1) * ldc + N) * e : 0, abytes = (static_cast<uint64_t>(M - 1) * lda + K) * e;
+    if (overlaps(dA, abytes, dC, cbytes) || overlaps(dA, abytes, W, wbytes))
+        return fail(MI_ERR_ALIASING, "%s: dA overlaps an input", fn);
+    hipStream_t s = static_cast<hipStream_t>(stream);
+    if (N == 0) {
+        if (mode == 1) return MI_OK;
+        const unsigned grid = static_cast<unsigned>(std::min<uint64_t>(ceil_div(static_cast<uint64_t>(M) * K, 256), 2048));
+        if (dtype == MI_F16) gemm_q8_bwd_zero_kernel<_Float16><<<grid, 256, 0, s>>>(static_cast<_Float16*>(dA), M, K, lda);
+        else gemm_q8_bwd_zero_kernel<float><<<grid, 256, 0, s>>>(static_cast<float*>(dA), M, K, lda);
+        return check_launch(fn);
+    }
+    Plan p = choose(M, N, K, dtype == MI_F32, workspace != nullptr);
+    if (part_bytes(M, K, p.splits) > workspace_bytes) p = choose(M, N, K, dtype == MI_F32, false);
+    const uint64_t need = part_bytes(M, K, p.splits);
+    if (need) {
+        if (!aligned(workspace, 16)) return fail(MI_ERR_ALIGNMENT, "%s: workspace must be 16-byte aligned", fn);
+        if (overlaps(workspace, need, dC, cbytes) || overlaps(workspace, need, W, wbytes) || overlaps(workspace, need, dA, abytes))
+            return fail(MI_ERR_ALIASING, "%s: workspace overlaps an operand", fn);
+    }
+    BwdArgs a{};
+    a.dC = dC;
+    a.W = static_cast<const uint8_t*>(W);
+    a.dA = dA;
+    a.part = need ? static_cast<float*>(workspace) : nullptr;
+    a.M = M;
+    a.N = N;
+    a.K = K;
+    a.ldc = ldc;
+    a.lda = lda;
+    a.mode = mode;
+    a.rowbytes = (K / 32) * 34;
+    a.vec = aligned(dA, 4 * e) && lda % 4 == 0 ? 1u : 0u;
+    const bool any = !aligned(dC, 16) || (ldc * e) % 16 || (N * e) % 16;
+    if (dtype == MI_F16) launch<_Float16>(a, p, any, s);
+    else launch<float>(a, p, any, s);
+    return check_launch(fn);
+}

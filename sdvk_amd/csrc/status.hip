@@ -86,6 +86,19 @@ extern "C" int mi_tuning_set(const char* name, const char* value) {
         t.gemm_cfg.store(static_cast<int>(a));
         return MI_OK;
     }
+    if (std::strcmp(name, "gemm_bwd_cfg") == 0) {
+        if (clear) {
+            t.gemm_bwd_cfg.store(-1);
+            t.gemm_bwd_splits.store(1);
+            return MI_OK;
+        }
+        if (!parse_pair(value, 0, mi::kGemmBwdBuilds - 1, 1, 64, 1, &a, &b))
+            return fail(MI_ERR_INVALID_ARG, "mi_tuning_set: gemm_bwd_cfg \"%s\" (want <0..%d>[:<1..64>])", value,
+                        mi::kGemmBwdBuilds - 1);
+        t.gemm_bwd_splits.store(static_cast<int>(b));
+        t.gemm_bwd_cfg.store(static_cast<int>(a));
+        return MI_OK;
+    }
     if (std::strcmp(name, "nn_kernel") == 0) {
         if (!clear && std::strcmp(value, "general") != 0)
             return fail(MI_ERR_INVALID_ARG, "mi_tuning_set: nn_kernel \"%s\" (want general)", value);
@@ -142,6 +155,8 @@ extern "C" void mi_tuning_reset(void) {
     t.attn_split_pieces.store(2);
     t.attn_direct_store.store(0);
     t.attn_simd_waves.store(0);
+    t.gemm_bwd_cfg.store(-1);
+    t.gemm_bwd_splits.store(1);
 }
 
 extern "C" const char* mi_status_string(int status) {

@@ -16,6 +16,8 @@ Names, argument meaning and error behaviour follow the reference
   BlockWeights / BlockDims / sdxl_block_forward (one transformer block)
       sdvkgen.cpp:1739-1763 with crossAttention :1283-1290
   block_ctx_kv / sdxl_block_forward_kv (the block with cached context K / V)
+  *_bwd: gradients of these operators for fine-tuning on frozen Q8_0 weights
+      (extension: the reference's SDXL path only runs forward)
 
 Where the reference calls exit(1) (unsupported attention shape, binding-count
 mismatch) these raise MiError / ValueError instead. Every call goes to
@@ -42,7 +44,8 @@ __all__ = [
     "q8_0_dequant",
     "q8_split_dequant", "q8_0_to_split", "q8_0_quantize", "Pg", "dispatch", "KERNELS", "layernorm", "geglu", "add2",
     "BlockWeights", "BlockDims", "block_workspace_bytes", "sdxl_block_forward", "block_ctx_kv_bytes", "block_ctx_kv",
-    "sdxl_block_forward_kv",
+    "sdxl_block_forward_kv", "gemm_nt_q8_0_bwd", "gemm_bwd_workspace_bytes", "gemm_nt_q8_0_geglu_bwd", "geglu_bwd",
+    "layernorm_bwd", "layernorm_bwd_ws_bytes",
 ]
 
 
@@ -365,6 +368,43 @@ def sdxl_block_forward_kv(w: BlockWeights, dims: BlockDims, x, kv, workspace, *,
     wc, dc = w.c(), dims.c()
     call("mi_sdxl_block_forward_kv", ctypes.byref(wc), ctypes.byref(dc), ptr(x), ptr(kv), getattr(kv, "nbytes", 0),
          ptr(ctx_len), ptr(workspace), nbytes, _s(stream))
+
+
+# ------------------------------------------------------------- backward passes --
+
+def gemm_bwd_workspace_bytes(M: int, N: int, K: int, *, dtype: int = MI_F32) -> int:
+    """Workspace gemm_nt_q8_0_bwd uses for this shape's split of N (0: no split)."""
+    return int(_lib.load().mi_gemm_nt_q8_0_bwd_ws_bytes(M, N, K, dtype))
+
+
+def gemm_nt_q8_0_bwd(dC, W, dA, M: int, N: int, K: int, *, dtype: int = MI_F32, mode: int = 0, ldc: int = 0, lda: int = 0,
+                     workspace=None, stream=None) -> None:
+    """Input gradient of gemm_nt_q8_0 (mi_gemm_nt_q8_0_bwd): dA[M,K] = dC[M,N] . deq(W[N,K]) (mode 1: dA += ...)."""
+    call("mi_gemm_nt_q8_0_bwd", ptr(dC), ptr(W), ptr(dA), dtype, M, N, K, mode, ldc, lda, *_ws(workspace), _s(stream))
+
+
+def gemm_nt_q8_0_geglu_bwd(A, W, dG, dH, M: int, F: int, K: int, *, bias=None, lda: int = 0, lddg: int = 0, lddh: int = 0,
+                           stream=None) -> None:
+    """Gradient of gemm_nt_q8_0_geglu_f16's projection (fp16 A, dG [M,F], dH [M,2F]), which is recomputed from A
+    (mi_gemm_nt_q8_0_geglu_bwd)."""
+    call("mi_gemm_nt_q8_0_geglu_bwd", ptr(A), ptr(W), ptr(bias), ptr(dG), ptr(dH), M, F, K, lda, lddg, lddh, _s(stream))
+
+
+def geglu_bwd(h, dy, dh, rows: int, F: int, *, dtype: int = MI_F32, stream=None) -> None:
+    """Gradient of geglu from a kept h [rows, 2F] fp32; dy [rows, F] and dh [rows, 2F] of `dtype` (mi_geglu_bwd)."""
+    call("mi_geglu_bwd", ptr(h), ptr(dy), ptr(dh), dtype, rows, F, _s(stream))
+
+
+def layernorm_bwd_ws_bytes(rows: int, d: int) -> int:
+    """Workspace layernorm_bwd needs for dgamma and dbeta."""
+    return int(_lib.load().mi_layernorm_bwd_ws_bytes(rows, d))
+
+
+def layernorm_bwd(x, gamma, dy, dx, dgamma, dbeta, workspace, rows: int, d: int, *, res=None, dy_dtype: int = MI_F32,
+                  eps: float = 1e-5, stream=None) -> None:
+    """Gradients of layernorm: dx (+ res), and dgamma / dbeta unless None (mi_layernorm_bwd)."""
+    call("mi_layernorm_bwd", ptr(x), ptr(gamma), ptr(dy), dy_dtype, ptr(res), ptr(dx), ptr(dgamma), ptr(dbeta), rows, d, eps,
+         *_ws(workspace), _s(stream))
 
 
 # --------------------------------------------- reference kernel-name dispatch --
