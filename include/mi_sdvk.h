@@ -472,6 +472,34 @@ int mi_sdxl_block_forward_kv(const mi_block_weights* w, const mi_block_dims* dim
  * (streams, captured graphs) need one each. Gradients are held in fp32 inside and
  * rounded once.                                                              */
 
+/* Gradients of mi_fused_attention / _ex / _ws from the call's inputs, its output and
+ * the output's gradient (P is recomputed; nothing else is kept from the forward pass):
+ *   delta = rowsum(dout out), dP = dout v^T, dS = P (dP - delta),
+ *   dq = scale dS k,  dk = scale dS^T q,  dv = P^T dout
+ * fwd: the forward call's arguments (out is read; precision is ignored). All tensors of
+ * one dtype: out_dtype == in_dtype, MI_F32 or MI_F16, and so dout, dq, dk, dv. The masks
+ * are the forward's: a query that sees no key gets dq = 0 and gives nothing to dk and
+ * dv; keys at or past kv_len[b] get dk = dv = 0, and their k and v are not read. Token
+ * strides 0 -> C (each < 2^22 elements), batch strides 0 -> T * ld; the batch rows of an
+ * output must not overlap. dq, dk and dv overlap no input and not each other, but may be
+ * column blocks of one [rows, 3C] matrix (equal strides). Tensors aligned to their
+ * element; the wide loads take hd % 8 == 0 with 16-byte aligned rows.
+ * MI_F16: P and dS rounded to fp16 once each, scaled so that small weights and gradients
+ * of any size keep their bits, fp32 sums. MI_F32: every operand as fp16 hi + lo (q, k, v
+ * within fp16's range, as in the forward pass; dout of any size).
+ * workspace: mi_fused_attention_bwd_ws_bytes(args) bytes (the sizes of fwd decide),
+ * 16-byte aligned, disjoint from the tensors. Tq == 0 stores zeros in dk and dv. */
+typedef struct mi_attn_bwd_args {
+    mi_attn_args fwd;
+    const void* dout;                        /* [batch][Tq][lddout] */
+    void *dq, *dk, *dv;                      /* [batch][T][ld] */
+    uint64_t lddout, lddq, lddk, lddv;       /* token strides, 0 -> C */
+    uint64_t sdout, sdq, sdk, sdv;           /* batch strides, 0 -> T * ld */
+} mi_attn_bwd_args;
+
+uint64_t mi_fused_attention_bwd_ws_bytes(const mi_attn_bwd_args* args);
+int mi_fused_attention_bwd(const mi_attn_bwd_args* args, void* workspace, uint64_t workspace_bytes, void* stream);
+
 /* Input gradient of mi_gemm_nt_q8_0 (C = A . deq(W)^T):
  *   dA[M,K] (=|+=) dC[M,N] . deq(W[N,K])
  * dC and dA of one dtype (MI_F32 / MI_F16), row strides ldc (0 -> N) and lda

@@ -35,6 +35,13 @@ class MiAttnArgs(ctypes.Structure):
     ]
 
 
+class MiAttnBwdArgs(ctypes.Structure):
+    """Mirror of mi_attn_bwd_args (include/mi_sdvk.h)."""
+    _fields_ = [("fwd", MiAttnArgs), ("dout", _vp), ("dq", _vp), ("dk", _vp), ("dv", _vp),
+                ("lddout", _u64), ("lddq", _u64), ("lddk", _u64), ("lddv", _u64),
+                ("sdout", _u64), ("sdq", _u64), ("sdk", _u64), ("sdv", _u64)]
+
+
 class MiBlockWeights(ctypes.Structure):
     """Mirror of mi_block_weights (include/mi_sdvk.h)."""
     _fields_ = [(n, _vp) for n in (
@@ -115,6 +122,8 @@ SIGNATURES = {
                                        _vp]),
     "mi_sdxl_block_forward_kv": (ctypes.c_int, [ctypes.POINTER(MiBlockWeights), ctypes.POINTER(MiBlockDims), _vp,
                                                 _vp, _u64, _vp, _vp, _u64, _vp]),
+    "mi_fused_attention_bwd_ws_bytes": (_u64, [ctypes.POINTER(MiAttnBwdArgs)]),
+    "mi_fused_attention_bwd": (ctypes.c_int, [ctypes.POINTER(MiAttnBwdArgs), _vp, _u64, _vp]),
     "mi_gemm_nt_q8_0_bwd_ws_bytes": (_u64, [_u32, _u32, _u32, ctypes.c_int]),
     "mi_gemm_nt_q8_0_bwd": (ctypes.c_int, [_vp, _vp, _vp, ctypes.c_int, _u32, _u32, _u32, _u32, _u32, _u32, _vp, _u64, _vp]),
     "mi_gemm_nt_q8_0_geglu_bwd": (ctypes.c_int, [_vp, _vp, _vp, _vp, _vp, _u32, _u32, _u32, _u32, _u32, _u32, _vp]),

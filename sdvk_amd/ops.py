@@ -32,7 +32,7 @@ from typing import Optional, Sequence
 from . import _lib
 from ._lib import (MI_ATTN_PREC_AUTO, MI_ATTN_PREC_FP16, MI_ATTN_PREC_SPLIT, MI_BLOCK_FP16_ACTIVATIONS,
                    MI_BLOCK_FP16_ATTENTION, MI_BLOCK_FUSED_EPILOGUES, MI_BLOCK_JOINT_QKV, MI_F16, MI_F32, MiAttnArgs,
-                   MiBlockDims, MiBlockWeights, MiError, call, ptr)
+                   MiAttnBwdArgs, MiBlockDims, MiBlockWeights, MiError, call, ptr)
 
 __all__ = [
     "MiError", "MI_F32", "MI_F16", "MI_ATTN_PREC_AUTO", "MI_ATTN_PREC_FP16", "MI_ATTN_PREC_SPLIT",
@@ -45,7 +45,7 @@ __all__ = [
     "q8_split_dequant", "q8_0_to_split", "q8_0_quantize", "Pg", "dispatch", "KERNELS", "layernorm", "geglu", "add2",
     "BlockWeights", "BlockDims", "block_workspace_bytes", "sdxl_block_forward", "block_ctx_kv_bytes", "block_ctx_kv",
     "sdxl_block_forward_kv", "gemm_nt_q8_0_bwd", "gemm_bwd_workspace_bytes", "gemm_nt_q8_0_geglu_bwd", "geglu_bwd",
-    "layernorm_bwd", "layernorm_bwd_ws_bytes",
+    "layernorm_bwd", "layernorm_bwd_ws_bytes", "fused_attention_bwd", "fused_attention_bwd_ws_bytes",
 ]
 
 
@@ -371,6 +371,26 @@ def sdxl_block_forward_kv(w: BlockWeights, dims: BlockDims, x, kv, workspace, *,
 
 
 # ------------------------------------------------------------- backward passes --
+
+def fused_attention_bwd_ws_bytes(*, batch: int, Tq: int, Tk: int, C: int, heads: int, dtype: int = MI_F32) -> int:
+    """Workspace fused_attention_bwd needs for these sizes."""
+    x = MiAttnBwdArgs(fwd=MiAttnArgs(batch=batch, Tq=Tq, Tk=Tk, C=C, heads=heads, in_dtype=dtype, out_dtype=dtype))
+    return int(_lib.load().mi_fused_attention_bwd_ws_bytes(ctypes.byref(x)))
+
+
+def fused_attention_bwd(q, k, v, out, dout, dq, dk, dv, workspace, *, batch: int, Tq: int, Tk: int, C: int, heads: int,
+                        causal: bool = False, dtype: int = MI_F32, ldq: int = 0, ldk: int = 0, ldv: int = 0, ldo: int = 0,
+                        sq: int = 0, sk: int = 0, sv: int = 0, so: int = 0, lddout: int = 0, lddq: int = 0, lddk: int = 0,
+                        lddv: int = 0, sdout: int = 0, sdq: int = 0, sdk: int = 0, sdv: int = 0, kv_len=None,
+                        scale: float = 0.0, stream=None) -> None:
+    """Gradients of the fused attention (mi_fused_attention_bwd): dq, dk, dv from q, k, v, out and dout, all of `dtype`."""
+    f = _attn_args(q, k, v, out, batch, Tq, Tk, C, heads, causal, dtype, dtype, ldq, ldk, ldv, ldo, sq, sk, sv, so, kv_len,
+                   scale)
+    x = MiAttnBwdArgs(fwd=f, dout=ptr(dout), dq=ptr(dq), dk=ptr(dk), dv=ptr(dv), lddout=lddout, lddq=lddq, lddk=lddk,
+                      lddv=lddv, sdout=sdout, sdq=sdq, sdk=sdk, sdv=sdv)
+    wp, wn = _ws(workspace)
+    call("mi_fused_attention_bwd", ctypes.byref(x), wp, wn, _s(stream))
+
 
 def gemm_bwd_workspace_bytes(M: int, N: int, K: int, *, dtype: int = MI_F32) -> int:
     """Workspace gemm_nt_q8_0_bwd uses for this shape's split of N (0: no split)."""

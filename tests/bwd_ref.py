@@ -295,10 +295,184 @@ def norm(be, *, rows, d, typ="f32", affine=True, res=True, weights=True, in_plac
         assert np.array_equal(be.get(bdb, np.float32, d).view(np.uint8), db.view(np.uint8))
 
 
-OPS = {"linear": linear, "geglu": geglu, "geglu_gemm": geglu_gemm, "norm": norm}
+# --------------------------------------------------------------- attention --
+
+def softmax_rows(S):
+    top = S.max(-1, keepdims=True, initial=-np.inf)
+    E = np.exp(S - np.where(np.isfinite(top), top, 0.0))
+    t = E.sum(-1, keepdims=True)
+    return E / np.where(t > 0, t, 1.0)
+
+
+def attn_head(q, k, v, do, scale, seen, typ, o_stored):
+    """One head in 64 bits: (dq, dk, dv), and bounds of what the kernels' roundings do to them.
+
+    o_stored: the output as the caller has it, rounded to its type: delta comes from it."""
+    S = np.where(seen, (q @ k.T) * scale, -np.inf)
+    P = softmax_rows(S)
+    dP = do @ v.T
+    delta = (do * o_stored).sum(1, keepdims=True)
+    true_delta = (P * dP).sum(1, keepdims=True)
+    dS = P * (dP - true_delta)
+    want = (scale * dS @ k, scale * dS.T @ q, P.T @ do)
+    T = max(q.shape[0], k.shape[0])
+    f16 = typ == "f16"
+    aq, ak, av, ag = np.abs(q), np.abs(k), np.abs(v), np.abs(do)
+    gm, gr = ag.max(initial=0.0), ag.max(1, keepdims=True, initial=0.0)
+    # a pair leaves 2^-22 of each operand and of the product of the low parts, and not less than 2^-25 of an operand as it
+    # is held: q, k and v as they are, dO with its largest element at 2^8 or more (of the row, or of the head)
+    pair, low = (0.0, 0.0) if f16 else (3 * 2.0 ** -22, TINY16)
+    gq, gk = (0.0, 0.0) if f16 else (gr * 2.0 ** -33, gm * 2.0 ** -33)
+    # scores: 64 terms; the exponent's fma, its argument, the row's maximum and log2 sum in fp32, at the size of the
+    # largest score seen; exp2 and the sum
+    eS = abs(scale) * ((aq @ ak.T) * (pair + 16 * U) + low * (aq.sum(1, keepdims=True) + ak.sum(1)[None, :]))
+    top = np.where(np.isfinite(S), np.abs(S), 0.0).max(1, keepdims=True, initial=0.0) + np.log(T + 1)
+    eP = P * (eS + eS.max(1, keepdims=True, initial=0.0) + 12 * U * top + (16 + T / 16) * U) * 1.1
+    ed = np.abs(delta - true_delta) + (ag * np.abs(o_stored)).sum(1, keepdims=True) * 70 * U
+    adP = ag @ av.T
+    # P and dS as operands: fp16 rounds them (H), a pair leaves 2^-22; not less than 2^-25 of what they are held at:
+    # P 2^14; dS in the key kernel 2^14 over the head's bound of |dP - delta|, to within a factor of two; in the query
+    # kernel exp2(s - m) (l is 1 at least) with the row's largest |dO| at 2^-4 (fp16) or 2^2 (fp32)
+    r = H * 1.01 if f16 else 2.0 ** -22
+    fP = TINY16 * 2.0 ** -14
+    fK = TINY16 * 2.0 ** -13 * (64 * gm * av.max(initial=0.0) + np.abs(delta).max(initial=0.0))
+    fQ = TINY16 * gr * (2.0 ** 4 if f16 else 2.0 ** -2)
+    chain = (T + 64) * U + pair
+
+    def d_score(gfloor, floor):
+        edP = adP * (pair + 16 * U) + gfloor * av.sum(1)[None, :] + low * ag.sum(1, keepdims=True)
+        e = P * (edP + ed) + eP * (np.abs(dP) + np.abs(true_delta) + edP + ed) + 6 * U * np.abs(dS)
+        return e + (np.abs(dS) + e) * r + floor * seen
+
+    eq, ek = d_score(gq, fQ), d_score(gk, fK)
+    aD = np.abs(dS)
+    e_dq = abs(scale) * (eq @ (ak + low) + aD @ (chain * ak + low))
+    e_dk = abs(scale) * (ek.T @ (aq + low) + aD.T @ (chain * aq + low))
+    e_p = eP + (P + eP) * r + fP * seen
+    e_dv = e_p.T @ (ag + gk) + P.T @ (chain * ag + gk)
+    return want, (e_dq, e_dk, e_dv)
+
+
+def attention(be, *, typ, batch=1, Tq, Tk, heads=1, hd=64, causal=False, lens=None, scale=0.0, gap=0, off=0, joint=False, gstd=None,
+              grow=False, peak=1.0, seed=5, poison=False, norm_check=True):
+    rng = rng_of(seed)
+    dt, esz, C = DT[typ], np.dtype(DT[typ]).itemsize, heads * hd
+    ld = 3 * C if joint else C + gap
+    std = gstd if gstd is not None else (1e-3 if typ == "f32" else 0.5)
+
+    def tensor(T, sd=1.0):
+        x = (rng.standard_normal((batch, T, C)) * sd).astype(dt)
+        return x
+
+    q, k, v, do = tensor(Tq, peak), tensor(Tk), tensor(Tk), tensor(Tq, std)
+    if grow:  # queries' gradients from 1e-6 to 1e2 of std, some zero
+        do = (f64(do) * 10.0 ** rng.uniform(-3 if typ == "f16" else -6, 2, (batch, Tq, 1))).astype(dt)
+        do[:, ::7] = 0
+    sc = scale if scale else 1 / math.sqrt(hd)
+    L = [Tk] * batch if lens is None else [min(max(x, 0), Tk) for x in lens]
+    i, j = np.arange(Tq)[:, None], np.arange(Tk)[None, :]
+    seen = [(j < L[b]) & ((j <= i) if causal else True) & (i >= 0) for b in range(batch)]
+    out = np.zeros((batch, Tq, C))
+    for b in range(batch):
+        for h in range(heads):
+            c = slice(h * hd, (h + 1) * hd)
+            S = np.where(seen[b], f64(q[b, :, c]) @ f64(k[b, :, c]).T * sc, -np.inf)
+            out[b, :, c] = softmax_rows(S) @ f64(v[b, :, c])
+    o = out.astype(dt)
+    if poison and lens is not None:  # what lies behind a row's keys is not read
+        for b in range(batch):
+            k[b, L[b]:], v[b, L[b]:] = np.nan, np.inf
+
+    A = Arena(be)
+
+    def place(x, l=ld):
+        T = x.shape[1]
+        buf = np.full(off + batch * T * l, SENTINEL, dtype=dt)
+        if x.size:
+            np.lib.stride_tricks.as_strided(buf[off:], x.shape, (T * l * esz, l * esz, esz))[...] = x
+        return buf
+
+    keep = [A.put(place(x)) for x in (q, k, v, o, do)]
+    pq, pk, pv, po, pg = (be.at(x, off * esz) for x in keep)
+    if joint:
+        n = off + batch * max(Tq, Tk) * ld
+        g = A.out(n, dt)
+        bufs = [(g, n, i * C) for i in range(3)]
+    else:
+        sizes = [off + batch * T * ld for T in (Tq, Tk, Tk)]
+        bufs = [(A.out(n, dt), n, 0) for n in sizes]
+    pd = [be.at(b, (off + o_) * esz) for b, _, o_ in bufs]
+    bl = A.put(np.asarray(lens, np.int32)) if lens is not None else None
+
+    import ctypes
+
+    from sdvk_amd._lib import MiAttnArgs, MiAttnBwdArgs
+    f = MiAttnArgs(q=pq, k=pk, v=pv, out=po, batch=batch, Tq=Tq, Tk=Tk, C=C, heads=heads, causal=int(causal), in_dtype=CODE[typ],
+                   out_dtype=CODE[typ], ldq=ld, ldk=ld, ldv=ld, ldo=ld, kv_len=bl.ptr if bl else None, scale=scale)
+    x = MiAttnBwdArgs(fwd=f, dout=pg, dq=pd[0], dk=pd[1], dv=pd[2], lddout=ld, lddq=ld, lddk=ld, lddv=ld)
+    need = be.value("mi_fused_attention_bwd_ws_bytes", ctypes.byref(x))
+    wsb = be.buf(np.full(max(need, 16), 0xff, np.uint8))
+    args = (ctypes.byref(x), wsb.ptr, need, None)
+    be.call("mi_fused_attention_bwd", *args)
+
+    flats = [be.get(b, dt, n) for b, n, _ in bufs]
+    grads = []
+    rests = [np.ones(fl.shape, bool) for fl in flats]
+    for (b, n, o_), fl, T, rest in zip(bufs, flats, (Tq, Tk, Tk), rests):
+        st = (T * ld, ld, 1)
+        grads.append(np.lib.stride_tricks.as_strided(fl[off + o_:], (batch, T, C), tuple(s * esz for s in st)))
+        np.lib.stride_tricks.as_strided(rest[off + o_:], (batch, T, C), st)[...] = False
+    if joint:
+        rests = [rests[0] & rests[1] & rests[2]] * 3
+    for fl, rest in zip(flats, rests):
+        assert np.all(fl[rest] == SENTINEL), "wrote outside the gradients"
+    rels = [[], [], []]
+    kz, vz = (np.where(np.isfinite(f64(t)), f64(t), 0.0) for t in (k, v))
+    for b in range(batch):
+        for h in range(heads):
+            c = slice(h * hd, (h + 1) * hd)
+            want, tol = attn_head(f64(q[b, :, c]), kz[b, :, c], vz[b, :, c], f64(do[b, :, c]), sc, seen[b], typ, f64(o[b, :, c]))
+            for n, (got, w, t) in enumerate(zip(grads, want, tol)):
+                rels[n].append(check(got[b, :, c], w, t * 1.02 + store_err(w, typ) * 1.01 + 1e-37, f"attention d{'qkv'[n]} batch {b} head {h}"))
+            for n in (1, 2):
+                assert np.all(grads[n][b, L[b]:, c] == 0), "a key past its row's length has a gradient"
+    if norm_check and Tq * Tk >= 4096 and not grow and scale == 0 and peak == 1:
+        # independent roundings, H / sqrt 3 each at most: P or dS, the result, and delta's (from the stored output) where a
+        # row has few keys (a peaked row's dS is the small difference of dP and delta: the bounds above hold it). fp32:
+        # 2^-22 of the operands of three products and of what is left out of them, 8 units of it in all
+        most = H if typ == "f16" else 8 * 2.0 ** -22
+        for n in range(3):
+            rel_check(max(rels[n]), most, f"attention d{'qkv'[n]}")
+    A.unchanged()
+    be.call("mi_fused_attention_bwd", *args)
+    for (b, n, _), fl in zip(bufs, flats):
+        assert np.array_equal(be.get(b, dt, n).view(np.uint8), fl.view(np.uint8)), "a second call gave other bits"
+
+
+OPS = {"attention": attention, "linear": linear, "geglu": geglu, "geglu_gemm": geglu_gemm, "norm": norm}
 
 # Small shapes where the operators can go wrong, on the emulator and on the GPU.
 CASES = {
+    "attention": [
+        dict(typ="f16", Tq=1, Tk=1), dict(typ="f32", Tq=1, Tk=1), dict(typ="f16", Tq=1, Tk=100, heads=2), dict(typ="f32", Tq=100, Tk=1, heads=2),
+        dict(typ="f16", Tq=100, Tk=150, heads=2), dict(typ="f32", Tq=70, Tk=130, heads=2), dict(typ="f16", Tq=130, Tk=77, batch=2, heads=2, lens=[77, 13]),
+        dict(typ="f32", Tq=66, Tk=77, batch=2, lens=[64, 1]), dict(typ="f16", Tq=65, Tk=70, batch=3, lens=[0, 65, -2], poison=True),
+        dict(typ="f32", Tq=33, Tk=70, batch=3, lens=[0, 64, 700], poison=True), dict(typ="f16", Tq=140, Tk=140, causal=True, heads=2),
+        dict(typ="f32", Tq=140, Tk=140, causal=True), dict(typ="f16", Tq=70, Tk=200, causal=True), dict(typ="f32", Tq=200, Tk=70, causal=True),
+        dict(typ="f16", Tq=77, Tk=77, causal=True, batch=2, lens=[77, 5]),
+        # head widths, rows off their 16-byte places, gaps, the joint [rows, 3C] gradient
+        dict(typ="f16", Tq=70, Tk=66, heads=3, hd=40), dict(typ="f32", Tq=70, Tk=66, heads=3, hd=40), dict(typ="f16", Tq=40, Tk=70, heads=2, hd=20),
+        dict(typ="f32", Tq=40, Tk=70, heads=2, hd=20), dict(typ="f16", Tq=40, Tk=70, heads=2, hd=37), dict(typ="f32", Tq=40, Tk=70, heads=3, hd=1),
+        dict(typ="f16", Tq=40, Tk=70, heads=2, off=1), dict(typ="f32", Tq=40, Tk=70, heads=2, off=1, gap=3), dict(typ="f16", Tq=40, Tk=70, heads=2, gap=8, off=8),
+        dict(typ="f16", Tq=70, Tk=70, heads=2, joint=True), dict(typ="f32", Tq=70, Tk=70, heads=2, joint=True, batch=2),
+        # scales, peaked rows, gradients of many sizes
+        dict(typ="f16", Tq=40, Tk=70, scale=-0.2), dict(typ="f32", Tq=40, Tk=70, scale=-0.2), dict(typ="f16", Tq=40, Tk=140, peak=30.0),
+        dict(typ="f32", Tq=40, Tk=140, peak=30.0), dict(typ="f16", Tq=140, Tk=70, grow=True), dict(typ="f32", Tq=140, Tk=70, grow=True),
+        dict(typ="f32", Tq=40, Tk=70, gstd=1e-20), dict(typ="f32", Tq=40, Tk=70, gstd=1e10), dict(typ="f16", Tq=40, Tk=70, gstd=2.0 ** -20, norm_check=False),
+        dict(typ="f16", Tq=40, Tk=70, gstd=0.0), dict(typ="f32", Tq=0, Tk=5), dict(typ="f16", Tq=5, Tk=0),
+        # parts of the queries
+        dict(typ="f16", Tq=300, Tk=40, heads=2), dict(typ="f32", Tq=260, Tk=140), dict(typ="f16", Tq=300, Tk=140, causal=True),
+    ],
     "linear": [
         dict(typ="f16", M=1, N=1, K=32), dict(typ="f32", M=1, N=1, K=32), dict(typ="f16", M=3, N=8, K=96),
         dict(typ="f32", M=2, N=96, K=64), dict(typ="f16", M=130, N=72, K=160), dict(typ="f32", M=70, N=36, K=160),
@@ -340,6 +514,13 @@ CASES = {
 }
 # Larger shapes, on the GPU alone: grids that stride over rows, splits as the rules choose them, tails.
 GPU_CASES = {
+    "attention": [
+        dict(typ="f16", Tq=1024, Tk=1024, heads=4, batch=2), dict(typ="f16", Tq=1024, Tk=77, heads=20, batch=2, lens=[77, 30]),
+        dict(typ="f32", Tq=900, Tk=900, heads=4), dict(typ="f32", Tq=1000, Tk=154, heads=5, batch=2, lens=[154, 100]), dict(typ="f16", Tq=2000, Tk=2000, heads=2),
+        dict(typ="f16", Tq=1500, Tk=1500, heads=2, causal=True), dict(typ="f32", Tq=1100, Tk=1100, heads=2, causal=True), dict(typ="f32", Tq=77, Tk=77, heads=12, causal=True),
+        dict(typ="f16", Tq=17, Tk=3000, heads=3), dict(typ="f32", Tq=5, Tk=2000, heads=2, hd=40), dict(typ="f16", Tq=3000, Tk=17, heads=3),
+        dict(typ="f16", Tq=1000, Tk=1000, heads=3, hd=20), dict(typ="f32", Tq=600, Tk=700, heads=3, hd=40),
+    ],
     "linear": [
         dict(typ="f32", M=2, N=1280, K=1280), dict(typ="f16", M=16, N=1280, K=640), dict(typ="f16", M=77, N=640, K=2048),
         dict(typ="f32", M=154, N=1280, K=2048), dict(typ="f16", M=1000, N=640, K=2560), dict(typ="f32", M=577, N=1280, K=1280),

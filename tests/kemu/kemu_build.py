@@ -31,7 +31,7 @@ LIB = OUT / "libkemu_sdvk.so"
 CXX = os.environ.get("KEMU_CXX", "/opt/rocm/llvm/bin/clang++")
 
 SOURCES = ["status.hip", "q8_0.hip", "gemm_q8.hip", "gemm_nn_q8.hip", "attention.hip", "glue.hip", "block.hip",
-           "glue_bwd.hip", "gemm_q8_bwd.hip", "gguf.cpp"]
+           "glue_bwd.hip", "gemm_q8_bwd.hip", "attention_bwd.hip", "gguf.cpp"]
 FLAGS = ["-std=c++17", "-O2", "-g0", "-fPIC", "-fno-strict-aliasing", "-Xclang", "-ffloat16-excess-precision=none",
          "-Wno-unused-command-line-argument", "-Wno-psabi"]
 

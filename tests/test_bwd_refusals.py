@@ -83,3 +83,37 @@ def test_layernorm(lib):
     for bad in (dict(dx=addr(0)), dict(dx=addr(2)), dict(dx=addr(3) + 16), dict(dx=addr(1)), dict(dg=addr(4)), dict(db=addr(5)), dict(dg=addr(1)),
                 dict(ws=addr(0)), dict(ws=addr(4)), dict(ws=addr(6))):
         assert call(**bad) == _lib.MI_ERR_ALIASING, bad
+
+
+def attn(lib, ws=addr(20), ws_bytes=None, **kw):
+    import ctypes
+
+    a = dict(q=addr(0), k=addr(1), v=addr(2), out=addr(3), batch=2, Tq=64, Tk=64, C=128, heads=2, in_dtype=1, out_dtype=1)
+    g = dict(dout=addr(4), dq=addr(5), dk=addr(6), dv=addr(7))
+    for name, v in kw.items():
+        (g if name in dict(_lib.MiAttnBwdArgs._fields_) else a)[name] = v
+    x = _lib.MiAttnBwdArgs(fwd=_lib.MiAttnArgs(**a), **g)
+    need = lib.mi_fused_attention_bwd_ws_bytes(ctypes.byref(x))
+    return lib.mi_fused_attention_bwd(ctypes.byref(x), ws, need if ws_bytes is None else ws_bytes, None)
+
+
+def test_attention(lib):
+    import ctypes
+
+    assert lib.mi_fused_attention_bwd(None, None, 0, None) == _lib.MI_ERR_INVALID_ARG
+    assert lib.mi_fused_attention_bwd_ws_bytes(None) == 0
+    assert attn(lib, Tq=0, Tk=0, ws=None) == _lib.MI_OK
+    for bad in (dict(in_dtype=2), dict(out_dtype=0), dict(batch=0), dict(q=None), dict(k=None), dict(v=None), dict(out=None), dict(dout=None),
+                dict(dq=None), dict(dk=None), dict(dv=None), dict(scale=float("inf")), dict(scale=float("nan")), dict(ldq=100), dict(lddk=64),
+                dict(sdq=100), dict(sdv=8000), dict(ws=None), dict(ws_bytes=100)):
+        assert attn(lib, **bad) == _lib.MI_ERR_INVALID_ARG, bad
+    for bad in (dict(C=130), dict(heads=3), dict(C=129, heads=1), dict(batch=70000), dict(ldk=1 << 22), dict(lddq=1 << 22),
+                dict(Tq=1 << 26, C=2, batch=8)):
+        assert attn(lib, **bad) == _lib.MI_ERR_UNSUPPORTED, bad
+    for bad in (dict(q=addr(0) + 1), dict(dv=addr(7) + 1), dict(ws=addr(20) + 8)):
+        assert attn(lib, **bad) == _lib.MI_ERR_ALIGNMENT, bad
+    for bad in (dict(dq=addr(0)), dict(dk=addr(3)), dict(dv=addr(4) + 64), dict(dk=addr(5)), dict(dv=addr(6) + 2), dict(ws=addr(2)), dict(ws=addr(7))):
+        assert attn(lib, **bad) == _lib.MI_ERR_ALIASING, bad
+    # column blocks of one [rows, 3C] matrix may not overlap each other either
+    assert attn(lib, dq=addr(5), dk=addr(5) + 128 * 2 - 2, dv=addr(5) + 512, lddq=384, lddk=384, lddv=384) == _lib.MI_ERR_ALIASING
+    assert ctypes.sizeof(_lib.MiAttnBwdArgs) == ctypes.sizeof(_lib.MiAttnArgs) + 4 * 8 + 8 * 8
