@@ -483,12 +483,16 @@ int mi_sdxl_block_forward_kv(const mi_block_weights* w, const mi_block_dims* dim
  * strides 0 -> C (each < 2^22 elements), batch strides 0 -> T * ld; the batch rows of an
  * output must not overlap. dq, dk and dv overlap no input and not each other, but may be
  * column blocks of one [rows, 3C] matrix (equal strides). Tensors aligned to their
- * element; the wide loads take hd % 8 == 0 with 16-byte aligned rows.
+ * element; MI_F16 with hd % 8 == 0 and 16-byte aligned rows is read in place, other
+ * tensors are packed into the workspace first (and gradients without 4-element aligned
+ * rows leave through it).
  * MI_F16: P and dS rounded to fp16 once each, scaled so that small weights and gradients
  * of any size keep their bits, fp32 sums. MI_F32: every operand as fp16 hi + lo (q, k, v
  * within fp16's range, as in the forward pass; dout of any size).
- * workspace: mi_fused_attention_bwd_ws_bytes(args) bytes (the sizes of fwd decide),
- * 16-byte aligned, disjoint from the tensors. Tq == 0 stores zeros in dk and dv. */
+ * workspace: mi_fused_attention_bwd_ws_bytes(args) bytes, 16-byte aligned, disjoint from
+ * the tensors. The bytes go by sizes and dtype, and by whether the addresses and strides
+ * are multiples of 16 bytes (of 4 elements, for dq, dk and dv; NULL counts as one).
+ * Tq == 0 stores zeros in dk and dv. */
 typedef struct mi_attn_bwd_args {
     mi_attn_args fwd;
     const void* dout;                        /* [batch][Tq][lddout] */

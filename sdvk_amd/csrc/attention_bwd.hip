@@ -6,30 +6,38 @@
 //   dQ = scale dS K,   dK = scale dS^T Q,   dV = P^T dO
 // P is never stored: two kernels recompute it, one for queries, one for keys.
 //
-// attn_bwd_q_kernel: a workgroup owns 128 queries of one (batch, head), 4 waves x 32, and walks over 64-key tiles of K
-// and V in LDS. S^T = K Q^T and dP^T = V dO^T leave a lane with one query and 32 keys, so the softmax is the forward
-// pass's online one: with the running maximum m, dQ accumulates exp2(s - m) (dP - delta) K and is rescaled with the row
-// sum l when m rises (lazily: kLazy); dQ = scale / l times that. Nothing but Q, K, V, O and dO is needed from the
-// forward pass; m + log2 l and delta of each row go to the workspace for the other kernel.
-// attn_bwd_k_kernel: a workgroup owns 128 keys, 4 waves x 32, and walks over 64-query tiles of Q and dO.
-// S = Q K^T and dP = dO V^T leave a lane with one key and 32 queries; P = exp2(s - (m + log2 l)). dV^T = dO^T P and
-// dK^T = Q^T dS take P and dS from the registers they are in (the MFMA's output order of the contracted index is the
-// order in which the other operand is read).
+// attn_bwd_q_kernel: blocks of 128 queries of one (batch, head), 4 waves x 32, walk over 64-key tiles of K and V in
+// LDS. S^T = K Q^T and dP^T = V dO^T leave a lane with one query and 32 keys, so the softmax is the forward pass's
+// online one: with a running reference m, dQ accumulates exp2(s - m) (dP - delta) K and is rescaled with the row sum l
+// when m rises (lazily); dQ = scale / l times that. Nothing but Q, K, V, O and dO is needed from the forward pass;
+// m + log2 l and delta of each row go to the workspace for the other kernel.
+// attn_bwd_k_kernel: blocks of 128 keys, 4 waves x 32, walk over 64-query tiles of Q and dO. S = Q K^T and dP = dO V^T
+// leave a lane with one key and 32 queries; P = exp2(s - (m + log2 l)). dV^T = dO^T P and dK^T = Q^T dS take P and dS
+// from the registers they are in (the MFMA's output order of the contracted index is the order in which the other
+// operand is read).
 // Every MFMA is v_mfma_f32_32x32x16_f16: seven products of Tq x Tk x 64 instead of five, for no atomic additions and
 // no dQ partials in memory (results repeat bit for bit).
 //
-// Each tile is staged row-major (64 rows x 64 columns fp16); 16-byte chunk c of row r lies at slot c ^ f(r), f the bit
-// reversal of (r / 2) % 8. That makes both uses free of bank conflicts: the 16-byte row fragments (16 rows of one chunk:
-// every slot of either half once) and the transposing reads of ds_read_b64_tr_b16 (four rows of four chunks: the
-// reversal puts rows r and r + 2 into different halves of a row).
+// Work is dealt in tiles: each workgroup (two per CU) takes as many whole blocks as there are for all, and the tiles of
+// the blocks left, in order, are cut into equal shares, so that a grid of 640 blocks does not take two rounds of 512, and
+// few blocks still fill the GPU. A workgroup whose share ends or begins inside a block writes its part of the block to
+// the workspace; a second kernel adds the parts of such blocks in order.
 //
-// fp32 tensors are carried as fp16 pairs x = hi + lo and three MFMAs per product (hi hi + hi lo + lo hi), as in the
-// forward pass; P and dS too. fp16's range is kept by powers of two, which are exact:
-//   * dS of a query row, in the first kernel, by the row's largest |dO| (kRowExp);
-//   * P, in the second kernel, by 2^14 (weights of 2^-28 are normal numbers then); dS by what keeps
+// Each tile is staged row-major (64 rows x 64 columns fp16) by loads straight into LDS; 16-byte chunk c of row r lies at
+// slot c ^ f(r), f the bit reversal of (r / 2) % 8. That makes both uses free of bank conflicts (counted: none): the
+// 16-byte row fragments (16 rows of one chunk: every slot of either half once) and the transposing reads of
+// ds_read_b64_tr_b16 (four rows of four chunks: the reversal puts rows r and r + 2 into different halves of a row).
+//
+// fp32 tensors, and fp16 ones whose rows are not 16-byte aligned or a multiple of 8 wide, are first packed into
+// [batch, head][token][64] fp16 planes in the workspace (attn_bwd_pack_kernel). fp32 becomes pairs x = hi + lo and takes
+// three MFMAs per product (hi hi + hi lo + lo hi), as in the forward pass; P and dS too. fp16's range is kept by powers
+// of two, which are exact:
+//   * in the query kernel, dS of a row by the row's largest |dO| (kRowExp), carried by exp2's argument;
+//   * in the key kernel, P by 2^14 (weights of 2^-28 are normal numbers then); dS by what keeps
 //     2^14 (64 max|dO| max|V| + max|delta|) under 2^15, max|dO| and max|delta| over the (batch, head), max|V| over the
-//     wave's keys: dS cannot overflow, and a weight of 2^-20 still has all its bits;
-//   * dO, fp32 only, by its largest element (of the row, or of the (batch, head)), taken to 2^8.
+//     block's keys: dS cannot overflow, and a weight of 2^-20 still has all its bits. fp16: that power of two is carried
+//     by V (its largest element stays in 2^-6 .. 2^12; P's power gives way beyond that);
+//   * dO of fp32, row by row, by its largest element, taken to 2^8.
 #include "common.hpp"
 
 #include <algorithm>
@@ -38,36 +46,52 @@
 namespace mi {
 namespace {
 
-constexpr int kB = 128;                  // queries (keys) per workgroup
+constexpr int kB = 128;                  // queries (keys) per block
 constexpr int kTile = 64;                // keys (queries) per staged tile
-// The running max rises when a score passes it by this (exp2 domain), and the power of two that a row's largest |dO| is
-// taken to in dS: exp2(s - m) (dP - delta) stays in fp16's range for |V| up to 32 even where 64 products agree in sign. A
-// pair's low part is a subnormal number where dS is small, so fp32 takes it larger and rescales more often.
+// A row's reference m rises when a lane's sum of exp2(s - m) passes 2^kLazy; kRowExp is the power of two that a row's
+// largest |dO| is taken to in dS: exp2(s - m) (dP - delta) stays in fp16's range for |V| up to 32 even where 64 products
+// agree in sign. A pair's low part is a subnormal number where dS is small, so fp32 takes it larger and rescales more often.
 template <int NP>
-constexpr float kLazy = NP == 2 ? 2.0f : 8.0f;
+constexpr int kLazy = NP == 2 ? 2 : 8;
 template <int NP>
 constexpr int kRowExp = NP == 2 ? 2 : -4;
-constexpr int kPairExp = 8;              // fp32: the power of two that the largest |dO| is taken to in its pairs
+constexpr int kPairExp = 8;              // fp32: the power of two that a row's largest |dO| is taken to in its pairs
 constexpr int kPExp = 14;                // P's power of two in the key kernel
 constexpr uint32_t kOob = 0x80000000u;   // a buffer offset past every record: the load returns zeros
 
 struct Tensor {
     const void* p;
-    uint64_t ld, s;  // token and batch strides, elements
+    uint64_t ld, s, sh;  // token, batch and head strides, elements
+};
+// An operand of the MFMA kernels: fp16 rows of whole 16-byte chunks, the head h of row t of batch b at
+// p + b s + h sh + t ld; the plane of the pairs' low parts `lo` elements further.
+struct Operand {
+    const _Float16* p;
+    uint64_t ld, s, sh, lo;
+};
+// How one kernel's blocks are dealt: NT tiles to a block (causal: fewer, see before()), nb blocks to a (batch, head),
+// `per` tiles to those. Each of wgs workgroups takes `whole` blocks, and an equal share of the tiles of the blocks left.
+struct Deal {
+    uint32_t NT, nb, per, wgs, whole;
 };
 struct BwdArgs {
     Tensor q, k, v, o, g;     // g: dO
     Tensor dq, dk, dv;
+    Operand xq, xk, xv, xg;
     uint32_t batch, Tq, Tk, heads, hd;
     int causal;
     const int32_t* kv_len;
     float c;                  // |scale| log2(e)
     float sgn, scale;         // the scale's sign, and itself
-    // workspace: per (batch, head) rows of qpad = 128 ceil(Tq / 128): m + log2 l (+inf: no key), delta; then per
-    // 128 queries max|dO| and max|delta|; then the query parts' dK and dV
+    // workspace: per (batch, head) rows of 128 ceil(Tq / 128): m + log2 l (+inf: no key), delta, and (packed) the row's
+    // exponent in the pairs; then per 128 queries max|dO| and max|delta|; then the parts of shared blocks
     float *lse, *delta, *maxes, *part;
-    uint32_t qblocks, kblocks, splits;
-    uint32_t vout;            // dq, dk and dv take 4-element stores
+    int* rexp;
+    uint32_t qblocks;
+    Deal qd, kd;
+    uint32_t ohd;             // columns of dq, dk and dv: hd, or 64 of planes in the workspace (unpacked by a kernel of its own)
+    Tensor user[3];           // (unpack) the caller's dq, dk and dv
+    uint32_t vin;             // (pack) the inputs take 16-byte loads
 };
 
 __device__ __forceinline__ uint32_t keys_of(const BwdArgs& a, uint32_t b) {
@@ -76,44 +100,110 @@ __device__ __forceinline__ uint32_t keys_of(const BwdArgs& a, uint32_t b) {
     return l < 0 ? 0u : min(static_cast<uint32_t>(l), a.Tk);
 }
 template <typename T>
-__device__ __forceinline__ const T* head_of(const Tensor& t, uint32_t b, uint32_t h, uint32_t hd) {
-    return static_cast<const T*>(t.p) + b * t.s + static_cast<uint64_t>(h) * hd;
+__device__ __forceinline__ T* head_of(const Tensor& t, uint32_t b, uint32_t h) {
+    return static_cast<T*>(const_cast<void*>(t.p)) + b * t.s + h * t.sh;
 }
+__device__ __forceinline__ const _Float16* head_of(const Operand& x, uint32_t b, uint32_t h) { return x.p + b * x.s + h * x.sh; }
+
+// ---- shares ------------------------------------------------------------------------------------------------------
+//
+// Tiles of the blocks before block i of a (batch, head). Causal: query block i sees keys up to its last query (2 i + 2
+// tiles, NT at most), key block i the queries from its first key on (NT - 2 i tiles; past the queries one, without work).
+template <bool KEYS>
+__host__ __device__ inline uint32_t before(uint32_t i, uint32_t NT, bool causal) {
+    if (!causal) return i * NT;
+    if (KEYS) {
+        const uint32_t half = (NT + 1) / 2, j = i < half ? i : half;
+        return j * (NT + 1 - j) + (i - j);
+    }
+    const uint32_t half = NT / 2, j = i < half ? i : half;
+    return j * (j + 1) + (i - j) * NT;
+}
+// The first tile of share w of `total`, counted from the first block that is dealt in shares.
+__host__ __device__ inline uint64_t share_start(const Deal& d, uint64_t total, uint64_t w) { return w * total / d.wgs; }
+__host__ __device__ inline uint32_t dealt_whole(const Deal& d) { return d.wgs * d.whole; }
+// Tiles that are dealt in shares (blocks are dealt whole only where all have NT tiles).
+__host__ __device__ inline uint64_t shared_tiles(const Deal& d, uint32_t bhs) {
+    return static_cast<uint64_t>(bhs) * d.per - static_cast<uint64_t>(dealt_whole(d)) * d.NT;
+}
+
+// The pieces of a workgroup's work, one after the other: tiles [t0, t1) of block blk of (batch, head) bh.
+template <bool KEYS>
+struct Pieces {
+    const Deal d;
+    const bool causal;
+    uint64_t base, at, end;  // tiles, counted from the first block of all
+    uint32_t id, blocks;     // the next whole block and those left
+    uint32_t bh, blk, t0, t1;
+    bool whole, first;       // the whole block; the first piece of the share
+
+    __device__ __forceinline__ Pieces(const Deal& d_, bool causal_, uint32_t bhs, uint32_t w) : d(d_), causal(causal_) {
+        const uint64_t total = shared_tiles(d, bhs);
+        base = static_cast<uint64_t>(dealt_whole(d)) * d.NT;
+        at = base + share_start(d, total, w);
+        end = base + share_start(d, total, w + 1);
+        base = at;
+        id = w * d.whole;
+        blocks = d.whole;
+    }
+    __device__ __forceinline__ bool next() {
+        if (blocks) {
+            bh = id / d.nb;
+            blk = id % d.nb;
+            t0 = 0;
+            t1 = d.NT;
+            whole = true;
+            ++id;
+            --blocks;
+            return true;
+        }
+        if (at >= end) return false;
+        first = at == base;
+        bh = static_cast<uint32_t>(at / d.per);
+        const uint32_t r = static_cast<uint32_t>(at % d.per);
+        uint32_t lo = 0, hi = d.nb;  // the last block with no more than r tiles before it
+        while (hi - lo > 1) {
+            const uint32_t mid = (lo + hi) / 2;
+            if (before<KEYS>(mid, d.NT, causal) <= r) lo = mid;
+            else hi = mid;
+        }
+        blk = lo;
+        const uint32_t b0 = before<KEYS>(blk, d.NT, causal), n = before<KEYS>(blk + 1, d.NT, causal) - b0;
+        t0 = r - b0;
+        t1 = static_cast<uint32_t>(min(static_cast<uint64_t>(n), t0 + (end - at)));
+        whole = t0 == 0 && t1 == n;
+        at += t1 - t0;
+        return true;
+    }
+};
+// The parts of a shared block: workgroups w0 .. w1 (equal: not shared); each keeps its part in slot 0 if its share
+// begins with it, else in slot 1.
+template <bool KEYS>
+struct Parts {
+    uint64_t total, u0;
+    uint32_t w0, w1;
+    __device__ __forceinline__ Parts(const Deal& d, bool causal, uint32_t bhs, uint32_t bh, uint32_t blk) {
+        w0 = w1 = 0;
+        if (bh * d.nb + blk < dealt_whole(d)) return;
+        total = shared_tiles(d, bhs);
+        const uint64_t skip = static_cast<uint64_t>(dealt_whole(d)) * d.NT;
+        u0 = static_cast<uint64_t>(bh) * d.per + before<KEYS>(blk, d.NT, causal) - skip;
+        const uint64_t u1 = static_cast<uint64_t>(bh) * d.per + before<KEYS>(blk + 1, d.NT, causal) - skip;
+        // share w begins at floor(w total / wgs): tile u is in the last share that begins at or before it
+        w0 = static_cast<uint32_t>(((u0 + 1) * d.wgs - 1) / total);
+        w1 = static_cast<uint32_t>((u1 * d.wgs - 1) / total);
+    }
+    __device__ __forceinline__ uint64_t slot(const Deal& d, uint32_t w) const {
+        return 2ull * w + (share_start(d, total, w) >= u0 ? 0 : 1);
+    }
+};
+constexpr uint32_t kQPart = kB * 64 + 2 * kB;  // floats of a query block's part: dQ rows, m, l
+constexpr uint32_t kKPart = 2 * kB * 64;       // of a key block's: dK and dV rows
+
+// ---- fragments ------------------------------------------------------------------------------------------------------
+
 // bit reversal of (r / 2) % 8
 __device__ __forceinline__ int swz(int r) { return ((r >> 3) & 1) | ((r >> 1) & 2) | ((r << 1) & 4); }
-
-// Eight consecutive elements of a row, those at or past `valid` zero, as fp16 and, for fp32, fp16 residuals, times sc.
-template <typename T, bool VEC>
-__device__ __forceinline__ void load8(const T* p, int valid, float sc, half8& hi, half8& lo) {
-    T x[8];
-#pragma unroll
-    for (int e = 0; e < 8; ++e) x[e] = static_cast<T>(0.0f);
-    if constexpr (VEC) {
-        typedef T V __attribute__((ext_vector_type(16 / sizeof(T))));
-        if (valid > 0) {
-#pragma unroll
-            for (int i = 0; i < 8 * static_cast<int>(sizeof(T)) / 16; ++i) {
-                const V v = reinterpret_cast<const V*>(p)[i];
-#pragma unroll
-                for (int e = 0; e < static_cast<int>(16 / sizeof(T)); ++e) x[i * (16 / sizeof(T)) + e] = v[e];
-            }
-        }
-    } else {
-#pragma unroll
-        for (int e = 0; e < 8; ++e)
-            if (e < valid) x[e] = p[e];
-    }
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-        if constexpr (sizeof(T) == 4) {
-            const float v = x[e] * sc;
-            hi[e] = static_cast<_Float16>(v);
-            lo[e] = static_cast<_Float16>(v - static_cast<float>(hi[e]));
-        } else {
-            hi[e] = sc < 0.0f ? -x[e] : x[e];  // fp16: the sign alone
-        }
-    }
-}
 __device__ __forceinline__ half8 zero8() { return half8{0, 0, 0, 0, 0, 0, 0, 0}; }
 
 __device__ __forceinline__ float wave_max(float v) {
@@ -123,87 +213,107 @@ __device__ __forceinline__ float wave_max(float v) {
 }
 // The exponent e of a positive x in [2^e, 2^(e+1)); zero and subnormals -127.
 __device__ __forceinline__ int exponent(float x) { return static_cast<int>(__float_as_uint(x) >> 23) - 127; }
+__device__ __forceinline__ int clamp(int x, int lo, int hi) { return max(lo, min(hi, x)); }
 
-// One staged operand: 64 rows of up to 64 columns of a [rows, ld] tensor, two LDS stages of NP planes.
-// fp16 rows of whole 16-byte chunks travel straight into LDS; others through registers (converted on the way).
-template <typename T, bool VEC>
-struct Stage {
-    static constexpr bool kDma = VEC && sizeof(T) == 2;
-    static constexpr int NP = sizeof(T) == 4 ? 2 : 1;
-    static constexpr int kPlane = kTile * 64, kHalves = 2 * NP * kPlane;
-    _Float16* lds;
-    const T* base;
-    uint64_t ld;
-    uint32_t rows;  // rows of the tensor that are read; others are zeros
-    int hd, tid;
-    float sc;       // fp32: the elements' power of two
-    half8 r[kDma ? 1 : 2][NP];
+// Row `t` of an operand's head, columns 16 s + 8 g .. + 7, both planes; zeros where !in or past hd.
+template <int NP>
+__device__ __forceinline__ void row_operand(const _Float16* head, const Operand& x, uint32_t t, int s, int g, bool in, int hd,
+                                            half8 (&f)[NP]) {
+    const int d = 16 * s + 8 * g;
+    const _Float16* p = head + (in ? t : 0u) * x.ld + (d < hd ? d : 0);
+#pragma unroll
+    for (int pl = 0; pl < NP; ++pl) {
+        f[pl] = zero8();
+        if (in && d < hd) f[pl] = *reinterpret_cast<const half8*>(p + pl * x.lo);
+    }
+}
 
-    __device__ __forceinline__ Stage(_Float16* l, const T* b, uint64_t ld_, uint32_t rows_, uint32_t hd_, int tid_, float sc_ = 1.0f)
-        : lds(l), base(b), ld(ld_), rows(rows_), hd(static_cast<int>(hd_)), tid(tid_), sc(sc_) {}
-    // chunk tid + 256 i of the tile: row c / 8, slot c % 8
-    __device__ __forceinline__ void load(uint32_t row0, int st) {
-        if constexpr (kDma) {
-            const uint32_t n = row0 < rows ? min(rows - row0, static_cast<uint32_t>(kTile)) : 0u;
-            const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(
-                const_cast<T*>(base + static_cast<uint64_t>(n ? row0 : 0u) * ld), 0,
-                n ? static_cast<int>(((n - 1) * ld + hd) * 2) : 0, 0x00020000);
-            const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
+// Where a lane's fragments lie in a staged tile (halves), the same in every stage and plane.
+struct Places {
+    int row[4], col[2][2];
+    __device__ __forceinline__ explicit Places(int lane) {
+        const int l32 = lane & 31, g = lane >> 5, rk = (lane >> 2) & 3;
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                const int piece = wave * 2 + i, row = 8 * piece + (lane >> 3), c = (lane & 7) ^ swz(row);
-                __builtin_amdgcn_raw_ptr_buffer_load_lds(
-                    rs, (__attribute__((address_space(3))) void*)(lds + st * NP * kPlane + piece * 512), 16,
-                    c * 8 < hd ? (row * static_cast<uint32_t>(ld) + c * 8) * 2u : kOob, 0, 0, 0);
+        for (int s = 0; s < 4; ++s) row[s] = l32 * 64 + (((2 * s + g) ^ swz(l32)) * 8);
+        // lane i of a 16-lane group supplies row i / 4, columns 4 (i % 4) .. + 3 of the group's 16
+#pragma unroll
+        for (int rd = 0; rd < 2; ++rd)
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                const int d = 32 * u + 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
+                col[rd][u] = (4 * g + rk) * 64 + (((d >> 3) ^ swz(8 * rd + 4 * g + rk)) * 8) + (d & 7);
             }
-        } else {
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                const int ch = tid + 256 * i, row = ch >> 3, c = (ch & 7) ^ swz(row);
-                const bool in = row0 + row < rows;
-                half8 lo = zero8();
-                load8<T, VEC>(base + static_cast<uint64_t>(in ? row0 + row : 0u) * ld + (c * 8 < hd ? c * 8 : 0), in ? hd - c * 8 : 0, sc,
-                              r[i][0], lo);
-                if constexpr (NP == 2) r[i][1] = lo;
-            }
-        }
-    }
-    __device__ __forceinline__ void store(int st) {
-        if constexpr (!kDma) {
-#pragma unroll
-            for (int i = 0; i < 2; ++i)
-#pragma unroll
-                for (int p = 0; p < NP; ++p)
-                    *reinterpret_cast<half8*>(lds + (st * NP + p) * kPlane + (tid + 256 * i) * 8) = r[i][p];
-        }
-    }
-    // this thread's loads of a tile are in LDS (before the barrier that hands it over)
-    __device__ __forceinline__ void settle() {
-        if constexpr (kDma) __builtin_amdgcn_s_waitcnt(0x0F70);
-    }
-    // rows 32 t + l32, columns 16 s + 8 g .. + 7
-    __device__ __forceinline__ half8 row_frag(int st, int p, int t, int s, int l32, int g) const {
-        return *reinterpret_cast<const half8*>(lds + (st * NP + p) * kPlane + (32 * t + l32) * 64 + (((2 * s + g) ^ swz(l32)) * 8));
-    }
-    // column 32 u + l32, rows 32 t + 16 sp + 4 g + {0..3, 8..11}
-    __device__ __forceinline__ half8 col_frag(int st, int p, int t, int sp, int u, int lane) const {
-        const int g = lane >> 5, rk = (lane >> 2) & 3, d = 32 * u + 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
-        half4 x[2];
-#pragma unroll
-        for (int rd = 0; rd < 2; ++rd) {
-            const int row = 32 * t + 16 * sp + 8 * rd + 4 * g + rk;
-            x[rd] = lds_read_tr16(lds + (st * NP + p) * kPlane + row * 64 + (((d >> 3) ^ swz(row)) * 8) + (d & 7));
-        }
-        return half8{x[0][0], x[0][1], x[0][2], x[0][3], x[1][0], x[1][1], x[1][2], x[1][3]};
     }
 };
+
+// One staged operand: 64 rows of up to 64 columns, NS LDS stages of NP planes. The stages are arrays of their own and known
+// at compile time: the compiler then knows that reads of one do not wait for the loads into another.
+template <int NP, int NS>
+struct Stage {
+    static constexpr int kPlane = kTile * 64, kHalves = NP * kPlane;
+    _Float16* lds[NS];
+    const _Float16* base;
+    uint64_t ld, lo;
+    uint32_t rows;  // rows of the tensor that are read; others are zeros
+    int wave, lane;
+    uint32_t off[2];
+
+    __device__ __forceinline__ void set(const _Float16* head, const Operand& x, uint32_t rows_, int hd, int wave_, int lane_) {
+        base = head;
+        ld = x.ld;
+        lo = x.lo;
+        rows = rows_;
+        wave = wave_;
+        lane = lane_;
+        // lane l brings slot l % 8 of row 8 piece + l / 8
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const int row = 8 * (wave * 2 + i) + (lane >> 3), c = (lane & 7) ^ swz(row);
+            off[i] = c * 8 < hd ? (row * static_cast<uint32_t>(ld) + c * 8) * 2u : kOob;
+        }
+        hd2 = hd;
+    }
+    int hd2;
+    template <int ST>
+    __device__ __forceinline__ void load(uint32_t row0) {
+        const uint32_t n = row0 < rows ? min(rows - row0, static_cast<uint32_t>(kTile)) : 0u;
+#pragma unroll
+        for (int p = 0; p < NP; ++p) {
+            const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(
+                const_cast<_Float16*>(base + p * lo + static_cast<uint64_t>(n ? row0 : 0u) * ld), 0,
+                n ? static_cast<int>(((n - 1) * ld + hd2) * 2) : 0, 0x00020000);
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+                __builtin_amdgcn_raw_ptr_buffer_load_lds(
+                    rs, (__attribute__((address_space(3))) void*)(lds[ST] + p * kPlane + (wave * 2 + i) * 512), 16, off[i], 0, 0, 0);
+        }
+    }
+    // rows 32 t + l32, columns 16 s + 8 g .. + 7
+    template <int ST>
+    __device__ __forceinline__ void row_frag(const Places& at, int t, int s, half8 (&f)[NP]) const {
+#pragma unroll
+        for (int p = 0; p < NP; ++p) f[p] = *reinterpret_cast<const half8*>(lds[ST] + p * kPlane + 32 * t * 64 + at.row[s]);
+    }
+    // column 32 u + l32, rows 32 t + 16 sp + 4 g + {0..3, 8..11}
+    template <int ST>
+    __device__ __forceinline__ void col_frag(const Places& at, int t, int sp, int u, half8 (&f)[NP]) const {
+#pragma unroll
+        for (int p = 0; p < NP; ++p) {
+            half4 x[2];
+#pragma unroll
+            for (int rd = 0; rd < 2; ++rd) x[rd] = lds_read_tr16(lds[ST] + p * kPlane + (32 * t + 16 * sp + 8 * rd) * 64 + at.col[rd][u]);
+            f[p] = half8{x[0][0], x[0][1], x[0][2], x[0][3], x[1][0], x[1][1], x[1][2], x[1][3]};
+        }
+    }
+};
+__device__ __forceinline__ void wait_loads() { __builtin_amdgcn_s_waitcnt(0x0F70); }  // vmcnt(0)
 
 // acc += a b of one 16-deep slice: one MFMA, or three of the pairs' planes (those with a residual first).
 template <int NP>
 __device__ __forceinline__ floatx16 mma(const half8 (&x)[NP], const half8 (&y)[NP], floatx16 acc) {
     if constexpr (NP == 2) {
-        acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(x[1], y[0], acc, 0, 0, 0);
-        acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(x[0], y[1], acc, 0, 0, 0);
+        acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(x[NP - 1], y[0], acc, 0, 0, 0);
+        acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(x[0], y[NP - 1], acc, 0, 0, 0);
     }
     return __builtin_amdgcn_mfma_f32_32x32x16_f16(x[0], y[0], acc, 0, 0, 0);
 }
@@ -221,428 +331,716 @@ __device__ __forceinline__ void operand(const float (&x)[16], int sp, half8 (&f)
     }
 }
 
-// Columns 32 u + 8 (r / 4) + 4 g + r % 4 of one row of T from two accumulator tiles, times f.
+// Columns 32 u + 8 (r / 4) + 4 g + r % 4 of one row of T from two accumulator tiles, times f; hd is a multiple of 4, the row
+// 4-element aligned (other gradients go through planes in the workspace).
 template <typename T>
-__device__ __forceinline__ void store_row(T* row, const floatx16 (&acc)[2], float f, int hd, int g, bool vec) {
+__device__ __forceinline__ void store_row(T* row, const floatx16 (&acc)[2], float f, int hd, int g) {
     typedef T T4 __attribute__((ext_vector_type(4)));
 #pragma unroll
     for (int u = 0; u < 2; ++u)
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
             const int d = 32 * u + 8 * q + 4 * g;
-            if (d >= hd) continue;
-            const T4 v = {static_cast<T>(acc[u][4 * q] * f), static_cast<T>(acc[u][4 * q + 1] * f),
-                          static_cast<T>(acc[u][4 * q + 2] * f), static_cast<T>(acc[u][4 * q + 3] * f)};
-            if (vec) {
-                *reinterpret_cast<T4*>(row + d) = v;
-            } else {
-#pragma unroll
-                for (int e = 0; e < 4; ++e)
-                    if (d + e < hd) row[d + e] = v[e];
-            }
+            if (d < hd)
+                *reinterpret_cast<T4*>(row + d) = T4{static_cast<T>(acc[u][4 * q] * f), static_cast<T>(acc[u][4 * q + 1] * f),
+                                                     static_cast<T>(acc[u][4 * q + 2] * f), static_cast<T>(acc[u][4 * q + 3] * f)};
         }
 }
 
-template <typename T, bool VEC>
-__global__ __launch_bounds__(256, 2) void attn_bwd_q_kernel(BwdArgs a) {
-    typedef Stage<T, VEC> St;
-    constexpr int NP = St::NP;
-    __shared__ __attribute__((aligned(16))) _Float16 smem[2 * St::kHalves];
+// ---- packing --------------------------------------------------------------------------------------------------------
+
+// q, k, v and dO (blockIdx.y) into fp16 planes [batch, head][token][64], columns past hd zero; for dO also delta of the
+// row and its exponent. Eight lanes a row; keys past their row's length are not read and become zeros.
+template <typename T>
+__global__ __launch_bounds__(256) void attn_bwd_pack_kernel(BwdArgs a) {
+    constexpr bool kPair = sizeof(T) == 4;
+    const uint32_t which = blockIdx.y;
+    // (fields one by one: a choice between the structures would copy them to memory)
+    auto of = [&](auto q, auto k, auto v, auto g) { return which == 0 ? q : which == 1 ? k : which == 2 ? v : g; };
+    const Tensor t{of(a.q.p, a.k.p, a.v.p, a.g.p), of(a.q.ld, a.k.ld, a.v.ld, a.g.ld), of(a.q.s, a.k.s, a.v.s, a.g.s), a.hd};
+    const Operand x{of(a.xq.p, a.xk.p, a.xv.p, a.xg.p), 64, of(a.xq.s, a.xk.s, a.xv.s, a.xg.s), of(a.xq.sh, a.xk.sh, a.xv.sh, a.xg.sh),
+                    of(a.xq.lo, a.xk.lo, a.xv.lo, a.xg.lo)};
+    const uint32_t len = which == 0 || which == 3 ? a.Tq : a.Tk;
+    const uint64_t rows = static_cast<uint64_t>(a.batch) * len * a.heads;
+    const uint64_t at = blockIdx.x * 32ull + (threadIdx.x >> 3);
+    const uint64_t tok = at / a.heads;
+    const uint32_t h = static_cast<uint32_t>(at % a.heads), b = static_cast<uint32_t>(tok / max(len, 1u)), i = static_cast<uint32_t>(tok % max(len, 1u));
+    const int d = (threadIdx.x & 7) * 8, hd = static_cast<int>(a.hd);
+    const bool in = at < rows && (which == 0 || which == 3 || i < keys_of(a, b));
+    auto read = [&](const Tensor& y, float (&v)[8]) {
+        const T* p = head_of<T>(y, in ? b : 0u, in ? h : 0u) + static_cast<uint64_t>(in ? i : 0u) * y.ld;
+        typedef T V __attribute__((ext_vector_type(16 / sizeof(T))));
+        constexpr int NV = 16 / sizeof(T);
+        if (a.vin && in && d < hd) {
+#pragma unroll
+            for (int k = 0; k < 8 / NV; ++k) {
+                const V w = reinterpret_cast<const V*>(p + d)[k];
+#pragma unroll
+                for (int e = 0; e < NV; ++e) v[k * NV + e] = static_cast<float>(w[e]);
+            }
+        } else {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] = in && d + e < hd ? static_cast<float>(p[d + e]) : 0.0f;
+        }
+    };
+    float v[8];
+    read(t, v);
+    int re = 0;
+    if (which == 3) {  // uniform in the workgroup
+        float o[8], delta = 0.0f, mx = 0.0f;
+        read(a.o, o);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            delta = __builtin_fmaf(v[e], o[e], delta);
+            mx = fmaxf(mx, fabsf(v[e]));
+        }
+#pragma unroll
+        for (int k = 1; k < 8; k <<= 1) {
+            delta += __shfl_xor(delta, k);
+            mx = fmaxf(mx, __shfl_xor(mx, k));
+        }
+        if (kPair) re = clamp(kPairExp - exponent(mx), -100, 100);
+        if (in && d == 0) {
+            const uint64_t row = (static_cast<uint64_t>(b) * a.heads + h) * a.qblocks * kB + i;
+            a.delta[row] = delta;
+            a.rexp[row] = re;
+        }
+    }
+    if (at >= rows) return;
+    _Float16* out = const_cast<_Float16*>(head_of(x, b, h)) + i * x.ld + d;
+    half8 hi, lo;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        const float w = kPair ? ldexpf(v[e], re) : v[e];
+        hi[e] = static_cast<_Float16>(w);
+        lo[e] = static_cast<_Float16>(w - static_cast<float>(hi[e]));
+    }
+    *reinterpret_cast<half8*>(out) = hi;
+    if (kPair) *reinterpret_cast<half8*>(out + x.lo) = lo;
+}
+
+// ---- queries --------------------------------------------------------------------------------------------------------
+
+// T: the type of O (read where !PACKED) and dQ.
+template <typename T, bool PACKED>
+__global__ __launch_bounds__(256, sizeof(T) == 4 ? 2 : 3) void attn_bwd_q_kernel(BwdArgs a) {
+    constexpr int NP = sizeof(T) == 4 ? 2 : 1;
+    constexpr int NS = 2;
+    static_assert(NP == 1 || PACKED, "fp32 is packed into pairs");
+    typedef Stage<NP, NS> St;
+    __shared__ __attribute__((aligned(16))) _Float16 ks0[St::kHalves], ks1[St::kHalves], vs0[St::kHalves], vs1[St::kHalves];
     __shared__ float wmax[2][4];
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int l32 = lane & 31, g = lane >> 5;
-    const uint32_t blk = xcd_swizzle(blockIdx.x, gridDim.x);
-    const uint32_t qb = blk % a.qblocks, bh = blk / a.qblocks;
-    const uint32_t h = bh % a.heads, b = bh / a.heads;
-    const uint32_t q0 = qb * kB, qi = q0 + wave * 32 + l32;
-    const int hd = static_cast<int>(a.hd);
-    const uint32_t L = keys_of(a, b);
-    const uint32_t kend = a.causal ? min(L, q0 + kB) : L;
-    // tiles that end at or before kfull need no mask for any query of this wave
-    uint32_t kfull = L / kTile * kTile;
-    if (a.causal) kfull = min(kfull, (q0 + wave * 32 + 1) / kTile * kTile);
+    const int hd = static_cast<int>(a.hd), ohd = static_cast<int>(a.ohd);
+    St K, V;
+    K.lds[0] = ks0;
+    K.lds[1] = ks1;
+    V.lds[0] = vs0;
+    V.lds[1] = vs1;
 
-    St K(smem, head_of<T>(a.k, b, h, a.hd), a.k.ld, kend, a.hd, tid);
-    St V(smem + St::kHalves, head_of<T>(a.v, b, h, a.hd), a.v.ld, kend, a.hd, tid);
-    const uint32_t ntiles = (kend + kTile - 1) / kTile;
-    if (ntiles) {
-        K.load(0, 0);
-        V.load(0, 0);
-    }
-
-    // this lane's query: fragments of Q (with the scale's sign) and dO, delta, max|dO|
-    const bool in = qi < a.Tq;
-    const T* qp = head_of<T>(a.q, b, h, a.hd) + static_cast<uint64_t>(in ? qi : 0u) * a.q.ld;
-    const T* op = head_of<T>(a.o, b, h, a.hd) + static_cast<uint64_t>(in ? qi : 0u) * a.o.ld;
-    const T* gp = head_of<T>(a.g, b, h, a.hd) + static_cast<uint64_t>(in ? qi : 0u) * a.g.ld;
-    half8 qf[4][NP], gf[4][NP];
-    float delta = 0.0f, gmax = 0.0f;
+    const Places places(lane);
+    const uint32_t wg = xcd_swizzle(blockIdx.x, gridDim.x);
+    Pieces<false> pc(a.qd, a.causal != 0, a.batch * a.heads, wg);
+    while (pc.next()) {
+        const uint32_t bh = pc.bh, h = bh % a.heads, b = bh / a.heads, qb = pc.blk;
+        const uint32_t q0 = qb * kB, qi = q0 + wave * 32 + l32;
+        // this lane's query: fragments of Q (with the scale's sign) and dO, delta, the row's power of two
+        const bool in = qi < a.Tq;
+        const uint64_t row = static_cast<uint64_t>(bh) * a.qblocks * kB + q0 + wave * 32 + l32;
+        half8 qf[4][NP], gf[4][NP], of[PACKED ? 1 : 4];
+        float delta = 0.0f, gmax = 0.0f;
+        int re = 0;
 #pragma unroll
-    for (int s = 0; s < 4; ++s) {
-        const int d = 16 * s + 8 * g, n = in ? hd - d : 0;
-        half8 lo = zero8();
-        load8<T, VEC>(qp + (d < hd ? d : 0), n, a.sgn, qf[s][0], lo);
-        if constexpr (NP == 2) qf[s][NP - 1] = lo;
-#pragma unroll
-        for (int e = 0; e < 8; ++e)
-            if (e < n) {
-                const float x = static_cast<float>(gp[d + e]);
-                delta = __builtin_fmaf(x, static_cast<float>(op[d + e]), delta);
-                gmax = fmaxf(gmax, fabsf(x));
-            }
-    }
-    delta += __shfl_xor(delta, 32);
-    gmax = fmaxf(gmax, __shfl_xor(gmax, 32));
-    // the row's power of two: max|dO| to 2^kRowExp in dS, to 2^kPairExp in the pairs
-    const int ge = max(-100, min(100, kRowExp<NP> - exponent(gmax)));
-    const float gsc = ldexpf(1.0f, ge);
-    constexpr float kPairUp = NP == 2 ? 64.0f : 1.0f;
-    static_assert(NP == 1 || kPairExp - kRowExp<2> == 6, "2^6 between the pairs of dO and dS");
-#pragma unroll
-    for (int s = 0; s < 4; ++s) {
-        const int d = 16 * s + 8 * g;
-        half8 lo = zero8();
-        load8<T, VEC>(gp + (d < hd ? d : 0), in ? hd - d : 0, NP == 2 ? gsc * kPairUp : 1.0f, gf[s][0], lo);
-        if constexpr (NP == 2) gf[s][NP - 1] = lo;
-    }
-    const float dscale = NP == 2 ? 1.0f / kPairUp : gsc;
-    const float ds0 = delta * gsc;
-    const float bmax = wave_max(gmax), dmax = wave_max(fabsf(delta));
-    if (lane == 0) {
-        wmax[0][wave] = bmax;
-        wmax[1][wave] = dmax;
-    }
-
-    floatx16 acc[2];
-#pragma unroll
-    for (int r = 0; r < 16; ++r) acc[0][r] = acc[1][r] = 0.0f;
-    float m = -INFINITY, l = 0.0f;
-    if (ntiles) {
-        K.store(0);
-        V.store(0);
-        K.settle();
-    }
-    __syncthreads();
-    for (uint32_t it = 0; it < ntiles; ++it) {
-        const int st = it & 1;
-        const bool more = it + 1 < ntiles;
-        if (more) {
-            K.load((it + 1) * kTile, st ^ 1);
-            V.load((it + 1) * kTile, st ^ 1);
-        }
-#pragma unroll
-        for (int t = 0; t < 2; ++t) {
-            floatx16 s, dp;
-#pragma unroll
-            for (int r = 0; r < 16; ++r) s[r] = dp[r] = 0.0f;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                half8 kf[NP], vf[NP];
-#pragma unroll
-                for (int p = 0; p < NP; ++p) {
-                    kf[p] = K.row_frag(st, p, t, i, l32, g);
-                    vf[p] = V.row_frag(st, p, t, i, l32, g);
-                }
-                s = mma(kf, qf[i], s);
-                dp = mma(vf, gf[i], dp);
-            }
-            const uint32_t k0 = it * kTile + 32 * t;
-            if (it * kTile >= kfull) {
-#pragma unroll
-                for (int r = 0; r < 16; ++r) {
-                    const uint32_t key = k0 + 8 * (r >> 2) + 4 * g + (r & 3);
-                    if (key >= L || (a.causal && key > qi)) s[r] = -INFINITY;
-                }
-            }
-            float mx = s[0];
-#pragma unroll
-            for (int r = 1; r < 16; ++r) mx = fmaxf(mx, s[r]);
-            mx = fmaxf(mx, __shfl_xor(mx, 32)) * a.c;
-            if (__any(mx > m + kLazy<NP>)) {
-                const float mn = fmaxf(m, mx);
-                const float alpha = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - mn);
-                m = mn;
-                l *= alpha;
-#pragma unroll
-                for (int r = 0; r < 16; ++r) {
-                    acc[0][r] *= alpha;
-                    acc[1][r] *= alpha;
-                }
-            }
-            const float mu = m == -INFINITY ? 0.0f : m;
-            float ds[16];
-#pragma unroll
-            for (int r = 0; r < 16; ++r) {
-                const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], a.c, -mu));
-                l += p;
-                ds[r] = p * __builtin_fmaf(dp[r], dscale, -ds0);
-            }
-#pragma unroll
-            for (int sp = 0; sp < 2; ++sp) {
-                half8 df[NP];
-                operand<NP>(ds, sp, df);
-#pragma unroll
-                for (int u = 0; u < 2; ++u) {
-                    half8 kt[NP];
-#pragma unroll
-                    for (int p = 0; p < NP; ++p) kt[p] = K.col_frag(st, p, t, sp, u, lane);
-                    acc[u] = mma(kt, df, acc[u]);
-                }
+        for (int s = 0; s < 4; ++s) {
+            row_operand<NP>(head_of(a.xq, b, h), a.xq, qi, s, g, in, PACKED ? 64 : hd, qf[s]);
+            row_operand<NP>(head_of(a.xg, b, h), a.xg, qi, s, g, in, PACKED ? 64 : hd, gf[s]);
+            if constexpr (!PACKED) {
+                const int d = 16 * s + 8 * g;
+                const T* op = head_of<T>(a.o, b, h) + static_cast<uint64_t>(in ? qi : 0u) * a.o.ld;
+                of[s] = zero8();
+                if (in && d < hd) of[s] = *reinterpret_cast<const half8*>(op + d);
             }
         }
-        if (more) {
-            K.store(st ^ 1);
-            V.store(st ^ 1);
-            K.settle();
+        if constexpr (PACKED) {
+            if (in) {
+                delta = a.delta[row];
+                re = a.rexp[row];
+            }
         }
+        const uint32_t L = keys_of(a, b);
+        const uint32_t kend = a.causal ? min(L, q0 + kB) : L;
+        // tiles that end at or before kfull need no mask for any query of this wave
+        uint32_t kfull = L / kTile * kTile;
+        if (a.causal) kfull = min(kfull, (q0 + wave * 32 + 1) / kTile * kTile);
+        const uint32_t ntiles = min(pc.t1, (kend + kTile - 1) / kTile);
+        K.set(head_of(a.xk, b, h), a.xk, kend, PACKED ? 64 : hd, wave, lane);
+        V.set(head_of(a.xv, b, h), a.xv, kend, PACKED ? 64 : hd, wave, lane);
+        uint32_t it = pc.t0;
+        if (it < ntiles) {
+            K.template load<0>(it * kTile);
+            V.template load<0>(it * kTile);
+        }
+
+#pragma unroll
+        for (int s = 0; s < 4; ++s) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                if constexpr (!PACKED) delta = __builtin_fmaf(static_cast<float>(gf[s][0][e]), static_cast<float>(of[s][e]), delta);
+                gmax = fmaxf(gmax, fabsf(static_cast<float>(gf[s][0][e])));
+            }
+            if (a.sgn < 0.0f) {
+#pragma unroll
+                for (int p = 0; p < NP; ++p) qf[s][p] = -qf[s][p];
+            }
+        }
+        gmax = fmaxf(gmax, __shfl_xor(gmax, 32));
+        if constexpr (!PACKED) delta += __shfl_xor(delta, 32);
+        // exp2(s - m) carries 2^ge; dP and delta carry 2^re
+        const int ge = clamp(kRowExp<NP> - exponent(gmax), -100, 100);
+        const float dl = ldexpf(delta, re);
+        const float thr = ldexpf(1.0f, kLazy<NP> + ge);
+        {
+            // the block's largest |dO| and |delta|, from its first part
+            const float x = wave_max(ldexpf(gmax, -re)), y = wave_max(fabsf(delta));
+            if (lane == 0) {
+                wmax[0][wave] = x;
+                wmax[1][wave] = y;
+            }
+        }
+
+        floatx16 acc[2];
+#pragma unroll
+        for (int r = 0; r < 16; ++r) acc[0][r] = acc[1][r] = 0.0f;
+        float m = 0.0f, l = 0.0f;  // m: the reference less ge, so that exp2(s - m) carries 2^ge
+        bool fresh = true;         // no reference yet
+        wait_loads();
         __syncthreads();
-    }
-    l += __shfl_xor(l, 32);
-    const uint64_t row = static_cast<uint64_t>(bh) * a.qblocks * kB + q0 + wave * 32 + l32;
-    if (g == 0) {
-        // a row without keys, or past Tq: its P is 0 in the key kernel whatever its scores
-        a.lse[row] = in && l > 0.0f ? m + __builtin_log2f(l) : INFINITY;
-        a.delta[row] = in ? delta : 0.0f;
-    }
-    if (tid < 2) {
-        float x = wmax[tid][0];
+        auto tile = [&](uint32_t j, auto ST) {
+            constexpr int st = decltype(ST)::value;
 #pragma unroll
-        for (int w = 1; w < 4; ++w) x = fmaxf(x, wmax[tid][w]);
-        a.maxes[(static_cast<uint64_t>(bh) * a.qblocks + qb) * 2 + tid] = x;
+            for (int t = 0; t < 2; ++t) {
+                __builtin_amdgcn_sched_barrier(0);  // one half's values live at a time
+                floatx16 s, dp;
+#pragma unroll
+                for (int r = 0; r < 16; ++r) s[r] = dp[r] = 0.0f;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    half8 kf[NP], vf[NP];
+                    K.template row_frag<st>(places, t, i, kf);
+                    V.template row_frag<st>(places, t, i, vf);
+                    s = mma<NP>(kf, qf[i], s);
+                    dp = mma<NP>(vf, gf[i], dp);
+                }
+                if (j * kTile >= kfull) {  // wave-uniform
+                    const uint32_t k0 = j * kTile + 32 * t;
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) {
+                        const uint32_t key = k0 + 8 * (r >> 2) + 4 * g + (r & 3);
+                        if (key >= L || (a.causal && key > qi)) s[r] = -INFINITY;
+                    }
+                }
+                auto largest = [&] {
+                    float mx = s[0];
+#pragma unroll
+                    for (int r = 1; r < 16; ++r) mx = fmaxf(mx, s[r]);
+                    return fmaxf(mx, __shfl_xor(mx, 32)) * a.c;
+                };
+                // The first half of a piece sets the reference to its largest score (every query that sees a key of the
+                // piece sees one there; the others keep l = 0). Later the lane's sum bounds each weight, so no maximum is
+                // taken until it passes the threshold.
+                if (fresh) {
+                    const float mx = largest();
+                    m = (mx == -INFINITY ? 0.0f : mx) - static_cast<float>(ge);
+                    fresh = false;
+                }
+                float p[16], ts = 0.0f;
+#pragma unroll
+                for (int r = 0; r < 16; ++r) {
+                    p[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], a.c, -m));
+                    ts += p[r];
+                }
+                if (__any(ts > thr)) {
+                    const float mx = largest() - static_cast<float>(ge);
+                    const float mn = fmaxf(m, mx);
+                    const float alpha = __builtin_amdgcn_exp2f(m - mn);
+                    m = mn;
+                    l *= alpha;
+                    ts = 0.0f;
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) {
+                        acc[0][r] *= alpha;
+                        acc[1][r] *= alpha;
+                        p[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], a.c, -m));
+                        ts += p[r];
+                    }
+                }
+                l += ts;
+#pragma unroll
+                for (int r = 0; r < 16; ++r) p[r] *= dp[r] - dl;
+#pragma unroll
+                for (int sp = 0; sp < 2; ++sp) {
+                    half8 df[NP];
+                    operand<NP>(p, sp, df);
+#pragma unroll
+                    for (int u = 0; u < 2; ++u) {
+                        half8 kt[NP];
+                        K.template col_frag<st>(places, t, sp, u, kt);
+                        acc[u] = mma<NP>(kt, df, acc[u]);
+                    }
+                }
+            }
+        };
+        auto step = [&](uint32_t j, auto ST) {
+            constexpr int nx = decltype(ST)::value ^ 1;
+            // (the last tile loads one past the piece, which is not used)
+            K.template load<nx>((j + 1) * kTile);
+            V.template load<nx>((j + 1) * kTile);
+            tile(j, ST);
+            wait_loads();
+            __syncthreads();
+        };
+        for (; it < ntiles; it += 2) {
+            step(it, std::integral_constant<int, 0>{});
+            if (it + 1 < ntiles) step(it + 1, std::integral_constant<int, 1>{});
+        }
+        l += __shfl_xor(l, 32);
+        if (pc.t0 == 0) {
+            // (packed rows have theirs; those past Tq get zeros here)
+            if (g == 0 && (!PACKED || !in)) a.delta[row] = in ? delta : 0.0f;
+            if (PACKED && g == 0 && !in) a.rexp[row] = 0;
+            if (tid < 2) {
+                float x = wmax[tid][0];
+#pragma unroll
+                for (int w = 1; w < 4; ++w) x = fmaxf(x, wmax[tid][w]);
+                a.maxes[(static_cast<uint64_t>(bh) * a.qblocks + qb) * 2 + tid] = x;
+            }
+        }
+        __syncthreads();  // wmax and the stages are free for the next piece
+        if (!pc.whole) {
+            float* P = a.part + (2ull * wg + (pc.first ? 0 : 1)) * kQPart;
+            const int r = wave * 32 + l32;
+            store_row(P + r * 64, acc, 1.0f, 64, g);
+            if (g == 0) {
+                P[kB * 64 + r] = l > 0.0f ? m : -INFINITY;
+                P[kB * 64 + kB + r] = l;
+            }
+            continue;
+        }
+        // a row without keys, or past Tq: its P is 0 in the key kernel whatever its scores
+        if (g == 0) a.lse[row] = in && l > 0.0f ? m + __builtin_log2f(l) : INFINITY;
+        if (in) {
+            const float f = l > 0.0f ? ldexpf(a.scale / l, -re) : 0.0f;
+            store_row(head_of<T>(a.dq, b, h) + static_cast<uint64_t>(qi) * a.dq.ld, acc, f, ohd, g);
+        }
     }
-    if (!in) return;
-    const float f = l > 0.0f ? ldexpf(a.scale / l, -ge) : 0.0f;
-    T* out = const_cast<T*>(head_of<T>(a.dq, b, h, a.hd)) + static_cast<uint64_t>(qi) * a.dq.ld;
-    store_row(out, acc, f, hd, g, a.vout);
 }
 
-template <typename T, bool VEC>
+// dQ and m + log2 l of the shared query blocks: sum_i 2^(m_i - M) part_i, M = max m_i, four parts at a time, in order. Four
+// workgroups a block; thread t takes query t / 8 of its 32, columns 8 (t % 8).
+template <typename T>
+__global__ __launch_bounds__(256) void attn_bwd_q_merge_kernel(BwdArgs a) {
+    typedef T T4 __attribute__((ext_vector_type(4)));
+    const uint32_t id = blockIdx.x / 4, bh = id / a.qblocks, qb = id % a.qblocks;
+    const Parts<false> ps(a.qd, a.causal != 0, a.batch * a.heads, bh, qb);
+    if (ps.w0 == ps.w1) return;
+    const int r = static_cast<int>(blockIdx.x % 4) * 32 + static_cast<int>(threadIdx.x >> 3), d = (threadIdx.x & 7) * 8;
+    const uint32_t qi = qb * kB + r;
+    const uint64_t row = static_cast<uint64_t>(bh) * a.qblocks * kB + qi;
+    const bool in = qi < a.Tq;
+    const int re = a.rexp && in ? a.rexp[row] : 0;
+    float M = -INFINITY, l = 0.0f;
+    floatx4 s0 = {0.0f, 0.0f, 0.0f, 0.0f}, s1 = s0;
+    for (uint32_t w = ps.w0; w <= ps.w1; w += 4) {
+        float mi[4], li[4];
+        floatx4 x0[4], x1[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {  // every load first; past the last part it again, without weight
+            const float* P = a.part + ps.slot(a.qd, min(w + i, ps.w1)) * kQPart;
+            mi[i] = P[kB * 64 + r];
+            li[i] = P[kB * 64 + kB + r];
+            x0[i] = *reinterpret_cast<const floatx4*>(P + r * 64 + d);
+            x1[i] = *reinterpret_cast<const floatx4*>(P + r * 64 + d + 4);
+        }
+        float mx = M;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) mx = fmaxf(mx, mi[i]);
+        const float keep = M == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(M - mx);
+        M = mx;
+        l *= keep;
+        s0 *= keep;
+        s1 *= keep;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            if (w + i > ps.w1 || mi[i] == -INFINITY) continue;
+            const float f = __builtin_amdgcn_exp2f(mi[i] - M);
+            l += f * li[i];
+            s0 += f * x0[i];
+            s1 += f * x1[i];
+        }
+    }
+    if (d == 0) a.lse[row] = in && l > 0.0f ? M + __builtin_log2f(l) : INFINITY;
+    const int ohd = static_cast<int>(a.ohd);
+    const float f = l > 0.0f ? ldexpf(a.scale / l, -re) : 0.0f;
+    T* out = head_of<T>(a.dq, bh / a.heads, bh % a.heads) + static_cast<uint64_t>(qi) * a.dq.ld + d;
+    s0 *= f;
+    s1 *= f;
+    if (in && d < ohd) *reinterpret_cast<T4*>(out) = T4{static_cast<T>(s0[0]), static_cast<T>(s0[1]), static_cast<T>(s0[2]), static_cast<T>(s0[3])};
+    if (in && d + 4 < ohd)
+        *reinterpret_cast<T4*>(out + 4) = T4{static_cast<T>(s1[0]), static_cast<T>(s1[1]), static_cast<T>(s1[2]), static_cast<T>(s1[3])};
+}
+
+// ---- keys -----------------------------------------------------------------------------------------------------------
+
+template <typename T, bool PACKED, bool CAUSAL>
 __global__ __launch_bounds__(256, 2) void attn_bwd_k_kernel(BwdArgs a) {
-    typedef Stage<T, VEC> St;
-    constexpr int NP = St::NP;
-    __shared__ __attribute__((aligned(16))) _Float16 smem[2 * St::kHalves];
-    __shared__ __attribute__((aligned(16))) float rowv[2][2][kTile];  // [stage][m + log2 l - kPExp, delta][query]
+    constexpr int NP = sizeof(T) == 4 ? 2 : 1;
+    constexpr int NS = 2;
+    typedef Stage<NP, NS> St;
+    __shared__ __attribute__((aligned(16))) _Float16 qs0[St::kHalves], qs1[St::kHalves], gs0[St::kHalves], gs1[St::kHalves];
+    // per stage and query: m + log2 l less P's power of two, and -delta in the unit of dP
+    __shared__ __attribute__((aligned(16))) float row0[2 * kTile], row1[2 * kTile];
+    __shared__ float wmax[4];
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int l32 = lane & 31, g = lane >> 5;
-    const uint32_t blk = xcd_swizzle(blockIdx.x, gridDim.x);
-    // parts of one key block are neighbours: they share its XCD with the head's other key blocks
-    const uint32_t part = blk % a.splits, kb = blk / a.splits % a.kblocks, bh = blk / a.splits / a.kblocks;
-    const uint32_t h = bh % a.heads, b = bh / a.heads;
-    const uint32_t k0 = kb * kB, kj = k0 + wave * 32 + l32;
-    const int hd = static_cast<int>(a.hd);
-    const uint32_t L = keys_of(a, b);
+    const int hd = static_cast<int>(a.hd), ohd = static_cast<int>(a.ohd);
+    St Q, G;
+    Q.lds[0] = qs0;
+    Q.lds[1] = qs1;
+    G.lds[0] = gs0;
+    G.lds[1] = gs1;
 
-    // max|dO| and max|delta| of the (batch, head)
-    float gm = 0.0f, dm = 0.0f;
-    for (uint32_t i = lane; i < a.qblocks; i += 64) {
-        const float* x = a.maxes + (static_cast<uint64_t>(bh) * a.qblocks + i) * 2;
-        gm = fmaxf(gm, x[0]);
-        dm = fmaxf(dm, x[1]);
-    }
-    gm = wave_max(gm);
-    dm = wave_max(dm);
-    const int ge = NP == 2 ? max(-100, min(100, kPairExp - exponent(gm))) : 0;  // fp32: dO times 2^ge
+    const Places places(lane);
+    const uint32_t wg = xcd_swizzle(blockIdx.x, gridDim.x);
+    Pieces<true> pc(a.kd, CAUSAL, a.batch * a.heads, wg);
+    while (pc.next()) {
+        const uint32_t bh = pc.bh, h = bh % a.heads, b = bh / a.heads;
+        const uint32_t k0 = pc.blk * kB, kj = k0 + wave * 32 + l32;
+        // query tiles of this piece; causal: counted from the first one with a query at or past the block's first key
+        const uint32_t tiles = (a.Tq + kTile - 1) / kTile;
+        const uint32_t first = CAUSAL ? min(k0 / kTile, tiles) : 0u;
+        uint32_t it = first + pc.t0;
+        const uint32_t tend = min(first + pc.t1, tiles);
+        Q.set(head_of(a.xq, b, h), a.xq, a.Tq, PACKED ? 64 : hd, wave, lane);
+        G.set(head_of(a.xg, b, h), a.xg, a.Tq, PACKED ? 64 : hd, wave, lane);
+        Q.template load<0>(it * kTile);
+        G.template load<0>(it * kTile);
 
-    // this lane's key: fragments of K (with the scale's sign) and V
-    const bool in = kj < L;
-    const T* kp = head_of<T>(a.k, b, h, a.hd) + static_cast<uint64_t>(in ? kj : 0u) * a.k.ld;
-    const T* vp = head_of<T>(a.v, b, h, a.hd) + static_cast<uint64_t>(in ? kj : 0u) * a.v.ld;
-    half8 kf[4][NP], vf[4][NP];
-    float vm = 0.0f;
+        // this lane's key: fragments of K (with the scale's sign) and V; zeros past the row's length
+        half8 kf[4][NP], vf[4][NP];
 #pragma unroll
-    for (int s = 0; s < 4; ++s) {
-        const int d = 16 * s + 8 * g, n = in ? hd - d : 0;
-        half8 lo = zero8();
-        load8<T, VEC>(kp + (d < hd ? d : 0), n, a.sgn, kf[s][0], lo);
-        if constexpr (NP == 2) kf[s][NP - 1] = lo;
-        load8<T, VEC>(vp + (d < hd ? d : 0), n, 1.0f, vf[s][0], lo);
-        if constexpr (NP == 2) vf[s][NP - 1] = lo;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) vm = fmaxf(vm, fabsf(static_cast<float>(vf[s][0][e])));
-    }
-    vm = wave_max(vm);
-    // dS times 2^(kPExp + se) stays under 2^15; dP already carries 2^ge
-    const int se = max(-100, min(100, 15 - kPExp - 1 - exponent(64.0f * gm * vm + dm)));
-    const float psc = ldexpf(1.0f, se - ge), dsc = ldexpf(1.0f, se);
-
-    // query tiles of this part; causal: from the first one with a query at or past the block's first key
-    const uint32_t tiles = (a.Tq + kTile - 1) / kTile;
-    const uint32_t first = a.causal ? min(k0 / kTile, tiles) : 0u;
-    const uint32_t t0 = first + static_cast<uint32_t>(static_cast<uint64_t>(tiles - first) * part / a.splits);
-    const uint32_t t1 = k0 < L ? first + static_cast<uint32_t>(static_cast<uint64_t>(tiles - first) * (part + 1) / a.splits) : t0;
-
-    St Q(smem, head_of<T>(a.q, b, h, a.hd), a.q.ld, a.Tq, a.hd, tid);
-    St G(smem + St::kHalves, head_of<T>(a.g, b, h, a.hd), a.g.ld, a.Tq, a.hd, tid, ldexpf(1.0f, ge));
-    const float* lse = a.lse + static_cast<uint64_t>(bh) * a.qblocks * kB;
-    const float* del = a.delta + static_cast<uint64_t>(bh) * a.qblocks * kB;
-    float rv = 0.0f;  // threads 0..127: the next tile's row values
-    auto load_rows = [&](uint32_t q0) {
-        if (tid < kTile) rv = lse[q0 + tid] - static_cast<float>(kPExp);
-        else if (tid < 2 * kTile) rv = del[q0 + tid - kTile];
-    };
-    auto store_rows = [&](int st) {
-        if (tid < 2 * kTile) rowv[st][tid >> 6][tid & 63] = rv;
-    };
-
-    floatx16 dk[2], dv[2];
-#pragma unroll
-    for (int r = 0; r < 16; ++r) dk[0][r] = dk[1][r] = dv[0][r] = dv[1][r] = 0.0f;
-    if (t0 < t1) {
-        Q.load(t0 * kTile, 0);
-        G.load(t0 * kTile, 0);
-        load_rows(t0 * kTile);
-        Q.store(0);
-        G.store(0);
-        store_rows(0);
-        Q.settle();
-    }
-    __syncthreads();
-    for (uint32_t it = t0; it < t1; ++it) {
-        const int st = (it - t0) & 1;
-        const bool more = it + 1 < t1;
-        if (more) {
-            Q.load((it + 1) * kTile, st ^ 1);
-            G.load((it + 1) * kTile, st ^ 1);
-            load_rows((it + 1) * kTile);
+        for (int s = 0; s < 4; ++s) {
+            row_operand<NP>(head_of(a.xk, b, h), a.xk, kj, s, g, kj < a.Tk, PACKED ? 64 : hd, kf[s]);
+            row_operand<NP>(head_of(a.xv, b, h), a.xv, kj, s, g, kj < a.Tk, PACKED ? 64 : hd, vf[s]);
         }
-        // causal: tiles that start at or past the wave's last key need no mask
-        const bool mask = a.causal && it * kTile < k0 + wave * 32 + 31;
+        // threads 0..63 bring m + log2 l, 64..127 delta (the others repeat them); the arrays hold 128 ceil(Tq / 128) rows, and
+        // a tile past them is loaded from the last one and not used
+        const bool second = (tid & kTile) != 0;
+        const uint64_t rbase = static_cast<uint64_t>(bh) * a.qblocks * kB + (tid & (kTile - 1));
+        const float* rows = (second ? a.delta : a.lse) + rbase;
+        float rv;
+        int rx = 0;
+        auto load_rows = [&](uint32_t j) {
+            const uint32_t o = min(j, 2 * a.qblocks - 1) * kTile;
+            rv = rows[o];
+            if constexpr (NP == 2) rx = a.rexp[rbase + o];
+        };
+        load_rows(it);
+        // max|dO| and max|delta| of the (batch, head)
+        float gm = 0.0f, dm = 0.0f;
+        for (uint32_t i = lane; i < a.qblocks; i += 64) {
+            const float* x = a.maxes + (static_cast<uint64_t>(bh) * a.qblocks + i) * 2;
+            gm = fmaxf(gm, x[0]);
+            dm = fmaxf(dm, x[1]);
+        }
+        const uint32_t L = keys_of(a, b);
+        const bool in = kj < L;
+        const uint32_t t1 = k0 < L ? tend : it;
+        gm = wave_max(gm);
+        dm = wave_max(dm);
+        float vm = 0.0f;
 #pragma unroll
-        for (int t = 0; t < 2; ++t) {
-            floatx16 s, dp;
+        for (int s = 0; s < 4; ++s) {
+#pragma unroll
+            for (int p = 0; p < NP; ++p) {
+                if (!in) kf[s][p] = vf[s][p] = zero8();
+                if (a.sgn < 0.0f) kf[s][p] = -kf[s][p];
+            }
+#pragma unroll
+            for (int e = 0; e < 8; ++e) vm = fmaxf(vm, fabsf(static_cast<float>(vf[s][0][e])));
+        }
+        vm = wave_max(vm);
+        if (lane == 0) wmax[wave] = vm;
+        __syncthreads();
+        vm = fmaxf(fmaxf(wmax[0], wmax[1]), fmaxf(wmax[2], wmax[3]));
+        // dS times 2^(pe + se) stays under 2^15. fp16: V carries 2^se, its largest element within 2^-6 .. 2^12, and P what
+        // is left. fp32: row i of dO carries 2^(e_i), P 2^(E - e_i) with E of the largest row, and the fma below the rest.
+        const int s0 = 15 - kPExp - 1 - exponent(64.0f * gm * vm + dm);
+        const int se = NP == 1 ? clamp(s0, -6 - exponent(vm), 12 - exponent(vm)) : clamp(s0, -100, 100);
+        const int pe = NP == 1 ? kPExp - max(0, se - s0) : kPExp;
+        const int E = NP == 2 ? clamp(kPairExp - exponent(gm), -100, 100) : 0;
+        const float psc = ldexpf(1.0f, se - E);
+        if constexpr (NP == 1) {
+            const float up = ldexpf(1.0f, clamp(se, -30, 30));
+#pragma unroll
+            for (int s = 0; s < 4; ++s)
+#pragma unroll
+                for (int e = 0; e < 8; ++e) vf[s][0][e] = static_cast<_Float16>(static_cast<float>(vf[s][0][e]) * up);
+        }
+
+        auto store_rows = [&](float* r) {
+            const float v = second ? -ldexpf(rv, NP == 2 ? rx - E + se : se) : rv - static_cast<float>(pe) + static_cast<float>(NP == 2 ? rx - E : 0);
+            if (tid < 2 * kTile) r[tid] = v;
+        };
+
+        floatx16 dk[2], dv[2];
+#pragma unroll
+        for (int r = 0; r < 16; ++r) dk[0][r] = dk[1][r] = dv[0][r] = dv[1][r] = 0.0f;
+        store_rows(row0);
+        wait_loads();
+        __syncthreads();
+        floatx16 s, dp;
+        half8 pf[2][NP], df[2][NP];
+        auto scores = [&](int t, auto ST) {
+            constexpr int st = decltype(ST)::value;
+            const float* rw = st ? row1 : row0;
 #pragma unroll
             for (int r = 0; r < 16; ++r) s[r] = dp[r] = 0.0f;
+            // fp16: dP's sum starts from -delta
+            if constexpr (NP == 1) {
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    const floatx4 dq = *reinterpret_cast<const floatx4*>(&rw[kTile + 32 * t + 8 * q + 4 * g]);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) dp[4 * q + e] = dq[e];
+                }
+            }
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 half8 qf[NP], gf[NP];
-#pragma unroll
-                for (int p = 0; p < NP; ++p) {
-                    qf[p] = Q.row_frag(st, p, t, i, l32, g);
-                    gf[p] = G.row_frag(st, p, t, i, l32, g);
-                }
-                s = mma(qf, kf[i], s);
-                dp = mma(gf, vf[i], dp);
+                Q.template row_frag<st>(places, t, i, qf);
+                G.template row_frag<st>(places, t, i, gf);
+                s = mma<NP>(qf, kf[i], s);
+                dp = mma<NP>(gf, vf[i], dp);
             }
+        };
+        auto weights = [&](uint32_t j, int t, auto ST) {
+            constexpr int st = decltype(ST)::value;
+            const float* rw = st ? row1 : row0;
             float p[16], ds[16];
 #pragma unroll
             for (int q = 0; q < 4; ++q) {
-                const floatx4 lq = *reinterpret_cast<const floatx4*>(&rowv[st][0][32 * t + 8 * q + 4 * g]);
-                const floatx4 dq = *reinterpret_cast<const floatx4*>(&rowv[st][1][32 * t + 8 * q + 4 * g]);
+                const floatx4 lq = *reinterpret_cast<const floatx4*>(&rw[32 * t + 8 * q + 4 * g]);
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const int r = 4 * q + e;
-                    p[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], a.c, -lq[e]));
-                    if (mask && it * kTile + 32 * t + 8 * q + 4 * g + e < kj) p[r] = 0.0f;
-                    ds[r] = p[r] * __builtin_fmaf(dp[r], psc, -dq[e] * dsc);
+                for (int e = 0; e < 4; ++e) p[4 * q + e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[4 * q + e], a.c, -lq[e]));
+                if constexpr (NP == 2) {
+                    const floatx4 dq = *reinterpret_cast<const floatx4*>(&rw[kTile + 32 * t + 8 * q + 4 * g]);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) dp[4 * q + e] = __builtin_fmaf(dp[4 * q + e], psc, dq[e]);
+                }
+            }
+            // causal: tiles that start at or past the wave's last key need no mask (wave-uniform)
+            if constexpr (CAUSAL) {
+                if (j * kTile < k0 + wave * 32 + 31) {
+#pragma unroll
+                    for (int r = 0; r < 16; ++r)
+                        if (j * kTile + 32 * t + 8 * (r >> 2) + 4 * g + (r & 3) < kj) p[r] = 0.0f;
                 }
             }
 #pragma unroll
+            for (int r = 0; r < 16; ++r) ds[r] = p[r] * dp[r];
+#pragma unroll
             for (int sp = 0; sp < 2; ++sp) {
-                half8 pf[NP], df[NP];
-                operand<NP>(p, sp, pf);
-                operand<NP>(ds, sp, df);
+                operand<NP>(p, sp, pf[sp]);
+                operand<NP>(ds, sp, df[sp]);
+            }
+        };
+        auto products = [&](int t, auto ST) {
+            constexpr int st = decltype(ST)::value;
+#pragma unroll
+            for (int sp = 0; sp < 2; ++sp)
 #pragma unroll
                 for (int u = 0; u < 2; ++u) {
                     half8 gt[NP], qt[NP];
-#pragma unroll
-                    for (int pl = 0; pl < NP; ++pl) {
-                        gt[pl] = G.col_frag(st, pl, t, sp, u, lane);
-                        qt[pl] = Q.col_frag(st, pl, t, sp, u, lane);
-                    }
-                    dv[u] = mma(gt, pf, dv[u]);
-                    dk[u] = mma(qt, df, dk[u]);
+                    G.template col_frag<st>(places, t, sp, u, gt);
+                    Q.template col_frag<st>(places, t, sp, u, qt);
+                    dv[u] = mma<NP>(gt, pf[sp], dv[u]);
+                    dk[u] = mma<NP>(qt, df[sp], dk[u]);
                 }
+        };
+        auto tile = [&](uint32_t j, auto ST) {
+            // one half's values live at a time (the scores of one half between the exponentials of the other: 225 us
+            // against 212 at 2 x 10 x 4096^2)
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+                __builtin_amdgcn_sched_barrier(0);
+                scores(t, ST);
+                weights(j, t, ST);
+                products(t, ST);
             }
+        };
+        auto step = [&](uint32_t j, auto ST) {
+            constexpr int nx = decltype(ST)::value ^ 1;
+            // (the last tile loads the one after it, which is not used)
+            Q.template load<nx>((j + 1) * kTile);
+            G.template load<nx>((j + 1) * kTile);
+            load_rows(j + 1);
+            tile(j, ST);
+            store_rows(nx ? row1 : row0);
+            wait_loads();
+            __syncthreads();
+        };
+        for (; it < t1; it += 2) {
+            step(it, std::integral_constant<int, 0>{});
+            if (it + 1 < t1) step(it + 1, std::integral_constant<int, 1>{});
         }
-        if (more) {
-            Q.store(st ^ 1);
-            G.store(st ^ 1);
-            store_rows(st ^ 1);
-            Q.settle();
-        }
-        __syncthreads();
-    }
-    if (kj >= a.Tk) return;
-    // keys past their row's length get zeros
-    const float fv = in ? ldexpf(1.0f, -kPExp - ge) : 0.0f;
-    const float fk = in ? ldexpf(a.scale, -kPExp - se) : 0.0f;
-    if (!in)
+        // keys past their row's length get zeros (their P is not: their scores are those of a zero key)
+        const float fv = ldexpf(1.0f, -pe - E), fk = ldexpf(a.scale, -pe - se);
+        if (!in)
 #pragma unroll
-        for (int r = 0; r < 16; ++r) dk[0][r] = dk[1][r] = dv[0][r] = dv[1][r] = 0.0f;
-    if (a.splits > 1) {
-        // [part][dk, dv][batch, head][Tk][64]
-        const uint64_t plane = static_cast<uint64_t>(a.batch) * a.heads * a.Tk * 64;
-        float* P = a.part + part * 2 * plane + (static_cast<uint64_t>(bh) * a.Tk + kj) * 64;
-        store_row(P, dk, fk, 64, g, true);
-        store_row(P + plane, dv, fv, 64, g, true);
-        return;
+            for (int r = 0; r < 16; ++r) dk[0][r] = dk[1][r] = dv[0][r] = dv[1][r] = 0.0f;
+        if (!pc.whole) {
+            float* P = a.part + (2ull * wg + (pc.first ? 0 : 1)) * kKPart + (wave * 32 + l32) * 64;
+            store_row(P, dk, fk, 64, g);
+            store_row(P + kB * 64, dv, fv, 64, g);
+        } else if (kj < a.Tk) {
+            store_row(head_of<T>(a.dk, b, h) + static_cast<uint64_t>(kj) * a.dk.ld, dk, fk, ohd, g);
+            store_row(head_of<T>(a.dv, b, h) + static_cast<uint64_t>(kj) * a.dv.ld, dv, fv, ohd, g);
+        }
     }
-    store_row(const_cast<T*>(head_of<T>(a.dk, b, h, a.hd)) + static_cast<uint64_t>(kj) * a.dk.ld, dk, fk, hd, g, a.vout);
-    store_row(const_cast<T*>(head_of<T>(a.dv, b, h, a.hd)) + static_cast<uint64_t>(kj) * a.dv.ld, dv, fv, hd, g, a.vout);
 }
 
-// The query parts' dK (blockIdx.y = 0) and dV (1), added in order: 16 threads a row of 64 columns.
+// dK (blockIdx.y = 0) and dV (1) of the shared key blocks: the parts added in order, four loaded at a time. Eight
+// workgroups a block; thread t takes key t / 16 of its 16, columns 4 (t % 16).
 template <typename T>
-__global__ __launch_bounds__(256) void attn_bwd_sum_kernel(BwdArgs a) {
+__global__ __launch_bounds__(256) void attn_bwd_k_merge_kernel(BwdArgs a) {
     typedef T T4 __attribute__((ext_vector_type(4)));
-    const uint64_t rows = static_cast<uint64_t>(a.batch) * a.heads * a.Tk, plane = rows * 64;
-    const uint64_t row = blockIdx.x * 16ull + (threadIdx.x >> 4);
-    const int d = (threadIdx.x & 15) * 4, hd = static_cast<int>(a.hd);
-    if (row >= rows || d >= hd) return;
-    const float* p = a.part + blockIdx.y * plane + row * 64 + d;
-    floatx4 v = *reinterpret_cast<const floatx4*>(p);
-    for (uint32_t s = 1; s < a.splits; ++s) v += *reinterpret_cast<const floatx4*>(p + s * 2 * plane);
-    const uint32_t bh = static_cast<uint32_t>(row / a.Tk), kj = static_cast<uint32_t>(row % a.Tk);
-    const Tensor& t = blockIdx.y ? a.dv : a.dk;
-    T* out = const_cast<T*>(head_of<T>(t, bh / a.heads, bh % a.heads, a.hd)) + static_cast<uint64_t>(kj) * t.ld + d;
-    if (a.vout) {
-        *reinterpret_cast<T4*>(out) = T4{static_cast<T>(v[0]), static_cast<T>(v[1]), static_cast<T>(v[2]), static_cast<T>(v[3])};
-    } else {
+    const uint32_t id = blockIdx.x / 8, bh = id / a.kd.nb, kb = id % a.kd.nb;
+    const Parts<true> ps(a.kd, a.causal != 0, a.batch * a.heads, bh, kb);
+    const int r = static_cast<int>(blockIdx.x % 8) * 16 + static_cast<int>(threadIdx.x >> 4), d = (threadIdx.x & 15) * 4;
+    const uint32_t kj = kb * kB + r;
+    if (ps.w0 == ps.w1 || kj >= a.Tk || d >= static_cast<int>(a.ohd)) return;
+    const float* P = a.part + blockIdx.y * kB * 64 + r * 64 + d;
+    floatx4 v = {0.0f, 0.0f, 0.0f, 0.0f};
+    for (uint32_t w = ps.w0; w <= ps.w1; w += 4) {
+        floatx4 x[4];
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
-            if (d + e < hd) out[e] = static_cast<T>(v[e]);
+        for (int i = 0; i < 4; ++i) x[i] = *reinterpret_cast<const floatx4*>(P + ps.slot(a.kd, min(w + i, ps.w1)) * kKPart);
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (w + i <= ps.w1) v += x[i];
+    }
+    const uint64_t ld = blockIdx.y ? a.dv.ld : a.dk.ld;
+    T* out = (blockIdx.y ? head_of<T>(a.dv, bh / a.heads, bh % a.heads) : head_of<T>(a.dk, bh / a.heads, bh % a.heads)) + kj * ld + d;
+    *reinterpret_cast<T4*>(out) = T4{static_cast<T>(v[0]), static_cast<T>(v[1]), static_cast<T>(v[2]), static_cast<T>(v[3])};
+}
+
+// dq, dk and dv (blockIdx.y) from planes in the workspace into tensors that take no 4-element stores.
+template <typename T>
+__global__ __launch_bounds__(256) void attn_bwd_unpack_kernel(BwdArgs a) {
+    const uint32_t which = blockIdx.y, len = which ? a.Tk : a.Tq;
+    const uint64_t rows = static_cast<uint64_t>(a.batch) * len * a.heads, n = rows * a.hd;
+    const T* from = static_cast<const T*>(which == 0 ? a.dq.p : which == 1 ? a.dk.p : a.dv.p);
+    T* to = static_cast<T*>(const_cast<void*>(which == 0 ? a.user[0].p : which == 1 ? a.user[1].p : a.user[2].p));
+    const uint64_t ld = which == 0 ? a.user[0].ld : which == 1 ? a.user[1].ld : a.user[2].ld;
+    const uint64_t sb = which == 0 ? a.user[0].s : which == 1 ? a.user[1].s : a.user[2].s;
+    for (uint64_t i = blockIdx.x * 256ull + threadIdx.x; i < n; i += static_cast<uint64_t>(gridDim.x) * 256) {
+        const uint64_t d = i % a.hd, at = i / a.hd, h = at % a.heads, tok = at / a.heads, b = tok / len, t = tok % len;
+        to[b * sb + t * ld + h * a.hd + d] = from[((b * a.heads + h) * len + t) * 64 + d];
     }
 }
 
-// Parts of the queries for the key kernel: as many as bring its grid to the GPU's CUs, each of two tiles at least.
-uint32_t query_parts(uint64_t blocks, uint32_t Tq) {
-    const uint64_t tiles = ceil_div(Tq, kTile);
-    return static_cast<uint32_t>(std::max<uint64_t>(1, std::min<uint64_t>(256 / std::max<uint64_t>(blocks, 1), tiles / 2)));
-}
-
-struct Layout {
-    uint64_t rows, maxes, part, total;  // bytes of one row array, offsets of the others
-};
-Layout layout(uint32_t batch, uint32_t heads, uint32_t Tq, uint32_t Tk, uint32_t splits) {
-    Layout l;
-    const uint64_t bh = static_cast<uint64_t>(batch) * heads, qb = ceil_div(Tq, kB);
-    l.rows = bh * qb * kB * 4;
-    l.maxes = 2 * l.rows;
-    l.part = (l.maxes + bh * qb * 8 + 255) / 256 * 256;
-    l.total = l.part + (splits > 1 ? static_cast<uint64_t>(splits) * 2 * bh * Tk * 64 * 4 : 0);
-    return l;
-}
-
-template <typename T, bool VEC>
-void launch(const BwdArgs& a, hipStream_t s) {
-    const unsigned bh = a.batch * a.heads;
-    attn_bwd_q_kernel<T, VEC><<<a.qblocks * bh, 256, 0, s>>>(a);
-    if (a.Tk == 0) return;
-    attn_bwd_k_kernel<T, VEC><<<a.kblocks * bh * a.splits, 256, 0, s>>>(a);
-    if (a.splits > 1) attn_bwd_sum_kernel<T><<<dim3(ceil_div(static_cast<uint64_t>(bh) * a.Tk, 16), 2), 256, 0, s>>>(a);
-}
-
-// Zeros, for a call without queries.
+// Zeros in dk and dv, for a call without queries.
 template <typename T>
 __global__ __launch_bounds__(256) void attn_bwd_zero_kernel(BwdArgs a) {
     const uint64_t C = static_cast<uint64_t>(a.heads) * a.hd, n = static_cast<uint64_t>(a.batch) * a.Tk * C;
     const Tensor& t = blockIdx.y ? a.dv : a.dk;
     for (uint64_t i = blockIdx.x * 256ull + threadIdx.x; i < n; i += static_cast<uint64_t>(gridDim.x) * 256) {
         const uint64_t r = i / C;
-        static_cast<T*>(const_cast<void*>(t.p))[r / a.Tk * t.s + r % a.Tk * t.ld + i % C] = static_cast<T>(0.0f);
+        head_of<T>(t, 0, 0)[r / a.Tk * t.s + r % a.Tk * t.ld + i % C] = static_cast<T>(0.0f);
     }
+}
+
+// ---- plan -----------------------------------------------------------------------------------------------------------
+
+constexpr uint32_t kSlots = 512;     // workgroups resident at once: two per CU
+constexpr uint32_t kMinShare = 4;    // tiles of a share, at least, where blocks are shared
+
+// Whole blocks, a workgroup each, where they fill rounds of kSlots well enough; else kSlots workgroups, or as many as get
+// kMinShare tiles.
+template <bool KEYS>
+Deal deal(uint32_t bhs, uint32_t T, uint32_t Tother, bool causal) {
+    Deal d;
+    d.NT = std::max(1u, ceil_div(Tother, kTile));
+    d.nb = ceil_div(T, kB);
+    d.per = before<KEYS>(d.nb, d.NT, causal);
+    const uint32_t blocks = bhs * d.nb;
+    const uint64_t total = static_cast<uint64_t>(bhs) * d.per;
+    d.wgs = blocks;
+    const bool alike = !causal || d.nb <= 1;  // all blocks have NT tiles
+    d.whole = alike ? 1 : 0;
+    const uint64_t rounds = (blocks + kSlots - 1) / kSlots;
+    const uint32_t shares = static_cast<uint32_t>(std::max<uint64_t>(1, std::min<uint64_t>(kSlots, total / kMinShare)));
+    if (blocks && blocks < rounds * kSlots * 9 / 10 && (blocks > kSlots || shares > blocks)) {
+        d.wgs = shares;
+        d.whole = alike ? blocks / shares : 0;
+    }
+    return d;
+}
+// No block is shared.
+bool all_whole(const Deal& d, uint32_t bhs) { return d.whole && dealt_whole(d) == bhs * d.nb; }
+
+struct Layout {
+    uint64_t delta, rexp, maxes, part, planes, outs, total;  // byte offsets
+    uint64_t qplane, kplane;                           // elements of a plane
+};
+Layout layout(uint32_t batch, uint32_t heads, uint32_t Tq, uint32_t Tk, bool packed, bool f32, bool vout) {
+    Layout l;
+    const uint64_t bh = static_cast<uint64_t>(batch) * heads, qb = ceil_div(Tq, kB), rows = bh * qb * kB * 4;
+    l.delta = rows;
+    l.rexp = 2 * rows;
+    l.maxes = l.rexp + (packed ? rows : 0);
+    l.part = (l.maxes + bh * qb * 8 + 255) / 256 * 256;
+    // (the same bytes for causal calls and others)
+    uint64_t parts = 0;
+    for (const bool causal : {false, true}) {
+        const uint32_t n = static_cast<uint32_t>(bh);
+        const Deal qd = deal<false>(n, Tq, Tk, causal), kd = deal<true>(n, Tk, Tq, causal);
+        parts = std::max(parts, std::max<uint64_t>(all_whole(qd, n) ? 0 : 8ull * qd.wgs * kQPart, all_whole(kd, n) ? 0 : 8ull * kd.wgs * kKPart));
+    }
+    l.planes = l.part + (parts + 255) / 256 * 256;
+    l.qplane = bh * Tq * 64;
+    l.kplane = bh * Tk * 64;
+    l.outs = l.planes + (packed ? (l.qplane + l.kplane) * 2 * 2 * (f32 ? 2 : 1) : 0);
+    l.total = l.outs + (vout ? 0 : (l.qplane + 2 * l.kplane) * (f32 ? 4 : 2));
+    return l;
+}
+
+template <typename T>
+void unpack(const BwdArgs& a, hipStream_t s) {
+    const uint64_t n = static_cast<uint64_t>(a.batch) * a.heads * std::max(a.Tq, a.Tk) * a.hd;
+    attn_bwd_unpack_kernel<T><<<dim3(static_cast<unsigned>(std::min<uint64_t>(ceil_div(n, 256), 4096)), 3), 256, 0, s>>>(a);
+}
+
+template <typename T, bool PACKED>
+void launch(const BwdArgs& a, hipStream_t s) {
+    const uint32_t bh = a.batch * a.heads;
+    if constexpr (PACKED) {
+        const uint64_t rows = static_cast<uint64_t>(bh) * std::max(a.Tq, a.Tk);
+        attn_bwd_pack_kernel<T><<<dim3(ceil_div(rows, 32), 4), 256, 0, s>>>(a);
+    }
+    attn_bwd_q_kernel<T, PACKED><<<a.qd.wgs, 256, 0, s>>>(a);
+    if (!all_whole(a.qd, bh)) attn_bwd_q_merge_kernel<T><<<bh * a.qblocks * 4, 256, 0, s>>>(a);
+    if (a.Tk == 0) {
+        if (a.user[0].ld) unpack<T>(a, s);
+        return;
+    }
+    if (a.causal) attn_bwd_k_kernel<T, PACKED, true><<<a.kd.wgs, 256, 0, s>>>(a);
+    else attn_bwd_k_kernel<T, PACKED, false><<<a.kd.wgs, 256, 0, s>>>(a);
+    if (!all_whole(a.kd, bh)) attn_bwd_k_merge_kernel<T><<<dim3(bh * a.kd.nb * 8, 2), 256, 0, s>>>(a);
+    if (a.user[0].ld) unpack<T>(a, s);
 }
 
 struct Span {
@@ -656,6 +1054,43 @@ bool interleaved(const Tensor& x, const Tensor& y, uint64_t C, uint64_t e) {
     const uintptr_t p = reinterpret_cast<uintptr_t>(x.p), q = reinterpret_cast<uintptr_t>(y.p);
     const uint64_t apart = (p > q ? p - q : q - p);
     return x.ld == y.ld && x.s == y.s && apart >= C * e && apart + C * e <= x.ld * e;
+}
+
+// Both kernels' shares; the launches' limits.
+int plan(const mi_attn_args& f, Deal& qd, Deal& kd, const char* fn) {
+    const uint64_t bh = static_cast<uint64_t>(f.batch) * f.heads;
+    const uint64_t qb = ceil_div(f.Tq, kB), kb = ceil_div(f.Tk, kB), qt = ceil_div(f.Tq, kTile) + 1, kt = ceil_div(f.Tk, kTile) + 1;
+    if (bh * std::max(qb, kb) >= (1u << 20) || qb * kt >= (1u << 31) || kb * qt >= (1u << 31))
+        return fail(MI_ERR_UNSUPPORTED, "%s: batch * heads * tokens too large", fn);
+    qd = deal<false>(static_cast<uint32_t>(bh), f.Tq, f.Tk, f.causal != 0);
+    kd = deal<true>(static_cast<uint32_t>(bh), f.Tk, f.Tq, f.causal != 0);
+    return MI_OK;
+}
+
+// Every row of the inputs in whole 16-byte chunks.
+bool wide(const mi_attn_bwd_args& x) {
+    const mi_attn_args& f = x.fwd;
+    const uint64_t e = f.in_dtype == MI_F16 ? 2 : 4;
+    const struct {
+        const void* p;
+        uint64_t ld, s;
+    } in[5] = {{f.q, f.ldq, f.sq}, {f.k, f.ldk, f.sk}, {f.v, f.ldv, f.sv}, {f.out, f.ldo, f.so}, {x.dout, x.lddout, x.sdout}};
+    bool w = f.C / f.heads % 8 == 0;
+    for (const auto& t : in) w = w && aligned(t.p, 16) && (t.ld ? t.ld : f.C) * e % 16 == 0 && (f.batch == 1 || t.s * e % 16 == 0);
+    return w;
+}
+
+// Gradients that take 4-element stores.
+bool wide_out(const mi_attn_bwd_args& x) {
+    const mi_attn_args& f = x.fwd;
+    const uint64_t e = f.in_dtype == MI_F16 ? 2 : 4;
+    const struct {
+        const void* p;
+        uint64_t ld, s;
+    } out[3] = {{x.dq, x.lddq, x.sdq}, {x.dk, x.lddk, x.sdk}, {x.dv, x.lddv, x.sdv}};
+    bool w = f.C / f.heads % 4 == 0;
+    for (const auto& t : out) w = w && aligned(t.p, 4 * e) && (t.ld ? t.ld : f.C) % 4 == 0 && (f.batch == 1 || t.s % 4 == 0);
+    return w;
 }
 
 int run(const mi_attn_bwd_args& x, void* ws, uint64_t ws_bytes, hipStream_t stream, const char* fn) {
@@ -685,7 +1120,7 @@ int run(const mi_attn_bwd_args& x, void* ws, uint64_t ws_bytes, hipStream_t stre
                {x.dout, x.lddout, x.sdout, f.Tq, &a.g, "dout"}, {x.dq, x.lddq, x.sdq, f.Tq, &a.dq, "dq"},
                {x.dk, x.lddk, x.sdk, f.Tk, &a.dk, "dk"},    {x.dv, x.lddv, x.sdv, f.Tk, &a.dv, "dv"}};
     Span span[8];
-    bool vec = f.C / f.heads % 8 == 0, vout = f.C / f.heads % 4 == 0;
+    const bool vec = wide(x), vout = wide_out(x);
     for (int i = 0; i < 8; ++i) {
         const uint64_t ld = in[i].ld ? in[i].ld : f.C, s = in[i].s ? in[i].s : in[i].T * ld;
         if (ld < f.C) return fail(MI_ERR_INVALID_ARG, "%s: token stride of %s < C", fn, in[i].name);
@@ -694,10 +1129,8 @@ int run(const mi_attn_bwd_args& x, void* ws, uint64_t ws_bytes, hipStream_t stre
         if (i >= 5 && f.batch > 1 && in[i].T && s < (in[i].T - 1) * ld + f.C)
             return fail(MI_ERR_INVALID_ARG, "%s: batch rows of %s overlap", fn, in[i].name);
         if (!aligned(in[i].p, e)) return fail(MI_ERR_ALIGNMENT, "%s: tensors must be aligned to their element size", fn);
-        *in[i].t = Tensor{in[i].p, ld, s};
+        *in[i].t = Tensor{in[i].p, ld, s, f.C / f.heads};
         span[i] = Span{in[i].p, in[i].T ? ((f.batch - 1) * s + (in[i].T - 1) * ld + f.C) * e : 0};
-        if (i < 5) vec = vec && aligned(in[i].p, 16) && ld * e % 16 == 0 && (f.batch == 1 || s * e % 16 == 0);
-        else vout = vout && aligned(in[i].p, 4 * e) && ld % 4 == 0 && (f.batch == 1 || s % 4 == 0);
     }
     for (int o = 5; o < 8; ++o)
         for (int i = 0; i < o; ++i)
@@ -714,8 +1147,7 @@ int run(const mi_attn_bwd_args& x, void* ws, uint64_t ws_bytes, hipStream_t stre
     a.scale = scale;
     a.sgn = scale < 0.0f ? -1.0f : 1.0f;
     a.c = fmaxf(fabsf(scale) * 1.4426950408889634f, 1e-30f);  // a masked score stays -inf
-    a.vout = vout ? 1u : 0u;
-    const uint64_t bh = static_cast<uint64_t>(f.batch) * f.heads;
+    a.ohd = a.hd;
     if (f.Tq == 0) {
         if (f.Tk == 0) return MI_OK;
         const uint64_t n = static_cast<uint64_t>(f.batch) * f.Tk * f.C;
@@ -725,11 +1157,11 @@ int run(const mi_attn_bwd_args& x, void* ws, uint64_t ws_bytes, hipStream_t stre
         return check_launch(fn);
     }
     a.qblocks = ceil_div(f.Tq, kB);
-    a.kblocks = ceil_div(f.Tk, kB);
-    a.splits = query_parts(bh * a.kblocks, f.Tq);
-    if (bh * a.qblocks >= (1u << 23) || bh * a.kblocks * a.splits >= (1u << 23))
-        return fail(MI_ERR_UNSUPPORTED, "%s: batch * heads * tokens too large", fn);
-    const Layout l = layout(f.batch, f.heads, f.Tq, f.Tk, a.splits);
+    const int st = plan(f, a.qd, a.kd, fn);
+    if (st) return st;
+    const bool packed = e == 4 || !vec;
+    const Layout l = layout(f.batch, f.heads, f.Tq, f.Tk, packed, e == 4, vout);
+    const uint64_t bhs = static_cast<uint64_t>(f.batch) * f.heads;
     if (!ws || ws_bytes < l.total)
         return fail(MI_ERR_INVALID_ARG, "%s: workspace %llu bytes < %llu needed", fn,
                     static_cast<unsigned long long>(ws ? ws_bytes : 0), static_cast<unsigned long long>(l.total));
@@ -738,13 +1170,44 @@ int run(const mi_attn_bwd_args& x, void* ws, uint64_t ws_bytes, hipStream_t stre
         if (overlaps(ws, l.total, span[i].p, span[i].bytes)) return fail(MI_ERR_ALIASING, "%s: workspace overlaps %s", fn, in[i].name);
     char* w = static_cast<char*>(ws);
     a.lse = reinterpret_cast<float*>(w);
-    a.delta = reinterpret_cast<float*>(w + l.rows);
+    a.delta = reinterpret_cast<float*>(w + l.delta);
+    a.rexp = packed ? reinterpret_cast<int*>(w + l.rexp) : nullptr;
     a.maxes = reinterpret_cast<float*>(w + l.maxes);
     a.part = reinterpret_cast<float*>(w + l.part);
-    if (e == 2 && vec) launch<_Float16, true>(a, stream);
-    else if (e == 2) launch<_Float16, false>(a, stream);
-    else if (vec) launch<float, true>(a, stream);
-    else launch<float, false>(a, stream);
+    a.vin = vec ? 1u : 0u;
+    if (!vout) {
+        char* p = w + l.outs;
+        Tensor* t[3] = {&a.dq, &a.dk, &a.dv};
+        for (int i = 0; i < 3; ++i) {
+            const uint64_t T = i ? f.Tk : f.Tq;
+            a.user[i] = *t[i];
+            *t[i] = Tensor{p, 64, f.heads * T * 64, T * 64};
+            p += bhs * T * 64 * e;
+        }
+        a.ohd = 64;
+    }
+    if (packed) {
+        _Float16* p = reinterpret_cast<_Float16*>(w + l.planes);
+        const uint64_t np = e == 4 ? 2 : 1;
+        auto take = [&](uint32_t T, uint64_t plane) {
+            const Operand x{p, 64, static_cast<uint64_t>(f.heads) * T * 64, static_cast<uint64_t>(T) * 64, plane};
+            p += np * plane;
+            return x;
+        };
+        a.xq = take(f.Tq, l.qplane);
+        a.xg = take(f.Tq, l.qplane);
+        a.xk = take(f.Tk, l.kplane);
+        a.xv = take(f.Tk, l.kplane);
+        if (e == 4) launch<float, true>(a, stream);
+        else launch<_Float16, true>(a, stream);
+    } else {
+        auto direct = [&](const Tensor& t) { return Operand{static_cast<const _Float16*>(t.p), t.ld, t.s, a.hd, 0}; };
+        a.xq = direct(a.q);
+        a.xg = direct(a.g);
+        a.xk = direct(a.k);
+        a.xv = direct(a.v);
+        launch<_Float16, false>(a, stream);
+    }
     return check_launch(fn);
 }
 
@@ -756,9 +1219,11 @@ using namespace mi;
 extern "C" uint64_t mi_fused_attention_bwd_ws_bytes(const mi_attn_bwd_args* args) {
     if (!args) return 0;
     const mi_attn_args& f = args->fwd;
-    if (!f.batch || !f.Tq || !mi_fused_attn_supported(f.C, f.heads)) return 0;
-    const uint64_t bh = static_cast<uint64_t>(f.batch) * f.heads;
-    return layout(f.batch, f.heads, f.Tq, f.Tk, query_parts(bh * ceil_div(f.Tk, kB), f.Tq)).total;
+    if (!f.batch || !f.Tq || !mi_fused_attn_supported(f.C, f.heads) || (f.in_dtype != MI_F32 && f.in_dtype != MI_F16)) return 0;
+    Deal qd, kd;
+    if (plan(f, qd, kd, "mi_fused_attention_bwd_ws_bytes") != MI_OK) return 0;
+    const bool f32 = f.in_dtype == MI_F32;
+    return layout(f.batch, f.heads, f.Tq, f.Tk, f32 || !wide(*args), f32, wide_out(*args)).total;
 }
 
 extern "C" int mi_fused_attention_bwd(const mi_attn_bwd_args* args, void* workspace, uint64_t workspace_bytes, void* stream) {

@@ -372,9 +372,11 @@ def sdxl_block_forward_kv(w: BlockWeights, dims: BlockDims, x, kv, workspace, *,
 
 # ------------------------------------------------------------- backward passes --
 
-def fused_attention_bwd_ws_bytes(*, batch: int, Tq: int, Tk: int, C: int, heads: int, dtype: int = MI_F32) -> int:
-    """Workspace fused_attention_bwd needs for these sizes."""
-    x = MiAttnBwdArgs(fwd=MiAttnArgs(batch=batch, Tq=Tq, Tk=Tk, C=C, heads=heads, in_dtype=dtype, out_dtype=dtype))
+def fused_attention_bwd_ws_bytes(*, batch: int, Tq: int, Tk: int, C: int, heads: int, dtype: int = MI_F32, wide: bool = True) -> int:
+    """Workspace fused_attention_bwd needs for these sizes; wide: every row of the tensors starts on 16 bytes (others
+    are packed into it)."""
+    x = MiAttnBwdArgs(fwd=MiAttnArgs(q=None if wide else 1, batch=batch, Tq=Tq, Tk=Tk, C=C, heads=heads,
+                                     in_dtype=dtype, out_dtype=dtype), dq=None if wide else 1)
     return int(_lib.load().mi_fused_attention_bwd_ws_bytes(ctypes.byref(x)))
 
 
