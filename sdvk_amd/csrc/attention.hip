@@ -468,16 +468,6 @@ constexpr int kResidNone = 0, kResidDiagonal = 1, kResidAll = 2;
 // TFLOP/s of the algorithm's operations), 1 x 10 x 4096^2 213 -> 171, 2 x 10 x 4096^2
 // with fp16 P 278 -> 226, cross 2 x 10 x 4096 x 77 22.2 -> 17.4; error against 64 bits
 // 6.8e-7 -> 4.5e-7 of the result's norm (2304 keys, N(0, 1) data).
-typedef float floatx2 __attribute__((ext_vector_type(2)));
-// Two values as fp16 (RNE) in one packed conversion.
-__device__ __forceinline__ half2 pack2(float x, float y) { return __builtin_convertvector(floatx2{x, y}, half2); }
-// fp16(x - hi): neg1 holds -1 in a register the compiler cannot see through, so
-// the subtraction stays a fma that rounds straight to fp16 (v_fma_mixlo/hi_f16).
-__device__ __forceinline__ half2 residual2(half2 hi, float x, float y, float neg1) {
-    return half2{static_cast<_Float16>(__builtin_fmaf(static_cast<float>(hi[0]), neg1, x)),
-                 static_cast<_Float16>(__builtin_fmaf(static_cast<float>(hi[1]), neg1, y))};
-}
-
 constexpr int kFLd = 72;                    // halves per staged row: 64 + 16-byte pad
 constexpr int kFPlane = kBKV * kFLd;        // halves of one staged plane (K or V, hi or lo)
 constexpr int kFStage = 4 * kFPlane;        // K hi, K lo, V hi, V lo

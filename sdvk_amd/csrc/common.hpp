@@ -171,6 +171,16 @@ __device__ __forceinline__ void interleave_step() {
     }
 }
 
+typedef float floatx2 __attribute__((ext_vector_type(2)));
+// Two values as fp16 (RNE) in one packed conversion.
+__device__ __forceinline__ half2 pack2(float x, float y) { return __builtin_convertvector(floatx2{x, y}, half2); }
+// fp16(x - hi): neg1 holds -1 in a register the compiler cannot see through, so
+// the subtraction stays a fma that rounds straight to fp16 (v_fma_mixlo/hi_f16).
+__device__ __forceinline__ half2 residual2(half2 hi, float x, float y, float neg1) {
+    return half2{static_cast<_Float16>(__builtin_fmaf(static_cast<float>(hi[0]), neg1, x)),
+                 static_cast<_Float16>(__builtin_fmaf(static_cast<float>(hi[1]), neg1, y))};
+}
+
 // Transposing LDS read: within each 16-lane group, lane i returns element i % 4
 // of the 8-byte pieces addressed by lanes i/4, i/4 + 4, i/4 + 8, i/4 + 12.
 __device__ __forceinline__ half4 lds_read_tr16(const _Float16* p) {

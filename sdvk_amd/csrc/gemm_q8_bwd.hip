@@ -173,6 +173,13 @@ __global__ __launch_bounds__(WM * WN * 64) void gemm_q8_bwd_kernel(BwdArgs a) {
     typedef T Unit __attribute__((ext_vector_type(AV)));
     Unit areg[2][A_IT];
     uint32_t wq[2][W_IT][QD + 1], wd[2][W_IT];
+    auto past = [](bool in) {
+        // (opaque: a select of the offset becomes a branch around the loads, and a load under a branch makes every later
+        // wait retire the loads in flight)
+        uint32_t top = in ? 0u : kPast;
+        asm volatile("" : "+v"(top));
+        return top;
+    };
     auto load_step = [&](uint32_t step, auto RS) {
         constexpr int rs = decltype(RS)::value;
         const uint32_t n0 = __builtin_amdgcn_readfirstlane(step * NS);
@@ -185,36 +192,41 @@ __global__ __launch_bounds__(WM * WN * 64) void gemm_q8_bwd_kernel(BwdArgs a) {
                 for (int e = 0; e < AV; ++e)
                     areg[rs][i][e] = row < rows && n + e < a.N ? panel[static_cast<uint64_t>(row) * a.ldc + n + e] : static_cast<T>(0.0f);
             } else {
-                const uint32_t off = n < a.N && a_off[i] != kPast ? a_off[i] + n * static_cast<uint32_t>(sizeof(T)) : kPast;
-                areg[rs][i] = __builtin_bit_cast(Unit, __builtin_amdgcn_raw_buffer_load_b128(rA, off, 0, 0));
+                // units past N read as zeros: offsets with the top bit set are out of range
+                const uint32_t off = (a_off[i] + ((tid + i * NT) & 7) * 16u) | past(n < a.N);
+                areg[rs][i] = __builtin_bit_cast(Unit, __builtin_amdgcn_raw_buffer_load_b128(rA, off, n0 * sizeof(T), 0));
             }
         }
+        const uint32_t soff = n0 * a.rowbytes;
 #pragma unroll
         for (int i = 0; i < W_IT; ++i) {
-            const bool in = n0 + w_n[i] < a.N;  // rows past N read as zeros
-            const uint32_t o = in ? w_off[i] + n0 * a.rowbytes : kPast;
+            const uint32_t out = past(n0 + w_n[i] < a.N);  // rows past N read as zeros
+            const uint32_t o = w_off[i] | out;
             if constexpr (QD == 8) {
-                const auto x0 = __builtin_amdgcn_raw_buffer_load_b128(rW, o, 0, 0);
-                const auto x1 = __builtin_amdgcn_raw_buffer_load_b128(rW, o + 16, 0, 0);
+                const auto x0 = __builtin_amdgcn_raw_buffer_load_b128(rW, o, soff, 0);
+                const auto x1 = __builtin_amdgcn_raw_buffer_load_b128(rW, o + 16, soff, 0);
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                     wq[rs][i][e] = x0[e];
                     wq[rs][i][QD / 2 + e] = x1[e];
                 }
             } else if constexpr (QD == 4) {
-                const auto x0 = __builtin_amdgcn_raw_buffer_load_b128(rW, o, 0, 0);
+                const auto x0 = __builtin_amdgcn_raw_buffer_load_b128(rW, o, soff, 0);
 #pragma unroll
                 for (int e = 0; e < 4; ++e) wq[rs][i][e] = x0[e];
             } else {
-                const auto x0 = __builtin_amdgcn_raw_buffer_load_b64(rW, o, 0, 0);
+                const auto x0 = __builtin_amdgcn_raw_buffer_load_b64(rW, o, soff, 0);
                 wq[rs][i][0] = x0[0];
                 wq[rs][i][1] = x0[1];
             }
-            wq[rs][i][QD] = __builtin_amdgcn_raw_buffer_load_b32(rW, o + 4 * QD, 0, 0);
-            wd[rs][i] = __builtin_amdgcn_raw_buffer_load_b16(rW, in ? w_d[i] + n0 * a.rowbytes : kPast, 0, 0);
+            // (the last block's window may end past W: the whole offset is in voffset, where the range check counts it)
+            wq[rs][i][QD] = __builtin_amdgcn_raw_buffer_load_b32(rW, (w_off[i] + soff + 4 * QD) | out, 0, 0);
+            wd[rs][i] = __builtin_amdgcn_raw_buffer_load_b16(rW, w_d[i] | out, soff, 0);
         }
     };
 
+    float neg1 = -1.0f;  // (residual2)
+    asm volatile("" : "+v"(neg1));
     int re[A_IT];  // fp32: the exponents of this thread's rows (the same in the eight threads of a row)
 #pragma unroll
     for (int i = 0; i < A_IT; ++i) re[i] = 127;
@@ -232,17 +244,15 @@ __global__ __launch_bounds__(WM * WN * 64) void gemm_q8_bwd_kernel(BwdArgs a) {
                 mx = dpp_max<0xb1>(mx);   // quad_perm [1, 0, 3, 2]
                 mx = dpp_max<0x4e>(mx);   // quad_perm [2, 3, 0, 1]
                 mx = dpp_max<0x141>(mx);  // row_half_mirror: the row's eight lanes
-                if (ldexpf(mx, re[i]) > kRowMax)
-                    re[i] = min(re[i], kRowExp + 127 - static_cast<int>(__float_as_uint(mx) >> 23));
-                half4 hi, lo;
+                const int low = min(re[i], kRowExp + 127 - static_cast<int>(__float_as_uint(mx) >> 23));
+                re[i] = ldexpf(mx, re[i]) > kRowMax ? low : re[i];
+                float v[4];
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const float v = ldexpf(x[e], re[i]);
-                    hi[e] = static_cast<_Float16>(v);
-                    lo[e] = static_cast<_Float16>(v - static_cast<float>(hi[e]));
-                }
-                *reinterpret_cast<half4*>(dst) = hi;
-                *reinterpret_cast<half4*>(dst + kAPlane) = lo;
+                for (int e = 0; e < 4; ++e) v[e] = ldexpf(x[e], re[i]);
+                const half2 h0 = pack2(v[0], v[1]), h1 = pack2(v[2], v[3]);
+                const half2 l0 = residual2(h0, v[0], v[1], neg1), l1 = residual2(h1, v[2], v[3], neg1);
+                *reinterpret_cast<half4*>(dst) = half4{h0[0], h0[1], h1[0], h1[1]};
+                *reinterpret_cast<half4*>(dst + kAPlane) = half4{l0[0], l0[1], l1[0], l1[1]};
                 if ((f & 7) == 0) rowexp[st * BM + (f >> 3)] = re[i];
             } else {
                 *reinterpret_cast<half8*>(dst) = __builtin_bit_cast(half8, areg[rs][i]);
@@ -263,11 +273,18 @@ __global__ __launch_bounds__(WM * WN * 64) void gemm_q8_bwd_kernel(BwdArgs a) {
                     const float s = static_cast<float>(d) * (1 << kWExp), s128 = -128.0f * s;
                     half8 hi, lo;
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) {
-                        const uint32_t byte = ((q[j + e / 4] ^ 0x80808080u) >> (8 * (e % 4))) & 0xffu;
-                        const float w = __builtin_fmaf(static_cast<float>(byte), s, s128);
-                        hi[e] = static_cast<_Float16>(w);
-                        lo[e] = static_cast<_Float16>(w - static_cast<float>(hi[e]));
+                    for (int e = 0; e < 8; e += 2) {
+                        float w[2];
+#pragma unroll
+                        for (int x = 0; x < 2; ++x) {
+                            const uint32_t byte = ((q[j + e / 4] ^ 0x80808080u) >> (8 * (e % 4 + x))) & 0xffu;
+                            w[x] = __builtin_fmaf(static_cast<float>(byte), s, s128);
+                        }
+                        const half2 h = pack2(w[0], w[1]), l = residual2(h, w[0], w[1], neg1);
+                        hi[e] = h[0];
+                        hi[e + 1] = h[1];
+                        lo[e] = l[0];
+                        lo[e + 1] = l[1];
                     }
                     *reinterpret_cast<half8*>(dst + 4 * j) = hi;
                     *reinterpret_cast<half8*>(dst + 4 * j + kWPlane) = lo;
@@ -345,6 +362,15 @@ __global__ __launch_bounds__(WM * WN * 64) void gemm_q8_bwd_kernel(BwdArgs a) {
     using S0 = std::integral_constant<int, 0>;
     using S1 = std::integral_constant<int, 1>;
 
+    // The step's MFMAs with the next fragment reads and a share of the conversions and LDS writes between them. Only the
+    // 256-row tiles have the CU to themselves; of the others two or three workgroups fill each other's gaps. us with and
+    // without the order, fp16: 256x128 1976x10240x1280 76.6 / 79.7, 8192x1920x640 37.9 / 41.2, 988x1280x5120 26.7 / 28.9;
+    // 128x128 2048x1280x5120 54.8 / 51.8; 64x64 576x1280x1280 11.7 / 10.8. fp32: 256x128 1976x10240x1280 212 / 214.
+    constexpr bool kMix = !ANY && BM == 256;
+    constexpr int kMfma = FM * FN * (NS / 16) * (kPair ? 3 : 1);
+    constexpr int kRead0 = NP * (FM + 2 * FN), kReads = kRead0 * (NS / 16);
+    constexpr int kWrites = NP * (A_IT + W_IT * QD / 2);
+    constexpr int kValu = kPair ? A_IT * 30 + W_IT * QD * 17 : W_IT * QD * 8;
     // Step j computes from LDS stage j & 1 while the loads of step j + 2 are in flight; those of step j + 1 are then
     // stored into the other stage. Loads past the last step re-read it and are not used.
     const uint32_t n_steps = s_end - s_begin, last = s_end - 1;
@@ -358,6 +384,7 @@ __global__ __launch_bounds__(WM * WN * 64) void gemm_q8_bwd_kernel(BwdArgs a) {
         __builtin_amdgcn_sched_barrier(0);
         compute(S0{});
         store_step(S1{}, S1{});
+        if constexpr (kMix) interleave_step<kMfma, kRead0, kReads - kRead0, kValu, kWrites>();
         __syncthreads();
         load_step(min(s_begin + j + 3, last), S1{});
         __builtin_amdgcn_sched_barrier(0);
@@ -365,6 +392,7 @@ __global__ __launch_bounds__(WM * WN * 64) void gemm_q8_bwd_kernel(BwdArgs a) {
         // an odd last step is the one just stored; an even one needs nothing more, and storing the last step again
         // would not change the sums, but would count its rows' exponents twice: the same exponents
         store_step(S0{}, S0{});
+        if constexpr (kMix) interleave_step<kMfma, kRead0, kReads - kRead0, kValu, kWrites>();
         __syncthreads();
     }
     if (j < n_steps) compute(S0{});
@@ -437,20 +465,50 @@ uint32_t launched_splits(uint32_t N, bool f32, uint32_t splits) {
     return ceil_div(steps, ceil_div(steps, splits));
 }
 
+// What a build costs, us: `base` (launch, first loads, last stores) and a step of its workgroups with 1, 2 or 3 of them on
+// a CU (LDS allows no more of the larger tiles). Fitted to a sweep of every build and number of parts over the layers of
+// 512- to 1024-pixel images (MI355X, operands of full entropy, calls back to back); examples in us, build:parts measured
+// (256x128, 128x128, 64x64): fp16 2048x1280x5120 54.5 / 47.6 / 77.8, 8192x1920x640 38.3 / 43.4 / 46.9, 576x1280x1280
+// 26.8 / 17.9 / 10.0, 1976x10240x1280 in 3 parts 76.7 / 83.7 / 130, unsplit 2:1 143; fp32 1152x1280x1280 28.8 in 5 parts /
+// 32.5 in 2 / 38.1 in 1, 8192x5120x640 218 in 3 / 256 in 3 / 311.
+struct Cost {
+    uint32_t bm, bk, per_cu;
+    double base, step[3];
+};
+constexpr Cost kCost[2][kGemmBwdBuilds] = {
+    {{256, 128, 1, 6.0, {1.13}}, {128, 128, 2, 4.5, {0.75, 1.25}}, {64, 64, 3, 2.8, {0.36, 0.62, 0.90}}},
+    {{256, 128, 1, 7.0, {1.60}}, {128, 128, 1, 5.0, {1.08}}, {64, 64, 3, 3.0, {0.62, 0.87, 1.18}}}};
+
+double cost_us(const Cost& c, uint32_t M, uint32_t K, uint32_t steps, uint32_t splits) {
+    const uint64_t wgs = static_cast<uint64_t>(ceil_div(M, c.bm)) * ceil_div(K, c.bk) * splits;
+    const uint64_t rounds = wgs / (kCUs * c.per_cu);
+    const uint32_t last = static_cast<uint32_t>(wgs % (kCUs * c.per_cu));
+    double us = static_cast<double>(rounds) * c.step[c.per_cu - 1];
+    if (last) us += c.step[ceil_div(last, kCUs) - 1];
+    us = c.base + us * ceil_div(steps, splits);
+    // the parts' planes are written and read back, by a launch of its own
+    if (splits > 1) us += 3.0 + static_cast<double>(splits) * M * K * 8 / 5.5e6;
+    return us;
+}
+
 Plan choose(uint32_t M, uint32_t N, uint32_t K, bool f32, bool allow_split) {
     const int forced = tuning().gemm_bwd_cfg.load(std::memory_order_relaxed);
     if (forced >= 0) {
         const uint32_t s = static_cast<uint32_t>(tuning().gemm_bwd_splits.load(std::memory_order_relaxed));
         return Plan{forced, allow_split ? launched_splits(N, f32, s) : 1u};
     }
-    auto tiles = [&](uint32_t bm, uint32_t bk) { return static_cast<uint64_t>(ceil_div(M, bm)) * ceil_div(K, bk); };
-    const uint64_t t256 = tiles(256, 128), t128 = tiles(128, 128), t64 = tiles(64, 64);
-    Plan p{t256 >= kCUs ? k256x128 : t128 > kCUs / 2 ? k128x128 : k64x64, 1};
-    if (!allow_split) return p;
-    const uint64_t t = p.build == k256x128 ? t256 : p.build == k128x128 ? t128 : t64;
-    if (p.build == k64x64 && t <= kCUs / 2)
-        p.splits = launched_splits(N, f32, static_cast<uint32_t>(std::min<uint64_t>(kCUs / t, std::max<uint32_t>(N / 128, 1))));
-    return p;
+    Plan best{k64x64, 1};
+    double best_us = 1e300;
+    for (int b = 0; b < kGemmBwdBuilds; ++b)
+        for (uint32_t splits : {1u, 2u, 3u, 4u, 5u, 8u, 12u, 16u}) {
+            if (splits > 1 && (!allow_split || launched_splits(N, f32, splits) != splits)) continue;
+            const double us = cost_us(kCost[f32][b], M, K, ceil_div(N, n_step(f32)), splits);
+            if (us < best_us) {
+                best_us = us;
+                best = Plan{b, splits};
+            }
+        }
+    return best;
 }
 
 uint64_t part_bytes(uint32_t M, uint32_t K, uint32_t splits) { return splits > 1 ? static_cast<uint64_t>(splits) * M * K * 4 : 0; }
