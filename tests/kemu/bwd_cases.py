@@ -1,4 +1,4 @@
-"""One case of tests/bwd_ref.py on the kernel emulator, in a process of its own (a fault in an emulated kernel ends
+"""One case of tests/bwd_ref.py or tests/bwd_block.py on the kernel emulator, in a process of its own (a fault in an emulated kernel ends
 that process with the emulator's report):
 
     python tests/kemu/bwd_cases.py '<json: {"op": name, "orders": [...], ...parameters}>'
@@ -12,6 +12,7 @@ from pathlib import Path
 HERE = Path(__file__).resolve().parent
 sys.path[:0] = [str(HERE.parent), str(HERE)]
 
+import bwd_block  # noqa: E402
 import bwd_ref  # noqa: E402
 import emu as kemu  # noqa: E402
 
@@ -45,9 +46,11 @@ def main(argv):
     spec = json.loads(argv[1])
     orders, op = spec.pop("orders"), spec.pop("op")
     be = Backend()
+    from sdvk_amd import _lib
+    _lib.load = lambda: be.E.lib  # sdvk_amd.ops on the emulated library
     for o in orders:
         be.E.order(o, bool(o))
-        bwd_ref.OPS[op](be, **spec)
+        {**bwd_ref.OPS, **bwd_block.OPS}[op](be, **spec)
         print(f"OK order {o}", flush=True)
 
 

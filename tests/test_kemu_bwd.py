@@ -12,6 +12,7 @@ from pathlib import Path
 
 import pytest
 
+import bwd_block
 import bwd_ref
 
 KEMU = Path(__file__).resolve().parent / "kemu"
@@ -32,11 +33,19 @@ def run(spec):
     return subprocess.run([sys.executable, str(KEMU / "bwd_cases.py"), json.dumps(spec)], capture_output=True, text=True, timeout=900)
 
 
-@pytest.mark.parametrize("op", list(bwd_ref.CASES))
-def test_backward_kernels_on_emulator(emulator, op):
-    specs = [dict(op=op, orders=ORDERS, **c) for c in bwd_ref.CASES[op]]
+def check(specs):
     with ThreadPoolExecutor(max(1, min(8, os.cpu_count() or 1))) as ex:
         results = list(ex.map(run, specs))
     failed = [f"{json.dumps(s)}\n{(r.stdout + r.stderr).strip()[-1200:]}" for s, r in zip(specs, results)
               if r.returncode != 0 or r.stdout.count("OK ") != len(ORDERS)]
     assert not failed, "\n\n".join(failed)
+
+
+@pytest.mark.parametrize("op", list(bwd_ref.CASES))
+def test_backward_kernels_on_emulator(emulator, op):
+    check([dict(op=op, orders=ORDERS, **c) for c in bwd_ref.CASES[op]])
+
+
+def test_block_backward_on_emulator(emulator):
+    """The operators run together: a transformer block's gradients, against 64 bits and against differences."""
+    check([dict(op=op, orders=ORDERS) for op in bwd_block.OPS])
