@@ -449,7 +449,7 @@ __global__ __launch_bounds__(256) void gemm_q8_bwd_zero_kernel(T* dA, uint32_t M
 
 constexpr uint32_t kCUs = 256;
 
-enum BuildId { k256x128 = 0, k128x128 = 1, k64x64 = 2 };
+enum BuildId { k256x128 = 0, k128x128 = 1, k64x64 = 2, kFew = 3 };
 static_assert(k64x64 + 1 == kGemmBwdBuilds, "mi_tuning_set bounds gemm_bwd_cfg by kGemmBwdBuilds");
 
 struct Plan {
@@ -463,6 +463,72 @@ uint32_t n_step(bool f32) { return f32 ? 32 : 64; }
 uint32_t launched_splits(uint32_t N, bool f32, uint32_t splits) {
     const uint32_t steps = ceil_div(N, n_step(f32));
     return ceil_div(steps, ceil_div(steps, splits));
+}
+
+// Few rows: dA = dC . deq(W) for up to MR rows in one launch, in fp32 for either type (w = d * q exact). What bounds it is
+// the latency of a launch and of its loads: a workgroup takes one 32-wide block of columns and all of N, a wave's lanes 8
+// rows n by the 8 dwords of a block, the 16 waves 128 rows at a time, kDeep times that in flight. The lanes of a column are
+// added by shuffles, the waves through LDS, always in the same order. 2x1280x1280 fp32: 6.3 us, of which a launch is 3.9
+// (64x64 tiles in 12 parts and their sum: 8.3).
+constexpr uint32_t kFewRows = 4;
+constexpr int kFewWaves = 16;
+
+template <typename T, int MR>
+__global__ __launch_bounds__(kFewWaves * 64) void gemm_q8_bwd_few_kernel(BwdArgs a) {
+    constexpr int kDeep = MR <= 2 ? 8 : 4;
+    constexpr uint32_t kRows = kFewWaves * 8;
+    __shared__ float sums[kFewWaves][MR][32];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, c = lane & 7;
+    const uint8_t* const col = a.W + static_cast<uint64_t>(blockIdx.x) * 34;
+    const T* const dC = static_cast<const T*>(a.dC);
+    float acc[MR][4];
+#pragma unroll
+    for (int m = 0; m < MR; ++m)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[m][e] = 0.0f;
+    for (uint32_t n0 = 0; n0 < a.N; n0 += kRows * kDeep) {
+        uint32_t q[kDeep];
+        _Float16 d[kDeep];
+        T x[kDeep][MR];
+#pragma unroll
+        for (int u = 0; u < kDeep; ++u) {
+            const uint32_t n = n0 + u * kRows + wave * 8 + (lane >> 3), at = min(n, a.N - 1);
+            const uint8_t* p = col + static_cast<uint64_t>(at) * a.rowbytes;
+            d[u] = *reinterpret_cast<const _Float16*>(p);
+            __builtin_memcpy(&q[u], p + 2 + 4 * c, 4);  // (2-byte aligned)
+#pragma unroll
+            for (int m = 0; m < MR; ++m) {
+                const T v = dC[static_cast<uint64_t>(min(static_cast<uint32_t>(m), a.M - 1)) * a.ldc + at];
+                x[u][m] = n < a.N ? v : static_cast<T>(0.0f);
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < kDeep; ++u) {
+            const float s = static_cast<float>(d[u]);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const float w = s * static_cast<float>(static_cast<int8_t>(q[u] >> (8 * e)));
+#pragma unroll
+                for (int m = 0; m < MR; ++m) acc[m][e] = __builtin_fmaf(static_cast<float>(x[u][m]), w, acc[m][e]);
+            }
+        }
+    }
+#pragma unroll
+    for (int m = 0; m < MR; ++m) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+#pragma unroll
+            for (int o = 8; o < 64; o <<= 1) acc[m][e] += __shfl_xor(acc[m][e], o);
+        if (lane < 8) *reinterpret_cast<floatx4*>(&sums[wave][m][4 * c]) = floatx4{acc[m][0], acc[m][1], acc[m][2], acc[m][3]};
+    }
+    __syncthreads();
+    const uint32_t m = tid / 32, k = tid % 32;
+    if (m >= a.M) return;  // (MR of the 32 rows that the threads cover have sums)
+    float v = 0.0f;
+#pragma unroll
+    for (int w = 0; w < kFewWaves; ++w) v += sums[w][m][k];
+    T* out = static_cast<T*>(a.dA) + static_cast<uint64_t>(m) * a.lda + blockIdx.x * 32 + k;
+    *out = static_cast<T>(a.mode ? static_cast<float>(*out) + v : v);
 }
 
 // What a build costs, us: `base` (launch, first loads, last stores) and a step of its workgroups with 1, 2 or 3 of them on
@@ -499,6 +565,14 @@ Plan choose(uint32_t M, uint32_t N, uint32_t K, bool f32, bool allow_split) {
     }
     Plan best{k64x64, 1};
     double best_us = 1e300;
+    // The kernel for few rows: one launch and no parts, but all of N in one workgroup, at a quarter of the loads in flight
+    // that the parts have. us against the best build and parts, fp32 / fp16: 1x1280x1280 5.7 : 8.3 / 5.6 : 7.6, 2x640x1280
+    // 4.7 : 7.8 / 4.7 : 6.0, 4x1280x1280 6.9 : 8.3 / 7.0 : 7.6, 2x5120x640 12.7 : 11.1 / 12.8 : 8.0; with eight rows
+    // 8x1280x1280 9.8 : 8.6 / 10.2 : 7.5.
+    if (M <= kFewRows) {
+        best = Plan{kFew, 1};
+        best_us = 4.0 + N * (0.0013 + 0.00025 * M);
+    }
     for (int b = 0; b < kGemmBwdBuilds; ++b)
         for (uint32_t splits : {1u, 2u, 3u, 4u, 5u, 8u, 12u, 16u}) {
             if (splits > 1 && (!allow_split || launched_splits(N, f32, splits) != splits)) continue;
@@ -524,8 +598,17 @@ void launch_build(BwdArgs a, uint32_t splits, hipStream_t s) {
 }
 
 template <typename T>
+void launch_few(const BwdArgs& a, hipStream_t s) {
+    const unsigned grid = a.K / 32, block = kFewWaves * 64;
+    if (a.M == 1) gemm_q8_bwd_few_kernel<T, 1><<<grid, block, 0, s>>>(a);
+    else if (a.M == 2) gemm_q8_bwd_few_kernel<T, 2><<<grid, block, 0, s>>>(a);
+    else gemm_q8_bwd_few_kernel<T, kFewRows><<<grid, block, 0, s>>>(a);
+}
+
+template <typename T>
 void launch(const BwdArgs& a, const Plan& p, bool any, hipStream_t s) {
-    if (any) launch_build<T, 64, 64, 2, 2, true>(a, p.splits, s);
+    if (p.build == kFew) launch_few<T>(a, s);
+    else if (any) launch_build<T, 64, 64, 2, 2, true>(a, p.splits, s);
     else if (p.build == k256x128) launch_build<T, 256, 128, 4, 2, false>(a, p.splits, s);
     else if (p.build == k128x128) launch_build<T, 128, 128, 4, 2, false>(a, p.splits, s);
     else launch_build<T, 64, 64, 2, 2, false>(a, p.splits, s);

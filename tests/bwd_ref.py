@@ -486,6 +486,10 @@ CASES = {
         dict(typ="f32", M=37, N=320, K=64, ramp=True), dict(typ="f32", M=20, N=320, K=64, ramp=True, ws=False),
         dict(typ="f32", M=9, N=64, K=32, std=1e-30), dict(typ="f32", M=9, N=64, K=32, std=1e25),
         dict(typ="f16", M=5, N=0, K=64), dict(typ="f32", M=5, N=0, K=64, mode=1),
+        # few rows: every number of them that has a kernel, N past one pass of the workgroup
+        dict(typ="f16", M=1, N=2100, K=32), dict(typ="f32", M=2, N=1025, K=64, ramp=True), dict(typ="f32", M=4, N=1030, K=32, mode=1),
+        dict(typ="f16", M=3, N=530, K=96, off=3, aoff=1, ldc=533, lda=97), dict(typ="f32", M=4, N=513, K=64, off=1, aoff=1, lda=65),
+        dict(typ="f32", M=3, N=64, K=32, std=1e-30), dict(typ="f16", M=3, N=40, K=64, cfg="2:1"),
         # every tile build, alone and with parts
         dict(typ="f16", M=300, N=136, K=288, cfg="0"), dict(typ="f32", M=300, N=68, K=288, cfg="0", mode=1),
         dict(typ="f16", M=150, N=200, K=288, cfg="1:3"), dict(typ="f32", M=150, N=100, K=160, cfg="1:2"),
