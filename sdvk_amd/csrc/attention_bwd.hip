@@ -979,7 +979,7 @@ Deal deal(uint32_t bhs, uint32_t T, uint32_t Tother, bool causal) {
     const uint32_t blocks = bhs * d.nb;
     const uint64_t total = static_cast<uint64_t>(bhs) * d.per;
     d.wgs = blocks;
-    const bool alike = !causal || d.nb <= 1;  // all blocks have NT tiles
+    const bool alike = d.per == d.nb * d.NT;  // all blocks have NT tiles
     d.whole = alike ? 1 : 0;
     const uint64_t rounds = (blocks + kSlots - 1) / kSlots;
     const uint32_t shares = static_cast<uint32_t>(std::max<uint64_t>(1, std::min<uint64_t>(kSlots, total / kMinShare)));

@@ -460,6 +460,7 @@ CASES = {
         dict(typ="f32", Tq=33, Tk=70, batch=3, lens=[0, 64, 700], poison=True), dict(typ="f16", Tq=140, Tk=140, causal=True, heads=2),
         dict(typ="f32", Tq=140, Tk=140, causal=True), dict(typ="f16", Tq=70, Tk=200, causal=True), dict(typ="f32", Tq=200, Tk=70, causal=True),
         dict(typ="f16", Tq=77, Tk=77, causal=True, batch=2, lens=[77, 5]),
+        dict(typ="f16", Tq=70, Tk=200, causal=True, heads=3), dict(typ="f32", Tq=100, Tk=300, causal=True, batch=2),
         # head widths, rows off their 16-byte places, gaps, the joint [rows, 3C] gradient
         dict(typ="f16", Tq=70, Tk=66, heads=3, hd=40), dict(typ="f32", Tq=70, Tk=66, heads=3, hd=40), dict(typ="f16", Tq=40, Tk=70, heads=2, hd=20),
         dict(typ="f32", Tq=40, Tk=70, heads=2, hd=20), dict(typ="f16", Tq=40, Tk=70, heads=2, hd=37), dict(typ="f32", Tq=40, Tk=70, heads=3, hd=1),
