@@ -73,6 +73,7 @@ struct Operand {
 // `per` tiles to those. Each of wgs workgroups takes `whole` blocks, and an equal share of the tiles of the blocks left.
 struct Deal {
     uint32_t NT, nb, per, wgs, whole;
+    uint32_t quo, rem, frac;  // the tiles dealt in shares are quo * wgs + rem (share_start)
 };
 struct BwdArgs {
     Tensor q, k, v, o, g;     // g: dO
@@ -119,32 +120,40 @@ __host__ __device__ inline uint32_t before(uint32_t i, uint32_t NT, bool causal)
     const uint32_t half = NT / 2, j = i < half ? i : half;
     return j * (j + 1) + (i - j) * NT;
 }
-// The first tile of share w of `total`, counted from the first block that is dealt in shares.
-__host__ __device__ inline uint64_t share_start(const Deal& d, uint64_t total, uint64_t w) { return w * total / d.wgs; }
-__host__ __device__ inline uint32_t dealt_whole(const Deal& d) { return d.wgs * d.whole; }
-// Tiles that are dealt in shares (blocks are dealt whole only where all have NT tiles).
-__host__ __device__ inline uint64_t shared_tiles(const Deal& d, uint32_t bhs) {
-    return static_cast<uint64_t>(bhs) * d.per - static_cast<uint64_t>(dealt_whole(d)) * d.NT;
+// The first tile of share w, counted from the first block that is dealt in shares: floor(w tiles / wgs), without a division
+// (frac: 2^32 rem / wgs rounded up; off by one in places for more than 65535 shares, where that changes nothing but the
+// balance); and the share of tile u.
+__host__ __device__ inline uint32_t share_start(const Deal& d, uint32_t w) {
+    return w * d.quo + static_cast<uint32_t>((static_cast<uint64_t>(w) * d.frac) >> 32);
 }
+__host__ __device__ inline uint32_t share_of(const Deal& d, uint32_t u) {
+    const uint64_t total = static_cast<uint64_t>(d.quo) * d.wgs + d.rem;
+    uint32_t w = static_cast<uint32_t>(static_cast<uint64_t>(u) * d.wgs / total);
+    while (share_start(d, w) > u) --w;
+    while (share_start(d, w + 1) <= u) ++w;
+    return w;
+}
+__host__ __device__ inline uint32_t dealt_whole(const Deal& d) { return d.wgs * d.whole; }
 
 // The pieces of a workgroup's work, one after the other: tiles [t0, t1) of block blk of (batch, head) bh.
 template <bool KEYS>
 struct Pieces {
     const Deal d;
     const bool causal;
-    uint64_t base, at, end;  // tiles, counted from the first block of all
+    uint32_t base, at, end;  // tiles, counted from the first block of all
     uint32_t id, blocks;     // the next whole block and those left
     uint32_t bh, blk, t0, t1;
     bool whole, first;       // the whole block; the first piece of the share
 
-    __device__ __forceinline__ Pieces(const Deal& d_, bool causal_, uint32_t bhs, uint32_t w) : d(d_), causal(causal_) {
-        const uint64_t total = shared_tiles(d, bhs);
-        base = static_cast<uint64_t>(dealt_whole(d)) * d.NT;
-        at = base + share_start(d, total, w);
-        end = base + share_start(d, total, w + 1);
-        base = at;
+    __device__ __forceinline__ Pieces(const Deal& d_, bool causal_, uint32_t w) : d(d_), causal(causal_) {
         id = w * d.whole;
         blocks = d.whole;
+        base = at = end = 0;
+        if (d.quo) {
+            const uint32_t skip = dealt_whole(d) * d.NT;
+            base = at = skip + share_start(d, w);
+            end = skip + share_start(d, w + 1);
+        }
     }
     __device__ __forceinline__ bool next() {
         if (blocks) {
@@ -159,8 +168,8 @@ struct Pieces {
         }
         if (at >= end) return false;
         first = at == base;
-        bh = static_cast<uint32_t>(at / d.per);
-        const uint32_t r = static_cast<uint32_t>(at % d.per);
+        bh = at / d.per;
+        const uint32_t r = at % d.per;
         uint32_t lo = 0, hi = d.nb;  // the last block with no more than r tiles before it
         while (hi - lo > 1) {
             const uint32_t mid = (lo + hi) / 2;
@@ -170,7 +179,7 @@ struct Pieces {
         blk = lo;
         const uint32_t b0 = before<KEYS>(blk, d.NT, causal), n = before<KEYS>(blk + 1, d.NT, causal) - b0;
         t0 = r - b0;
-        t1 = static_cast<uint32_t>(min(static_cast<uint64_t>(n), t0 + (end - at)));
+        t1 = min(n, t0 + (end - at));
         whole = t0 == 0 && t1 == n;
         at += t1 - t0;
         return true;
@@ -180,22 +189,15 @@ struct Pieces {
 // begins with it, else in slot 1.
 template <bool KEYS>
 struct Parts {
-    uint64_t total, u0;
-    uint32_t w0, w1;
-    __device__ __forceinline__ Parts(const Deal& d, bool causal, uint32_t bhs, uint32_t bh, uint32_t blk) {
-        w0 = w1 = 0;
+    uint32_t u0, w0, w1;
+    __device__ __forceinline__ Parts(const Deal& d, bool causal, uint32_t bh, uint32_t blk) {
+        u0 = w0 = w1 = 0;
         if (bh * d.nb + blk < dealt_whole(d)) return;
-        total = shared_tiles(d, bhs);
-        const uint64_t skip = static_cast<uint64_t>(dealt_whole(d)) * d.NT;
-        u0 = static_cast<uint64_t>(bh) * d.per + before<KEYS>(blk, d.NT, causal) - skip;
-        const uint64_t u1 = static_cast<uint64_t>(bh) * d.per + before<KEYS>(blk + 1, d.NT, causal) - skip;
-        // share w begins at floor(w total / wgs): tile u is in the last share that begins at or before it
-        w0 = static_cast<uint32_t>(((u0 + 1) * d.wgs - 1) / total);
-        w1 = static_cast<uint32_t>((u1 * d.wgs - 1) / total);
+        u0 = bh * d.per + before<KEYS>(blk, d.NT, causal) - dealt_whole(d) * d.NT;
+        w0 = share_of(d, u0);
+        w1 = share_of(d, u0 + (before<KEYS>(blk + 1, d.NT, causal) - before<KEYS>(blk, d.NT, causal)) - 1);
     }
-    __device__ __forceinline__ uint64_t slot(const Deal& d, uint32_t w) const {
-        return 2ull * w + (share_start(d, total, w) >= u0 ? 0 : 1);
-    }
+    __device__ __forceinline__ uint64_t slot(const Deal& d, uint32_t w) const { return 2ull * w + (share_start(d, w) >= u0 ? 0 : 1); }
 };
 constexpr uint32_t kQPart = kB * 64 + 2 * kB;  // floats of a query block's part: dQ rows, m, l
 constexpr uint32_t kKPart = 2 * kB * 64;       // of a key block's: dK and dV rows
@@ -320,14 +322,21 @@ __device__ __forceinline__ floatx16 mma(const half8 (&x)[NP], const half8 (&y)[N
 // Elements 8 sp .. 8 sp + 7 of x as an MFMA operand. The empty register constraint holds the fp32 value: the rounding to hi
 // must not fuse into the multiplication that made it (a mixed-precision fma rounds the exact product), or lo, the rest of
 // the fp32 value, would belong to another hi now and then (a row in a hundred off by 1e-4).
+// neg1: residual2's.
 template <int NP>
-__device__ __forceinline__ void operand(const float (&x)[16], int sp, half8 (&f)[NP]) {
+__device__ __forceinline__ void operand(const float (&x)[16], int sp, half8 (&f)[NP], float neg1) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        float v = x[8 * sp + i];
-        if constexpr (NP == 2) asm volatile("" : "+v"(v));
-        f[0][i] = static_cast<_Float16>(v);
-        if constexpr (NP == 2) f[NP - 1][i] = static_cast<_Float16>(v - static_cast<float>(f[0][i]));
+    for (int i = 0; i < 8; i += 2) {
+        float v = x[8 * sp + i], w = x[8 * sp + i + 1];
+        if constexpr (NP == 2) asm volatile("" : "+v"(v), "+v"(w));
+        const half2 hi = pack2(v, w);
+        f[0][i] = hi[0];
+        f[0][i + 1] = hi[1];
+        if constexpr (NP == 2) {
+            const half2 lo = residual2(hi, v, w, neg1);
+            f[NP - 1][i] = lo[0];
+            f[NP - 1][i + 1] = lo[1];
+        }
     }
 }
 
@@ -426,6 +435,9 @@ template <typename T, bool PACKED>
 __global__ __launch_bounds__(256, sizeof(T) == 4 ? 2 : 3) void attn_bwd_q_kernel(BwdArgs a) {
     constexpr int NP = sizeof(T) == 4 ? 2 : 1;
     constexpr int NS = 2;
+    // The fragments of a product are read from LDS ahead of the one before it: fp32 2x20x256^2 45.1 us with and 47.2 without.
+    // fp16 has no registers for it at three waves per SIMD (2x10x4096x77 47.9 and 46.5).
+    constexpr int kAhead = NP == 2 ? 1 : 0;
     static_assert(NP == 1 || PACKED, "fp32 is packed into pairs");
     typedef Stage<NP, NS> St;
     __shared__ __attribute__((aligned(16))) _Float16 ks0[St::kHalves], ks1[St::kHalves], vs0[St::kHalves], vs1[St::kHalves];
@@ -441,14 +453,18 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 ? 2 : 3) void attn_bwd_q_kernel
     V.lds[1] = vs1;
 
     const Places places(lane);
+    float neg1 = -1.0f;  // (residual2)
+    asm volatile("" : "+v"(neg1));
     const uint32_t wg = xcd_swizzle(blockIdx.x, gridDim.x);
-    Pieces<false> pc(a.qd, a.causal != 0, a.batch * a.heads, wg);
+    Pieces<false> pc(a.qd, a.causal != 0, wg);
     while (pc.next()) {
         const uint32_t bh = pc.bh, h = bh % a.heads, b = bh / a.heads, qb = pc.blk;
         const uint32_t q0 = qb * kB, qi = q0 + wave * 32 + l32;
         // this lane's query: fragments of Q (with the scale's sign) and dO, delta, the row's power of two
         const bool in = qi < a.Tq;
         const uint64_t row = static_cast<uint64_t>(bh) * a.qblocks * kB + q0 + wave * 32 + l32;
+        const uint32_t L = keys_of(a, b);  // (first: what is behind it waits for it alone)
+        __builtin_amdgcn_sched_barrier(0);
         half8 qf[4][NP], gf[4][NP], of[PACKED ? 1 : 4];
         float delta = 0.0f, gmax = 0.0f;
         int re = 0;
@@ -469,7 +485,6 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 ? 2 : 3) void attn_bwd_q_kernel
                 re = a.rexp[row];
             }
         }
-        const uint32_t L = keys_of(a, b);
         const uint32_t kend = a.causal ? min(L, q0 + kB) : L;
         // tiles that end at or before kfull need no mask for any query of this wave
         uint32_t kfull = L / kTile * kTile;
@@ -525,13 +540,18 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 ? 2 : 3) void attn_bwd_q_kernel
                 floatx16 s, dp;
 #pragma unroll
                 for (int r = 0; r < 16; ++r) s[r] = dp[r] = 0.0f;
+                half8 kf[kAhead + 1][NP], vf[kAhead + 1][NP];
+                auto rows = [&](int i) {
+                    K.template row_frag<st>(places, t, i, kf[i & kAhead]);
+                    V.template row_frag<st>(places, t, i, vf[i & kAhead]);
+                };
+                if (kAhead) rows(0);
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    half8 kf[NP], vf[NP];
-                    K.template row_frag<st>(places, t, i, kf);
-                    V.template row_frag<st>(places, t, i, vf);
-                    s = mma<NP>(kf, qf[i], s);
-                    dp = mma<NP>(vf, gf[i], dp);
+                    if (i + kAhead < 4) rows(i + kAhead);
+                    if (kAhead) __builtin_amdgcn_sched_barrier(0);
+                    s = mma<NP>(kf[i & kAhead], qf[i], s);
+                    dp = mma<NP>(vf[i & kAhead], gf[i], dp);
                 }
                 if (j * kTile >= kfull) {  // wave-uniform
                     const uint32_t k0 = j * kTile + 32 * t;
@@ -579,16 +599,16 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 ? 2 : 3) void attn_bwd_q_kernel
                 l += ts;
 #pragma unroll
                 for (int r = 0; r < 16; ++r) p[r] *= dp[r] - dl;
+                half8 df[2][NP], kt[kAhead + 1][NP];
+                auto columns = [&](int n) { K.template col_frag<st>(places, t, n >> 1, n & 1, kt[n & kAhead]); };
+                if (kAhead) columns(0);
+                operand<NP>(p, 0, df[0], neg1);
+                operand<NP>(p, 1, df[1], neg1);
 #pragma unroll
-                for (int sp = 0; sp < 2; ++sp) {
-                    half8 df[NP];
-                    operand<NP>(p, sp, df);
-#pragma unroll
-                    for (int u = 0; u < 2; ++u) {
-                        half8 kt[NP];
-                        K.template col_frag<st>(places, t, sp, u, kt);
-                        acc[u] = mma<NP>(kt, df, acc[u]);
-                    }
+                for (int n = 0; n < 4; ++n) {
+                    if (n + kAhead < 4) columns(n + kAhead);
+                    if (kAhead) __builtin_amdgcn_sched_barrier(0);
+                    acc[n & 1] = mma<NP>(kt[n & kAhead], df[n >> 1], acc[n & 1]);
                 }
             }
         };
@@ -643,7 +663,7 @@ template <typename T>
 __global__ __launch_bounds__(256) void attn_bwd_q_merge_kernel(BwdArgs a) {
     typedef T T4 __attribute__((ext_vector_type(4)));
     const uint32_t id = blockIdx.x / 4, bh = id / a.qblocks, qb = id % a.qblocks;
-    const Parts<false> ps(a.qd, a.causal != 0, a.batch * a.heads, bh, qb);
+    const Parts<false> ps(a.qd, a.causal != 0, bh, qb);
     if (ps.w0 == ps.w1) return;
     const int r = static_cast<int>(blockIdx.x % 4) * 32 + static_cast<int>(threadIdx.x >> 3), d = (threadIdx.x & 7) * 8;
     const uint32_t qi = qb * kB + r;
@@ -697,6 +717,9 @@ template <typename T, bool PACKED, bool CAUSAL>
 __global__ __launch_bounds__(256, 2) void attn_bwd_k_kernel(BwdArgs a) {
     constexpr int NP = sizeof(T) == 4 ? 2 : 1;
     constexpr int NS = 2;
+    // The fragments of a product are read from LDS ahead of the one before it, where registers allow: fp16 2x20x1024^2 90.7 us
+    // with and 92.1 without; fp32 would spill (1x8x2048^2 causal 105 and 103).
+    constexpr int kAhead = NP == 1 ? 1 : 0;
     typedef Stage<NP, NS> St;
     __shared__ __attribute__((aligned(16))) _Float16 qs0[St::kHalves], qs1[St::kHalves], gs0[St::kHalves], gs1[St::kHalves];
     // per stage and query: m + log2 l less P's power of two, and -delta in the unit of dP
@@ -713,8 +736,10 @@ __global__ __launch_bounds__(256, 2) void attn_bwd_k_kernel(BwdArgs a) {
     G.lds[1] = gs1;
 
     const Places places(lane);
+    float neg1 = -1.0f;  // (residual2)
+    asm volatile("" : "+v"(neg1));
     const uint32_t wg = xcd_swizzle(blockIdx.x, gridDim.x);
-    Pieces<true> pc(a.kd, CAUSAL, a.batch * a.heads, wg);
+    Pieces<true> pc(a.kd, CAUSAL, wg);
     while (pc.next()) {
         const uint32_t bh = pc.bh, h = bh % a.heads, b = bh / a.heads;
         const uint32_t k0 = pc.blk * kB, kj = k0 + wave * 32 + l32;
@@ -723,6 +748,7 @@ __global__ __launch_bounds__(256, 2) void attn_bwd_k_kernel(BwdArgs a) {
         const uint32_t first = CAUSAL ? min(k0 / kTile, tiles) : 0u;
         uint32_t it = first + pc.t0;
         const uint32_t tend = min(first + pc.t1, tiles);
+        const uint32_t L = keys_of(a, b);
         Q.set(head_of(a.xq, b, h), a.xq, a.Tq, PACKED ? 64 : hd, wave, lane);
         G.set(head_of(a.xg, b, h), a.xg, a.Tq, PACKED ? 64 : hd, wave, lane);
         Q.template load<0>(it * kTile);
@@ -755,7 +781,6 @@ __global__ __launch_bounds__(256, 2) void attn_bwd_k_kernel(BwdArgs a) {
             gm = fmaxf(gm, x[0]);
             dm = fmaxf(dm, x[1]);
         }
-        const uint32_t L = keys_of(a, b);
         const bool in = kj < L;
         const uint32_t t1 = k0 < L ? tend : it;
         gm = wave_max(gm);
@@ -817,13 +842,18 @@ __global__ __launch_bounds__(256, 2) void attn_bwd_k_kernel(BwdArgs a) {
                     for (int e = 0; e < 4; ++e) dp[4 * q + e] = dq[e];
                 }
             }
+            half8 qf[kAhead + 1][NP], gf[kAhead + 1][NP];
+            auto rows = [&](int i) {
+                Q.template row_frag<st>(places, t, i, qf[i & kAhead]);
+                G.template row_frag<st>(places, t, i, gf[i & kAhead]);
+            };
+            if (kAhead) rows(0);
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                half8 qf[NP], gf[NP];
-                Q.template row_frag<st>(places, t, i, qf);
-                G.template row_frag<st>(places, t, i, gf);
-                s = mma<NP>(qf, kf[i], s);
-                dp = mma<NP>(gf, vf[i], dp);
+                if (i + kAhead < 4) rows(i + kAhead);
+                if (kAhead) __builtin_amdgcn_sched_barrier(0);
+                s = mma<NP>(qf[i & kAhead], kf[i], s);
+                dp = mma<NP>(gf[i & kAhead], vf[i], dp);
             }
         };
         auto weights = [&](uint32_t j, int t, auto ST) {
@@ -853,22 +883,25 @@ __global__ __launch_bounds__(256, 2) void attn_bwd_k_kernel(BwdArgs a) {
             for (int r = 0; r < 16; ++r) ds[r] = p[r] * dp[r];
 #pragma unroll
             for (int sp = 0; sp < 2; ++sp) {
-                operand<NP>(p, sp, pf[sp]);
-                operand<NP>(ds, sp, df[sp]);
+                operand<NP>(p, sp, pf[sp], neg1);
+                operand<NP>(ds, sp, df[sp], neg1);
             }
         };
         auto products = [&](int t, auto ST) {
             constexpr int st = decltype(ST)::value;
+            half8 gt[kAhead + 1][NP], qt[kAhead + 1][NP];
+            auto columns = [&](int n) {
+                G.template col_frag<st>(places, t, n >> 1, n & 1, gt[n & kAhead]);
+                Q.template col_frag<st>(places, t, n >> 1, n & 1, qt[n & kAhead]);
+            };
+            if (kAhead) columns(0);
 #pragma unroll
-            for (int sp = 0; sp < 2; ++sp)
-#pragma unroll
-                for (int u = 0; u < 2; ++u) {
-                    half8 gt[NP], qt[NP];
-                    G.template col_frag<st>(places, t, sp, u, gt);
-                    Q.template col_frag<st>(places, t, sp, u, qt);
-                    dv[u] = mma<NP>(gt, pf[sp], dv[u]);
-                    dk[u] = mma<NP>(qt, df[sp], dk[u]);
-                }
+            for (int n = 0; n < 4; ++n) {
+                if (n + kAhead < 4) columns(n + kAhead);
+                if (kAhead) __builtin_amdgcn_sched_barrier(0);
+                dv[n & 1] = mma<NP>(gt[n & kAhead], pf[n >> 1], dv[n & 1]);
+                dk[n & 1] = mma<NP>(qt[n & kAhead], df[n >> 1], dk[n & 1]);
+            }
         };
         auto tile = [&](uint32_t j, auto ST) {
             // one half's values live at a time (the scores of one half between the exponentials of the other: 225 us
@@ -918,7 +951,7 @@ template <typename T>
 __global__ __launch_bounds__(256) void attn_bwd_k_merge_kernel(BwdArgs a) {
     typedef T T4 __attribute__((ext_vector_type(4)));
     const uint32_t id = blockIdx.x / 8, bh = id / a.kd.nb, kb = id % a.kd.nb;
-    const Parts<true> ps(a.kd, a.causal != 0, a.batch * a.heads, bh, kb);
+    const Parts<true> ps(a.kd, a.causal != 0, bh, kb);
     const int r = static_cast<int>(blockIdx.x % 8) * 16 + static_cast<int>(threadIdx.x >> 4), d = (threadIdx.x & 15) * 4;
     const uint32_t kj = kb * kB + r;
     if (ps.w0 == ps.w1 || kj >= a.Tk || d >= static_cast<int>(a.ohd)) return;
@@ -966,13 +999,16 @@ __global__ __launch_bounds__(256) void attn_bwd_zero_kernel(BwdArgs a) {
 // ---- plan -----------------------------------------------------------------------------------------------------------
 
 constexpr uint32_t kSlots = 512;     // workgroups resident at once: two per CU
-constexpr uint32_t kMinShare = 4;    // tiles of a share, at least, where blocks are shared
+// Tiles of a share, at least, where blocks are shared. us with 4 / 2 / 1: fp16 2x20x1024x77 33.8 / 36.9 / 55, 2x20x256^2
+// 23.8 / 34.3 / 42, fp32 2x20x1024x77 60.0 / 61.5 / 82 (and with 3: 38.4, 44, 63.6): smaller shares are mostly first loads, and
+// their parts are written, read back and added.
+constexpr uint32_t kMinShare = 4;
 
 // Whole blocks, a workgroup each, where they fill rounds of kSlots well enough; else kSlots workgroups, or as many as get
 // kMinShare tiles.
 template <bool KEYS>
 Deal deal(uint32_t bhs, uint32_t T, uint32_t Tother, bool causal) {
-    Deal d;
+    Deal d{};
     d.NT = std::max(1u, ceil_div(Tother, kTile));
     d.nb = ceil_div(T, kB);
     d.per = before<KEYS>(d.nb, d.NT, causal);
@@ -981,11 +1017,22 @@ Deal deal(uint32_t bhs, uint32_t T, uint32_t Tother, bool causal) {
     d.wgs = blocks;
     const bool alike = d.per == d.nb * d.NT;  // all blocks have NT tiles
     d.whole = alike ? 1 : 0;
+    if (total >= 1ull << 31) {  // (the tiles are counted in 32 bits; the last of so many rounds matters little)
+        d.wgs = blocks;
+        d.whole = 1;
+        return d;
+    }
     const uint64_t rounds = (blocks + kSlots - 1) / kSlots;
     const uint32_t shares = static_cast<uint32_t>(std::max<uint64_t>(1, std::min<uint64_t>(kSlots, total / kMinShare)));
     if (blocks && blocks < rounds * kSlots * 9 / 10 && (blocks > kSlots || shares > blocks)) {
         d.wgs = shares;
         d.whole = alike ? blocks / shares : 0;
+    }
+    if (d.wgs) {
+        const uint32_t shared = static_cast<uint32_t>(total) - dealt_whole(d) * d.NT;
+        d.quo = shared / d.wgs;
+        d.rem = shared % d.wgs;
+        d.frac = static_cast<uint32_t>(((static_cast<uint64_t>(d.rem) << 32) + d.wgs - 1) / d.wgs);
     }
     return d;
 }
