@@ -156,12 +156,13 @@ __global__ __launch_bounds__(WM * WN * 64) void gemm_q8_bwd_kernel(BwdArgs a) {
         const uint32_t row = (tid + i * NT) >> 3;
         a_off[i] = row < rows ? row * a.ldc * sizeof(T) : kPast;
     }
-    // W: thread u handles part u / W_BLOCKS of block u % W_BLOCKS: row n = block / KB, column block % KB. 64 (32) rows
+    // W: thread u handles part u % PARTS of block u / PARTS: row n = block / KB, column block % KB (a wave writes runs of
+    // whole rows to LDS; parts a wave apart, four lanes met in a bank: 2048x1280x5120 fp16 51.0 us, now 45.8). 64 (32) rows
     // of 34 * K / 32 bytes are a multiple of 4 bytes, so a thread's place in its dwords is the same every step.
     uint32_t w_off[W_IT], w_n[W_IT], w_sel[W_IT], w_d[W_IT];
 #pragma unroll
     for (int i = 0; i < W_IT; ++i) {
-        const uint32_t u = tid + i * NT, blk = u % W_BLOCKS, pt = u / W_BLOCKS;
+        const uint32_t u = tid + i * NT, blk = u / PARTS, pt = u % PARTS;
         w_n[i] = blk / KB;
         const uint32_t byte = w_n[i] * a.rowbytes + min(k0 / 32 + blk % KB, a.K / 32 - 1) * 34;
         const uint32_t q = byte + 2 + pt * (QD * 4);
@@ -260,7 +261,7 @@ __global__ __launch_bounds__(WM * WN * 64) void gemm_q8_bwd_kernel(BwdArgs a) {
         }
 #pragma unroll
         for (int i = 0; i < W_IT; ++i) {
-            const int u = tid + i * NT, blk = u % W_BLOCKS, pt = u / W_BLOCKS;
+            const int u = tid + i * NT, blk = u / PARTS, pt = u % PARTS;
             _Float16* dst = Ws + (blk / KB) * LDW + (blk % KB) * 32 + pt * (QD * 4);
             const _Float16 d = __builtin_bit_cast(_Float16, static_cast<uint16_t>(wd[rs][i]));
             uint32_t q[QD];
