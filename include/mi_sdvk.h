@@ -80,8 +80,9 @@ int mi_version(void);
  *                       instead of whole rows through LDS
  *   "attn_simd_waves"   "2" | "3": fp16 attention build of 2 or 3 waves per
  *                       SIMD (fp16-precision, non-causal, 4-wave launches)
- *   "gemm_bwd_cfg"      "<build 0..2>[:<N parts>]" (input-gradient GEMM tile
- *                       build; the parts apply to calls with a workspace)
+ *   "gemm_bwd_cfg"      "<build 0..3>[:<N parts>]" (input-gradient GEMM tile
+ *                       build; 3 is fp32 only and runs as 0 for fp16; the
+ *                       parts apply to calls with a workspace)
  * MI_ERR_INVALID_ARG for an unknown name or a malformed value. Not
  * synchronised with calls in flight on other threads.                      */
 int mi_tuning_set(const char* name, const char* value);

@@ -32,7 +32,7 @@ int check_launch(const char* what);
 // sizes only: no override changes an operator's arithmetic beyond the
 // summation order of a different plan.
 constexpr int kGemmBuilds = 7;  // tile builds of gemm_q8.hip (kNumCfg)
-constexpr int kGemmBwdBuilds = 3;  // tile builds of gemm_q8_bwd.hip
+constexpr int kGemmBwdBuilds = 4;  // tile builds of gemm_q8_bwd.hip
 struct Tuning {
     std::atomic<int> gemm_cfg{-1};          // tile build, or -1
     std::atomic<int> gemm_splits{1};        // K splits with gemm_cfg (workspace entries)

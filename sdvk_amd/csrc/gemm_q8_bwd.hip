@@ -450,8 +450,8 @@ __global__ __launch_bounds__(256) void gemm_q8_bwd_zero_kernel(T* dA, uint32_t M
 
 constexpr uint32_t kCUs = 256;
 
-enum BuildId { k256x128 = 0, k128x128 = 1, k64x64 = 2, kFew = 3 };
-static_assert(k64x64 + 1 == kGemmBwdBuilds, "mi_tuning_set bounds gemm_bwd_cfg by kGemmBwdBuilds");
+enum BuildId { k256x128 = 0, k128x128 = 1, k64x64 = 2, k256x256 = 3, kFew = 4 };
+static_assert(k256x256 + 1 == kGemmBwdBuilds, "mi_tuning_set bounds gemm_bwd_cfg by kGemmBwdBuilds");
 
 struct Plan {
     int build;
@@ -535,16 +535,18 @@ __global__ __launch_bounds__(kFewWaves * 64) void gemm_q8_bwd_few_kernel(BwdArgs
 // What a build costs, us: `base` (launch, first loads, last stores) and a step of its workgroups with 1, 2 or 3 of them on
 // a CU (LDS allows no more of the larger tiles). Fitted to a sweep of every build and number of parts over the layers of
 // 512- to 1024-pixel images (MI355X, operands of full entropy, calls back to back); examples in us, build:parts measured
-// (256x128, 128x128, 64x64): fp16 2048x1280x5120 54.5 / 47.6 / 77.8, 8192x1920x640 38.3 / 43.4 / 46.9, 576x1280x1280
-// 26.8 / 17.9 / 10.0, 1976x10240x1280 in 3 parts 76.7 / 83.7 / 130, unsplit 2:1 143; fp32 1152x1280x1280 28.8 in 5 parts /
-// 32.5 in 2 / 38.1 in 1, 8192x5120x640 218 in 3 / 256 in 3 / 311.
+// (256x128, 128x128, 64x64, 256x256): fp16 2048x1280x5120 48.0 / 45.9 / 72.7 / 46.5, 8192x1920x640 33.1 / 40.0 / 51.3 /
+// 46.0, 576x1280x1280 16.9 / 14.4 / 9.7, 1976x10240x1280 in 3 parts 71.8 / 83.1, in 5 parts 256x256 78.6; fp32
+// 1152x1280x1280 29.0 in 5 parts / 30.3 in 2 / 34.9 / 32.9 in 8, 2048x1280x5120 142 / 130 / - / 105, 1976x10240x1280 203 in
+// 3 parts / 236 / - / 184 in 5. fp32's three products per pair of fragments gain from 256x256 tiles, fp16's one does not: it
+// has no such build.
 struct Cost {
     uint32_t bm, bk, per_cu;
     double base, step[3];
 };
 constexpr Cost kCost[2][kGemmBwdBuilds] = {
-    {{256, 128, 1, 6.0, {1.13}}, {128, 128, 2, 4.5, {0.75, 1.25}}, {64, 64, 3, 2.8, {0.36, 0.62, 0.90}}},
-    {{256, 128, 1, 7.0, {1.60}}, {128, 128, 1, 5.0, {1.08}}, {64, 64, 3, 3.0, {0.62, 0.87, 1.18}}}};
+    {{256, 128, 1, 6.0, {1.00}}, {128, 128, 2, 4.5, {0.68, 1.25}}, {64, 64, 3, 2.8, {0.35, 0.62, 0.90}}, {}},
+    {{256, 128, 1, 7.0, {1.60}}, {128, 128, 1, 5.0, {1.08}}, {64, 64, 3, 3.0, {0.62, 0.87, 1.18}}, {256, 256, 1, 9.0, {2.41}}}};
 
 double cost_us(const Cost& c, uint32_t M, uint32_t K, uint32_t steps, uint32_t splits) {
     const uint64_t wgs = static_cast<uint64_t>(ceil_div(M, c.bm)) * ceil_div(K, c.bk) * splits;
@@ -574,7 +576,7 @@ Plan choose(uint32_t M, uint32_t N, uint32_t K, bool f32, bool allow_split) {
         best = Plan{kFew, 1};
         best_us = 4.0 + N * (0.0013 + 0.00025 * M);
     }
-    for (int b = 0; b < kGemmBwdBuilds; ++b)
+    for (int b = 0; b < (f32 ? kGemmBwdBuilds : kGemmBwdBuilds - 1); ++b)
         for (uint32_t splits : {1u, 2u, 3u, 4u, 5u, 8u, 12u, 16u}) {
             if (splits > 1 && (!allow_split || launched_splits(N, f32, splits) != splits)) continue;
             const double us = cost_us(kCost[f32][b], M, K, ceil_div(N, n_step(f32)), splits);
@@ -610,7 +612,8 @@ template <typename T>
 void launch(const BwdArgs& a, const Plan& p, bool any, hipStream_t s) {
     if (p.build == kFew) launch_few<T>(a, s);
     else if (any) launch_build<T, 64, 64, 2, 2, true>(a, p.splits, s);
-    else if (p.build == k256x128) launch_build<T, 256, 128, 4, 2, false>(a, p.splits, s);
+    else if (sizeof(T) == 4 && p.build == k256x256) launch_build<float, 256, 256, 4, 2, false>(a, p.splits, s);
+    else if (p.build == k256x128 || p.build == k256x256) launch_build<T, 256, 128, 4, 2, false>(a, p.splits, s);
     else if (p.build == k128x128) launch_build<T, 128, 128, 4, 2, false>(a, p.splits, s);
     else launch_build<T, 64, 64, 2, 2, false>(a, p.splits, s);
     if (!a.part) return;

@@ -496,6 +496,7 @@ CASES = {
         dict(typ="f16", M=150, N=200, K=288, cfg="1:3"), dict(typ="f32", M=150, N=100, K=160, cfg="1:2"),
         dict(typ="f16", M=150, N=200, K=160, cfg="2:2"), dict(typ="f32", M=70, N=100, K=96, cfg="2:3", mode=1),
         dict(typ="f16", M=260, N=64, K=160, cfg="0", lda=161), dict(typ="f32", M=130, N=96, K=160, cfg="1", ws=False),
+        dict(typ="f32", M=300, N=100, K=288, cfg="3:2"), dict(typ="f32", M=260, N=100, K=320, cfg="3", mode=1), dict(typ="f32", M=200, N=320, K=96, cfg="3", ramp=True),
         dict(typ="f32", M=260, N=320, K=160, cfg="0", ramp=True), dict(typ="f32", M=130, N=320, K=160, cfg="1", ramp=True),
     ],
     "geglu": [
