@@ -55,7 +55,7 @@ constexpr int kB = 128;                  // queries (keys) per block
 constexpr int kTile = 64;                // keys (queries) per staged tile
 // A row's reference m rises when a lane's sum of exp2(s - m) passes 2^kLazy; kRowExp is the power of two that a row's
 // largest |dO| is taken to in dS: exp2(s - m) (dP - delta) stays in fp16's range for |V| up to 32 even where 64 products
-// agree in sign. A pair's low part is a subnormal number where dS is small, so fp32 takes it larger and rescales more often.
+// agree in sign; where it would not, m rises further. A pair's low part is a subnormal number where dS is small, so fp32 takes it larger and rescales more often.
 template <int NP>
 constexpr int kLazy = NP == 2 ? 2 : 8;
 template <int NP>
@@ -602,8 +602,26 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 ? 2 : 3) void attn_bwd_q_kernel
                     }
                 }
                 l += ts;
+                float big = 0.0f;
 #pragma unroll
-                for (int r = 0; r < 16; ++r) p[r] *= dp[r] - dl;
+                for (int r = 0; r < 16; ++r) {
+                    p[r] *= dp[r] - dl;
+                    big = fmaxf(big, fabsf(p[r]));
+                }
+                // large values of V: the reference rises until the row's dS is under 2^15 (at 2^13 or more)
+                if (__any(big > 32768.0f)) {
+                    const float most = fmaxf(big, __shfl_xor(big, 32));
+                    const int k = max(0, min(exponent(most), 100) - 13);
+                    const float alpha = ldexpf(1.0f, -k);
+                    m += static_cast<float>(k);
+                    l *= alpha;
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) {
+                        acc[0][r] *= alpha;
+                        acc[1][r] *= alpha;
+                        p[r] *= alpha;
+                    }
+                }
                 half8 df[2][NP], kt[kAhead + 1][NP];
                 auto columns = [&](int n) { K.template col_frag<st>(places, t, n >> 1, n & 1, kt[n & kAhead]); };
                 if (kAhead) columns(0);

@@ -332,11 +332,12 @@ def attn_head(q, k, v, do, scale, seen, typ, o_stored):
     adP = ag @ av.T
     # P and dS as operands: fp16 rounds them (H), a pair leaves 2^-22; not less than 2^-25 of what they are held at:
     # P 2^14; dS in the key kernel 2^14 over the head's bound of |dP - delta|, to within a factor of two; in the query
-    # kernel exp2(s - m) (l is 1 at least) with the row's largest |dO| at 2^-4 (fp16) or 2^2 (fp32)
+    # kernel exp2(s - m) (l is 1 at least) with the row's largest |dO| at 2^-4 (fp16) or 2^2 (fp32), or, where the row's dS
+    # would pass 2^15 there, with its largest (|dP - delta| at most) at 2^13 or more
     r = H * 1.01 if f16 else 2.0 ** -22
     fP = TINY16 * 2.0 ** -14
     fK = TINY16 * 2.0 ** -13 * (64 * gm * av.max(initial=0.0) + np.abs(delta).max(initial=0.0))
-    fQ = TINY16 * gr * (2.0 ** 4 if f16 else 2.0 ** -2)
+    fQ = TINY16 * (gr * (2.0 ** 4 if f16 else 2.0 ** -2) + 2.0 ** -13 * np.abs(dP - true_delta).max(1, keepdims=True, initial=0.0))
     chain = (T + 64) * U + pair
 
     def d_score(gfloor, floor):
@@ -354,7 +355,7 @@ def attn_head(q, k, v, do, scale, seen, typ, o_stored):
 
 
 def attention(be, *, typ, batch=1, Tq, Tk, heads=1, hd=64, causal=False, lens=None, scale=0.0, gap=0, off=0, joint=False, gstd=None,
-              grow=False, peak=1.0, seed=5, poison=False, norm_check=True):
+              grow=False, peak=1.0, vsize=0.0, seed=5, poison=False, norm_check=True):
     rng = rng_of(seed)
     dt, esz, C = DT[typ], np.dtype(DT[typ]).itemsize, heads * hd
     ld = 3 * C if joint else C + gap
@@ -365,6 +366,9 @@ def attention(be, *, typ, batch=1, Tq, Tk, heads=1, hd=64, causal=False, lens=No
         return x
 
     q, k, v, do = tensor(Tq, peak), tensor(Tk), tensor(Tk), tensor(Tq, std)
+    if vsize:  # values of this size, each key's of one sign, and the gradients of one: no product cancels another
+        v = (np.sign(rng.standard_normal((batch, Tk, 1))) * np.abs(f64(v)) * vsize).astype(dt)
+        do = np.abs(do)
     if grow:  # queries' gradients from 1e-6 to 1e2 of std, some zero
         do = (f64(do) * 10.0 ** rng.uniform(-3 if typ == "f16" else -6, 2, (batch, Tq, 1))).astype(dt)
         do[:, ::7] = 0
@@ -470,6 +474,8 @@ CASES = {
         dict(typ="f16", Tq=40, Tk=70, scale=-0.2), dict(typ="f32", Tq=40, Tk=70, scale=-0.2), dict(typ="f16", Tq=40, Tk=140, peak=30.0),
         dict(typ="f32", Tq=40, Tk=140, peak=30.0), dict(typ="f16", Tq=140, Tk=70, grow=True), dict(typ="f32", Tq=140, Tk=70, grow=True),
         dict(typ="f32", Tq=40, Tk=70, gstd=1e-20), dict(typ="f32", Tq=40, Tk=70, gstd=1e10), dict(typ="f16", Tq=40, Tk=70, gstd=2.0 ** -20, norm_check=False),
+        dict(typ="f16", Tq=70, Tk=150, vsize=2000.0, gstd=0.01, norm_check=False), dict(typ="f32", Tq=70, Tk=150, vsize=2000.0, norm_check=False),
+        dict(typ="f16", Tq=40, Tk=70, vsize=100.0, causal=True, peak=5.0, gstd=0.1, norm_check=False),
         dict(typ="f16", Tq=40, Tk=70, gstd=0.0), dict(typ="f32", Tq=0, Tk=5), dict(typ="f16", Tq=5, Tk=0),
         # parts of the queries
         dict(typ="f16", Tq=300, Tk=40, heads=2), dict(typ="f32", Tq=260, Tk=140), dict(typ="f16", Tq=300, Tk=140, causal=True),
