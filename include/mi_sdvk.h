@@ -552,7 +552,7 @@ int mi_geglu_bwd(const float* h, const void* dy, void* dh, int dtype, uint32_t r
  * stream; dx may be res itself, and overlaps nothing else. dgamma and dbeta both NULL
  * or both set; set, they need `workspace` of mi_layernorm_bwd_ws_bytes(rows, d) bytes,
  * 16-byte aligned, disjoint from the tensors (rows added in a fixed order). rows <=
- * 2^31; any d; d % 4 == 0, d <= 4096 and 16-byte aligned tensors (8-byte for an fp16
+ * 2^31, d <= 2^30; d % 4 == 0, d <= 4096 and 16-byte aligned tensors (8-byte for an fp16
  * dy) is the fast path. rows == 0 stores zeros in dgamma and dbeta.          */
 uint64_t mi_layernorm_bwd_ws_bytes(uint32_t rows, uint32_t d);
 int mi_layernorm_bwd(const float* x, const float* gamma, const void* dy, int dy_dtype, const float* res, float* dx,

@@ -26,6 +26,7 @@ namespace {
 constexpr uint32_t kMaxParts = 512;  // partial rows of dgamma / dbeta: two workgroups per CU
 constexpr int kColRows = 64;         // rows per workgroup of the general column sums, at least
 constexpr uint32_t kMaxRows = 1u << 31;
+constexpr uint32_t kMaxCols = 1u << 30;  // 2 d columns of sums and a stride of 64 are counted in 32 bits
 constexpr uint32_t kMaxGrid = 1u << 20;  // workgroups of a launch that strides over rows
 
 // The wave's sum in every lane, the same bits in each (glue.hip's order: quads, half rows, rows, halves).
@@ -347,7 +348,7 @@ extern "C" int mi_layernorm_bwd(const float* x, const float* gamma, const void* 
     if (dy_dtype != MI_F32 && dy_dtype != MI_F16) return fail(MI_ERR_INVALID_ARG, "%s: dy_dtype %d", fn, dy_dtype);
     if ((dgamma == nullptr) != (dbeta == nullptr)) return fail(MI_ERR_INVALID_ARG, "%s: dgamma and dbeta go together", fn);
     if (d == 0) return fail(MI_ERR_INVALID_ARG, "%s: d == 0", fn);
-    if (rows > kMaxRows) return fail(MI_ERR_UNSUPPORTED, "%s: rows %u > 2^31", fn, rows);
+    if (rows > kMaxRows || d > kMaxCols) return fail(MI_ERR_UNSUPPORTED, "%s: rows %u > 2^31 or d %u > 2^30", fn, rows, d);
     const uint64_t ey = dy_dtype == MI_F16 ? 2 : 4;
     if (!aligned(x, 4) || !aligned(gamma, 4) || !aligned(dy, ey) || !aligned(res, 4) || !aligned(dx, 4) ||
         !aligned(dgamma, 4) || !aligned(dbeta, 4))

@@ -77,6 +77,7 @@ def test_layernorm(lib):
     for bad in (dict(x=None), dict(dy=None), dict(dx=None), dict(dt=5), dict(dg=None), dict(db=None), dict(d=0), dict(ws=None), dict(ws_bytes=64)):
         assert call(**bad) == _lib.MI_ERR_INVALID_ARG, bad
     assert call(rows=(1 << 31) + 1, d=1) == _lib.MI_ERR_UNSUPPORTED
+    assert call(rows=1, d=(1 << 30) + 1) == _lib.MI_ERR_UNSUPPORTED  # the columns are counted in 32 bits
     for bad in (dict(x=addr(0) + 2), dict(gamma=addr(1) + 2), dict(dy=addr(2) + 1, dt=1), dict(dx=addr(4) + 2), dict(res=addr(3) + 1),
                 dict(dg=addr(5) + 2), dict(ws=addr(7) + 8)):
         assert call(**bad) == _lib.MI_ERR_ALIGNMENT, bad
