@@ -480,7 +480,7 @@ int mi_sdxl_block_forward_kv(const mi_block_weights* w, const mi_block_dims* dim
  * fwd: the forward call's arguments (out is read; precision is ignored). All tensors of
  * one dtype: out_dtype == in_dtype, MI_F32 or MI_F16, and so dout, dq, dk, dv. The masks
  * are the forward's: a query that sees no key gets dq = 0 and gives nothing to dk and
- * dv; keys at or past kv_len[b] get dk = dv = 0, and their k and v are not read. Token
+ * dv; keys at or past kv_len[b] get dk = dv = 0, whatever their k and v hold. Token
  * strides 0 -> C (each < 2^22 elements), batch strides 0 -> T * ld; the batch rows of an
  * output must not overlap. dq, dk and dv overlap no input and not each other, but may be
  * column blocks of one [rows, 3C] matrix (equal strides). Tensors aligned to their
