@@ -15,7 +15,7 @@
 //
 // Measured (MI355X): LayerNorm 8192 x 640 fp32 with res 16.2 us (84 MB: 5.2 TB/s, what a copy of that size reaches in the
 // last-level cache) and 3.9 us for the sum of the partial rows; 77 x 768 with an fp16 dy 4.8 and 2.7 us (latency). GEGLU
-// 2048 x 5120 fp32 30.8 us alone, 39.7 us one call behind the other (210 MB: 5.3 TB/s).
+// 2048 x 5120 fp32 30.8 us alone, 40.0 us one call behind the other (210 MB: 5.3 TB/s).
 #include "common.hpp"
 
 #include <algorithm>
