@@ -1,0 +1,98 @@
+"""Backward operators on tensors whose rows and batches lie more than 4 GiB apart: the bits of the same data packed."""
+import numpy as np
+import pytest
+
+import bwd_ref
+from sdvk_amd import ops
+from sdvk_amd.hip import DeviceBuffer, synchronize
+
+pytestmark = pytest.mark.gpu
+
+H = np.float16
+
+
+@pytest.fixture(autouse=True)
+def plans(gpu):
+    ops.tuning_reset()
+
+
+def test_attention_batches(gpu):
+    """fp16 inputs in one allocation, the second batch 4.3 GB behind the first; gradients far apart too."""
+    print("[case] attention, batch stride 2^31 + 64 elements", flush=True)
+    B, T, C, heads, s = 2, 150, 128, 2, (1 << 31) + 64
+    r = bwd_ref.rng_of(41)
+    x = [(r.standard_normal((B, T, C)) * f).astype(H) for f in (1, 1, 1, 1, 0.1)]
+    ws = DeviceBuffer(ops.fused_attention_bwd_ws_bytes(batch=B, Tq=T, Tk=T, C=C, heads=heads, dtype=ops.MI_F16))
+    near = [DeviceBuffer.from_array(a.reshape(-1)) for a in x]
+    out = [DeviceBuffer.from_array(np.full(B * T * C, 7, H)) for _ in range(3)]
+    kw = dict(batch=B, Tq=T, Tk=T, C=C, heads=heads, dtype=ops.MI_F16)
+    ops.fused_attention_bwd(*near, *out, ws, **kw)
+    synchronize()
+    want = [b.download(H, B * T * C).reshape(B, T, C) for b in out]
+    assert all(np.all(np.isfinite(w)) and np.any(w) for w in want)
+
+    step = T * C * 2
+    far = DeviceBuffer((s * 2) + 5 * step)
+    for i, a in enumerate(x):
+        for b in range(B):
+            far.upload(a[b].reshape(-1), offset=i * step + b * s * 2)
+    grads = DeviceBuffer(s * 2 + step)
+    small = [DeviceBuffer.from_array(np.full(B * T * C, 7, H)) for _ in range(2)]
+    strides = dict(sq=s, sk=s, sv=s, so=s, sdout=s)
+    for n in range(3):  # each gradient far apart once
+        d = [small[0], small[1]]
+        d.insert(n, grads)
+        ops.fused_attention_bwd(*(far.value + i * step for i in range(5)), *d, ws, **kw, **strides, **{"sd" + "qkv"[n]: s})
+        synchronize()
+        for b in range(B):
+            got = grads.download(H, T * C, offset=b * s * 2).reshape(T, C)
+            assert np.array_equal(got.view(np.uint16), want[n][b].view(np.uint16)), ("qkv"[n], b)
+
+
+@pytest.mark.parametrize("typ", ["f16", "f32"])
+def test_linear_rows(gpu, typ):
+    """Rows of dC and dA a few MB apart, the last ones past 4 GiB."""
+    print(f"[case] linear {typ}, row strides of 2^21 elements and more", flush=True)
+    dt, code = bwd_ref.DT[typ], bwd_ref.CODE[typ]
+    e = np.dtype(dt).itemsize
+    ld = (1 << 22) // e * 2 - 8
+    M, N, K = (1 << 32) // (ld * e) + 40, 72, 96
+    r = bwd_ref.rng_of(42)
+    c = (r.standard_normal((M, N)) * 0.1).astype(dt)
+    raw, _ = bwd_ref.q8_blocks(r.standard_normal((N, K)) * 0.05)
+    W, near = DeviceBuffer.from_array(raw), DeviceBuffer.from_array(c.reshape(-1))
+    out = DeviceBuffer.from_array(np.full(M * K, 7, dt))
+    ops.gemm_nt_q8_0_bwd(near, W, out, M, N, K, dtype=code)
+    synchronize()
+    want = out.download(dt, M * K).reshape(M, K)
+    assert np.all(np.isfinite(want)) and np.any(want)
+    far, res = DeviceBuffer(M * ld * e), DeviceBuffer(M * ld * e)
+    for m in range(M):
+        far.upload(c[m], offset=m * ld * e)
+    ops.gemm_nt_q8_0_bwd(far, W, res, M, N, K, dtype=code, ldc=ld, lda=ld)
+    synchronize()
+    got = np.stack([res.download(dt, K, offset=m * ld * e) for m in range(M)])
+    assert np.array_equal(got.view(np.uint8), want.view(np.uint8))
+
+
+def test_geglu_gemm_rows(gpu):
+    """Rows of dG and dH a few MB apart, the last ones past 4 GiB."""
+    print("[case] geglu_gemm, row strides of 2^21 - 8 elements", flush=True)
+    ld, F, K = (1 << 21) - 8, 40, 64
+    M = (1 << 32) // (ld * 2) + 40
+    r = bwd_ref.rng_of(43)
+    a, g = r.standard_normal((M, K)).astype(H), (r.standard_normal((M, F)) * 0.1).astype(H)
+    raw, _ = bwd_ref.q8_blocks(r.standard_normal((2 * F, K)) * 0.05)
+    A, W, near = DeviceBuffer.from_array(a.reshape(-1)), DeviceBuffer.from_array(raw), DeviceBuffer.from_array(g.reshape(-1))
+    out = DeviceBuffer.from_array(np.full(M * 2 * F, 7, H))
+    ops.gemm_nt_q8_0_geglu_bwd(A, W, near, out, M, F, K)
+    synchronize()
+    want = out.download(H, M * 2 * F).reshape(M, 2 * F)
+    assert np.all(np.isfinite(want)) and np.any(want)
+    far, res = DeviceBuffer(M * ld * 2), DeviceBuffer(M * ld * 2)
+    for m in range(M):
+        far.upload(g[m], offset=m * ld * 2)
+    ops.gemm_nt_q8_0_geglu_bwd(A, W, far, res, M, F, K, lddg=ld, lddh=ld)
+    synchronize()
+    got = np.stack([res.download(H, 2 * F, offset=m * ld * 2) for m in range(M)])
+    assert np.array_equal(got.view(np.uint16), want.view(np.uint16))
