@@ -154,7 +154,7 @@ struct Pieces {
         id = w * d.whole;
         blocks = d.whole;
         base = at = end = 0;
-        if (d.quo) {
+        if (d.quo | d.rem) {
             const uint32_t skip = dealt_whole(d) * d.NT;
             base = at = skip + share_start(d, w);
             end = skip + share_start(d, w + 1);

@@ -478,7 +478,7 @@ CASES = {
         dict(typ="f16", Tq=40, Tk=70, vsize=100.0, causal=True, peak=5.0, gstd=0.1, norm_check=False),
         dict(typ="f16", Tq=40, Tk=70, gstd=0.0), dict(typ="f32", Tq=0, Tk=5), dict(typ="f16", Tq=5, Tk=0),
         # parts of the queries
-        dict(typ="f16", Tq=300, Tk=40, heads=2), dict(typ="f32", Tq=260, Tk=140), dict(typ="f16", Tq=300, Tk=140, causal=True),
+        dict(typ="f16", batch=541, Tq=3, Tk=5, hd=8), dict(typ="f16", Tq=300, Tk=40, heads=2), dict(typ="f32", Tq=260, Tk=140), dict(typ="f16", Tq=300, Tk=140, causal=True),
     ],
     "linear": [
         dict(typ="f16", M=1, N=1, K=32), dict(typ="f32", M=1, N=1, K=32), dict(typ="f16", M=3, N=8, K=96),
@@ -527,6 +527,9 @@ CASES = {
 # Larger shapes, on the GPU alone: grids that stride over rows, splits as the rules choose them, tails.
 GPU_CASES = {
     "attention": [
+        # more than 512 blocks of few tiles, not a multiple of the workgroups
+        dict(typ="f32", batch=7, heads=11, Tq=800, Tk=77, hd=8), dict(typ="f16", batch=7, heads=11, Tq=800, Tk=40, hd=8),
+        dict(typ="f16", batch=11, heads=7, Tq=77, Tk=1000, hd=16, causal=True),
         dict(typ="f16", Tq=1024, Tk=1024, heads=4, batch=2), dict(typ="f16", Tq=1024, Tk=77, heads=20, batch=2, lens=[77, 30]),
         dict(typ="f32", Tq=900, Tk=900, heads=4), dict(typ="f32", Tq=1000, Tk=154, heads=5, batch=2, lens=[154, 100]), dict(typ="f16", Tq=2000, Tk=2000, heads=2),
         dict(typ="f16", Tq=1500, Tk=1500, heads=2, causal=True), dict(typ="f32", Tq=1100, Tk=1100, heads=2, causal=True), dict(typ="f32", Tq=77, Tk=77, heads=12, causal=True),
