@@ -78,7 +78,7 @@ struct Operand {
 // `per` tiles to those. Each of wgs workgroups takes `whole` blocks, and an equal share of the tiles of the blocks left.
 struct Deal {
     uint32_t NT, nb, per, wgs, whole;
-    uint32_t quo, rem, frac;  // the tiles dealt in shares are quo * wgs + rem (share_start)
+    uint32_t quo, rem, frac;  // the tiles dealt in shares are quo * wgs + rem (share_start), none or quo > 0
 };
 struct BwdArgs {
     Tensor q, k, v, o, g;     // g: dO
@@ -154,7 +154,7 @@ struct Pieces {
         id = w * d.whole;
         blocks = d.whole;
         base = at = end = 0;
-        if (d.quo | d.rem) {
+        if (d.quo) {
             const uint32_t skip = dealt_whole(d) * d.NT;
             base = at = skip + share_start(d, w);
             end = skip + share_start(d, w + 1);
@@ -1051,12 +1051,16 @@ Deal deal(uint32_t bhs, uint32_t T, uint32_t Tother, bool causal) {
         d.wgs = shares;
         d.whole = alike ? blocks / shares : 0;
     }
-    if (d.wgs) {
-        const uint32_t shared = static_cast<uint32_t>(total) - dealt_whole(d) * d.NT;
-        d.quo = shared / d.wgs;
-        d.rem = shared % d.wgs;
-        d.frac = static_cast<uint32_t>(((static_cast<uint64_t>(d.rem) << 32) + d.wgs - 1) / d.wgs);
+    if (!d.wgs) return d;
+    const uint32_t shared = static_cast<uint32_t>(total) - dealt_whole(d) * d.NT;
+    if (shared && shared < d.wgs) {  // (alike: the parts of a block are of workgroups one after the other, none without a tile)
+        d.wgs = blocks;
+        d.whole = 1;
+        return d;
     }
+    d.quo = shared / d.wgs;
+    d.rem = shared % d.wgs;
+    d.frac = static_cast<uint32_t>(((static_cast<uint64_t>(d.rem) << 32) + d.wgs - 1) / d.wgs);
     return d;
 }
 // No block is shared.
