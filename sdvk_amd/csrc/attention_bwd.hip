@@ -1027,10 +1027,17 @@ constexpr uint32_t kSlots = 512;     // workgroups resident at once: two per CU
 // their parts are written, read back and added.
 constexpr uint32_t kMinShare = 4;
 
+// Tiles that sharing has to take off the longest workgroup where there are more blocks than kSlots, to be worth its parts
+// and their merge; without it the blocks of the second round start as those of the first end. us shared / whole: fp16
+// 2x10x4096x256 66.6 / 56.4 (3 tiles off the queries' kernel), x1024 126 / 119 (12), x2048 212 / 205 (24), x4096 365 / 382
+// (48), 2x18x2048^2 192 / 199 (28); fp32 2x10x4096x512 175 / 171 (6), x1024 278 / 277 (12), x2048 482 / 489 (24).
+constexpr uint32_t kMinSaved[2] = {24, 12};  // fp16, fp32
+
 // Whole blocks, a workgroup each, where they fill rounds of kSlots well enough; else kSlots workgroups, or as many as get
 // kMinShare tiles.
+
 template <bool KEYS>
-Deal deal(uint32_t bhs, uint32_t T, uint32_t Tother, bool causal) {
+Deal deal(uint32_t bhs, uint32_t T, uint32_t Tother, bool causal, bool f32) {
     Deal d{};
     d.NT = std::max(1u, ceil_div(Tother, kTile));
     d.nb = ceil_div(T, kB);
@@ -1047,7 +1054,8 @@ Deal deal(uint32_t bhs, uint32_t T, uint32_t Tother, bool causal) {
     }
     const uint64_t rounds = (blocks + kSlots - 1) / kSlots;
     const uint32_t shares = static_cast<uint32_t>(std::max<uint64_t>(1, std::min<uint64_t>(kSlots, total / kMinShare)));
-    if (blocks && blocks < rounds * kSlots * 9 / 10 && (blocks > kSlots || shares > blocks)) {
+    const bool worth = !alike || rounds * d.NT > total / kSlots + kMinSaved[f32];
+    if (blocks && blocks < rounds * kSlots * 9 / 10 && (blocks > kSlots ? worth : shares > blocks)) {
         d.wgs = shares;
         d.whole = alike ? blocks / shares : 0;
     }
@@ -1081,7 +1089,7 @@ Layout layout(uint32_t batch, uint32_t heads, uint32_t Tq, uint32_t Tk, bool pac
     uint64_t parts = 0;
     for (const bool causal : {false, true}) {
         const uint32_t n = static_cast<uint32_t>(bh);
-        const Deal qd = deal<false>(n, Tq, Tk, causal), kd = deal<true>(n, Tk, Tq, causal);
+        const Deal qd = deal<false>(n, Tq, Tk, causal, f32), kd = deal<true>(n, Tk, Tq, causal, f32);
         parts = std::max(parts, std::max<uint64_t>(all_whole(qd, n) ? 0 : 8ull * qd.wgs * kQPart, all_whole(kd, n) ? 0 : 8ull * kd.wgs * kKPart));
     }
     l.planes = l.part + (parts + 255) / 256 * 256;
@@ -1136,8 +1144,8 @@ int plan(const mi_attn_args& f, Deal& qd, Deal& kd, const char* fn) {
     const uint64_t qb = ceil_div(f.Tq, kB), kb = ceil_div(f.Tk, kB), qt = ceil_div(f.Tq, kTile) + 1, kt = ceil_div(f.Tk, kTile) + 1;
     if (bh * std::max(qb, kb) >= (1u << 20) || qb * kt >= (1u << 31) || kb * qt >= (1u << 31))
         return fail(MI_ERR_UNSUPPORTED, "%s: batch * heads * tokens too large", fn);
-    qd = deal<false>(static_cast<uint32_t>(bh), f.Tq, f.Tk, f.causal != 0);
-    kd = deal<true>(static_cast<uint32_t>(bh), f.Tk, f.Tq, f.causal != 0);
+    qd = deal<false>(static_cast<uint32_t>(bh), f.Tq, f.Tk, f.causal != 0, f.in_dtype == MI_F32);
+    kd = deal<true>(static_cast<uint32_t>(bh), f.Tk, f.Tq, f.causal != 0, f.in_dtype == MI_F32);
     return MI_OK;
 }
 

@@ -530,6 +530,8 @@ GPU_CASES = {
         # more than 512 blocks of few tiles, not a multiple of the workgroups
         dict(typ="f32", batch=7, heads=11, Tq=800, Tk=77, hd=8), dict(typ="f16", batch=7, heads=11, Tq=800, Tk=40, hd=8),
         dict(typ="f16", batch=11, heads=7, Tq=77, Tk=1000, hd=16, causal=True),
+        # more than 512 blocks, some whole and the others shared
+        dict(typ="f32", heads=77, Tq=900, Tk=1200, hd=4),
         dict(typ="f16", Tq=1024, Tk=1024, heads=4, batch=2), dict(typ="f16", Tq=1024, Tk=77, heads=20, batch=2, lens=[77, 30]),
         dict(typ="f32", Tq=900, Tk=900, heads=4), dict(typ="f32", Tq=1000, Tk=154, heads=5, batch=2, lens=[154, 100]), dict(typ="f16", Tq=2000, Tk=2000, heads=2),
         dict(typ="f16", Tq=1500, Tk=1500, heads=2, causal=True), dict(typ="f32", Tq=1100, Tk=1100, heads=2, causal=True), dict(typ="f32", Tq=77, Tk=77, heads=12, causal=True),
