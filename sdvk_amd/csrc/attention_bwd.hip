@@ -33,10 +33,12 @@
 // three MFMAs per product (hi hi + hi lo + lo hi), as in the forward pass; P and dS too. fp16's range is kept by powers
 // of two, which are exact:
 //   * in the query kernel, dS of a row by the row's largest |dO| (kRowExp), carried by exp2's argument;
-//   * in the key kernel, P by 2^14 (weights of 2^-28 are normal numbers then); dS by what keeps
-//     2^14 (64 max|dO| max|V| + max|delta|) under 2^15, max|dO| and max|delta| over the (batch, head), max|V| over the
-//     block's keys: dS cannot overflow, and a weight of 2^-20 still has all its bits. fp16: that power of two is carried
-//     by V (its largest element stays in 2^-6 .. 2^12; P's power gives way beyond that);
+//   * in the key kernel, P by 2^14 (weights of 2^-28 are normal numbers then), whatever V and dO are; dS by what keeps
+//     2^14 (|dP| + |delta|) under 2^15, for the largest |delta| of the (batch, head) and the bound of |dP| that its rows of
+//     dO and the block's of V give: fp32 64 max|dO| max|V|, fp16 the product of the largest rows' norms. dS cannot
+//     overflow, and a weight of 2^-20 still has all its bits. fp16: that power of two is carried by V, whose largest
+//     element stays in 2^-6 .. 2^12, and by dS itself beyond that, in a multiplication that only such blocks make: with the
+//     elements' bound N(0, 1) tensors made it (2x10x4096^2 fp16 357 us, with the norms 351);
 //   * dO of fp32, row by row, by its largest element, taken to 2^8.
 //
 // Measured (MI355X, us a call; a call of the kernels that its sizes take): fp16 2x10x4096^2 hd 64 350 (keys 205, queries 180,
@@ -471,7 +473,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 ? 2 : 3) void attn_bwd_q_kernel
         const uint32_t L = keys_of(a, b);  // (first: what is behind it waits for it alone)
         __builtin_amdgcn_sched_barrier(0);
         half8 qf[4][NP], gf[4][NP], of[PACKED ? 1 : 4];
-        float delta = 0.0f, gmax = 0.0f;
+        float delta = 0.0f, gmax = 0.0f, gsq = 0.0f;
         int re = 0;
 #pragma unroll
         for (int s = 0; s < 4; ++s) {
@@ -508,7 +510,9 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 ? 2 : 3) void attn_bwd_q_kernel
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
                 if constexpr (!PACKED) delta = __builtin_fmaf(static_cast<float>(gf[s][0][e]), static_cast<float>(of[s][e]), delta);
-                gmax = fmaxf(gmax, fabsf(static_cast<float>(gf[s][0][e])));
+                const float x = static_cast<float>(gf[s][0][e]);
+                gmax = fmaxf(gmax, fabsf(x));
+                if constexpr (NP == 1) gsq = __builtin_fmaf(x, x, gsq);
             }
             if (a.sgn < 0.0f) {
 #pragma unroll
@@ -516,14 +520,15 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 ? 2 : 3) void attn_bwd_q_kernel
             }
         }
         gmax = fmaxf(gmax, __shfl_xor(gmax, 32));
+        if constexpr (NP == 1) gsq += __shfl_xor(gsq, 32);
         if constexpr (!PACKED) delta += __shfl_xor(delta, 32);
         // exp2(s - m) carries 2^ge; dP and delta carry 2^re
         const int ge = clamp(kRowExp<NP> - exponent(gmax), -100, 100);
         const float dl = ldexpf(delta, re);
         const float thr = ldexpf(1.0f, kLazy<NP> + ge);
         {
-            // the block's largest |dO| and |delta|, from its first part
-            const float x = wave_max(ldexpf(gmax, -re)), y = wave_max(fabsf(delta));
+            // the block's largest |dO| (fp16: row of it, in the Euclidean norm) and |delta|, from its first part
+            const float x = wave_max(NP == 1 ? sqrtf(gsq) : ldexpf(gmax, -re)), y = wave_max(fabsf(delta));
             if (lane == 0) {
                 wmax[0][wave] = x;
                 wmax[1][wave] = y;
@@ -747,7 +752,7 @@ __global__ __launch_bounds__(256, 2) void attn_bwd_k_kernel(BwdArgs a) {
     __shared__ __attribute__((aligned(16))) _Float16 qs0[St::kHalves], qs1[St::kHalves], gs0[St::kHalves], gs1[St::kHalves];
     // per stage and query: m + log2 l less P's power of two, and -delta in the unit of dP
     __shared__ __attribute__((aligned(16))) float row0[2 * kTile], row1[2 * kTile];
-    __shared__ float wmax[4];
+    __shared__ float wmax[2][4];
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int l32 = lane & 31, g = lane >> 5;
@@ -797,7 +802,7 @@ __global__ __launch_bounds__(256, 2) void attn_bwd_k_kernel(BwdArgs a) {
             if constexpr (NP == 2) rx = a.rexp[rbase + o];
         };
         load_rows(it);
-        // max|dO| and max|delta| of the (batch, head)
+        // max|dO| (fp16: the largest row's norm) and max|delta| of the (batch, head)
         float gm = 0.0f, dm = 0.0f;
         for (uint32_t i = lane; i < a.qblocks; i += 64) {
             const float* x = a.maxes + (static_cast<uint64_t>(bh) * a.qblocks + i) * 2;
@@ -808,7 +813,7 @@ __global__ __launch_bounds__(256, 2) void attn_bwd_k_kernel(BwdArgs a) {
         const uint32_t t1 = k0 < L ? tend : it;
         gm = wave_max(gm);
         dm = wave_max(dm);
-        float vm = 0.0f;
+        float vm = 0.0f, vsq = 0.0f;
 #pragma unroll
         for (int s = 0; s < 4; ++s) {
 #pragma unroll
@@ -817,21 +822,34 @@ __global__ __launch_bounds__(256, 2) void attn_bwd_k_kernel(BwdArgs a) {
                 if (a.sgn < 0.0f) kf[s][p] = -kf[s][p];
             }
 #pragma unroll
-            for (int e = 0; e < 8; ++e) vm = fmaxf(vm, fabsf(static_cast<float>(vf[s][0][e])));
+            for (int e = 0; e < 8; ++e) {
+                const float x = static_cast<float>(vf[s][0][e]);
+                vm = fmaxf(vm, fabsf(x));
+                if constexpr (NP == 1) vsq = __builtin_fmaf(x, x, vsq);
+            }
         }
         vm = wave_max(vm);
-        if (lane == 0) wmax[wave] = vm;
+        if constexpr (NP == 1) vsq = wave_max(vsq + __shfl_xor(vsq, 32));
+        if (lane == 0) {
+            wmax[0][wave] = vm;
+            wmax[1][wave] = vsq;
+        }
         __syncthreads();
-        vm = fmaxf(fmaxf(wmax[0], wmax[1]), fmaxf(wmax[2], wmax[3]));
-        // dS times 2^(pe + se) stays under 2^15. fp16: V carries 2^se, its largest element within 2^-6 .. 2^12, and P what
-        // is left. fp32: row i of dO carries 2^(e_i), P 2^(E - e_i) with E of the largest row, and the fma below the rest.
-        const int s0 = 15 - kPExp - 1 - exponent(64.0f * gm * vm + dm);
-        const int se = NP == 1 ? clamp(s0, -6 - exponent(vm), 12 - exponent(vm)) : clamp(s0, -100, 100);
-        const int pe = NP == 1 ? kPExp - max(0, se - s0) : kPExp;
+        auto largest = [&](int i) { return fmaxf(fmaxf(wmax[i][0], wmax[i][1]), fmaxf(wmax[i][2], wmax[i][3])); };
+        vm = largest(0);
+        // dS times 2^(kPExp + s0) stays under 2^15. fp16: V and delta carry 2^se (where the block has no values, delta
+        // alone), V's largest element within 2^-6 .. 2^12, and dS what is left, 2^rest, by a multiplication of its own.
+        // fp32: row i of dO carries 2^(e_i), P 2^(E - e_i) with E of the largest row, and the fma below the rest.
         const int E = NP == 2 ? clamp(kPairExp - exponent(gm), -100, 100) : 0;
+        const float bound = gm * (NP == 1 ? sqrtf(largest(1)) : 64.0f * vm) + dm;  // of |dP| and |delta|
+        const int s0 = NP == 2 || bound > 0.0f ? 15 - kPExp - 1 - exponent(bound) : 0;
+        const int sv = NP == 1 && vm > 0.0f ? clamp(s0, -6 - exponent(vm), 12 - exponent(vm)) : s0;
+        const int se = NP == 1 ? clamp(sv, -30, 30) : clamp(s0, -100, 100);
+        const int rest = NP == 1 ? clamp(s0 - se, -100, 100) : 0;
+        const float rsc = ldexpf(1.0f, rest);
         const float psc = ldexpf(1.0f, se - E);
         if constexpr (NP == 1) {
-            const float up = ldexpf(1.0f, clamp(se, -30, 30));
+            const float up = ldexpf(1.0f, se);
 #pragma unroll
             for (int s = 0; s < 4; ++s)
 #pragma unroll
@@ -839,7 +857,7 @@ __global__ __launch_bounds__(256, 2) void attn_bwd_k_kernel(BwdArgs a) {
         }
 
         auto store_rows = [&](float* r) {
-            const float v = second ? -ldexpf(rv, NP == 2 ? rx - E + se : se) : rv - static_cast<float>(pe) + static_cast<float>(NP == 2 ? rx - E : 0);
+            const float v = second ? -ldexpf(rv, NP == 2 ? rx - E + se : se) : rv - static_cast<float>(kPExp) + static_cast<float>(NP == 2 ? rx - E : 0);
             if (tid < 2 * kTile) r[tid] = v;
         };
 
@@ -904,6 +922,12 @@ __global__ __launch_bounds__(256, 2) void attn_bwd_k_kernel(BwdArgs a) {
             }
 #pragma unroll
             for (int r = 0; r < 16; ++r) ds[r] = p[r] * dp[r];
+            if constexpr (NP == 1) {
+                if (rest) {  // uniform in the workgroup
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) ds[r] *= rsc;
+                }
+            }
 #pragma unroll
             for (int sp = 0; sp < 2; ++sp) {
                 operand<NP>(p, sp, pf[sp], neg1);
@@ -953,7 +977,7 @@ __global__ __launch_bounds__(256, 2) void attn_bwd_k_kernel(BwdArgs a) {
             if (it + 1 < t1) step(it + 1, std::integral_constant<int, 1>{});
         }
         // keys past their row's length get zeros (their P is not: their scores are those of a zero key)
-        const float fv = ldexpf(1.0f, -pe - E), fk = ldexpf(a.scale, -pe - se);
+        const float fv = ldexpf(1.0f, -kPExp - E), fk = ldexpf(a.scale, -kPExp - se - rest);
         if (!in)
 #pragma unroll
             for (int r = 0; r < 16; ++r) dk[0][r] = dk[1][r] = dv[0][r] = dv[1][r] = 0.0f;

@@ -355,7 +355,7 @@ def attn_head(q, k, v, do, scale, seen, typ, o_stored):
 
 
 def attention(be, *, typ, batch=1, Tq, Tk, heads=1, hd=64, causal=False, lens=None, scale=0.0, gap=0, off=0, joint=False, gstd=None,
-              grow=False, peak=1.0, vsize=0.0, seed=5, poison=False, norm_check=True):
+              grow=False, peak=1.0, vsize=0.0, vblocks=(), seed=5, poison=False, norm_check=True):
     rng = rng_of(seed)
     dt, esz, C = DT[typ], np.dtype(DT[typ]).itemsize, heads * hd
     ld = 3 * C if joint else C + gap
@@ -369,6 +369,8 @@ def attention(be, *, typ, batch=1, Tq, Tk, heads=1, hd=64, causal=False, lens=No
     if vsize:  # values of this size, each key's of one sign, and the gradients of one: no product cancels another
         v = (np.sign(rng.standard_normal((batch, Tk, 1))) * np.abs(f64(v)) * vsize).astype(dt)
         do = np.abs(do)
+    for k0, k1, factor in vblocks:  # values of these keys times factor
+        v[:, k0:k1] = (f64(v[:, k0:k1]) * factor).astype(dt)
     if grow:  # queries' gradients from 1e-6 to 1e2 of std, some zero
         do = (f64(do) * 10.0 ** rng.uniform(-3 if typ == "f16" else -6, 2, (batch, Tq, 1))).astype(dt)
         do[:, ::7] = 0
@@ -477,6 +479,18 @@ CASES = {
         dict(typ="f16", Tq=70, Tk=150, vsize=2000.0, gstd=0.01, norm_check=False), dict(typ="f32", Tq=70, Tk=150, vsize=2000.0, norm_check=False),
         dict(typ="f16", Tq=40, Tk=70, vsize=100.0, causal=True, peak=5.0, gstd=0.1, norm_check=False),
         dict(typ="f16", Tq=40, Tk=70, gstd=0.0), dict(typ="f32", Tq=0, Tk=5), dict(typ="f16", Tq=5, Tk=0),
+        # blocks of 128 keys whose values are all zero, next to others: whole, one key, packed, causal, shared by workgroups
+        *(dict(typ=t, norm_check=False, **c) for t in ("f16", "f32") for c in (
+            dict(Tq=40, Tk=150, vblocks=[[128, 150, 0.0]]), dict(Tq=64, Tk=129, vblocks=[[128, 129, 0.0]]),
+            dict(Tq=40, Tk=154, hd=40, off=1, vblocks=[[77, 154, 0.0]]), dict(Tq=128, Tk=256, gstd=100.0, vblocks=[[128, 256, 0.0]]),
+            dict(Tq=200, Tk=200, causal=True, heads=2, vblocks=[[128, 200, 0.0]]), dict(Tq=600, Tk=150, heads=2, vblocks=[[128, 150, 0.0]]),
+            dict(Tq=40, Tk=300, batch=2, lens=[300, 129], gstd=100.0, vblocks=[[100, 256, 0.0]], poison=True),
+            dict(Tq=40, Tk=70, vblocks=[[0, 70, 0.0]]))),
+        # large gradients on small values, so that the weights' and the scores' powers of two lie far apart
+        dict(typ="f16", Tq=40, Tk=400, gstd=3000.0, peak=6.0, norm_check=False), dict(typ="f16", Tq=128, Tk=256, gstd=8000.0, vblocks=[[128, 256, 2.0 ** -24]], norm_check=False),
+        dict(typ="f16", Tq=128, Tk=256, gstd=8000.0, vblocks=[[128, 256, 2.0 ** -20]], norm_check=False), dict(typ="f16", Tq=128, Tk=256, gstd=100.0, vblocks=[[128, 256, 1e-7]], norm_check=False),
+        dict(typ="f16", Tq=40, Tk=400, gstd=3000.0, peak=6.0, hd=40, off=1, norm_check=False), dict(typ="f16", Tq=140, Tk=140, gstd=3000.0, peak=4.0, causal=True, norm_check=False),
+        dict(typ="f16", Tq=64, Tk=70, gstd=0.5, vblocks=[[0, 70, 2.0 ** -24]], norm_check=False), dict(typ="f16", Tq=64, Tk=200, gstd=1e-6, vblocks=[[0, 128, 2.0 ** -23], [128, 200, 1e4]], norm_check=False),
         # parts of the queries
         dict(typ="f16", batch=541, Tq=3, Tk=5, hd=8), dict(typ="f16", Tq=300, Tk=40, heads=2), dict(typ="f32", Tq=260, Tk=140), dict(typ="f16", Tq=300, Tk=140, causal=True),
     ],
