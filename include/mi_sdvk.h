@@ -489,7 +489,8 @@ int mi_sdxl_block_forward_kv(const mi_block_weights* w, const mi_block_dims* dim
  * rows leave through it).
  * MI_F16: P and dS rounded to fp16 once each, scaled so that small weights and gradients
  * of any size keep their bits, fp32 sums. MI_F32: every operand as fp16 hi + lo (q, k, v
- * within fp16's range, as in the forward pass; dout of any size).
+ * within fp16's range, as in the forward pass; dout's rows with their largest element
+ * within 1e-30 .. 1e30, or zero).
  * workspace: mi_fused_attention_bwd_ws_bytes(args) bytes, 16-byte aligned, disjoint from
  * the tensors. The bytes go by sizes and dtype, and by whether the addresses and strides
  * are multiples of 16 bytes (of 4 elements, for dq, dk and dv; NULL counts as one).

@@ -839,12 +839,13 @@ __global__ __launch_bounds__(256, 2) void attn_bwd_k_kernel(BwdArgs a) {
         vm = largest(0);
         // dS times 2^(kPExp + s0) stays under 2^15. fp16: V and delta carry 2^se (where the block has no values, delta
         // alone), V's largest element within 2^-6 .. 2^12, and dS what is left, 2^rest, by a multiplication of its own.
-        // fp32: row i of dO carries 2^(e_i), P 2^(E - e_i) with E of the largest row, and the fma below the rest.
+        // fp32: row i of dO carries 2^(e_i), P 2^(E - e_i) with E of the largest row, and the fma below the rest: se
+        // is held where 2^(se - E) is finite (without values in the block, se goes by delta, E by dO).
         const int E = NP == 2 ? clamp(kPairExp - exponent(gm), -100, 100) : 0;
         const float bound = gm * (NP == 1 ? sqrtf(largest(1)) : 64.0f * vm) + dm;  // of |dP| and |delta|
-        const int s0 = NP == 2 || bound > 0.0f ? 15 - kPExp - 1 - exponent(bound) : 0;
+        const int s0 = bound > 0.0f ? 15 - kPExp - 1 - exponent(bound) : 0;
         const int sv = NP == 1 && vm > 0.0f ? clamp(s0, -6 - exponent(vm), 12 - exponent(vm)) : s0;
-        const int se = NP == 1 ? clamp(sv, -30, 30) : clamp(s0, -100, 100);
+        const int se = NP == 1 ? clamp(sv, -30, 30) : clamp(s0, -126, min(100, E + 100));
         const int rest = NP == 1 ? clamp(s0 - se, -100, 100) : 0;
         const float rsc = ldexpf(1.0f, rest);
         const float psc = ldexpf(1.0f, se - E);

@@ -486,6 +486,8 @@ CASES = {
             dict(Tq=200, Tk=200, causal=True, heads=2, vblocks=[[128, 200, 0.0]]), dict(Tq=600, Tk=150, heads=2, vblocks=[[128, 150, 0.0]]),
             dict(Tq=40, Tk=300, batch=2, lens=[300, 129], gstd=100.0, vblocks=[[100, 256, 0.0]], poison=True),
             dict(Tq=40, Tk=70, vblocks=[[0, 70, 0.0]]))),
+        dict(typ="f32", Tq=40, Tk=70, gstd=1e12, vblocks=[[0, 70, 0.0]], norm_check=False), dict(typ="f32", Tq=40, Tk=150, gstd=1e12, vblocks=[[128, 150, 0.0]], norm_check=False),
+        dict(typ="f32", Tq=40, Tk=70, gstd=2e29, vblocks=[[0, 35, 1e3]], norm_check=False), dict(typ="f32", Tq=40, Tk=70, gstd=1e-30),
         # large gradients on small values, so that the weights' and the scores' powers of two lie far apart
         dict(typ="f16", Tq=40, Tk=400, gstd=3000.0, peak=6.0, norm_check=False), dict(typ="f16", Tq=128, Tk=256, gstd=8000.0, vblocks=[[128, 256, 2.0 ** -24]], norm_check=False),
         dict(typ="f16", Tq=128, Tk=256, gstd=8000.0, vblocks=[[128, 256, 2.0 ** -20]], norm_check=False), dict(typ="f16", Tq=128, Tk=256, gstd=100.0, vblocks=[[128, 256, 1e-7]], norm_check=False),
