@@ -1156,11 +1156,13 @@ struct Span {
 };
 
 // Two outputs whose byte spans overlap without sharing an element: column blocks of one matrix (the joint Q / K / V
-// gradient [rows, 3C]), the same strides and C columns apart at least.
-bool interleaved(const Tensor& x, const Tensor& y, uint64_t C, uint64_t e) {
+// gradient [rows, 3C]), the same strides and C columns apart at least; the last row of a batch (the further block's, of Tx
+// or Ty rows) ends before the next batch begins.
+bool interleaved(const Tensor& x, const Tensor& y, uint64_t Tx, uint64_t Ty, uint64_t batch, uint64_t C, uint64_t e) {
     const uintptr_t p = reinterpret_cast<uintptr_t>(x.p), q = reinterpret_cast<uintptr_t>(y.p);
-    const uint64_t apart = (p > q ? p - q : q - p);
-    return x.ld == y.ld && x.s == y.s && apart >= C * e && apart + C * e <= x.ld * e;
+    const uint64_t apart = (p > q ? p - q : q - p), T = p > q ? Tx : Ty;
+    return x.ld == y.ld && x.s == y.s && apart >= C * e && apart + C * e <= x.ld * e &&
+           (batch == 1 || apart + ((T - 1) * x.ld + C) * e <= x.s * e);
 }
 
 // Both kernels' shares; the launches' limits.
@@ -1242,7 +1244,7 @@ int run(const mi_attn_bwd_args& x, void* ws, uint64_t ws_bytes, hipStream_t stre
     for (int o = 5; o < 8; ++o)
         for (int i = 0; i < o; ++i)
             if (overlaps(span[o].p, span[o].bytes, span[i].p, span[i].bytes) &&
-                !(i >= 5 && interleaved(*in[o].t, *in[i].t, f.C, e)))
+                !(i >= 5 && interleaved(*in[o].t, *in[i].t, in[o].T, in[i].T, f.batch, f.C, e)))
                 return fail(MI_ERR_ALIASING, "%s: %s overlaps %s", fn, in[o].name, in[i].name);
     a.batch = f.batch;
     a.Tq = f.Tq;

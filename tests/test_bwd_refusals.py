@@ -117,4 +117,19 @@ def test_attention(lib):
         assert attn(lib, **bad) == _lib.MI_ERR_ALIASING, bad
     # column blocks of one [rows, 3C] matrix may not overlap each other either
     assert attn(lib, dq=addr(5), dk=addr(5) + 128 * 2 - 2, dv=addr(5) + 512, lddq=384, lddk=384, lddv=384) == _lib.MI_ERR_ALIASING
+    # ... nor the next batch's: the last row of dk (dv) of one batch in the first of dq (dq or dk) of the next
+    joint = dict(dq=addr(5), dk=addr(5) + 256, dv=addr(5) + 512, lddq=384, lddk=384, lddv=384)
+    for s in (63 * 384 + 128, 63 * 384 + 256, 64 * 384 - 1):
+        assert attn(lib, **joint, sdq=s, sdk=s, sdv=s) == _lib.MI_ERR_ALIASING, s
+    s = 63 * 384 + 128  # dq's own rows end before the next batch; dk's begin behind dq's of the next batch
+    assert attn(lib, dq=addr(5), dk=addr(5) + 256, lddq=384, lddk=384, sdq=s, sdk=s) == _lib.MI_ERR_ALIASING
+    assert attn(lib, dq=addr(5) + 256, dk=addr(5), lddq=384, lddk=384, sdq=s, sdk=s) == _lib.MI_ERR_ALIASING
+    # of different lengths: the longer one's last row counts
+    s = 64 * 384
+    assert attn(lib, dq=addr(5) + 512, dk=addr(5), dv=addr(5) + 256, Tq=65, lddq=384, lddk=384, lddv=384, sdq=s, sdk=s, sdv=s) == _lib.MI_ERR_INVALID_ARG
+    s = 64 * 384 + 128
+    assert attn(lib, dq=addr(5), dk=addr(5) + 256, Tk=65, lddq=384, lddk=384, sdq=s, sdk=s) == _lib.MI_ERR_ALIASING
+    # what fits gets past this check, to the workspace's
+    for kw in (dict(), dict(sdq=64 * 384, sdk=64 * 384, sdv=64 * 384), dict(batch=1, sdq=1, sdk=1, sdv=1)):
+        assert attn(lib, **{**joint, **kw}, ws=None) == _lib.MI_ERR_INVALID_ARG, kw
     assert ctypes.sizeof(_lib.MiAttnBwdArgs) == ctypes.sizeof(_lib.MiAttnArgs) + 4 * 8 + 8 * 8
