@@ -27,7 +27,7 @@ constexpr uint32_t kMaxParts = 512;  // partial rows of dgamma / dbeta: two work
 constexpr int kColRows = 64;         // rows per workgroup of the general column sums, at least
 constexpr uint32_t kMaxRows = 1u << 31;
 constexpr uint32_t kMaxCols = 1u << 30;  // 2 d columns of sums and a stride of 64 are counted in 32 bits
-constexpr uint32_t kMaxGrid = 1u << 20;  // workgroups of a launch that strides over rows
+constexpr uint32_t kMaxGrid = 1u << 20;  // workgroups of a launch that strides over rows or columns (2^32 threads are refused)
 
 // The wave's sum in every lane, the same bits in each (glue.hip's order: quads, half rows, rows, halves).
 template <int CTRL>
@@ -188,57 +188,62 @@ __global__ __launch_bounds__(256) void layernorm_bwd_kernel(const float* x, cons
     }
 }
 
-// Column sums of rows [y * per, (y + 1) * per) at 64 columns: four row groups of a workgroup, added in order.
+// Column sums of rows [y * per, (y + 1) * per) at 64 columns at a time: four row groups of a workgroup, added in order.
 template <typename TD>
 __global__ __launch_bounds__(256) void layernorm_cols_kernel(const float* x, const TD* dy, const float* stats, float* part,
                                                              uint32_t rows, uint32_t d, uint32_t per) {
     __shared__ float sums[2][4][64];
     const uint32_t lane = threadIdx.x & 63, grp = threadIdx.x >> 6;
-    const uint32_t j = blockIdx.x * 64 + lane;
     const uint32_t r0 = blockIdx.y * per, r1 = min(rows, r0 + per);
-    float sg = 0.0f, sb = 0.0f;
-    if (j < d)
-        for (uint32_t r = r0 + grp; r < r1; r += 4) {
-            const uint64_t at = static_cast<uint64_t>(r) * d + j;
-            const float w = static_cast<float>(dy[at]);
-            sg += w * ((x[at] - stats[2 * static_cast<uint64_t>(r)]) * stats[2 * static_cast<uint64_t>(r) + 1]);
-            sb += w;
-        }
-    sums[0][grp][lane] = sg;
-    sums[1][grp][lane] = sb;
-    __syncthreads();
-    if (grp < 2 && j < d)
-        part[(static_cast<uint64_t>(blockIdx.y) * 2 + grp) * d + j] =
-            ((sums[grp][0][lane] + sums[grp][1][lane]) + sums[grp][2][lane]) + sums[grp][3][lane];
+    for (uint32_t j0 = blockIdx.x * 64; j0 < d; j0 += gridDim.x * 64) {
+        const uint32_t j = j0 + lane;
+        float sg = 0.0f, sb = 0.0f;
+        if (j < d)
+            for (uint32_t r = r0 + grp; r < r1; r += 4) {
+                const uint64_t at = static_cast<uint64_t>(r) * d + j;
+                const float w = static_cast<float>(dy[at]);
+                sg += w * ((x[at] - stats[2 * static_cast<uint64_t>(r)]) * stats[2 * static_cast<uint64_t>(r) + 1]);
+                sb += w;
+            }
+        sums[0][grp][lane] = sg;
+        sums[1][grp][lane] = sb;
+        __syncthreads();
+        if (grp < 2 && j < d)
+            part[(static_cast<uint64_t>(blockIdx.y) * 2 + grp) * d + j] =
+                ((sums[grp][0][lane] + sums[grp][1][lane]) + sums[grp][2][lane]) + sums[grp][3][lane];
+        __syncthreads();  // the sums are free for the next columns
+    }
 }
 
-// dgamma and dbeta from `parts` partial rows of [2][d]: 32 columns per workgroup, 32 groups of rows (g, g + 32, ...)
+// dgamma and dbeta from `parts` partial rows of [2][d]: 32 columns at a time, 32 groups of rows (g, g + 32, ...)
 // whose sums are added in a fixed tree.
 __global__ __launch_bounds__(1024) void layernorm_parts_kernel(const float* part, float* dgamma, float* dbeta,
                                                                uint32_t parts, uint32_t d) {
     __shared__ float sums[32][33];
     const uint32_t lane = threadIdx.x & 31, grp = threadIdx.x >> 5;
-    const uint32_t j = blockIdx.x * 32 + lane;
     const uint64_t width = 2ull * d;
-    float s = 0.0f;
-    if (j < width) {
-        uint32_t p = grp;
-        for (; p + 96 < parts; p += 128) {
-            const float* q = part + static_cast<uint64_t>(p) * width + j;
-            const float a = q[0], b = q[32 * width], c = q[64 * width], e = q[96 * width];
-            s += (a + b) + (c + e);
+    for (uint64_t j0 = blockIdx.x * 32ull; j0 < width; j0 += gridDim.x * 32ull) {
+        const uint64_t j = j0 + lane;
+        float s = 0.0f;
+        if (j < width) {
+            uint32_t p = grp;
+            for (; p + 96 < parts; p += 128) {
+                const float* q = part + static_cast<uint64_t>(p) * width + j;
+                const float a = q[0], b = q[32 * width], c = q[64 * width], e = q[96 * width];
+                s += (a + b) + (c + e);
+            }
+            for (; p < parts; p += 32) s += part[static_cast<uint64_t>(p) * width + j];
         }
-        for (; p < parts; p += 32) s += part[static_cast<uint64_t>(p) * width + j];
-    }
-    sums[grp][lane] = s;
-    __syncthreads();
-    for (uint32_t o = 16; o > 0; o >>= 1) {
-        if (grp < o) sums[grp][lane] += sums[grp + o][lane];
+        sums[grp][lane] = s;
         __syncthreads();
-    }
-    if (grp == 0 && j < width) {
-        if (j < d) dgamma[j] = sums[0][lane];
-        else dbeta[j - d] = sums[0][lane];
+        for (uint32_t o = 16; o > 0; o >>= 1) {
+            if (grp < o) sums[grp][lane] += sums[grp + o][lane];
+            __syncthreads();
+        }
+        if (grp == 0 && j < width) {  // (a lane reads what it alone writes for the next columns)
+            if (j < d) dgamma[j] = sums[0][lane];
+            else dbeta[j - d] = sums[0][lane];
+        }
     }
 }
 
@@ -277,9 +282,9 @@ void launch_norm(const float* x, const float* gamma, const TD* dy, const float* 
         if (!dgamma) return;
         const uint32_t per = ceil_div(rows, col_parts(rows));
         parts = ceil_div(rows, per);
-        layernorm_cols_kernel<TD><<<dim3(ceil_div(d, 64), parts), 256, 0, s>>>(x, dy, stats, part, rows, d, per);
+        layernorm_cols_kernel<TD><<<dim3(std::min(ceil_div(d, 64), kMaxGrid), parts), 256, 0, s>>>(x, dy, stats, part, rows, d, per);
     }
-    if (dgamma) layernorm_parts_kernel<<<ceil_div(2ull * d, 32), 1024, 0, s>>>(part, dgamma, dbeta, parts, d);
+    if (dgamma) layernorm_parts_kernel<<<std::min(ceil_div(2ull * d, 32), kMaxGrid), 1024, 0, s>>>(part, dgamma, dbeta, parts, d);
 }
 
 // Thread (x, y) of the grid takes columns 4 (blockIdx.x * 256 + tid) .. + 3 of rows blockIdx.y, + gridDim.y, ...
@@ -379,7 +384,7 @@ extern "C" int mi_layernorm_bwd(const float* x, const float* gamma, const void* 
     hipStream_t s = static_cast<hipStream_t>(stream);
     if (rows == 0) {
         // sums over no rows
-        if (dgamma) layernorm_parts_kernel<<<ceil_div(2ull * d, 32), 1024, 0, s>>>(nullptr, dgamma, dbeta, 0, d);
+        if (dgamma) layernorm_parts_kernel<<<std::min(ceil_div(2ull * d, 32), kMaxGrid), 1024, 0, s>>>(nullptr, dgamma, dbeta, 0, d);
         return check_launch(fn);
     }
     const bool vec = d % 4 == 0 && d <= kLayerNormVecMax && aligned(x, 16) && aligned(dx, 16) && aligned(dy, 4 * ey) &&

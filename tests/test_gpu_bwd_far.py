@@ -96,3 +96,30 @@ def test_geglu_gemm_rows(gpu):
     synchronize()
     got = np.stack([res.download(H, 2 * F, offset=m * ld * 2) for m in range(M)])
     assert np.array_equal(got.view(np.uint16), want.view(np.uint16))
+
+
+def test_layernorm_columns(gpu):
+    """More columns than a launch has threads for at 32 columns a workgroup of 1024. Signs that alternate every 64 (x) and
+    every 128 columns (dy): every sum over columns is exact, mean(dy) = mean(dy xh) = 0, and what is left is the rounding of
+    1 / sqrt(var + eps), three operations, and of the products."""
+    d = (1 << 26) + 256
+    print(f"[case] LayerNorm of {d} columns", flush=True)
+    s = np.where(np.arange(d) // 64 % 2 == 0, 1, -1).astype(np.float32)
+    t = np.where(np.arange(d) // 128 % 2 == 0, 1, -1).astype(np.float32)
+    a, b = np.float32([1, 2]), np.float32([3, 0.5])
+    x, dy = (DeviceBuffer.from_array((f[:, None] * v).reshape(-1)) for f, v in ((a, s), (b, t)))
+    ws = DeviceBuffer(ops.layernorm_bwd_ws_bytes(2, d))
+    dx, dg, db = (DeviceBuffer.from_array(np.full(n * d, 7, np.float32)) for n in (2, 1, 1))
+    ops.layernorm_bwd(x, None, dy, dx, dg, db, ws, 2, d)
+    synchronize()
+    inv = 1 / np.sqrt(np.float64(a) ** 2 + np.float64(np.float32(1e-5)))
+    tol = 8 * bwd_ref.U
+    got = dx.download(np.float32, 2 * d).reshape(2, d)
+    for r in range(2):
+        assert np.max(np.abs(got[r] - (inv[r] * b[r]) * t)) <= tol * inv[r] * b[r], r
+    want = float((a * b * inv).sum())
+    assert np.max(np.abs(dg.download(np.float32, d) - want * (s * t))) <= tol * want
+    assert np.array_equal(db.download(np.float32, d), 3.5 * t)
+    ops.layernorm_bwd(x, None, dy, dx, dg, db, ws, 0, d)
+    synchronize()
+    assert not dg.download(np.float32, d).any() and not db.download(np.float32, d).any()
