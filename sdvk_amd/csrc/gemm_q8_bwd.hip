@@ -477,6 +477,7 @@ uint32_t launched_splits(uint32_t N, bool f32, uint32_t splits) {
 // (64x64 tiles in 12 parts and their sum: 8.3).
 constexpr uint32_t kFewRows = 4;
 constexpr int kFewWaves = 16;
+constexpr uint32_t kFewMaxK = 1u << 27;  // K / 32 workgroups of 1024 threads: a launch counts them in 32 bits
 
 template <typename T, int MR>
 __global__ __launch_bounds__(kFewWaves * 64) void gemm_q8_bwd_few_kernel(BwdArgs a) {
@@ -576,7 +577,7 @@ Plan choose(uint32_t M, uint32_t N, uint32_t K, bool f32, bool allow_split) {
     // that the parts have. us against the best build and parts, fp32 / fp16: 1x1280x1280 5.7 : 8.3 / 5.6 : 7.6, 2x640x1280
     // 4.7 : 7.8 / 4.7 : 6.0, 4x1280x1280 6.9 : 8.3 / 7.0 : 7.6, 2x5120x640 12.7 : 11.1 / 12.8 : 8.0; with eight rows
     // 8x1280x1280 9.8 : 8.6 / 10.2 : 7.5.
-    if (M <= kFewRows) {
+    if (M <= kFewRows && K < kFewMaxK) {
         best = Plan{kFew, 1};
         best_us = 4.0 + N * (0.0013 + 0.00025 * M);
     }

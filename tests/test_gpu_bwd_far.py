@@ -123,3 +123,18 @@ def test_layernorm_columns(gpu):
     ops.layernorm_bwd(x, None, dy, dx, dg, db, ws, 0, d)
     synchronize()
     assert not dg.download(np.float32, d).any() and not db.download(np.float32, d).any()
+
+
+def test_linear_columns(gpu):
+    """One row and more 32-wide blocks of columns than a launch has workgroups of 1024 threads: a weight of one row whose
+    quants count through -127 .. 127, its scales powers of two, so that every product is exact."""
+    K = (1 << 27) + 64
+    print(f"[case] linear of {K} columns, one row", flush=True)
+    q = (np.arange(K) % 255 - 127).astype(np.int8).reshape(-1, 32)
+    d = np.float16(2.0) ** (np.arange(K // 32) % 7 - 3).astype(np.float16)
+    W = DeviceBuffer.from_array(np.concatenate([d[:, None].view(np.uint8), q.view(np.uint8)], 1).reshape(-1))
+    dC, dA = DeviceBuffer.from_array(np.float32([3.0])), DeviceBuffer.from_array(np.full(K, 7, np.float32))
+    ops.gemm_nt_q8_0_bwd(dC, W, dA, 1, 1, K)
+    synchronize()
+    want = 3 * q.astype(np.float32) * d.astype(np.float32)[:, None]
+    assert np.array_equal(dA.download(np.float32, K), want.reshape(-1))
