@@ -118,18 +118,26 @@ __device__ __forceinline__ float gelu_erf(float v) {
 // GEGLU's gradient: y = v * gelu(x), gelu(x) = x cdf(x), gelu'(x) = cdf(x) + x pdf(x) with the normal
 // distribution's cdf and pdf:
 //   dv = dy * x * cdf(x),   dx = dy * v * (cdf(x) + x * pdf(x)).
-// The cdf's tail q = (1 - erf(|x| / sqrt 2)) / 2 is half the rational approximation of gelu_erf (7.1.26,
-// |error| <= 0.75e-7 of the cdf) times exp(-x^2 / 2), and that exponential is the pdf's too, so the two
-// derivatives cost one v_exp_f32 and one v_rcp_f32. Taking the tail itself (cdf = q for x < 0, 1 - q for
-// x >= 0) avoids the cancellation of 1 + erf at negative x. Contraction is off: every kernel that inlines
-// this computes the same bits.
+// The cdf's tail q = erfc(z) / 2, z = |x| / sqrt 2, is exp(-z^2) times half of erfcx(z) = exp(z^2) erfc(z), which is
+// fitted by t P(t), t = 1 / (1 + 0.38 z), in relative error (a weighted least-squares iteration towards the minimax fit on
+// z <= 9.6, past which q is no normal number: 4e-8 with these coefficients). The tail itself keeps its relative accuracy, as
+// 1 + erf would not at negative x (gelu_erf's polynomial, bounded absolutely, left dv 4e-3 of itself off at x = -6; now 2e-6,
+// mostly the exponential's argument). exp(-x^2 / 2) is the pdf's too, so the two derivatives cost one v_exp_f32 and one
+// v_rcp_f32. Contraction is off and every fma is written out: every kernel that inlines this computes the same bits.
 __device__ __forceinline__ void geglu_grad(float v, float x, float dy, float& dv, float& dx) {
 #pragma clang fp contract(off)
-    const float ax = fabsf(x) * 0.70710678118654752440f;
-    const float t = __builtin_amdgcn_rcpf(1.0f + 0.3275911f * ax);
-    const float poly = ((((1.061405429f * t - 1.453152027f) * t + 1.421413741f) * t - 0.284496736f) * t + 0.254829592f) * t;
-    const float e = __builtin_amdgcn_exp2f(-ax * ax * 1.44269504088896341f);
-    const float q = 0.5f * poly * e;
+    const float t = __builtin_amdgcn_rcpf(__builtin_fmaf(fabsf(x), 0.38f * 0.70710678118654752440f, 1.0f));
+    float p = 0.058896184f;
+    p = __builtin_fmaf(p, t, -0.261921495f);
+    p = __builtin_fmaf(p, t, 0.363080382f);
+    p = __builtin_fmaf(p, t, -0.160515264f);
+    p = __builtin_fmaf(p, t, 0.229332566f);
+    p = __builtin_fmaf(p, t, 0.138964981f);
+    p = __builtin_fmaf(p, t, 0.203820139f);
+    p = __builtin_fmaf(p, t, 0.213932395f);
+    p = __builtin_fmaf(p, t, 0.214410126f);
+    const float e = __builtin_amdgcn_exp2f(x * x * -0.72134752044448170368f);
+    const float q = 0.5f * t * p * e;
     const float cdf = x >= 0.0f ? 1.0f - q : q;
     dv = dy * (x * cdf);
     dx = dy * (v * (cdf + x * (0.39894228040143267794f * e)));

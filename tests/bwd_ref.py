@@ -165,13 +165,27 @@ def geglu_tol(v, g, dy, dvg, typ):
             np.abs(dy * v) * 2 * e + 4 * U * np.abs(dvg[1]) + store_err(dvg[1], typ) * 1.01)
 
 
-def geglu(be, *, typ, rows, F, off=0, in_place=False, wide=False, seed=2):
+def geglu_tail_tol(v, g, y, want):
+    """Relative bounds where the gates are far below zero. The cdf's tail: the fit 1 u, its coefficients' and the Horner
+    form's roundings 10 steps of at most 1.9 times the value (the sum of the coefficients' magnitudes), 3 u of t times
+    d ln q / d ln t <= 3, exp2 and two products 6 u, and x^2 u from the exponential's argument and half as much from its
+    constant: 35 + 1.5 x^2 in all; x pdf(x) the exponential's alone. Then three products and a sum."""
+    cdf = 0.5 * np.vectorize(math.erfc)(-g / math.sqrt(2))
+    xpdf = np.abs(g) * np.exp(-g * g / 2) / math.sqrt(2 * math.pi)
+    k = 1.5 * g * g
+    return (np.abs(want[0]) * (38 + k) * U * 1.05 + 1e-37,
+            np.abs(y * v) * (cdf * (36 + k) + xpdf * (8 + k)) * U * 1.05 + 3 * U * np.abs(want[1]) + 1e-37)
+
+
+def geglu(be, *, typ, rows, F, off=0, in_place=False, wide=False, tail=False, seed=2):
     rng = rng_of(seed)
     dt, esz = DT[typ], np.dtype(DT[typ]).itemsize
     h = (rng.standard_normal((rows, 2 * F)) * (6.0 if wide else 1.5)).astype(np.float32)
     dy = (rng.standard_normal((rows, F)) * 0.5).astype(dt)
     if wide and h.size:
         h[0, F:F + min(F, 5)] = [0.0, -0.0, 40.0, -40.0, 1e-30][:min(F, 5)]
+    if tail:  # gates from -12 up
+        h[:, F:] = np.linspace(-12, 3, rows * F).reshape(rows, F)
     A = Arena(be)
     pad = np.full(off, SENTINEL, dt)
     bdy = A.put(np.concatenate([pad, dy.reshape(-1)]))
@@ -190,7 +204,7 @@ def geglu(be, *, typ, rows, F, off=0, in_place=False, wide=False, seed=2):
     got = flat[off:].reshape(rows, 2 * F)
     v, g, y = f64(h[:, :F]), f64(h[:, F:]), f64(dy)
     want = geglu_parts(v, g, y)
-    tol = geglu_tol(v, g, y, want, typ)
+    tol = geglu_tail_tol(v, g, y, want) if tail else geglu_tol(v, g, y, want, typ)
     check(got[:, :F], want[0], tol[0], "geglu dv")
     check(got[:, F:], want[1], tol[1], "geglu dg")
     A.unchanged()
@@ -524,6 +538,7 @@ CASES = {
     "geglu": [
         dict(typ="f32", rows=3, F=64), dict(typ="f16", rows=5, F=36), dict(typ="f32", rows=7, F=37), dict(typ="f16", rows=4, F=1),
         dict(typ="f32", rows=2, F=64, off=1), dict(typ="f16", rows=3, F=64, off=1), dict(typ="f32", rows=5, F=40, in_place=True),
+        dict(typ="f32", rows=40, F=100, tail=True), dict(typ="f32", rows=40, F=101, tail=True),
         dict(typ="f32", rows=5, F=41, in_place=True), dict(typ="f32", rows=40, F=100, wide=True), dict(typ="f16", rows=40, F=100, wide=True),
     ],
     "geglu_gemm": [
