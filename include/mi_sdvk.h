@@ -68,7 +68,9 @@ int mi_version(void);
  * tests that pin one kernel plan. Process-wide; the library never reads the
  * environment. An override picks tiles, K splits or workgroup sizes only, so
  * results stay within the operators' documented error (a different plan can
- * change the summation order, never the arithmetic). value NULL or "" clears.
+ * change the summation order; the arithmetic only where "gemm_bwd_cfg" takes up
+ * to four rows to the tiles, which round or split the weights). value NULL or ""
+ * clears.
  *   "gemm_cfg"          "<build 0..6>[:<K splits>]" (Q8 NT GEMM tile build;
  *                       the splits apply to the workspace entries)
  *   "nn_kernel"         "general": the NN GEMM's untiled kernel for every shape
@@ -490,7 +492,9 @@ int mi_sdxl_block_forward_kv(const mi_block_weights* w, const mi_block_dims* dim
  * MI_F16: P and dS rounded to fp16 once each, scaled so that small weights and gradients
  * of any size keep their bits, fp32 sums. MI_F32: every operand as fp16 hi + lo (q, k, v
  * within fp16's range, as in the forward pass; dout's rows with their largest element
- * within 1e-30 .. 1e30, or zero).
+ * within 1e-30 .. 1e30, or zero). delta comes from out as it is stored: an fp16 out whose
+ * rows of v share a mean far above their spread leaves its rounding in dq and dk (a mean of
+ * 30 times the spread: 7e-3 of them).
  * workspace: mi_fused_attention_bwd_ws_bytes(args) bytes, 16-byte aligned, disjoint from
  * the tensors. The bytes go by sizes and dtype, and by whether the addresses and strides
  * are multiples of 16 bytes (of 4 elements, for dq, dk and dv; NULL counts as one).
@@ -517,7 +521,8 @@ int mi_fused_attention_bwd(const mi_attn_bwd_args* args, void* workspace, uint64
  * carried as fp16 hi + lo (weights below 1023 in magnitude; a row of dC of any
  * size, by an exponent of its own): the accuracy of an fp32 product; an infinity in
  * dC leaves NaN in its row of dA. Up to four rows may run in fp32 arithmetic with
- * unrounded weights, for either type. N == 0 stores zeros in mode 0.
+ * unrounded weights, for either type (by the sizes and by whether a workspace lets
+ * the tiles split N: whichever is faster). N == 0 stores zeros in mode 0.
  * workspace (or NULL): grids too small to fill the GPU split N into parts, fp32,
  * added in order, when it holds mi_gemm_nt_q8_0_bwd_ws_bytes(M, N, K, dtype) bytes
  * (16-byte aligned, disjoint from the operands); with less the call runs unsplit.

@@ -4,6 +4,11 @@
 //   delta_i = sum_d dO_id O_id          (= sum_j P_ij dP_ij)
 //   dP = dO V^T,   dS = P (dP - delta)
 //   dQ = scale dS K,   dK = scale dS^T Q,   dV = P^T dO
+// delta is taken from O as the caller has it. In fp16 that carries O's rounding, up to 2^-11 of |O|, into dS: nothing beside
+// the rounding of dS where the rows of V differ as much as they are large, but where they share a mean of 5, 30 or 300 times
+// their spread dQ and dK come out 1.5e-3, 7e-3 or 0.1 off. (The sum of exp2(s - m) (dP - delta), kept beside l, says what
+// delta is off by; handed to the key kernel it mends dK alone, at 3% of 2x10x4096^2 and 2x20x1024x77, and dQ would take an
+// eighth product, P K.)
 // P is never stored: two kernels recompute it, one for queries, one for keys.
 //
 // attn_bwd_q_kernel: blocks of 128 queries of one (batch, head), 4 waves x 32, walk over 64-key tiles of K and V in
@@ -41,10 +46,15 @@
 //     elements' bound N(0, 1) tensors made it (2x10x4096^2 fp16 357 us, with the norms 351);
 //   * dO of fp32, row by row, by its largest element, taken to 2^8.
 //
-// Measured (MI355X, us a call; a call of the kernels that its sizes take): fp16 2x10x4096^2 hd 64 350 (keys 205, queries 180,
-// their merges 10 and 7; 860 TFLOP/s over the seven products, MFMAs busy 47% of cycles at the 1.8 GHz that the power limit
-// leaves: what bounds it), 2x20x1024x77 30 and fp32 causal 12x77 29 (three launches of first loads and one or two tiles:
-// latency), fp32 10x2304^2 189 (keys 98, queries 81, packing 11, merges 10 and 7, each timed alone; 760 TFLOP/s over its 21 products).
+// P and dS are rounded to fp16 for fp16 tensors (2^-11 of each, beside the result's own 2^-11; pairs as for fp32 would take 21
+// products for seven).
+//
+// Measured (MI355X, us a call; a call of the kernels that its sizes take): fp16 2x10x4096^2 hd 64 358 (keys 207, queries 189,
+// their merges 10 and 7, each timed alone; 840 TFLOP/s over the seven products), 2x20x1024x77 30 and fp32 causal 12x77 29
+// (three launches of first loads and one or two tiles: latency), fp32 10x2304^2 189 (keys 99, queries 83, packing 11, merges
+// 10 and 8; 760 TFLOP/s over its 21 products). What bounds the large calls: no unit is full. Of the cycles (1.7 to 1.8 GHz)
+// MFMAs are busy 50% in the key and 39% in the query kernel, VALUs 42% and 55%, LDS 38% and 20% (fp32: 49 and 42, 32 and 42, 21
+// and 15). A wave's scores, exponentials and products follow one another, and two or three waves a SIMD do not fill the gaps.
 #include "common.hpp"
 
 #include <algorithm>

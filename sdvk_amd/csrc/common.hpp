@@ -30,7 +30,8 @@ int check_launch(const char* what);
 // with one atomic load per call, never from the environment. Defaults mean
 // "the built-in rules decide". They pick tiles, split counts and workgroup
 // sizes only: no override changes an operator's arithmetic beyond the
-// summation order of a different plan.
+// summation order of a different plan, but for gemm_bwd_cfg with up to four
+// rows (their own kernel does not round the weights, the tiles do).
 constexpr int kGemmBuilds = 7;  // tile builds of gemm_q8.hip (kNumCfg)
 constexpr int kGemmBwdBuilds = 4;  // tile builds of gemm_q8_bwd.hip
 struct Tuning {

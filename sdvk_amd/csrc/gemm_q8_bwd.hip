@@ -9,7 +9,9 @@
 //     out of LDS (row stride BN + 32 halves, so that the four rows of a 32-lane read cover all banks);
 //   * v_mfma_f32_32x32x16_f16 of the transposed product (a lane holds one row of dA and runs of four columns).
 //
-// fp16: dC as it is, w = fp16(d * q), fp32 sums, dA rounded once.
+// fp16: dC as it is, w = fp16(d * q), fp32 sums, dA rounded once. The forward product rounds the weights alike: this is the
+//   gradient of what ran (3e-4 of unrounded weights' in the mean, with the result's own rounding, which alone is 2e-4;
+//   weights as pairs would take two products).
 // fp32: both operands as fp16 pairs x = hi + lo and three products (hi hi + hi lo + lo hi): what is dropped is
 //   2^-22 of a product, the accuracy of an fp32 product summed in fp32. fp16's range is kept by powers of two, which
 //   are exact: the weights times 2^6 (|w| < 1023; the pair's absolute error 2^-31 is then 2^-25 of a weight of 0.02);
@@ -17,8 +19,8 @@
 //   of 1e4 keep all their bits). A row's exponent falls by a step only when an element would pass 2^14 (its first
 //   elements are taken to 2^9 .. 2^10), and the row's sums are then brought down with it.
 //
-// Measured (MI355X, us a call): fp16 2048x1280x5120 (M x N x K) 44 (610 TFLOP/s: 640 tiles of 128x128 on 512 places, MFMAs
-// busy 27% of cycles, LDS reads and a barrier per step between them), 1976x10240x1280 71; fp32 1152x1280x1280 28 (five parts,
+// Measured (MI355X, us a call): fp16 2048x1280x5120 (M x N x K) 45 (600 TFLOP/s: 640 tiles of 128x128 on 512 places, MFMAs
+// busy 29% of cycles, LDS 48%, and a barrier per step), 1976x10240x1280 71; fp32 1152x1280x1280 29 (five parts,
 // 23 and 6 for their sum), 2048x1280x5120 105; 2x1280x1280 6.1 (gemm_q8_bwd_few_kernel).
 //
 // Grids too small to fill the GPU split N when the caller gives a workspace: each part stores its sums, fp32, and a
