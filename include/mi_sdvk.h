@@ -491,10 +491,15 @@ int mi_sdxl_block_forward_kv(const mi_block_weights* w, const mi_block_dims* dim
  * rows leave through it).
  * MI_F16: P and dS rounded to fp16 once each, scaled so that small weights and gradients
  * of any size keep their bits, fp32 sums. MI_F32: every operand as fp16 hi + lo (q, k, v
- * within fp16's range, as in the forward pass; dout's rows with their largest element
- * within 1e-30 .. 1e30, or zero). delta comes from out as it is stored: an fp16 out whose
- * rows of v share a mean far above their spread leaves its rounding in dq and dk (a mean of
- * 30 times the spread: 7e-3 of them).
+ * within fp16's range, as in the forward pass; each row of dout zero, or its largest
+ * element within 1e-30 .. 1e30). What bounds the accuracy beside that:
+ *   - dk (MI_F32: dv too) is held to 2^-38 of the (batch, head)'s largest row of dout: a
+ *     key that only rows 1e-8 of that or smaller reach loses bits;
+ *   - MI_F16: values below 2^-8 of the largest of their 128 keys' enter dk at up to 2^-19
+ *     of that one;
+ *   - MI_F16: delta takes out as it is stored. Where the rows of v share a mean far above
+ *     their spread, out's rounding shows in dq and dk (a mean of 30 times the spread: 7e-3
+ *     of them).
  * workspace: mi_fused_attention_bwd_ws_bytes(args) bytes, 16-byte aligned, disjoint from
  * the tensors. The bytes go by sizes and dtype, and by whether the addresses and strides
  * are multiples of 16 bytes (of 4 elements, for dq, dk and dv; NULL counts as one).

@@ -42,8 +42,9 @@
 //     2^14 (|dP| + |delta|) under 2^15, for the largest |delta| of the (batch, head) and the bound of |dP| that its rows of
 //     dO and the block's of V give: fp32 64 max|dO| max|V|, fp16 the product of the largest rows' norms. dS cannot
 //     overflow, and a weight of 2^-20 still has all its bits. fp16: that power of two is carried by V, whose largest
-//     element stays in 2^-6 .. 2^12, and by dS itself beyond that, in a multiplication that only such blocks make: with the
-//     elements' bound N(0, 1) tensors made it (2x10x4096^2 fp16 357 us, with the norms 351);
+//     element stays in 2^-6 .. 2^12 (an element under 2^-8 of it may lose bits, 2^-19 of it at most), and by dS itself
+//     beyond that, in a multiplication that only such blocks make: with the elements' bound N(0, 1) tensors made it
+//     (2x10x4096^2 fp16 357 us, with the norms 351);
 //   * dO of fp32, row by row, by its largest element, taken to 2^8.
 //
 // P and dS are rounded to fp16 for fp16 tensors (2^-11 of each, beside the result's own 2^-11; pairs as for fp32 would take 21
