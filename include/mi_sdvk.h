@@ -53,6 +53,7 @@ typedef enum mi_status {
 typedef enum mi_dtype {
     MI_F32 = 0,
     MI_F16 = 1,
+    MI_I8 = 2, /* rows of 8-bit codes with a scale each: mi_groupnorm's y alone */
 } mi_dtype;
 
 /* ---------------------------------------------------------------- misc -- */
@@ -569,6 +570,90 @@ uint64_t mi_layernorm_bwd_ws_bytes(uint32_t rows, uint32_t d);
 int mi_layernorm_bwd(const float* x, const float* gamma, const void* dy, int dy_dtype, const float* res, float* dx,
                      float* dgamma, float* dbeta, uint32_t rows, uint32_t d, float eps, void* workspace,
                      uint64_t workspace_bytes, void* stream);
+
+/* ------------------------------------------- GroupNorm and 8-bit linears -- *
+ * What lies between a ResBlock and a transformer's first linear. (Extension: the
+ * reference runs its norms and linears in fp32 / Q8_0.) Contract as for every entry:
+ * nothing is allocated, work is ordered on the stream, results repeat bit for bit, an
+ * entry may be captured into a HIP graph. A workspace is used in stream order; calls
+ * that may overlap in time (streams, captured graphs) need one each.              */
+
+/* GroupNorm with an optional activation over channels-last tensors (pixels are rows):
+ *   z = (x - mean) / sqrt(var + eps) gamma + beta,  y = z (MI_ACT_NONE) or z sigma(z) (MI_ACT_SILU)
+ * mean and var over the channels / groups neighbouring channels of all pixels of an image.
+ * x: MI_F32 or MI_F16; y: MI_F32, MI_F16, or MI_I8, rows of codes with a scale each
+ * (mi_quantize_rows_i8's, of the fp32 result): y_scale[image * pixels + pixel] (the rows
+ * that mi_gemm_nt_i8 takes as A). gamma, beta: fp32 or NULL (1, 0). Row strides ldx, ldy
+ * (0 -> channels) and image strides sx, sy (0 -> pixels * ld) in elements, so a tensor may
+ * be a column block of a wider one, or hold the images' rows in turn; rows of y must not
+ * overlap. stats (or NULL): batch * groups * 4 floats, 16-byte aligned, kept for the
+ * backward pass: a group's mean, what the mean's rounding to fp32 left, 1 / sqrt(var + eps), 0.
+ * Means and variances keep their accuracy whatever the mean's size (values below 1e18 in
+ * magnitude: squares are summed in fp32). groups divides channels; batch and channels <=
+ * 2^20, batch * pixels <= 2^31. Tensors aligned to their element. Fast: channels and strides
+ * multiples of 16 bytes (MI_I8: of 16 codes), 16-byte aligned tensors, channels <= 4096. y, y_scale,
+ * stats and workspace overlap no input and not each other. workspace:
+ * mi_groupnorm_ws_bytes(...) bytes, 16-byte aligned. batch or pixels 0: nothing is written. */
+enum { MI_ACT_NONE = 0, MI_ACT_SILU = 1 };
+
+typedef struct mi_groupnorm_args {
+    const void* x;                           /* [batch][pixels][ldx] */
+    const float *gamma, *beta;               /* [channels] or NULL */
+    void* y;                                 /* [batch][pixels][ldy] */
+    float* y_scale;                          /* [batch * pixels] for MI_I8, else NULL */
+    float* stats;                            /* [batch][groups][4] or NULL */
+    uint32_t batch, pixels, channels, groups;
+    int32_t x_dtype, y_dtype;                /* mi_dtype */
+    int32_t act;                             /* MI_ACT_* */
+    float eps;
+    uint64_t ldx, ldy, sx, sy;
+} mi_groupnorm_args;
+
+uint64_t mi_groupnorm_ws_bytes(uint32_t batch, uint32_t pixels, uint32_t channels, uint32_t groups);
+int mi_groupnorm(const mi_groupnorm_args* args, void* workspace, uint64_t workspace_bytes, void* stream);
+
+/* Gradients of mi_groupnorm from x and dy: with xh = (x - mean) inv and w = dy act'(z),
+ *   dx = inv (w gamma - mean_g(w gamma) - xh mean_g(w gamma xh)) (+ res)
+ *   dgamma = sum over images and pixels of w xh,  dbeta = sum of w
+ * fwd: the forward call's arguments; y and y_scale are not read, y_dtype is dy's type
+ * (MI_F32 or MI_F16). fwd.stats: what the forward pass kept, or NULL: computed again from
+ * x. dx and res of x's type, res (or NULL) the gradient that reaches x past the norm; dx may
+ * be res itself (equal strides) and overlaps nothing else. dgamma and dbeta both NULL or
+ * both set. Strides as in the forward call. Sums in fp32 over at most 2048 rows, then in 64
+ * bits, in a fixed order. workspace: mi_groupnorm_bwd_ws_bytes(...) bytes, 16-byte aligned,
+ * disjoint from the tensors. batch or pixels 0 stores zeros in dgamma and dbeta.       */
+typedef struct mi_groupnorm_bwd_args {
+    mi_groupnorm_args fwd;
+    const void *dy, *res;                    /* [batch][pixels][ld] */
+    void* dx;
+    float *dgamma, *dbeta;                   /* [channels] or NULL */
+    uint64_t lddy, ldres, lddx;              /* row strides, 0 -> channels */
+    uint64_t sdy, sres, sdx;                 /* image strides, 0 -> pixels * ld */
+} mi_groupnorm_bwd_args;
+
+uint64_t mi_groupnorm_bwd_ws_bytes(uint32_t batch, uint32_t pixels, uint32_t channels, uint32_t groups);
+int mi_groupnorm_bwd(const mi_groupnorm_bwd_args* args, void* workspace, uint64_t workspace_bytes, void* stream);
+
+/* Rows of 8-bit codes: scale[r] = max(max|x[r]|, 127 * 2^-126) / 127 in fp32, q[r, c] = x[r, c] /
+ * scale[r] rounded to the nearest integer, ties to even (of the exact quotient: -127 ..
+ * 127). A row with an infinity or a NaN gets the scale NaN and codes 0. x MI_F32 or MI_F16
+ * (dtype); row strides ldx, ldq in elements (0 -> cols). For weights, one scale a channel:
+ * mi_q8_0_dequant, then this. Tensors aligned to their element; cols % 16 == 0 with 16-byte
+ * aligned rows and cols <= 8192 is the fast path. q and scale overlap nothing.               */
+int mi_quantize_rows_i8(const void* x, int dtype, int8_t* q, float* scale, uint32_t rows, uint32_t cols, uint32_t ldx,
+                        uint32_t ldq, void* stream);
+
+/* Product of 8-bit rows with a scale for each token and channel:
+ *   C[m,n] (=|+=) a_scale[m] w_scale[n] sum_k A[m,k] W[n,k] (+ bias[n])
+ * The sum is exact (32-bit integers; any codes -128 .. 127, K <= 131071), the rest fp32:
+ * fma(float(sum) a_scale, w_scale, bias), so a call's bits do not depend on the sizes around it.
+ * C MI_F32 or MI_F16 (c_dtype, rounded once); mode 0 stores, 1 adds without the bias, 2 adds
+ * with it (the residual). Row strides lda, ldw (0 -> K) and ldc (0 -> N). bias fp32 or NULL.
+ * Fast: K % 16 == 0, A and W 16-byte aligned with strides of 16, A's and W's rows within
+ * 4 GiB. C overlaps no input.                                                       */
+int mi_gemm_nt_i8(const int8_t* A, const float* a_scale, const int8_t* W, const float* w_scale, const float* bias, void* C,
+                  int c_dtype, uint32_t M, uint32_t N, uint32_t K, uint32_t mode, uint32_t lda, uint32_t ldw, uint32_t ldc,
+                  void* stream);
 
 /* ---------------------------------------------------------------- GGUF -- *
  * Checkpoint access: the container reader and the upload of its tensors into

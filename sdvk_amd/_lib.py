@@ -14,7 +14,8 @@ LIB_PATH = Path(__file__).resolve().parent / "libmi_sdvk.so"
 
 (MI_OK, MI_ERR_INVALID_ARG, MI_ERR_UNSUPPORTED, MI_ERR_ALIGNMENT, MI_ERR_ALIASING, MI_ERR_HIP, MI_ERR_IO,
  MI_ERR_NOT_FOUND) = range(8)
-MI_F32, MI_F16 = 0, 1
+MI_F32, MI_F16, MI_I8 = 0, 1, 2
+MI_ACT_NONE, MI_ACT_SILU = 0, 1
 MI_ATTN_PREC_AUTO, MI_ATTN_PREC_FP16, MI_ATTN_PREC_SPLIT = 0, 1, 2
 
 # Every function declared in include/mi_sdvk.h, with its ctypes signature.
@@ -40,6 +41,20 @@ class MiAttnBwdArgs(ctypes.Structure):
     _fields_ = [("fwd", MiAttnArgs), ("dout", _vp), ("dq", _vp), ("dk", _vp), ("dv", _vp),
                 ("lddout", _u64), ("lddq", _u64), ("lddk", _u64), ("lddv", _u64),
                 ("sdout", _u64), ("sdq", _u64), ("sdk", _u64), ("sdv", _u64)]
+
+
+class MiGroupnormArgs(ctypes.Structure):
+    """Mirror of mi_groupnorm_args (include/mi_sdvk.h)."""
+    _fields_ = [("x", _vp), ("gamma", _vp), ("beta", _vp), ("y", _vp), ("y_scale", _vp), ("stats", _vp),
+                ("batch", _u32), ("pixels", _u32), ("channels", _u32), ("groups", _u32),
+                ("x_dtype", _i32), ("y_dtype", _i32), ("act", _i32), ("eps", ctypes.c_float),
+                ("ldx", _u64), ("ldy", _u64), ("sx", _u64), ("sy", _u64)]
+
+
+class MiGroupnormBwdArgs(ctypes.Structure):
+    """Mirror of mi_groupnorm_bwd_args (include/mi_sdvk.h)."""
+    _fields_ = [("fwd", MiGroupnormArgs), ("dy", _vp), ("res", _vp), ("dx", _vp), ("dgamma", _vp), ("dbeta", _vp),
+                ("lddy", _u64), ("ldres", _u64), ("lddx", _u64), ("sdy", _u64), ("sres", _u64), ("sdx", _u64)]
 
 
 class MiBlockWeights(ctypes.Structure):
@@ -131,6 +146,12 @@ SIGNATURES = {
     "mi_layernorm_bwd_ws_bytes": (_u64, [_u32, _u32]),
     "mi_layernorm_bwd": (ctypes.c_int, [_vp, _vp, _vp, ctypes.c_int, _vp, _vp, _vp, _vp, _u32, _u32, ctypes.c_float, _vp,
                                         _u64, _vp]),
+    "mi_groupnorm_ws_bytes": (_u64, [_u32, _u32, _u32, _u32]),
+    "mi_groupnorm": (ctypes.c_int, [ctypes.POINTER(MiGroupnormArgs), _vp, _u64, _vp]),
+    "mi_groupnorm_bwd_ws_bytes": (_u64, [_u32, _u32, _u32, _u32]),
+    "mi_groupnorm_bwd": (ctypes.c_int, [ctypes.POINTER(MiGroupnormBwdArgs), _vp, _u64, _vp]),
+    "mi_quantize_rows_i8": (ctypes.c_int, [_vp, ctypes.c_int, _vp, _vp, _u32, _u32, _u32, _u32, _vp]),
+    "mi_gemm_nt_i8": (ctypes.c_int, [_vp, _vp, _vp, _vp, _vp, _vp, ctypes.c_int, _u32, _u32, _u32, _u32, _u32, _u32, _u32, _vp]),
     "mi_gguf_open": (ctypes.c_int, [ctypes.c_char_p, ctypes.c_char_p, ctypes.POINTER(_vp)]),
     "mi_gguf_close": (None, [_vp]),
     "mi_gguf_info": (ctypes.c_int, [_vp, ctypes.POINTER(_u32), ctypes.POINTER(_u64), ctypes.POINTER(_u64),

@@ -1,0 +1,565 @@
+// groupnorm.hip -- GroupNorm with an optional SiLU on channels-last tensors for gfx950, forward and backward.
+//
+// x [batch][pixels][C]; group g of an image is channels g cg .. g cg + cg - 1 (cg = C / groups) of all its pixels, n = pixels cg
+// values with mean m and variance v:
+//   xh = (x - m) inv, inv = 1 / sqrt(v + eps);  z = xh gamma + beta;  y = z or z sigma(z)
+//   w  = dy act'(z);  dgamma = sum over batch and pixels of w xh,  dbeta = sum of w
+//   dx = inv (w gamma - mean_g(w gamma) - xh mean_g(w gamma xh)) (+ res)
+// y may leave as 8-bit rows (one pixel's channels) with a scale each: quant.hpp.
+//
+// Statistics: an image's rows are cut into chunks. A chunk's sums are taken about a shift, the mean of some of its own values,
+// so that neither a large common mean nor an outlier cancels the variance (the shift lies within sqrt(n / m) standard
+// deviations of the chunk's mean, m the values that made it); the chunks' means and squared deviations are then joined in
+// 64 bits. A mean is held as two floats: with the first alone x - m would be off by 2^-24 m, which a large mean over a
+// small spread shows.
+#include "common.hpp"
+#include "quant.hpp"
+
+#include <algorithm>
+
+namespace mi {
+namespace {
+
+constexpr uint32_t kMaxGrid = 1u << 20;   // workgroups of a launch that strides over its units
+constexpr uint32_t kChunkMin = 16;        // rows of a chunk, at least (but for the last) ...
+constexpr uint32_t kChunkMax = 2048;      // ... and at most: the longest chain of fp32 additions
+constexpr uint32_t kChunks = 512;         // chunks of all images, about: two workgroups per CU
+
+struct Stat {  // of one group of one image, 16 bytes: what `stats` holds
+    float mean, low, inv, zero;
+};
+struct Part {  // of one group of one chunk: mean = shift + rest, m2 = sum of (x - mean)^2
+    float shift, rest, m2, zero;
+};
+
+struct GnArgs {
+    const void* x;
+    const float *gamma, *beta;
+    void* y;
+    float* y_scale;
+    Stat* stats;
+    Part* part;
+    uint32_t batch, pixels, C, groups, cg;
+    uint32_t chunk, nchunk;  // rows of a chunk, chunks of an image
+    float eps;
+    uint64_t ldx, ldy, sx, sy;
+};
+
+struct GnBwdArgs {
+    GnArgs f;
+    const void *dy, *res;
+    void* dx;
+    float *dgamma, *dbeta;
+    float* cpart;  // [batch][nchunk][2][C]: sums of w and of w xh
+    float* gsum;   // [batch][groups][2]: mean(w gamma), mean(w gamma xh)
+    uint64_t lddy, ldres, lddx, sdy, sres, sdx;
+};
+
+__device__ __forceinline__ double wave_sum(double v) {
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) v += __shfl_xor(v, o);
+    return v;
+}
+
+// z = xh gamma + beta as one fma of x - mean: s.low inv gamma is far below beta's rounding unless the mean is large.
+struct Coef {
+    float mean, a, b;
+};
+__device__ __forceinline__ Coef coef(const Stat& s, float gamma, float beta) {
+    const float a = s.inv * gamma;
+    return Coef{s.mean, a, __builtin_fmaf(-s.low, a, beta)};
+}
+__device__ __forceinline__ float apply(float x, const Coef& k) { return __builtin_fmaf(x - k.mean, k.a, k.b); }
+
+constexpr float kLog2e = 1.44269504088896340736f;
+// z sigma(z). The exponential and the reciprocal are the hardware's (1 ulp each); the exponent's argument is off by 2^-24 of
+// itself, which is |z| 2^-24 of the result: no more than z's own rounding does to it. Below z = -87.3 e is held at 2^126: what
+// is left, |z| 2^-126 at most, stands for results below 1e-36.
+template <int ACT>
+__device__ __forceinline__ float activate(float z) {
+    if constexpr (ACT == MI_ACT_NONE) return z;
+    return z * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(fminf(-kLog2e * z, 126.0f)));
+}
+// act'(z) = sigma(z) (1 + z sigma(-z)), sigma(-z) = e sigma(z)
+template <int ACT>
+__device__ __forceinline__ float slope(float z) {
+    if constexpr (ACT == MI_ACT_NONE) return 1.0f;
+    const float e = __builtin_amdgcn_exp2f(fminf(-kLog2e * z, 126.0f));
+    const float s = __builtin_amdgcn_rcpf(1.0f + e);
+    return s * __builtin_fmaf(z, e * s, 1.0f);
+}
+
+// ---- any shape and alignment -------------------------------------------------------
+
+// One group of one chunk per workgroup; two passes over its values, sums in 64 bits.
+template <typename TX>
+__global__ __launch_bounds__(256) void gn_part_any_kernel(GnArgs a) {
+    __shared__ double red[3][4];
+    const uint32_t tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
+    const uint64_t units = static_cast<uint64_t>(a.batch) * a.nchunk * a.groups;
+    const uint32_t step_r = 256 / a.cg, step_c = 256 % a.cg;
+    for (uint64_t u = blockIdx.x; u < units; u += gridDim.x) {
+        const uint32_t g = static_cast<uint32_t>(u % a.groups);
+        const uint64_t bc = u / a.groups;
+        const uint32_t c = static_cast<uint32_t>(bc % a.nchunk), b = static_cast<uint32_t>(bc / a.nchunk);
+        const uint32_t r0 = c * a.chunk, rows = min(a.chunk, a.pixels - r0);
+        const TX* x = static_cast<const TX*>(a.x) + b * a.sx + r0 * a.ldx + static_cast<uint64_t>(g) * a.cg;
+        const uint64_t n = static_cast<uint64_t>(rows) * a.cg;
+        const uint32_t first_r = tid / a.cg, first_c = tid % a.cg;
+        double s = wave_sum(first_r < rows ? static_cast<double>(x[first_r * a.ldx + first_c]) : 0.0);
+        if (lane == 0) red[0][wave] = s;
+        __syncthreads();
+        const float shift = static_cast<float>(((red[0][0] + red[0][1]) + (red[0][2] + red[0][3])) /
+                                               static_cast<double>(min(n, static_cast<uint64_t>(256))));
+        double d1 = 0.0, d2 = 0.0;
+        for (uint32_t r = first_r, ch = first_c; r < rows;) {
+            const double d = static_cast<double>(static_cast<float>(x[r * a.ldx + ch])) - static_cast<double>(shift);
+            d1 += d;
+            d2 += d * d;
+            r += step_r;
+            ch += step_c;
+            if (ch >= a.cg) {
+                ch -= a.cg;
+                ++r;
+            }
+        }
+        d1 = wave_sum(d1);
+        d2 = wave_sum(d2);
+        if (lane == 0) {
+            red[1][wave] = d1;
+            red[2][wave] = d2;
+        }
+        __syncthreads();
+        if (tid == 0) {
+            d1 = (red[1][0] + red[1][1]) + (red[1][2] + red[1][3]);
+            d2 = (red[2][0] + red[2][1]) + (red[2][2] + red[2][3]);
+            const double rest = d1 / static_cast<double>(n);
+            a.part[bc * a.groups + g] = Part{shift, static_cast<float>(rest), static_cast<float>(d2 - d1 * rest), 0.0f};
+        }
+        __syncthreads();  // the sums are free for the next unit
+    }
+}
+
+// Joins the chunks of a group (a wave each): the mean of the means, then each chunk's deviations about it.
+__global__ __launch_bounds__(256) void gn_join_kernel(GnArgs a) {
+    const uint32_t lane = threadIdx.x & 63;
+    const uint64_t units = static_cast<uint64_t>(a.batch) * a.groups;
+    for (uint64_t u = blockIdx.x * 4ull + (threadIdx.x >> 6); u < units; u += gridDim.x * 4ull) {
+        const uint64_t b = u / a.groups, g = u % a.groups;
+        const Part* p = a.part + b * a.nchunk * a.groups + g;
+        const double total = static_cast<double>(a.pixels) * a.cg;
+        double s = 0.0;
+        for (uint32_t c = lane; c < a.nchunk; c += 64) {
+            const Part q = p[static_cast<uint64_t>(c) * a.groups];
+            const double n = static_cast<double>(min(a.chunk, a.pixels - c * a.chunk)) * a.cg;
+            s += n * (static_cast<double>(q.shift) + static_cast<double>(q.rest));
+        }
+        const double mean = wave_sum(s) / total;
+        s = 0.0;
+        for (uint32_t c = lane; c < a.nchunk; c += 64) {
+            const Part q = p[static_cast<uint64_t>(c) * a.groups];
+            const double n = static_cast<double>(min(a.chunk, a.pixels - c * a.chunk)) * a.cg;
+            const double d = (static_cast<double>(q.shift) - mean) + static_cast<double>(q.rest);
+            s += static_cast<double>(q.m2) + n * d * d;
+        }
+        const double var = wave_sum(s) / total;
+        if (lane == 0) {
+            const float hi = static_cast<float>(mean);
+            a.stats[u] = Stat{hi, static_cast<float>(mean - static_cast<double>(hi)),
+                              static_cast<float>(1.0 / sqrt(var + static_cast<double>(a.eps))), 0.0f};
+        }
+    }
+}
+
+// A wave takes a row at a time.
+template <typename TX, typename TY, int ACT>
+__global__ __launch_bounds__(256) void gn_apply_any_kernel(GnArgs a) {
+    const uint32_t lane = threadIdx.x & 63;
+    const uint64_t rows = static_cast<uint64_t>(a.batch) * a.pixels;
+    for (uint64_t row = blockIdx.x * 4ull + (threadIdx.x >> 6); row < rows; row += gridDim.x * 4ull) {
+        const uint64_t b = row / a.pixels, r = row % a.pixels;
+        const TX* x = static_cast<const TX*>(a.x) + b * a.sx + r * a.ldx;
+        TY* y = static_cast<TY*>(a.y) + b * a.sy + r * a.ldy;
+        const Stat* st = a.stats + b * a.groups;
+        auto value = [&](uint32_t c) {
+            const Coef k = coef(st[c / a.cg], a.gamma ? a.gamma[c] : 1.0f, a.beta ? a.beta[c] : 0.0f);
+            return activate<ACT>(apply(static_cast<float>(x[c]), k));
+        };
+        if constexpr (sizeof(TY) == 1) {
+            uint32_t top = 0;
+            for (uint32_t c = lane; c < a.C; c += 64) top = max(top, magnitude_bits(value(c)));
+            const RowScale s = row_scale(wave_max(top));
+            for (uint32_t c = lane; c < a.C; c += 64) y[c] = static_cast<int8_t>(quant_code(value(c), s));
+            if (lane == 0) a.y_scale[row] = s.scale;
+        } else {
+            for (uint32_t c = lane; c < a.C; c += 64) y[c] = static_cast<TY>(value(c));
+        }
+    }
+}
+
+// Sums of w and w xh over a chunk's rows, 64 channels at a time: four row groups of a workgroup, added in order.
+template <typename TX, typename TD, int ACT>
+__global__ __launch_bounds__(256) void gn_bwd_cols_any_kernel(GnBwdArgs a) {
+    __shared__ float sums[2][4][64];
+    const GnArgs& f = a.f;
+    const uint32_t lane = threadIdx.x & 63, grp = threadIdx.x >> 6;
+    const uint32_t blocks = (f.C + 63) / 64;
+    const uint64_t units = static_cast<uint64_t>(f.batch) * f.nchunk * blocks;
+    for (uint64_t u = blockIdx.x; u < units; u += gridDim.x) {
+        const uint32_t c = static_cast<uint32_t>(u % blocks) * 64 + lane;
+        const uint64_t bc = u / blocks, b = bc / f.nchunk;
+        const uint64_t r0 = (bc % f.nchunk) * f.chunk;
+        const uint32_t rows = min(f.chunk, static_cast<uint32_t>(f.pixels - r0));
+        float s1 = 0.0f, s2 = 0.0f;
+        if (c < f.C) {
+            const Stat st = f.stats[b * f.groups + c / f.cg];
+            const Coef one = coef(st, 1.0f, 0.0f);
+            const float gamma = f.gamma ? f.gamma[c] : 1.0f, beta = f.beta ? f.beta[c] : 0.0f;
+            const TX* x = static_cast<const TX*>(f.x) + b * f.sx + r0 * f.ldx + c;
+            const TD* dy = static_cast<const TD*>(a.dy) + b * a.sdy + r0 * a.lddy + c;
+            for (uint32_t r = grp; r < rows; r += 4) {
+                const float xh = apply(static_cast<float>(x[r * f.ldx]), one);
+                const float w = static_cast<float>(dy[r * a.lddy]) * slope<ACT>(__builtin_fmaf(xh, gamma, beta));
+                s1 += w;
+                s2 += w * xh;
+            }
+        }
+        sums[0][grp][lane] = s1;
+        sums[1][grp][lane] = s2;
+        __syncthreads();
+        if (grp < 2 && c < f.C)
+            a.cpart[(bc * 2 + grp) * f.C + c] = ((sums[grp][0][lane] + sums[grp][1][lane]) + sums[grp][2][lane]) + sums[grp][3][lane];
+        __syncthreads();  // the sums are free for the next unit
+    }
+}
+
+// A group's sums over the chunks' columns (a wave each), in 64 bits.
+__global__ __launch_bounds__(256) void gn_bwd_groups_kernel(GnBwdArgs a) {
+    const GnArgs& f = a.f;
+    const uint32_t lane = threadIdx.x & 63;
+    const uint64_t units = static_cast<uint64_t>(f.batch) * f.groups;
+    for (uint64_t u = blockIdx.x * 4ull + (threadIdx.x >> 6); u < units; u += gridDim.x * 4ull) {
+        const uint64_t b = u / f.groups;
+        const uint32_t c0 = static_cast<uint32_t>(u % f.groups) * f.cg;
+        const float* p = a.cpart + b * f.nchunk * 2 * f.C;
+        double s1 = 0.0, s2 = 0.0;
+        for (uint32_t k = 0; k < f.nchunk; ++k, p += 2ull * f.C)
+            for (uint32_t c = lane; c < f.cg; c += 64) {
+                const double gamma = f.gamma ? static_cast<double>(f.gamma[c0 + c]) : 1.0;
+                s1 += gamma * static_cast<double>(p[c0 + c]);
+                s2 += gamma * static_cast<double>(p[f.C + c0 + c]);
+            }
+        const double n = static_cast<double>(f.pixels) * f.cg;
+        s1 = wave_sum(s1) / n;
+        s2 = wave_sum(s2) / n;
+        if (lane == 0) {
+            a.gsum[2 * u] = static_cast<float>(s1);
+            a.gsum[2 * u + 1] = static_cast<float>(s2);
+        }
+    }
+}
+
+// dgamma and dbeta: 64 channels at a time, four groups of partial rows, in 64 bits. parts == 0: sums over nothing.
+__global__ __launch_bounds__(256) void gn_bwd_params_kernel(const float* cpart, float* dgamma, float* dbeta, uint64_t parts, uint32_t C) {
+    __shared__ double sums[2][4][64];
+    const uint32_t lane = threadIdx.x & 63, grp = threadIdx.x >> 6;
+    for (uint32_t c0 = blockIdx.x * 64; c0 < C; c0 += gridDim.x * 64) {
+        const uint32_t c = c0 + lane;
+        double s1 = 0.0, s2 = 0.0;
+        if (c < C)
+            for (uint64_t p = grp; p < parts; p += 4) {
+                s1 += static_cast<double>(cpart[p * 2 * C + c]);
+                s2 += static_cast<double>(cpart[(p * 2 + 1) * C + c]);
+            }
+        sums[0][grp][lane] = s1;
+        sums[1][grp][lane] = s2;
+        __syncthreads();
+        if (grp < 2 && c < C) {
+            const double s = (sums[grp][0][lane] + sums[grp][1][lane]) + (sums[grp][2][lane] + sums[grp][3][lane]);
+            (grp ? dgamma : dbeta)[c] = static_cast<float>(s);
+        }
+        __syncthreads();
+    }
+}
+
+template <typename TX, typename TD, int ACT>
+__global__ __launch_bounds__(256) void gn_bwd_apply_any_kernel(GnBwdArgs a) {
+    const GnArgs& f = a.f;
+    const uint32_t lane = threadIdx.x & 63;
+    const uint64_t rows = static_cast<uint64_t>(f.batch) * f.pixels;
+    for (uint64_t row = blockIdx.x * 4ull + (threadIdx.x >> 6); row < rows; row += gridDim.x * 4ull) {
+        const uint64_t b = row / f.pixels, r = row % f.pixels;
+        const TX* x = static_cast<const TX*>(f.x) + b * f.sx + r * f.ldx;
+        const TD* dy = static_cast<const TD*>(a.dy) + b * a.sdy + r * a.lddy;
+        const TX* res = a.res ? static_cast<const TX*>(a.res) + b * a.sres + r * a.ldres : nullptr;
+        TX* dx = static_cast<TX*>(a.dx) + b * a.sdx + r * a.lddx;
+        for (uint32_t c = lane; c < f.C; c += 64) {
+            const uint64_t g = b * f.groups + c / f.cg;
+            const Stat st = f.stats[g];
+            const float gamma = f.gamma ? f.gamma[c] : 1.0f, beta = f.beta ? f.beta[c] : 0.0f;
+            const float xh = apply(static_cast<float>(x[c]), coef(st, 1.0f, 0.0f));
+            const float w = static_cast<float>(dy[c]) * slope<ACT>(__builtin_fmaf(xh, gamma, beta));
+            const float t = __builtin_fmaf(w, gamma, -a.gsum[2 * g]);
+            const float d = st.inv * __builtin_fmaf(-xh, a.gsum[2 * g + 1], t);
+            dx[c] = static_cast<TX>(res ? d + static_cast<float>(res[c]) : d);
+        }
+    }
+}
+
+// ---- host ------------------------------------------------------------------------------
+
+constexpr uint32_t kMaxBatch = 1u << 20, kMaxChannels = 1u << 20;
+constexpr uint64_t kMaxRows = 1ull << 31;
+
+void set_chunks(GnArgs& a) {
+    const uint64_t most = std::max<uint64_t>((static_cast<uint64_t>(a.pixels) + kChunkMin - 1) / kChunkMin, 1);
+    const uint64_t least = std::max<uint64_t>((static_cast<uint64_t>(a.pixels) + kChunkMax - 1) / kChunkMax, 1);
+    const uint64_t want = std::max<uint64_t>(std::min<uint64_t>(most, kChunks / std::max(a.batch, 1u)), least);
+    a.chunk = ceil_div(std::max(a.pixels, 1u), want);
+    a.nchunk = ceil_div(std::max(a.pixels, 1u), a.chunk);
+}
+
+bool sizes_ok(uint32_t batch, uint32_t pixels, uint32_t channels, uint32_t groups) {
+    return channels != 0 && groups != 0 && channels % groups == 0 && batch <= kMaxBatch && channels <= kMaxChannels &&
+           static_cast<uint64_t>(batch) * pixels <= kMaxRows;
+}
+
+uint64_t up(uint64_t n) { return (n + 255) / 256 * 256; }
+uint64_t stat_bytes(const GnArgs& a) { return up(static_cast<uint64_t>(a.batch) * a.groups * sizeof(Stat)); }
+uint64_t part_bytes(const GnArgs& a) { return up(static_cast<uint64_t>(a.batch) * a.nchunk * a.groups * sizeof(Part)); }
+uint64_t cpart_bytes(const GnArgs& a) { return up(static_cast<uint64_t>(a.batch) * a.nchunk * 2 * a.C * 4); }
+uint64_t gsum_bytes(const GnArgs& a) { return up(static_cast<uint64_t>(a.batch) * a.groups * 8); }
+
+GnArgs sized(uint32_t batch, uint32_t pixels, uint32_t channels, uint32_t groups) {
+    GnArgs a{};
+    a.batch = batch;
+    a.pixels = pixels;
+    a.C = channels;
+    a.groups = groups;
+    a.cg = channels / groups;
+    set_chunks(a);
+    return a;
+}
+
+unsigned grid_of(uint64_t units) { return static_cast<unsigned>(std::min<uint64_t>(units, kMaxGrid)); }
+
+struct Span {
+    const void* p;
+    uint64_t bytes;
+};
+// The bytes from a strided tensor's first element to behind its last; false where that passes 2^62.
+bool span(const void* p, uint32_t batch, uint32_t pixels, uint32_t C, uint64_t ld, uint64_t s, uint64_t esz, Span& out) {
+    const __uint128_t last = static_cast<__uint128_t>(batch - 1) * s + static_cast<__uint128_t>(pixels - 1) * ld + C;
+    if (last > (static_cast<__uint128_t>(1) << 60)) return false;
+    out = Span{p, static_cast<uint64_t>(last) * esz};
+    return true;
+}
+// Whether no two rows of an output overlap: image after image, or the images' rows in turn.
+bool rows_apart(uint32_t batch, uint32_t pixels, uint32_t C, uint64_t ld, uint64_t s) {
+    if (batch <= 1) return true;
+    const __uint128_t image = static_cast<__uint128_t>(pixels - 1) * ld + C;
+    if (pixels <= 1) return s >= C;
+    return s >= image || (s >= C && ld >= static_cast<__uint128_t>(batch - 1) * s + C);
+}
+
+uint64_t esize(int dtype) { return dtype == MI_F32 ? 4 : dtype == MI_F16 ? 2 : 1; }
+
+// What both directions check of the forward call's arguments, strides filled in. need_y: the forward call itself.
+int check_args(const char* fn, const mi_groupnorm_args* g, GnArgs& a, bool need_y, Span& x, Span& y) {
+    if (!g) return fail(MI_ERR_INVALID_ARG, "%s: null arguments", fn);
+    if (g->x_dtype != MI_F32 && g->x_dtype != MI_F16) return fail(MI_ERR_INVALID_ARG, "%s: x_dtype %d", fn, g->x_dtype);
+    if (g->y_dtype != MI_F32 && g->y_dtype != MI_F16 && !(need_y && g->y_dtype == MI_I8))
+        return fail(MI_ERR_INVALID_ARG, "%s: y_dtype %d", fn, g->y_dtype);
+    if (g->act != MI_ACT_NONE && g->act != MI_ACT_SILU) return fail(MI_ERR_INVALID_ARG, "%s: act %d", fn, g->act);
+    if (!(g->eps >= 0.0f) || g->eps > 3.4e38f) return fail(MI_ERR_INVALID_ARG, "%s: eps %g", fn, static_cast<double>(g->eps));
+    if (g->channels == 0 || g->groups == 0 || g->channels % g->groups != 0)
+        return fail(MI_ERR_INVALID_ARG, "%s: %u channels in %u groups", fn, g->channels, g->groups);
+    if (!sizes_ok(g->batch, g->pixels, g->channels, g->groups))
+        return fail(MI_ERR_UNSUPPORTED, "%s: batch %u > 2^20, batch * pixels > 2^31 or channels %u > 2^20", fn, g->batch, g->channels);
+    a = sized(g->batch, g->pixels, g->channels, g->groups);
+    a.x = g->x;
+    a.gamma = g->gamma;
+    a.beta = g->beta;
+    a.y = g->y;
+    a.y_scale = g->y_scale;
+    a.eps = g->eps;
+    a.ldx = g->ldx ? g->ldx : g->channels;
+    a.ldy = g->ldy ? g->ldy : g->channels;
+    a.sx = g->sx ? g->sx : a.ldx * g->pixels;
+    a.sy = g->sy ? g->sy : a.ldy * g->pixels;
+    if (g->batch == 0 || g->pixels == 0) return MI_OK;
+    if (!g->x || (need_y && !g->y)) return fail(MI_ERR_INVALID_ARG, "%s: null pointer", fn);
+    if (need_y && (g->y_dtype == MI_I8) != (g->y_scale != nullptr))
+        return fail(MI_ERR_INVALID_ARG, "%s: y_scale belongs to MI_I8 rows", fn);
+    if (a.ldx < g->channels || (need_y && a.ldy < g->channels))
+        return fail(MI_ERR_INVALID_ARG, "%s: a row stride below %u channels", fn, g->channels);
+    if (!span(a.x, a.batch, a.pixels, a.C, a.ldx, a.sx, esize(g->x_dtype), x) ||
+        (need_y && !span(a.y, a.batch, a.pixels, a.C, a.ldy, a.sy, esize(g->y_dtype), y)))
+        return fail(MI_ERR_UNSUPPORTED, "%s: a tensor spans 2^60 elements or more", fn);
+    if (need_y && !rows_apart(a.batch, a.pixels, a.C, a.ldy, a.sy))
+        return fail(MI_ERR_INVALID_ARG, "%s: rows of y overlap each other", fn);
+    if (!aligned(a.x, esize(g->x_dtype)) || (need_y && !aligned(a.y, esize(g->y_dtype))) || !aligned(a.gamma, 4) || !aligned(a.beta, 4) ||
+        !aligned(a.y_scale, 4))
+        return fail(MI_ERR_ALIGNMENT, "%s: tensors must be aligned to their element size", fn);
+    if (!aligned(g->stats, 16)) return fail(MI_ERR_ALIGNMENT, "%s: stats must be 16-byte aligned", fn);
+    return MI_OK;
+}
+
+// No output overlaps an input or another output; same[o] (or -1) names the input that output o may be itself.
+int check_overlaps(const char* fn, const Span* out, int nout, const Span* in, int nin, int may_o, int may_i) {
+    for (int o = 0; o < nout; ++o) {
+        for (int i = 0; i < nin; ++i)
+            if (overlaps(out[o].p, out[o].bytes, in[i].p, in[i].bytes) && !(o == may_o && i == may_i && out[o].p == in[i].p))
+                return fail(MI_ERR_ALIASING, "%s: an output or the workspace overlaps an input", fn);
+        for (int q = 0; q < o; ++q)
+            if (overlaps(out[o].p, out[o].bytes, out[q].p, out[q].bytes))
+                return fail(MI_ERR_ALIASING, "%s: outputs or the workspace overlap each other", fn);
+    }
+    return MI_OK;
+}
+
+int check_ws(const char* fn, const void* ws, uint64_t have, uint64_t need) {
+    if (!ws || have < need)
+        return fail(MI_ERR_INVALID_ARG, "%s: workspace %llu bytes < %llu needed", fn, static_cast<unsigned long long>(ws ? have : 0),
+                    static_cast<unsigned long long>(need));
+    if (!aligned(ws, 16)) return fail(MI_ERR_ALIGNMENT, "%s: workspace must be 16-byte aligned", fn);
+    return MI_OK;
+}
+
+template <typename TX>
+void launch_stats(const GnArgs& a, hipStream_t s) {
+    gn_part_any_kernel<TX><<<grid_of(static_cast<uint64_t>(a.batch) * a.nchunk * a.groups), 256, 0, s>>>(a);
+    gn_join_kernel<<<grid_of((static_cast<uint64_t>(a.batch) * a.groups + 3) / 4), 256, 0, s>>>(a);
+}
+
+template <typename TX, typename TY>
+void launch_apply(const GnArgs& a, int act, hipStream_t s) {
+    const unsigned grid = grid_of((static_cast<uint64_t>(a.batch) * a.pixels + 3) / 4);
+    if (act == MI_ACT_SILU) gn_apply_any_kernel<TX, TY, MI_ACT_SILU><<<grid, 256, 0, s>>>(a);
+    else gn_apply_any_kernel<TX, TY, MI_ACT_NONE><<<grid, 256, 0, s>>>(a);
+}
+
+template <typename TX>
+void launch_forward(const GnArgs& a, int y_dtype, int act, hipStream_t s) {
+    launch_stats<TX>(a, s);
+    if (y_dtype == MI_F32) launch_apply<TX, float>(a, act, s);
+    else if (y_dtype == MI_F16) launch_apply<TX, _Float16>(a, act, s);
+    else launch_apply<TX, int8_t>(a, act, s);
+}
+
+template <typename TX, typename TD, int ACT>
+void launch_backward(const GnBwdArgs& a, bool stats, hipStream_t s) {
+    const GnArgs& f = a.f;
+    if (stats) launch_stats<TX>(f, s);
+    gn_bwd_cols_any_kernel<TX, TD, ACT><<<grid_of(static_cast<uint64_t>(f.batch) * f.nchunk * ceil_div(f.C, 64)), 256, 0, s>>>(a);
+    gn_bwd_groups_kernel<<<grid_of((static_cast<uint64_t>(f.batch) * f.groups + 3) / 4), 256, 0, s>>>(a);
+    if (a.dgamma)
+        gn_bwd_params_kernel<<<grid_of(ceil_div(f.C, 64)), 256, 0, s>>>(a.cpart, a.dgamma, a.dbeta, static_cast<uint64_t>(f.batch) * f.nchunk, f.C);
+    gn_bwd_apply_any_kernel<TX, TD, ACT><<<grid_of((static_cast<uint64_t>(f.batch) * f.pixels + 3) / 4), 256, 0, s>>>(a);
+}
+
+template <typename TX, typename TD>
+void launch_backward(const GnBwdArgs& a, int act, bool stats, hipStream_t s) {
+    if (act == MI_ACT_SILU) launch_backward<TX, TD, MI_ACT_SILU>(a, stats, s);
+    else launch_backward<TX, TD, MI_ACT_NONE>(a, stats, s);
+}
+
+}  // namespace
+}  // namespace mi
+
+using namespace mi;
+
+extern "C" uint64_t mi_groupnorm_ws_bytes(uint32_t batch, uint32_t pixels, uint32_t channels, uint32_t groups) {
+    if (!sizes_ok(batch, pixels, channels, groups) || batch == 0 || pixels == 0) return 0;
+    const GnArgs a = sized(batch, pixels, channels, groups);
+    return stat_bytes(a) + part_bytes(a);
+}
+
+extern "C" int mi_groupnorm(const mi_groupnorm_args* args, void* workspace, uint64_t workspace_bytes, void* stream) {
+    const char* fn = "mi_groupnorm";
+    GnArgs a;
+    Span x{}, y{};
+    if (int st = check_args(fn, args, a, true, x, y)) return st;
+    if (a.batch == 0 || a.pixels == 0) return MI_OK;
+    const uint64_t need = mi_groupnorm_ws_bytes(a.batch, a.pixels, a.C, a.groups), cols = static_cast<uint64_t>(a.C) * 4;
+    if (int st = check_ws(fn, workspace, workspace_bytes, need)) return st;
+    const Span in[3] = {x, {a.gamma, cols}, {a.beta, cols}};
+    const Span out[4] = {y, {a.y_scale, static_cast<uint64_t>(a.batch) * a.pixels * 4},
+                         {args->stats, static_cast<uint64_t>(a.batch) * a.groups * sizeof(Stat)}, {workspace, need}};
+    if (int st = check_overlaps(fn, out, 4, in, 3, -1, -1)) return st;
+    a.stats = args->stats ? reinterpret_cast<Stat*>(args->stats) : static_cast<Stat*>(workspace);
+    a.part = reinterpret_cast<Part*>(static_cast<char*>(workspace) + stat_bytes(a));
+    hipStream_t s = static_cast<hipStream_t>(stream);
+    if (args->x_dtype == MI_F32) launch_forward<float>(a, args->y_dtype, args->act, s);
+    else launch_forward<_Float16>(a, args->y_dtype, args->act, s);
+    return check_launch(fn);
+}
+
+extern "C" uint64_t mi_groupnorm_bwd_ws_bytes(uint32_t batch, uint32_t pixels, uint32_t channels, uint32_t groups) {
+    if (!sizes_ok(batch, pixels, channels, groups) || batch == 0 || pixels == 0) return 0;
+    const GnArgs a = sized(batch, pixels, channels, groups);
+    return stat_bytes(a) + part_bytes(a) + gsum_bytes(a) + cpart_bytes(a);
+}
+
+extern "C" int mi_groupnorm_bwd(const mi_groupnorm_bwd_args* args, void* workspace, uint64_t workspace_bytes, void* stream) {
+    const char* fn = "mi_groupnorm_bwd";
+    if (!args) return fail(MI_ERR_INVALID_ARG, "%s: null arguments", fn);
+    GnBwdArgs a{};
+    Span x{}, none{}, dy{}, res{}, dx{};
+    if (int st = check_args(fn, &args->fwd, a.f, false, x, none)) return st;
+    const GnArgs& f = a.f;
+    const mi_groupnorm_args& g = args->fwd;
+    if ((args->dgamma == nullptr) != (args->dbeta == nullptr)) return fail(MI_ERR_INVALID_ARG, "%s: dgamma and dbeta go together", fn);
+    if (!aligned(args->dgamma, 4) || !aligned(args->dbeta, 4))
+        return fail(MI_ERR_ALIGNMENT, "%s: tensors must be aligned to their element size", fn);
+    a.dgamma = args->dgamma;
+    a.dbeta = args->dbeta;
+    const uint64_t cols = static_cast<uint64_t>(f.C) * 4;
+    hipStream_t s = static_cast<hipStream_t>(stream);
+    if (f.batch == 0 || f.pixels == 0) {
+        if (!a.dgamma) return MI_OK;
+        if (overlaps(a.dgamma, cols, a.dbeta, cols)) return fail(MI_ERR_ALIASING, "%s: outputs overlap each other", fn);
+        gn_bwd_params_kernel<<<grid_of(ceil_div(f.C, 64)), 256, 0, s>>>(nullptr, a.dgamma, a.dbeta, 0, f.C);
+        return check_launch(fn);
+    }
+    if (!args->dy || !args->dx) return fail(MI_ERR_INVALID_ARG, "%s: null pointer", fn);
+    a.dy = args->dy;
+    a.res = args->res;
+    a.dx = args->dx;
+    a.lddy = args->lddy ? args->lddy : f.C;
+    a.ldres = args->ldres ? args->ldres : f.C;
+    a.lddx = args->lddx ? args->lddx : f.C;
+    a.sdy = args->sdy ? args->sdy : a.lddy * f.pixels;
+    a.sres = args->sres ? args->sres : a.ldres * f.pixels;
+    a.sdx = args->sdx ? args->sdx : a.lddx * f.pixels;
+    if (a.lddy < f.C || a.lddx < f.C || (a.res && a.ldres < f.C))
+        return fail(MI_ERR_INVALID_ARG, "%s: a row stride below %u channels", fn, f.C);
+    const uint64_t ex = esize(g.x_dtype), ed = esize(g.y_dtype);
+    if (!span(a.dy, f.batch, f.pixels, f.C, a.lddy, a.sdy, ed, dy) || !span(a.dx, f.batch, f.pixels, f.C, a.lddx, a.sdx, ex, dx) ||
+        (a.res && !span(a.res, f.batch, f.pixels, f.C, a.ldres, a.sres, ex, res)))
+        return fail(MI_ERR_UNSUPPORTED, "%s: a tensor spans 2^60 elements or more", fn);
+    if (!rows_apart(f.batch, f.pixels, f.C, a.lddx, a.sdx)) return fail(MI_ERR_INVALID_ARG, "%s: rows of dx overlap each other", fn);
+    if (!aligned(a.dy, ed) || !aligned(a.dx, ex) || !aligned(a.res, ex))
+        return fail(MI_ERR_ALIGNMENT, "%s: tensors must be aligned to their element size", fn);
+    const uint64_t need = mi_groupnorm_bwd_ws_bytes(f.batch, f.pixels, f.C, f.groups);
+    if (int st = check_ws(fn, workspace, workspace_bytes, need)) return st;
+    const Span in[6] = {x, {f.gamma, cols}, {f.beta, cols}, dy, {g.stats, static_cast<uint64_t>(f.batch) * f.groups * sizeof(Stat)}, res};
+    const Span out[4] = {dx, {a.dgamma, cols}, {a.dbeta, cols}, {workspace, need}};
+    // dx may be res itself: a value is read before it is written, by the same lane
+    const bool same = a.res == a.dx && a.ldres == a.lddx && a.sres == a.sdx;
+    if (int st = check_overlaps(fn, out, 4, in, 6, same ? 0 : -1, 5)) return st;
+    char* ws = static_cast<char*>(workspace);
+    a.f.stats = g.stats ? reinterpret_cast<Stat*>(g.stats) : reinterpret_cast<Stat*>(ws);
+    a.f.part = reinterpret_cast<Part*>(ws + stat_bytes(f));
+    a.gsum = reinterpret_cast<float*>(ws + stat_bytes(f) + part_bytes(f));
+    a.cpart = reinterpret_cast<float*>(ws + stat_bytes(f) + part_bytes(f) + gsum_bytes(f));
+    const bool stats = !g.stats;
+    if (g.x_dtype == MI_F32) {
+        if (g.y_dtype == MI_F32) launch_backward<float, float>(a, g.act, stats, s);
+        else launch_backward<float, _Float16>(a, g.act, stats, s);
+    } else {
+        if (g.y_dtype == MI_F32) launch_backward<_Float16, float>(a, g.act, stats, s);
+        else launch_backward<_Float16, _Float16>(a, g.act, stats, s);
+    }
+    return check_launch(fn);
+}

@@ -16,6 +16,8 @@ Names, argument meaning and error behaviour follow the reference
   BlockWeights / BlockDims / sdxl_block_forward (one transformer block)
       sdvkgen.cpp:1739-1763 with crossAttention :1283-1290
   block_ctx_kv / sdxl_block_forward_kv (the block with cached context K / V)
+  groupnorm / quantize_rows_i8 / gemm_nt_i8: GroupNorm with its activation,
+      8-bit rows and their product (extensions)
   *_bwd: gradients of these operators for fine-tuning on frozen Q8_0 weights
       (extension: the reference's SDXL path only runs forward)
 
@@ -31,8 +33,9 @@ from typing import Optional, Sequence
 
 from . import _lib
 from ._lib import (MI_ATTN_PREC_AUTO, MI_ATTN_PREC_FP16, MI_ATTN_PREC_SPLIT, MI_BLOCK_FP16_ACTIVATIONS,
-                   MI_BLOCK_FP16_ATTENTION, MI_BLOCK_FUSED_EPILOGUES, MI_BLOCK_JOINT_QKV, MI_F16, MI_F32, MiAttnArgs,
-                   MiAttnBwdArgs, MiBlockDims, MiBlockWeights, MiError, call, ptr)
+                   MI_BLOCK_FP16_ATTENTION, MI_BLOCK_FUSED_EPILOGUES, MI_BLOCK_JOINT_QKV, MI_F16, MI_F32, MI_I8, MI_ACT_NONE,
+                   MI_ACT_SILU, MiAttnArgs, MiAttnBwdArgs, MiBlockDims, MiBlockWeights, MiError, MiGroupnormArgs,
+                   MiGroupnormBwdArgs, call, ptr)
 
 __all__ = [
     "MiError", "MI_F32", "MI_F16", "MI_ATTN_PREC_AUTO", "MI_ATTN_PREC_FP16", "MI_ATTN_PREC_SPLIT",
@@ -46,6 +49,8 @@ __all__ = [
     "BlockWeights", "BlockDims", "block_workspace_bytes", "sdxl_block_forward", "block_ctx_kv_bytes", "block_ctx_kv",
     "sdxl_block_forward_kv", "gemm_nt_q8_0_bwd", "gemm_bwd_workspace_bytes", "gemm_nt_q8_0_geglu_bwd", "geglu_bwd",
     "layernorm_bwd", "layernorm_bwd_ws_bytes", "fused_attention_bwd", "fused_attention_bwd_ws_bytes",
+    "MI_I8", "MI_ACT_NONE", "MI_ACT_SILU", "groupnorm", "groupnorm_ws_bytes", "groupnorm_bwd", "groupnorm_bwd_ws_bytes",
+    "quantize_rows_i8", "gemm_nt_i8",
 ]
 
 
@@ -427,6 +432,55 @@ def layernorm_bwd(x, gamma, dy, dx, dgamma, dbeta, workspace, rows: int, d: int,
     """Gradients of layernorm: dx (+ res), and dgamma / dbeta unless None (mi_layernorm_bwd)."""
     call("mi_layernorm_bwd", ptr(x), ptr(gamma), ptr(dy), dy_dtype, ptr(res), ptr(dx), ptr(dgamma), ptr(dbeta), rows, d, eps,
          *_ws(workspace), _s(stream))
+
+
+# -------------------------------------------------- GroupNorm and 8-bit linears --
+
+def groupnorm_ws_bytes(*, batch: int, pixels: int, C: int, groups: int) -> int:
+    """Workspace groupnorm needs for these sizes."""
+    return int(_lib.load().mi_groupnorm_ws_bytes(batch, pixels, C, groups))
+
+
+def groupnorm(x, gamma, beta, y, workspace, *, batch: int, pixels: int, C: int, groups: int, act: int = MI_ACT_NONE, eps: float = 1e-5,
+              x_dtype: int = MI_F32, y_dtype: int = MI_F32, y_scale=None, stats=None, ldx: int = 0, ldy: int = 0, sx: int = 0,
+              sy: int = 0, stream=None) -> None:
+    """GroupNorm (+ SiLU) of channels-last x (mi_groupnorm); y_dtype MI_I8 leaves rows of codes with scales in y_scale. stats:
+    batch * groups * 4 floats kept for groupnorm_bwd."""
+    a = MiGroupnormArgs(ptr(x), ptr(gamma), ptr(beta), ptr(y), ptr(y_scale), ptr(stats), batch, pixels, C, groups, x_dtype, y_dtype,
+                        act, eps, ldx, ldy, sx, sy)
+    wp, wn = _ws(workspace)
+    call("mi_groupnorm", ctypes.byref(a), wp, wn, _s(stream))
+
+
+def groupnorm_bwd_ws_bytes(*, batch: int, pixels: int, C: int, groups: int) -> int:
+    """Workspace groupnorm_bwd needs for these sizes."""
+    return int(_lib.load().mi_groupnorm_bwd_ws_bytes(batch, pixels, C, groups))
+
+
+def groupnorm_bwd(x, gamma, beta, dy, dx, dgamma, dbeta, workspace, *, batch: int, pixels: int, C: int, groups: int,
+                  act: int = MI_ACT_NONE, eps: float = 1e-5, x_dtype: int = MI_F32, dy_dtype: int = MI_F32, res=None, stats=None,
+                  ldx: int = 0, lddy: int = 0, lddx: int = 0, ldres: int = 0, sx: int = 0, sdy: int = 0, sdx: int = 0, sres: int = 0,
+                  stream=None) -> None:
+    """Gradients of groupnorm: dx (+ res) of x's type, and dgamma / dbeta unless None (mi_groupnorm_bwd). stats: what the
+    forward call kept, or None: computed again."""
+    f = MiGroupnormArgs(ptr(x), ptr(gamma), ptr(beta), None, None, ptr(stats), batch, pixels, C, groups, x_dtype, dy_dtype, act, eps,
+                        ldx, 0, sx, 0)
+    a = MiGroupnormBwdArgs(f, ptr(dy), ptr(res), ptr(dx), ptr(dgamma), ptr(dbeta), lddy, ldres, lddx, sdy, sres, sdx)
+    wp, wn = _ws(workspace)
+    call("mi_groupnorm_bwd", ctypes.byref(a), wp, wn, _s(stream))
+
+
+def quantize_rows_i8(x, q, scale, rows: int, cols: int, *, dtype: int = MI_F32, ldx: int = 0, ldq: int = 0, stream=None) -> None:
+    """Codes q = x / scale, scale = max|x| / 127 of each row (mi_quantize_rows_i8)."""
+    call("mi_quantize_rows_i8", ptr(x), dtype, ptr(q), ptr(scale), rows, cols, ldx, ldq, _s(stream))
+
+
+def gemm_nt_i8(A, a_scale, W, w_scale, C, M: int, N: int, K: int, *, bias=None, c_dtype: int = MI_F32, mode: int = 0, lda: int = 0,
+               ldw: int = 0, ldc: int = 0, stream=None) -> None:
+    """C[m,n] = a_scale[m] w_scale[n] (A . W^T)[m,n] + bias[n] of 8-bit codes, the sum exact (mi_gemm_nt_i8); mode 1 adds,
+    mode 2 adds with the bias."""
+    call("mi_gemm_nt_i8", ptr(A), ptr(a_scale), ptr(W), ptr(w_scale), ptr(bias), ptr(C), c_dtype, M, N, K, mode, lda, ldw, ldc,
+         _s(stream))
 
 
 # --------------------------------------------- reference kernel-name dispatch --

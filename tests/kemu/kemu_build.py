@@ -31,7 +31,8 @@ LIB = OUT / "libkemu_sdvk.so"
 CXX = os.environ.get("KEMU_CXX", "/opt/rocm/llvm/bin/clang++")
 
 SOURCES = ["status.hip", "q8_0.hip", "gemm_q8.hip", "gemm_nn_q8.hip", "attention.hip", "glue.hip", "block.hip",
-           "glue_bwd.hip", "gemm_q8_bwd.hip", "attention_bwd.hip", "gguf.cpp"]
+           "glue_bwd.hip", "gemm_q8_bwd.hip", "attention_bwd.hip", "groupnorm.hip", "gemm_i8.hip",
+           "gguf.cpp"]
 FLAGS = ["-std=c++17", "-O2", "-g0", "-fPIC", "-fno-strict-aliasing", "-Xclang", "-ffloat16-excess-precision=none",
          "-Wno-unused-command-line-argument", "-Wno-psabi"]
 
@@ -58,7 +59,7 @@ def transform(text: str) -> str:
 
 
 def _inputs() -> list[Path]:
-    return ([CSRC / s for s in SOURCES] + [CSRC / "common.hpp", ROOT / "include" / "mi_sdvk.h", HERE / "kemu.cpp",
+    return ([CSRC / s for s in SOURCES] + [CSRC / "common.hpp", CSRC / "quant.hpp", ROOT / "include" / "mi_sdvk.h", HERE / "kemu.cpp",
              HERE / "kemu.hpp", HERE / "include" / "hip" / "hip_runtime.h", Path(__file__).resolve()])
 
 
@@ -79,7 +80,8 @@ def build(force: bool = False) -> Path:
     (OUT / "src").mkdir(parents=True, exist_ok=True)
     inc = ["-I", str(HERE / "include"), "-I", str(CSRC), "-I", str(ROOT / "include")]
     # next to the rewritten sources, where their quoted includes look first
-    (OUT / "src" / "common.hpp").write_text(transform((CSRC / "common.hpp").read_text()))
+    for h in ("common.hpp", "quant.hpp"):
+        (OUT / "src" / h).write_text(transform((CSRC / h).read_text()))
     jobs = []
     for s in SOURCES:
         dst = OUT / "src" / (Path(s).stem + ".cpp")
