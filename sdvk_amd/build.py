@@ -74,7 +74,7 @@ def build(save_temps: str | None = None, verbose: bool = False) -> Path:
         with concurrent.futures.ThreadPoolExecutor(max_workers=len(jobs)) as ex:
             list(ex.map(lambda j: _run(j[0], cwd, verbose), jobs))
         link = [hipcc(), "--offload-arch=gfx950", "-shared", "-fPIC", *[o for _, o in jobs],
-                "-o", str(LIB) + ".tmp", f"-Wl,-rpath,{ROCM / 'lib'}"]
+                "-o", str(LIB) + ".tmp", f"-Wl,-rpath,{ROCM / 'lib'}", "-Wl,-z,defs"]
         _run(link, cwd, verbose)
     os.replace(str(LIB) + ".tmp", LIB)
     return LIB

@@ -34,6 +34,7 @@ int check_launch(const char* what);
 // rows (their own kernel does not round the weights, the tiles do).
 constexpr int kGemmBuilds = 7;  // tile builds of gemm_q8.hip (kNumCfg)
 constexpr int kGemmBwdBuilds = 4;  // tile builds of gemm_q8_bwd.hip
+constexpr int kGemmI8Builds = 10;  // builds of gemm_i8.hip
 struct Tuning {
     std::atomic<int> gemm_cfg{-1};          // tile build, or -1
     std::atomic<int> gemm_splits{1};        // K splits with gemm_cfg (workspace entries)
@@ -46,6 +47,7 @@ struct Tuning {
     std::atomic<int> attn_simd_waves{0};    // fp16 attention build: 2 or 3 waves per SIMD, or 0
     std::atomic<int> gemm_bwd_cfg{-1};      // input-gradient GEMM tile build, or -1
     std::atomic<int> gemm_bwd_splits{1};    // N parts with gemm_bwd_cfg (with a workspace)
+    std::atomic<int> gemm_i8_cfg{-1};       // 8-bit product's build, or -1
 };
 Tuning& tuning();
 

@@ -8,12 +8,14 @@
 #include "quant.hpp"
 
 #include <algorithm>
+#include <type_traits>
 
 namespace mi {
 namespace {
 
 constexpr uint32_t kMaxGrid = 1u << 20;  // workgroups of a launch that strides over its units
 constexpr uint32_t kMaxK = 131071;       // 2^31 / 2^14
+constexpr uint64_t kMaxLd = 1u << 22;    // row strides that 256 rows address in 31 bits
 
 struct I8Args {
     const int8_t *A, *W;
@@ -21,16 +23,54 @@ struct I8Args {
     void* C;
     uint32_t M, N, K, mode;
     uint64_t lda, ldw, ldc;
+    uint32_t tiles_m, tiles_n, group_m;
+    uint32_t wide;  // C's rows take 16-byte stores
 };
 
-// mode 0 stores, mode 1 adds, mode 2 adds with the bias (NULL for mode 1).
+constexpr uint32_t kPast = 0x80000000u;  // a buffer offset past every record: the load returns zeros
+
+// C from a sum: mode 0 stores, mode 1 adds, mode 2 adds with the bias (NULL for mode 1).
+__device__ __forceinline__ float result(int acc, float sa, float sw, float bias) {
+    return __builtin_fmaf(static_cast<float>(acc) * sa, sw, bias);
+}
 template <typename TC>
 __device__ __forceinline__ void store_one(const I8Args& a, uint32_t m, uint32_t n, int acc, float sa) {
-    const float b = a.bias ? a.bias[n] : 0.0f;
-    float v = __builtin_fmaf(static_cast<float>(acc) * sa, a.sw[n], b);
+    float v = result(acc, sa, a.sw[n], a.bias ? a.bias[n] : 0.0f);
     TC* p = static_cast<TC*>(a.C) + m * a.ldc + n;
     if (a.mode) v += static_cast<float>(*p);
     *p = static_cast<TC>(v);
+}
+
+// The scales and biases of V columns.
+template <int V>
+struct Columns {
+    float sw[V], bias[V];
+};
+// V neighbouring results of row m: whole runs (16-byte aligned, in range), or element by element.
+template <typename TC, int V>
+__device__ __forceinline__ void store_run(const I8Args& a, uint32_t m, uint32_t n, const int (&acc)[V], float sa, const Columns<V>& c, bool whole) {
+    typedef TC Run __attribute__((ext_vector_type(V)));
+    TC* p = static_cast<TC*>(a.C) + m * a.ldc + n;
+    if (whole) {
+        Run r;
+        if (a.mode) {
+            const Run old = *reinterpret_cast<const Run*>(p);
+#pragma unroll
+            for (int e = 0; e < V; ++e) r[e] = static_cast<TC>(result(acc[e], sa, c.sw[e], c.bias[e]) + static_cast<float>(old[e]));
+        } else {
+#pragma unroll
+            for (int e = 0; e < V; ++e) r[e] = static_cast<TC>(result(acc[e], sa, c.sw[e], c.bias[e]));
+        }
+        *reinterpret_cast<Run*>(p) = r;
+        return;
+    }
+#pragma unroll
+    for (int e = 0; e < V; ++e)
+        if (n + e < a.N) {
+            float v = result(acc[e], sa, c.sw[e], c.bias[e]);
+            if (a.mode) v += static_cast<float>(p[e]);
+            p[e] = static_cast<TC>(v);
+        }
 }
 
 // Any K, any alignment: a 64 x 64 tile in steps of 32 codes, 4 x 4 outputs a thread.
@@ -79,6 +119,363 @@ __global__ __launch_bounds__(256) void gemm_i8_any_kernel(I8Args a) {
     }
 }
 
+// ---- tiles ---------------------------------------------------------------------------
+//
+// A workgroup computes a BM x BN tile of C in steps of 128 codes. A step's rows go from memory straight into LDS
+// (buffer loads with an LDS destination: 8 rows of 128 bytes an instruction), two stages deep. An LDS row is 128 bytes, its
+// eight 16-byte slots in the order slot ^ (row / 2) % 8, so that the 16 rows that a fragment read takes at a time lie in
+// different banks; the loads' lanes permute their addresses accordingly (the 128 bytes of a row stay one segment).
+// The product is transposed (W is the MFMA's A operand): a lane holds one row m of C and runs of four columns.
+// Codes past K are zeros in both operands, rows past M or N are out of the resources' range.
+typedef int intx4 __attribute__((ext_vector_type(4)));
+typedef int intx16 __attribute__((ext_vector_type(16)));
+
+__device__ __forceinline__ uint32_t swz(uint32_t row) { return (row >> 1) & 7u; }
+__device__ __forceinline__ void wait_loads() { __builtin_amdgcn_s_waitcnt(0x0F70); }  // vmcnt(0)
+__device__ __forceinline__ void wait_lds() { __builtin_amdgcn_s_waitcnt(0xC07F); }    // lgkmcnt(0)
+
+// 16 bytes a lane from `off` of the `bytes` at base (zeros past them) to LDS: lane l's to dst + 16 l.
+__device__ __forceinline__ void load_lds(const int8_t* base, int bytes, int8_t* dst, uint32_t off) {
+    const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(const_cast<int8_t*>(base), 0, bytes, 0x00020000);
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (__attribute__((address_space(3))) void*)(dst), 16, off, 0, 0, 0);
+}
+
+// Rows of one operand: IT load instructions a wave brings into LDS (rows 8 (IT wave + i) .. + 7).
+template <int IT>
+struct Rows {
+    const int8_t* base;
+    int bytes;                    // that the rows span
+    uint32_t off[IT], col[2], K;  // col: the lane's place in 128 codes, by the parity of its eight rows
+    int at;                       // bytes into a stage
+    // rows r0 .. r0 + count - 1 of X at stride ld
+    __device__ __forceinline__ Rows(const int8_t* X, uint64_t ld, uint32_t r0, uint32_t count, uint32_t K_, int wave, int lane) : K(K_) {
+        base = X + r0 * ld;
+        bytes = static_cast<int>((count - 1) * ld + K);
+        at = wave * IT * 1024;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) col[i] = ((lane & 7) ^ swz(8 * (wave * IT + i) + (lane >> 3))) * 16;
+#pragma unroll
+        for (int i = 0; i < IT; ++i) off[i] = (8 * (wave * IT + i) + (lane >> 3)) * static_cast<uint32_t>(ld) + col[i & 1];
+    }
+    __device__ __forceinline__ void load(int8_t* stage, uint32_t k0) const {
+#pragma unroll
+        for (int i = 0; i < IT; ++i) load_lds(base, bytes, stage + at + i * 1024, k0 + col[i & 1] < K ? off[i] + k0 : kPast);
+    }
+};
+
+// Rows and columns of the tile that workgroup `b` of tiles_m x tiles_n computes: neighbouring workgroups of an XCD share
+// group_m rows of tiles.
+__device__ __forceinline__ void tile_of(const I8Args& a, uint32_t b, uint32_t& tm, uint32_t& tn) {
+    const uint32_t t = xcd_swizzle(b, a.tiles_m * a.tiles_n);
+    const uint32_t per = a.group_m * a.tiles_n, g = t / per, i = t % per;
+    const uint32_t rows = min(a.group_m, a.tiles_m - g * a.group_m);
+    tm = g * a.group_m + i % rows;
+    tn = i / rows;
+}
+
+// A wave's sums of 32 rows and TN columns leave through LDS (a region of its own), so that whole runs of a row are stored.
+template <typename TC, int TN>
+struct Out {
+    static constexpr int kLd = TN + 4, kInts = 32 * kLd;
+    static constexpr int V = 16 / static_cast<int>(sizeof(TC)), LPR = TN / V, RPI = 64 / LPR;  // columns a lane, lanes a row, rows at a time
+};
+
+// KG groups of WM x WN waves take the steps in turn; with two, each hands the other the sums of half its rows at the end.
+template <typename TC, int BM, int BN, int WM, int WN, int KG>
+__global__ __launch_bounds__(KG * WM * WN * 64) void gemm_i8_tile_kernel(I8Args a) {
+    constexpr int NW = WM * WN, TM = BM / WM, TN = BN / WN, FM = TM / 32, FN = TN / 32;
+    constexpr int A_IT = BM / 8 / NW, W_IT = BN / 8 / NW, FO = FM / KG;  // FO: 32-row blocks of a wave's own at the end
+    typedef Out<TC, TN> O;
+    static_assert(BM % (8 * NW) == 0 && BN % (8 * NW) == 0 && FM % KG == 0, "loads and rows divide evenly");
+    constexpr int P = KG * 128 * (BM > BN ? BM : BN) / (O::kInts * 4), Q = KG * 128 * (BM > BN ? BN : BM) / (O::kInts * 4);
+    static_assert(2 * (P + Q) >= KG * NW, "the epilogue's regions fit the stages");
+    static_assert(KG == 1 || (KG == 2 && NW == 4 && FO * FN * 4096 * 2 <= KG * 128 * (BM < BN ? BM : BN)), "the exchanged sums fit the stages");
+    // arrays of their own: the compiler then knows that reads of one stage do not wait for the loads into the other
+    __shared__ __attribute__((aligned(16))) int8_t as0[KG * BM * 128], as1[KG * BM * 128], ws0[KG * BN * 128], ws1[KG * BN * 128];
+    // the tile's scales and biases, read while the first codes are on their way: from memory in the epilogue each would cost a
+    // round trip
+    __shared__ __attribute__((aligned(16))) float sas[BM], sws[BN], biases[BN];
+    const int tid = threadIdx.x, lane = tid & 63;
+    const int wv = __builtin_amdgcn_readfirstlane(tid >> 6), kg = wv / NW, wave = wv % NW;
+    const int l32 = lane & 31, g = lane >> 5, wm = wave % WM, wn = wave / WM;
+    uint32_t tm, tn;
+    tile_of(a, blockIdx.x, tm, tn);
+    const uint32_t m0 = tm * BM, n0 = tn * BN;
+    const Rows<A_IT> ra(a.A, a.lda, m0, min(static_cast<uint32_t>(BM), a.M - m0), a.K, wave, lane);
+    const Rows<W_IT> rw(a.W, a.ldw, n0, min(static_cast<uint32_t>(BN), a.N - n0), a.K, wave, lane);
+    int at[4];  // the lane's piece of a 32-row block, for each 32 codes of a step
+#pragma unroll
+    for (int s = 0; s < 4; ++s) at[s] = l32 * 128 + (((2 * s + g) ^ swz(l32)) * 16);
+    intx16 acc[FM][FN];
+#pragma unroll
+    for (int i = 0; i < FM; ++i)
+#pragma unroll
+        for (int j = 0; j < FN; ++j)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) acc[i][j][r] = 0;
+    // the fragments of the next 32 codes are read ahead of the products of these
+    auto compute = [&](const int8_t* as, const int8_t* ws) {
+        const int8_t* ap = as + kg * BM * 128 + wm * TM * 128;
+        const int8_t* wp = ws + kg * BN * 128 + wn * TN * 128;
+        intx4 x[2][FM], w[2][FN];
+        auto read = [&](auto S) {
+            constexpr int s = decltype(S)::value;
+#pragma unroll
+            for (int i = 0; i < FM; ++i) x[s & 1][i] = *reinterpret_cast<const intx4*>(ap + i * 4096 + at[s]);
+#pragma unroll
+            for (int j = 0; j < FN; ++j) w[s & 1][j] = *reinterpret_cast<const intx4*>(wp + j * 4096 + at[s]);
+        };
+        auto multiply = [&](auto S) {
+            constexpr int s = decltype(S)::value;
+#pragma unroll
+            for (int i = 0; i < FM; ++i)
+#pragma unroll
+                for (int j = 0; j < FN; ++j) acc[i][j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(w[s & 1][j], x[s & 1][i], acc[i][j], 0, 0, 0);
+        };
+        read(std::integral_constant<int, 0>{});
+        __builtin_amdgcn_sched_barrier(0);
+        read(std::integral_constant<int, 1>{});
+        multiply(std::integral_constant<int, 0>{});
+        __builtin_amdgcn_sched_barrier(0);
+        read(std::integral_constant<int, 2>{});
+        multiply(std::integral_constant<int, 1>{});
+        __builtin_amdgcn_sched_barrier(0);
+        read(std::integral_constant<int, 3>{});
+        multiply(std::integral_constant<int, 2>{});
+        __builtin_amdgcn_sched_barrier(0);
+        multiply(std::integral_constant<int, 3>{});
+    };
+    auto load = [&](int8_t* as, int8_t* ws, uint32_t k) {  // past K: zeros
+        ra.load(as + kg * BM * 128, k);
+        rw.load(ws + kg * BN * 128, k);
+    };
+    constexpr uint32_t kStep = 128 * KG;
+    const uint32_t kk = 128 * kg;
+    load(as0, ws0, kk);
+    for (int i = tid; i < BM; i += KG * NW * 64) sas[i] = a.sa[min(m0 + i, a.M - 1)];
+    for (int i = tid; i < BN; i += KG * NW * 64) {
+        sws[i] = a.sw[min(n0 + i, a.N - 1)];
+        biases[i] = a.bias ? a.bias[min(n0 + i, a.N - 1)] : 0.0f;
+    }
+    wait_loads();
+    __syncthreads();
+    // two steps a trip, an odd last one behind them (leaving the loop in its middle would copy every sum)
+    const uint32_t steps = (a.K + kStep - 1) / kStep;
+    uint32_t k = kk;
+    for (uint32_t p = steps / 2; p > 0; --p, k += 2 * kStep) {
+        load(as1, ws1, k + kStep);
+        compute(as0, ws0);
+        wait_loads();
+        __syncthreads();
+        load(as0, ws0, k + 2 * kStep);
+        compute(as1, ws1);
+        wait_loads();
+        __syncthreads();
+    }
+    if (steps & 1) {
+        compute(as0, ws0);
+        __syncthreads();
+    }
+    // (every wave has read its last step, no load is in flight: the stages are free)
+    if constexpr (KG == 2) {
+        int8_t* const space = wave == 0 ? as0 : wave == 1 ? as1 : wave == 2 ? ws0 : ws1;
+        // a wave's slot: (wave, group), its partner's rows in register order
+        intx4* const out = reinterpret_cast<intx4*>(space) + (kg * FO * FN * 4) * 64 + lane;
+#pragma unroll
+        for (int i = 0; i < FO; ++i)
+#pragma unroll
+            for (int j = 0; j < FN; ++j)
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    const intx16 v = kg ? acc[i][j] : acc[FO + i][j];
+                    out[((i * FN + j) * 4 + q) * 64] = intx4{v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]};
+                }
+        __syncthreads();
+        const intx4* const in = reinterpret_cast<const intx4*>(space) + ((1 - kg) * FO * FN * 4) * 64 + lane;
+#pragma unroll
+        for (int i = 0; i < FO; ++i)
+#pragma unroll
+            for (int j = 0; j < FN; ++j) {
+                intx16 v = kg ? acc[FO + i][j] : acc[i][j];
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    const intx4 y = in[((i * FN + j) * 4 + q) * 64];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) v[4 * q + e] += y[e];
+                }
+                acc[i][j] = v;
+            }
+        __syncthreads();
+    }
+    // P waves' regions in each of the two larger arrays, Q in each of the others
+    int8_t* const big = (BM > BN ? wv < P ? as0 : as1 : wv < P ? ws0 : ws1) + wv % P * O::kInts * 4;
+    int8_t* const small = (BM > BN ? wv - 2 * P < Q ? ws0 : ws1 : wv - 2 * P < Q ? as0 : as1) + (wv - 2 * P + 2 * P * Q) % Q * O::kInts * 4;
+    int* const stage = reinterpret_cast<int*>(wv < 2 * P ? big : small);
+    const int col = wn * TN + (lane % O::LPR) * O::V;
+    const uint32_t n = n0 + col;
+    Columns<O::V> cols;
+#pragma unroll
+    for (int e = 0; e < O::V; ++e) {
+        cols.sw[e] = sws[col + e];
+        cols.bias[e] = biases[col + e];
+    }
+    auto rows = [&](int i, auto WHOLE) {
+        const int r0 = wm * TM + 32 * (kg * FO + i);
+#pragma unroll
+        for (int j = 0; j < FN; ++j)
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+                *reinterpret_cast<intx4*>(&stage[l32 * O::kLd + 32 * j + 8 * q + 4 * g]) =
+                    intx4{acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]};
+        __builtin_amdgcn_wave_barrier();
+#pragma unroll
+        for (int t = 0; t < 32 / O::RPI; ++t) {
+            const int row = t * O::RPI + lane / O::LPR;
+            const uint32_t m = m0 + r0 + row;
+            int v[O::V];
+#pragma unroll
+            for (int e = 0; e < O::V; e += 4) {
+                const intx4 x = *reinterpret_cast<const intx4*>(&stage[row * O::kLd + (lane % O::LPR) * O::V + e]);
+#pragma unroll
+                for (int y = 0; y < 4; ++y) v[e + y] = x[y];
+            }
+            if constexpr (decltype(WHOLE)::value) store_run<TC, O::V>(a, m, n, v, sas[r0 + row], cols, true);
+            else if (m < a.M && n < a.N) store_run<TC, O::V>(a, m, n, v, sas[r0 + row], cols, a.wide && n + O::V <= a.N);
+        }
+        __builtin_amdgcn_wave_barrier();  // every read of these rows precedes the next rows' writes
+    };
+    if (a.wide && m0 + BM <= a.M && n0 + BN <= a.N) {
+#pragma unroll
+        for (int i = 0; i < FO; ++i) rows(i, std::true_type{});
+    } else {
+#pragma unroll
+        for (int i = 0; i < FO; ++i) rows(i, std::false_type{});
+    }
+}
+
+// ---- small grids: a workgroup's waves split K ---------------------------------------------
+//
+// Eight waves compute the same 32 x 32 tile, each from the 128-code steps wave, wave + 8, ... through LDS stages of its own
+// (no barrier: a wave waits for its own loads alone), and add their sums through LDS. One launch, no workspace.
+template <typename TC>
+__global__ __launch_bounds__(512) void gemm_i8_split_kernel(I8Args a) {
+    constexpr int kWave = 64 * 128;  // bytes of a wave's stage: 32 rows of A, 32 of W
+    constexpr int kLd = 36;
+    __shared__ __attribute__((aligned(16))) int8_t st0[8 * kWave], st1[8 * kWave];
+    const int tid = threadIdx.x, lane = tid & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int l32 = lane & 31, g = lane >> 5;
+    uint32_t tm, tn;
+    tile_of(a, blockIdx.x, tm, tn);
+    const uint32_t m0 = tm * 32, n0 = tn * 32;
+    const Rows<4> ra(a.A, a.lda, m0, min(32u, a.M - m0), a.K, 0, lane), rw(a.W, a.ldw, n0, min(32u, a.N - n0), a.K, 0, lane);
+    int8_t* const s0 = st0 + wave * kWave;
+    int8_t* const s1 = st1 + wave * kWave;
+    intx16 acc;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) acc[r] = 0;
+    auto load = [&](int8_t* st, uint32_t k) {
+        wait_lds();  // reads of what the loads replace
+        ra.load(st, k);
+        rw.load(st + 4096, k);
+    };
+    auto compute = [&](const int8_t* st) {
+        __builtin_amdgcn_wave_barrier();  // (a wave's wait is for the loads of all its lanes)
+#pragma unroll
+        for (int s = 0; s < 4; ++s) {
+            const int at = l32 * 128 + (((2 * s + g) ^ swz(l32)) * 16);
+            acc = __builtin_amdgcn_mfma_i32_32x32x32_i8(*reinterpret_cast<const intx4*>(st + 4096 + at),
+                                                        *reinterpret_cast<const intx4*>(st + at), acc, 0, 0, 0);
+        }
+    };
+    uint32_t k = wave * 128;
+    if (k < a.K) load(s0, k);
+    while (k < a.K) {
+        if (k + 1024 < a.K) {
+            load(s1, k + 1024);
+            __builtin_amdgcn_s_waitcnt(0x0F78);  // vmcnt(8): the other stage's loads
+        } else {
+            wait_loads();
+        }
+        compute(s0);
+        k += 1024;
+        if (k >= a.K) break;
+        if (k + 1024 < a.K) {
+            load(s0, k + 1024);
+            __builtin_amdgcn_s_waitcnt(0x0F78);
+        } else {
+            wait_loads();
+        }
+        compute(s1);
+        k += 1024;
+    }
+    __syncthreads();
+    int* const red = reinterpret_cast<int*>(st0);
+#pragma unroll
+    for (int q = 0; q < 4; ++q)
+        *reinterpret_cast<intx4*>(&red[(wave * 32 + l32) * kLd + 8 * q + 4 * g]) = intx4{acc[4 * q], acc[4 * q + 1], acc[4 * q + 2], acc[4 * q + 3]};
+    __syncthreads();
+    if (tid >= 256) return;
+    const uint32_t row = tid >> 3, c = (tid & 7) * 4, m = m0 + row, n = n0 + c;
+    if (m >= a.M || n >= a.N) return;
+    Columns<4> cols;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        cols.sw[e] = a.sw[min(n + e, a.N - 1)];
+        cols.bias[e] = a.bias ? a.bias[min(n + e, a.N - 1)] : 0.0f;
+    }
+    const float sa = a.sa[m];
+    int v[4] = {0, 0, 0, 0};
+#pragma unroll
+    for (int w = 0; w < 8; ++w) {
+        const intx4 x = *reinterpret_cast<const intx4*>(&red[(w * 32 + row) * kLd + c]);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] += x[e];
+    }
+    store_run<TC, 4>(a, m, n, v, sa, cols, a.wide && n + 4 <= a.N);
+}
+
+// ---- few rows ------------------------------------------------------------------------------
+//
+// Up to 16 rows (single tokens): a workgroup takes 16 columns and its eight waves the 256-code pieces of K in turn, the
+// weights straight from memory into MFMA operands (16 rows x 64 bytes an instruction); the sums are added through LDS.
+constexpr uint32_t kFewRows = 16;
+
+template <typename TC>
+__global__ __launch_bounds__(512) void gemm_i8_few_kernel(I8Args a) {
+    constexpr int kLd = 20;
+    __shared__ __attribute__((aligned(16))) int red[8][16 * kLd];
+    const int tid = threadIdx.x, lane = tid & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const uint32_t l16 = lane & 15, c = lane >> 4, n0 = blockIdx.x * 16;
+    const uint32_t rows = min(16u, a.N - n0);
+    const __amdgpu_buffer_rsrc_t rA = __builtin_amdgcn_make_buffer_rsrc(const_cast<int8_t*>(a.A), 0, static_cast<int>((a.M - 1) * a.lda + a.K), 0x00020000);
+    const __amdgpu_buffer_rsrc_t rW = __builtin_amdgcn_make_buffer_rsrc(const_cast<int8_t*>(a.W + n0 * a.ldw), 0,
+                                                                        static_cast<int>((rows - 1) * a.ldw + a.K), 0x00020000);
+    const uint32_t oa = l16 < a.M ? l16 * static_cast<uint32_t>(a.lda) : kPast, ow = l16 < rows ? l16 * static_cast<uint32_t>(a.ldw) : kPast;
+    intx4 acc = {0, 0, 0, 0};
+    for (uint32_t k0 = wave * 256; k0 < a.K; k0 += 2048) {
+        intx4 x[4], w[4];
+#pragma unroll
+        for (int s = 0; s < 4; ++s) {
+            const uint32_t k = k0 + 64 * s + 16 * c;
+            w[s] = __builtin_bit_cast(intx4, __builtin_amdgcn_raw_buffer_load_b128(rW, k < a.K && l16 < rows ? ow + k : kPast, 0, 0));
+            x[s] = __builtin_bit_cast(intx4, __builtin_amdgcn_raw_buffer_load_b128(rA, k < a.K && l16 < a.M ? oa + k : kPast, 0, 0));
+        }
+#pragma unroll
+        for (int s = 0; s < 4; ++s) acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(w[s], x[s], acc, 0, 0, 0);
+    }
+    *reinterpret_cast<intx4*>(&red[wave][l16 * kLd + 4 * c]) = acc;  // row m = l16, columns 4c .. 4c + 3
+    __syncthreads();
+    if (tid >= 256) return;
+    const uint32_t m = tid >> 4, col = tid & 15, n = n0 + col;
+    if (m >= a.M || n >= a.N) return;
+    int v = 0;
+#pragma unroll
+    for (int w = 0; w < 8; ++w) v += red[w][m * kLd + col];
+    store_one<TC>(a, m, n, v, a.sa[m]);
+}
+
 // A wave takes a row at a time: its largest magnitude, then its codes.
 template <typename T>
 __global__ __launch_bounds__(256) void quantize_rows_any_kernel(const T* x, int8_t* q, float* scale, uint64_t rows, uint32_t cols,
@@ -98,9 +495,50 @@ unsigned grid_of(uint64_t units) { return static_cast<unsigned>(std::min<uint64_
 
 uint64_t span(uint64_t rows, uint64_t ld, uint64_t cols) { return rows ? (rows - 1) * ld + cols : 0; }
 
+// Builds: 0 any shape, 1 few rows, 2 waves split K (32 x 32), the others tiles.
+struct Tile {
+    uint32_t bm, bn;
+};
+constexpr Tile kTiles[kGemmI8Builds] = {{64, 64}, {16, 16}, {32, 32}, {64, 64}, {128, 64}, {128, 128}, {128, 128}, {256, 128}, {192, 256}, {256, 256}};
+enum { kAny = 0, kFew = 1, kSplitK = 2 };
+
+int choose(const I8Args& a) {
+    const bool vec = a.K % 16 == 0 && a.lda % 16 == 0 && a.ldw % 16 == 0 && aligned(a.A, 16) && aligned(a.W, 16) &&
+                     a.lda <= kMaxLd && a.ldw <= kMaxLd;
+    if (!vec) return kAny;
+    const int cfg = tuning().gemm_i8_cfg.load();
+    if (cfg >= 0 && (cfg != kFew || a.M <= kFewRows)) return cfg;
+    if (a.M <= kFewRows) return kFew;
+    const uint64_t t64 = static_cast<uint64_t>(ceil_div(a.M, 64)) * ceil_div(a.N, 64);
+    if (t64 <= 128) return kSplitK;
+    if (t64 <= 512) return 3;
+    const uint64_t t256 = static_cast<uint64_t>(ceil_div(a.M, 256)) * ceil_div(a.N, 256);
+    return t256 >= 200 ? 9 : 5;
+}
+
 template <typename TC>
-void launch_product(const I8Args& a, hipStream_t s) {
-    gemm_i8_any_kernel<TC><<<grid_of(static_cast<uint64_t>(ceil_div(a.M, 64)) * ceil_div(a.N, 64)), 256, 0, s>>>(a);
+void launch_product(I8Args a, hipStream_t s) {
+    const int build = choose(a);
+    if (build == kAny) {
+        gemm_i8_any_kernel<TC><<<grid_of(static_cast<uint64_t>(ceil_div(a.M, 64)) * ceil_div(a.N, 64)), 256, 0, s>>>(a);
+        return;
+    }
+    a.wide = a.ldc % (16 / sizeof(TC)) == 0 && aligned(a.C, 16);
+    a.tiles_m = ceil_div(a.M, kTiles[build].bm);
+    a.tiles_n = ceil_div(a.N, kTiles[build].bn);
+    a.group_m = std::min(a.tiles_m, 8u);
+    const unsigned grid = a.tiles_m * a.tiles_n;
+    switch (build) {
+        case kFew: gemm_i8_few_kernel<TC><<<grid, 512, 0, s>>>(a); break;
+        case kSplitK: gemm_i8_split_kernel<TC><<<grid, 512, 0, s>>>(a); break;
+        case 3: gemm_i8_tile_kernel<TC, 64, 64, 2, 2, 1><<<grid, 256, 0, s>>>(a); break;
+        case 4: gemm_i8_tile_kernel<TC, 128, 64, 2, 2, 1><<<grid, 256, 0, s>>>(a); break;
+        case 5: gemm_i8_tile_kernel<TC, 128, 128, 2, 2, 1><<<grid, 256, 0, s>>>(a); break;
+        case 6: gemm_i8_tile_kernel<TC, 128, 128, 2, 2, 2><<<grid, 512, 0, s>>>(a); break;
+        case 7: gemm_i8_tile_kernel<TC, 256, 128, 4, 2, 1><<<grid, 512, 0, s>>>(a); break;
+        case 8: gemm_i8_tile_kernel<TC, 192, 256, 2, 4, 1><<<grid, 512, 0, s>>>(a); break;
+        default: gemm_i8_tile_kernel<TC, 256, 256, 2, 4, 1><<<grid, 512, 0, s>>>(a); break;
+    }
 }
 
 template <typename T>
@@ -140,7 +578,7 @@ extern "C" int mi_gemm_nt_i8(const int8_t* A, const float* a_scale, const int8_t
     if (M == 0 || N == 0) return MI_OK;
     if (K == 0 || K > kMaxK) return fail(MI_ERR_UNSUPPORTED, "%s: K %u (1 .. %u: the sum is held in 32 bits)", fn, K, kMaxK);
     if (!A || !a_scale || !W || !w_scale || !C) return fail(MI_ERR_INVALID_ARG, "%s: null pointer", fn);
-    I8Args a{A, W, a_scale, w_scale, mode == 1 ? nullptr : bias, C, M, N, K, mode, lda ? lda : K, ldw ? ldw : K, ldc ? ldc : N};
+    I8Args a{A, W, a_scale, w_scale, mode == 1 ? nullptr : bias, C, M, N, K, mode, lda ? lda : K, ldw ? ldw : K, ldc ? ldc : N, 0, 0, 0, 0};
     if (a.lda < K || a.ldw < K || a.ldc < N) return fail(MI_ERR_INVALID_ARG, "%s: a row stride below its row", fn);
     const uint64_t e = c_dtype == MI_F16 ? 2 : 4;
     if (!aligned(a_scale, 4) || !aligned(w_scale, 4) || !aligned(bias, 4) || !aligned(C, e))

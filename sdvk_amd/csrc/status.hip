@@ -99,6 +99,12 @@ extern "C" int mi_tuning_set(const char* name, const char* value) {
         t.gemm_bwd_cfg.store(static_cast<int>(a));
         return MI_OK;
     }
+    if (std::strcmp(name, "gemm_i8_cfg") == 0) {
+        if (!clear && !parse_int(value, value + std::strlen(value), 0, mi::kGemmI8Builds - 1, &a))
+            return fail(MI_ERR_INVALID_ARG, "mi_tuning_set: gemm_i8_cfg \"%s\" (want 0..%d)", value, mi::kGemmI8Builds - 1);
+        t.gemm_i8_cfg.store(clear ? -1 : static_cast<int>(a));
+        return MI_OK;
+    }
     if (std::strcmp(name, "nn_kernel") == 0) {
         if (!clear && std::strcmp(value, "general") != 0)
             return fail(MI_ERR_INVALID_ARG, "mi_tuning_set: nn_kernel \"%s\" (want general)", value);
@@ -157,6 +163,7 @@ extern "C" void mi_tuning_reset(void) {
     t.attn_simd_waves.store(0);
     t.gemm_bwd_cfg.store(-1);
     t.gemm_bwd_splits.store(1);
+    t.gemm_i8_cfg.store(-1);
 }
 
 extern "C" const char* mi_status_string(int status) {

@@ -304,6 +304,50 @@ inline f4v mfma_16x16x32_f16(h8 a, h8 b, f4v c, int cbsz, int abid, int blgp) {
     return d;
 }
 
+// v_mfma_i32_32x32x32_i8 and v_mfma_i32_16x16x64_i8: lane l supplies row l % R of A and column l % R of B (R = 32, 16), 16
+// codes each, k = 16 (l / R) + 0..15; D / C as in the fp16 forms above. Sums wrap at 32 bits.
+typedef int i4v __attribute__((ext_vector_type(4)));
+typedef int i16v __attribute__((ext_vector_type(16)));
+template <int R, class V>
+struct MfmaI8In {
+    i4v a, b;
+    V c;
+};
+template <int R, class V>
+inline void mfma_i8_fn(const unsigned char (*ins)[256], unsigned char (*outs)[256], const void*) {
+    constexpr int KD = 16 * 64 / R, NR = R * R / 64;
+    int8_t A[R][KD], B[KD][R];
+    MfmaI8In<R, V> x[64];
+    for (int l = 0; l < 64; ++l) {
+        std::memcpy(&x[l], ins[l], sizeof x[l]);
+        int8_t a[16], b[16];
+        std::memcpy(a, &x[l].a, 16);
+        std::memcpy(b, &x[l].b, 16);
+        for (int e = 0; e < 16; ++e) {
+            A[l % R][16 * (l / R) + e] = a[e];
+            B[16 * (l / R) + e][l % R] = b[e];
+        }
+    }
+    for (int l = 0; l < 64; ++l) {
+        V d;
+        for (int r = 0; r < NR; ++r) {
+            const int i = R == 32 ? 8 * (r / 4) + 4 * (l / 32) + r % 4 : 4 * (l / 16) + r;
+            uint32_t s = static_cast<uint32_t>(x[l].c[r]);
+            for (int k = 0; k < KD; ++k) s += static_cast<uint32_t>(A[i][k] * B[k][l % R]);
+            d[r] = static_cast<int>(s);
+        }
+        std::memcpy(outs[l], &d, sizeof d);
+    }
+}
+template <int R, class V>
+inline V mfma_i8(i4v a, i4v b, V c, int cbsz, int abid, int blgp) {
+    if (cbsz || abid || blgp) die("mfma: broadcast controls are not emulated");
+    const MfmaI8In<R, V> x{a, b, c};
+    V d;
+    wave_op("mfma_i32_i8", &x, sizeof x, &d, sizeof d, mfma_i8_fn<R, V>, nullptr);
+    return d;
+}
+
 struct DppCtl {
     int ctrl;
 };
@@ -495,6 +539,8 @@ inline T __shfl_xor(T v, int mask, int width = 64) {
 #define __builtin_amdgcn_raw_buffer_store_b32 ::kemu::buffer_store_b32
 #define __builtin_amdgcn_mfma_f32_32x32x16_f16 ::kemu::mfma_32x32x16_f16
 #define __builtin_amdgcn_mfma_f32_16x16x32_f16 ::kemu::mfma_16x16x32_f16
+#define __builtin_amdgcn_mfma_i32_32x32x32_i8 (::kemu::mfma_i8<32, ::kemu::i16v>)
+#define __builtin_amdgcn_mfma_i32_16x16x64_i8 (::kemu::mfma_i8<16, ::kemu::i4v>)
 #define __builtin_amdgcn_mov_dpp ::kemu::mov_dpp
 #define __builtin_amdgcn_readfirstlane ::kemu::readfirstlane
 #define __builtin_amdgcn_mbcnt_lo ::kemu::mbcnt_lo

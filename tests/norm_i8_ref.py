@@ -304,7 +304,7 @@ def quantize(be, *, rows, cols, typ="f32", kind="normal", ldx=0, ldq=0, off=0, q
     A.unchanged()
 
 
-def product(be, *, M, N, K, out="f32", mode=0, bias=True, lda=0, ldw=0, ldc=0, off=0, woff=0, coff=0, extreme=False, broken=False, seed=4):
+def product(be, *, M, N, K, out="f32", mode=0, bias=True, lda=0, ldw=0, ldc=0, off=0, woff=0, coff=0, extreme=False, broken=False, cfg=None, seed=4):
     rng = rng_of(seed)
     lo = -128 if extreme else -127
     a, w = (rng.integers(lo, 128, (r, K)).astype(np.int8) for r in (M, N))
@@ -330,8 +330,12 @@ def product(be, *, M, N, K, out="f32", mode=0, bias=True, lda=0, ldw=0, ldc=0, o
     if mode:
         view(init, coff, 1, M, N, lc, 0)[0] = old
     bc = A.out(0, dt, init.copy())
+    if cfg:
+        be.tune("gemm_i8_cfg", cfg)
     be.call("mi_gemm_nt_i8", be.at(ba, off), bsa.ptr, be.at(bw, woff), bsw.ptr, bb.ptr if bias else None, be.at(bc, coff * np.dtype(dt).itemsize),
             {"f32": 0, "f16": 1}[out], M, N, K, mode, lda, ldw, ldc, None)
+    if cfg:
+        be.tune("gemm_i8_cfg", None)
     flat = be.get(bc, dt, nc)
     got = view(flat, coff, 1, M, N, lc, 0)[0].copy()
     assert np.all(outside(flat, coff, 1, M, N, lc, 0) == dt(SENTINEL)), "wrote outside C"
@@ -350,6 +354,7 @@ def product(be, *, M, N, K, out="f32", mode=0, bias=True, lda=0, ldw=0, ldc=0, o
     if not mode:
         be.call("mi_gemm_nt_i8", be.at(ba, off), bsa.ptr, be.at(bw, woff), bsw.ptr, bb.ptr if bias else None, be.at(bc, coff * np.dtype(dt).itemsize),
                 {"f32": 0, "f16": 1}[out], M, N, K, mode, lda, ldw, ldc, None)
+        # by the rules, if the first call was pinned to a build: every build gives the same bits
         assert np.array_equal(be.get(bc, dt, nc).view(np.uint8), flat.view(np.uint8)), "a second call gave other bits"
 
 
@@ -397,6 +402,14 @@ CASES = {
         dict(M=20, N=40, K=64, lda=65, ldw=67), dict(M=20, N=40, K=64, off=1), dict(M=20, N=40, K=64, woff=8), dict(M=20, N=40, K=64, coff=1, out="f16"), dict(M=20, N=40, K=64, coff=1), dict(M=40, N=40, K=1040, extreme=True), dict(M=4, N=9, K=131071, extreme=True),
         dict(M=9, N=40, K=4096, extreme=True), dict(M=9, N=20, K=64, broken=True), dict(M=40, N=20, K=64, broken=True, mode=2), dict(M=1, N=300, K=1280), dict(M=8, N=20, K=2064, out="f16"), dict(M=77, N=64, K=2048),
         dict(M=150, N=130, K=128, out="f16"), dict(M=300, N=270, K=192), dict(M=260, N=300, K=64, out="f16", ldc=304), dict(M=300, N=260, K=320, mode=2),
+        # every build, with tails of rows, columns and codes
+        dict(M=20, N=40, K=64, cfg="0"), dict(M=16, N=40, K=80, cfg="1"), dict(M=40, N=40, K=80, cfg="1"), dict(M=1, N=33, K=16, cfg="2"), dict(M=65, N=47, K=2448, cfg="2", extreme=True),
+        dict(M=65, N=47, K=2448, cfg="2", out="f16", mode=2), dict(M=1, N=33, K=16, cfg="3"), dict(M=65, N=70, K=400, cfg="3", out="f16"), dict(M=130, N=100, K=272, cfg="3", lda=288, ldw=304, ldc=101),
+        dict(M=1, N=33, K=16, cfg="4"), dict(M=129, N=131, K=400, cfg="4", extreme=True), dict(M=140, N=264, K=272, cfg="4", out="f16", mode=2, ldc=272), dict(M=140, N=134, K=128, cfg="4", out="f16"),
+        dict(M=1, N=33, K=16, cfg="5"), dict(M=257, N=259, K=400, cfg="5", extreme=True), dict(M=300, N=264, K=272, cfg="5", out="f16", mode=2, ldc=272), dict(M=300, N=261, K=256, cfg="5", out="f16"),
+        dict(M=300, N=516, K=144, cfg="5", mode=1), dict(M=1, N=33, K=16, cfg="6"), dict(M=129, N=131, K=400, cfg="6", extreme=True), dict(M=140, N=264, K=656, cfg="6", out="f16", mode=2, ldc=272),
+        dict(M=257, N=131, K=400, cfg="7", extreme=True), dict(M=300, N=264, K=256, cfg="7", out="f16", mode=2, ldc=272), dict(M=193, N=259, K=400, cfg="8", extreme=True),
+        dict(M=200, N=264, K=272, cfg="8", out="f16"), dict(M=257, N=259, K=400, cfg="9", extreme=True), dict(M=300, N=264, K=272, cfg="9", out="f16", mode=2, ldc=272),
     ],
 }
 # Larger shapes, on the GPU alone: grids that stride, many chunks, tails.
