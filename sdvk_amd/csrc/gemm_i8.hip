@@ -173,10 +173,10 @@ __device__ __forceinline__ void tile_of(const I8Args& a, uint32_t b, uint32_t& t
     tn = i / rows;
 }
 
-// A wave's sums of 32 rows and TN columns leave through LDS (a region of its own), so that whole runs of a row are stored.
-template <typename TC, int TN>
+// A wave's sums of R rows and TN columns at a time leave through LDS (a region of its own), so that whole runs of a row are stored.
+template <typename TC, int TN, int R_>
 struct Out {
-    static constexpr int kLd = TN + 4, kInts = 32 * kLd;
+    static constexpr int R = R_, kLd = TN + 4, kInts = R * kLd;
     static constexpr int V = 16 / static_cast<int>(sizeof(TC)), LPR = TN / V, RPI = 64 / LPR;  // columns a lane, lanes a row, rows at a time
 };
 
@@ -185,11 +185,11 @@ template <typename TC, int BM, int BN, int WM, int WN, int KG>
 __global__ __launch_bounds__(KG * WM * WN * 64) void gemm_i8_tile_kernel(I8Args a) {
     constexpr int NW = WM * WN, TM = BM / WM, TN = BN / WN, FM = TM / 32, FN = TN / 32;
     constexpr int A_IT = BM / 8 / NW, W_IT = BN / 8 / NW, FO = FM / KG;  // FO: 32-row blocks of a wave's own at the end
-    typedef Out<TC, TN> O;
+    typedef Out<TC, TN, (TN > 128 ? 16 : 32)> O;
     static_assert(BM % (8 * NW) == 0 && BN % (8 * NW) == 0 && FM % KG == 0, "loads and rows divide evenly");
     constexpr int P = KG * 128 * (BM > BN ? BM : BN) / (O::kInts * 4), Q = KG * 128 * (BM > BN ? BN : BM) / (O::kInts * 4);
     static_assert(2 * (P + Q) >= KG * NW, "the epilogue's regions fit the stages");
-    static_assert(KG == 1 || (KG == 2 && NW == 4 && FO * FN * 4096 * 2 <= KG * 128 * (BM < BN ? BM : BN)), "the exchanged sums fit the stages");
+    static_assert(KG == 1 || (KG == 2 && FO * FN * 4096 * ((NW + 1) / 2) <= KG * 128 * (BM < BN ? BM : BN)), "the exchanged sums fit the stages");
     // arrays of their own: the compiler then knows that reads of one stage do not wait for the loads into the other
     __shared__ __attribute__((aligned(16))) int8_t as0[KG * BM * 128], as1[KG * BM * 128], ws0[KG * BN * 128], ws1[KG * BN * 128];
     // the tile's scales and biases, read while the first codes are on their way: from memory in the epilogue each would cost a
@@ -278,9 +278,12 @@ __global__ __launch_bounds__(KG * WM * WN * 64) void gemm_i8_tile_kernel(I8Args 
     }
     // (every wave has read its last step, no load is in flight: the stages are free)
     if constexpr (KG == 2) {
-        int8_t* const space = wave == 0 ? as0 : wave == 1 ? as1 : wave == 2 ? ws0 : ws1;
-        // a wave's slot: (wave, group), its partner's rows in register order
-        intx4* const out = reinterpret_cast<intx4*>(space) + (kg * FO * FN * 4) * 64 + lane;
+        // slots of (wave, group) in turn over the four arrays, the partner's rows in register order
+        auto slot = [&](int i) {
+            int8_t* const p = (i & 3) == 0 ? as0 : (i & 3) == 1 ? as1 : (i & 3) == 2 ? ws0 : ws1;
+            return reinterpret_cast<intx4*>(p) + (i >> 2) * (FO * FN * 4 * 64) + lane;
+        };
+        intx4* const out = slot(2 * wave + kg);
 #pragma unroll
         for (int i = 0; i < FO; ++i)
 #pragma unroll
@@ -291,7 +294,7 @@ __global__ __launch_bounds__(KG * WM * WN * 64) void gemm_i8_tile_kernel(I8Args 
                     out[((i * FN + j) * 4 + q) * 64] = intx4{v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]};
                 }
         __syncthreads();
-        const intx4* const in = reinterpret_cast<const intx4*>(space) + ((1 - kg) * FO * FN * 4) * 64 + lane;
+        const intx4* const in = slot(2 * wave + 1 - kg);
 #pragma unroll
         for (int i = 0; i < FO; ++i)
 #pragma unroll
@@ -311,38 +314,46 @@ __global__ __launch_bounds__(KG * WM * WN * 64) void gemm_i8_tile_kernel(I8Args 
     int8_t* const big = (BM > BN ? wv < P ? as0 : as1 : wv < P ? ws0 : ws1) + wv % P * O::kInts * 4;
     int8_t* const small = (BM > BN ? wv - 2 * P < Q ? ws0 : ws1 : wv - 2 * P < Q ? as0 : as1) + (wv - 2 * P + 2 * P * Q) % Q * O::kInts * 4;
     int* const stage = reinterpret_cast<int*>(wv < 2 * P ? big : small);
-    const int col = wn * TN + (lane % O::LPR) * O::V;
-    const uint32_t n = n0 + col;
+    const int lrow = lane / O::LPR, lcol = lane % O::LPR * O::V;
+    const bool busy = lane < O::LPR * O::RPI;
+    const uint32_t n = n0 + wn * TN + lcol;
     Columns<O::V> cols;
 #pragma unroll
     for (int e = 0; e < O::V; ++e) {
-        cols.sw[e] = sws[col + e];
-        cols.bias[e] = biases[col + e];
+        cols.sw[e] = sws[wn * TN + lcol + e];
+        cols.bias[e] = biases[wn * TN + lcol + e];
     }
     auto rows = [&](int i, auto WHOLE) {
-        const int r0 = wm * TM + 32 * (kg * FO + i);
 #pragma unroll
-        for (int j = 0; j < FN; ++j)
+        for (int h = 0; h < 32; h += O::R) {
+            const int r0 = wm * TM + 32 * (kg * FO + i) + h;
+            if (O::R == 32 || (l32 & 16) == h) {
 #pragma unroll
-            for (int q = 0; q < 4; ++q)
-                *reinterpret_cast<intx4*>(&stage[l32 * O::kLd + 32 * j + 8 * q + 4 * g]) =
-                    intx4{acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]};
-        __builtin_amdgcn_wave_barrier();
+                for (int j = 0; j < FN; ++j)
 #pragma unroll
-        for (int t = 0; t < 32 / O::RPI; ++t) {
-            const int row = t * O::RPI + lane / O::LPR;
-            const uint32_t m = m0 + r0 + row;
-            int v[O::V];
-#pragma unroll
-            for (int e = 0; e < O::V; e += 4) {
-                const intx4 x = *reinterpret_cast<const intx4*>(&stage[row * O::kLd + (lane % O::LPR) * O::V + e]);
-#pragma unroll
-                for (int y = 0; y < 4; ++y) v[e + y] = x[y];
+                    for (int q = 0; q < 4; ++q)
+                        *reinterpret_cast<intx4*>(&stage[(l32 % O::R) * O::kLd + 32 * j + 8 * q + 4 * g]) =
+                            intx4{acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]};
             }
-            if constexpr (decltype(WHOLE)::value) store_run<TC, O::V>(a, m, n, v, sas[r0 + row], cols, true);
-            else if (m < a.M && n < a.N) store_run<TC, O::V>(a, m, n, v, sas[r0 + row], cols, a.wide && n + O::V <= a.N);
+            __builtin_amdgcn_wave_barrier();
+#pragma unroll
+            for (int t = 0; t < O::R; t += O::RPI) {
+                const int row = t + lrow;
+                if (busy && row < O::R) {
+                    const uint32_t m = m0 + r0 + row;
+                    int v[O::V];
+#pragma unroll
+                    for (int e = 0; e < O::V; e += 4) {
+                        const intx4 x = *reinterpret_cast<const intx4*>(&stage[row * O::kLd + lcol + e]);
+#pragma unroll
+                        for (int y = 0; y < 4; ++y) v[e + y] = x[y];
+                    }
+                    if constexpr (decltype(WHOLE)::value) store_run<TC, O::V>(a, m, n, v, sas[r0 + row], cols, true);
+                    else if (m < a.M && n < a.N) store_run<TC, O::V>(a, m, n, v, sas[r0 + row], cols, a.wide && n + O::V <= a.N);
+                }
+            }
+            __builtin_amdgcn_wave_barrier();  // every read of these rows precedes the next rows' writes
         }
-        __builtin_amdgcn_wave_barrier();  // every read of these rows precedes the next rows' writes
     };
     if (a.wide && m0 + BM <= a.M && n0 + BN <= a.N) {
 #pragma unroll
@@ -495,12 +506,22 @@ unsigned grid_of(uint64_t units) { return static_cast<unsigned>(std::min<uint64_
 
 uint64_t span(uint64_t rows, uint64_t ld, uint64_t cols) { return rows ? (rows - 1) * ld + cols : 0; }
 
-// Builds: 0 any shape, 1 few rows, 2 waves split K (32 x 32), the others tiles.
-struct Tile {
-    uint32_t bm, bn;
+// Builds: 0 any shape, 1 few rows, 2 waves split K (32 x 32), the others tiles; 5 is 4 with two groups of waves, which take the
+// steps in turn.
+//
+// us of a tile build = 3 + n (tile + steps step), n tiles on the fullest of 256 CUs, fitted to a sweep (MI355X). A step is bound by LDS:
+// 8.7 cycles a fragment read and 18.6 a KB loaded into it predict all of them but 64 x 64's. Sweep, us, fp16 C, the five tiles in
+// order: 1024x1280x1280 6.6 / 10.8 / 9.8 / 15.1 / 23.5, 2048x1280x5120 26.9 / 31.5 / 25.4 / 44.1 / 66.0, 8192x640x2560 27.7 / 21.6 / 30.3 / 27.1 / 38.9,
+// 2048x10240x1280 48.9 / 37.0 / 43.8 / 36.1 / 32.4, 8192x5120x640 60.2 / 43.7 / 63.6 / 47.3 / 43.2. 256 x 256 and 256 x 128 tiles were
+// between their neighbours everywhere.
+struct Build {
+    uint32_t bm, bn, step;   // codes of a step
+    float tile_us, step_us;
 };
-constexpr Tile kTiles[kGemmI8Builds] = {{64, 64}, {16, 16}, {32, 32}, {64, 64}, {128, 64}, {128, 128}, {128, 128}, {256, 128}, {192, 256}, {256, 256}};
-enum { kAny = 0, kFew = 1, kSplitK = 2 };
+constexpr Build kBuilds[kGemmI8Builds] = {{64, 64, 32, 0, 0}, {16, 16, 0, 0, 0}, {32, 32, 0, 0, 0}, {64, 64, 128, 0.2f, 0.22f}, {128, 128, 128, 1.6f, 0.42f},
+                                          {128, 128, 256, 2.2f, 1.05f}, {192, 256, 128, 3.4f, 0.94f}, {256, 320, 128, 7.7f, 1.38f}};
+enum { kAny = 0, kFew = 1, kSplitK = 2, k64 = 3, k128 = 4, k128x2 = 5, k192 = 6, k256 = 7 };
+constexpr float kAlone128 = 0.68f;  // us a step of 128 x 128 with no second tile on the CU to fill its waits
 
 int choose(const I8Args& a) {
     const bool vec = a.K % 16 == 0 && a.lda % 16 == 0 && a.ldw % 16 == 0 && aligned(a.A, 16) && aligned(a.W, 16) &&
@@ -509,11 +530,19 @@ int choose(const I8Args& a) {
     const int cfg = tuning().gemm_i8_cfg.load();
     if (cfg >= 0 && (cfg != kFew || a.M <= kFewRows)) return cfg;
     if (a.M <= kFewRows) return kFew;
-    const uint64_t t64 = static_cast<uint64_t>(ceil_div(a.M, 64)) * ceil_div(a.N, 64);
-    if (t64 <= 128) return kSplitK;
-    if (t64 <= 512) return 3;
-    const uint64_t t256 = static_cast<uint64_t>(ceil_div(a.M, 256)) * ceil_div(a.N, 256);
-    return t256 >= 200 ? 9 : 5;
+    if (static_cast<uint64_t>(ceil_div(a.M, 64)) * ceil_div(a.N, 64) <= 128) return kSplitK;
+    int best = k64;
+    float least = 0.0f;
+    for (int b = k64; b <= k256; ++b) {
+        const uint64_t tiles = static_cast<uint64_t>(ceil_div(a.M, kBuilds[b].bm)) * ceil_div(a.N, kBuilds[b].bn);
+        const float n = static_cast<float>((tiles + 255) / 256);
+        const float us = n * (kBuilds[b].tile_us + ceil_div(a.K, kBuilds[b].step) * (b == k128 && tiles <= 256 ? kAlone128 : kBuilds[b].step_us));
+        if (b == k64 || us < least) {
+            best = b;
+            least = us;
+        }
+    }
+    return best;
 }
 
 template <typename TC>
@@ -524,20 +553,18 @@ void launch_product(I8Args a, hipStream_t s) {
         return;
     }
     a.wide = a.ldc % (16 / sizeof(TC)) == 0 && aligned(a.C, 16);
-    a.tiles_m = ceil_div(a.M, kTiles[build].bm);
-    a.tiles_n = ceil_div(a.N, kTiles[build].bn);
+    a.tiles_m = ceil_div(a.M, kBuilds[build].bm);
+    a.tiles_n = ceil_div(a.N, kBuilds[build].bn);
     a.group_m = std::min(a.tiles_m, 8u);
     const unsigned grid = a.tiles_m * a.tiles_n;
     switch (build) {
         case kFew: gemm_i8_few_kernel<TC><<<grid, 512, 0, s>>>(a); break;
         case kSplitK: gemm_i8_split_kernel<TC><<<grid, 512, 0, s>>>(a); break;
-        case 3: gemm_i8_tile_kernel<TC, 64, 64, 2, 2, 1><<<grid, 256, 0, s>>>(a); break;
-        case 4: gemm_i8_tile_kernel<TC, 128, 64, 2, 2, 1><<<grid, 256, 0, s>>>(a); break;
-        case 5: gemm_i8_tile_kernel<TC, 128, 128, 2, 2, 1><<<grid, 256, 0, s>>>(a); break;
-        case 6: gemm_i8_tile_kernel<TC, 128, 128, 2, 2, 2><<<grid, 512, 0, s>>>(a); break;
-        case 7: gemm_i8_tile_kernel<TC, 256, 128, 4, 2, 1><<<grid, 512, 0, s>>>(a); break;
-        case 8: gemm_i8_tile_kernel<TC, 192, 256, 2, 4, 1><<<grid, 512, 0, s>>>(a); break;
-        default: gemm_i8_tile_kernel<TC, 256, 256, 2, 4, 1><<<grid, 512, 0, s>>>(a); break;
+        case k64: gemm_i8_tile_kernel<TC, 64, 64, 2, 2, 1><<<grid, 256, 0, s>>>(a); break;
+        case k128: gemm_i8_tile_kernel<TC, 128, 128, 2, 2, 1><<<grid, 256, 0, s>>>(a); break;
+        case k128x2: gemm_i8_tile_kernel<TC, 128, 128, 2, 2, 2><<<grid, 512, 0, s>>>(a); break;
+        case k192: gemm_i8_tile_kernel<TC, 192, 256, 2, 4, 1><<<grid, 512, 0, s>>>(a); break;
+        default: gemm_i8_tile_kernel<TC, 256, 320, 4, 2, 1><<<grid, 512, 0, s>>>(a); break;
     }
 }
 

@@ -406,10 +406,9 @@ CASES = {
         dict(M=20, N=40, K=64, cfg="0"), dict(M=16, N=40, K=80, cfg="1"), dict(M=40, N=40, K=80, cfg="1"), dict(M=1, N=33, K=16, cfg="2"), dict(M=65, N=47, K=2448, cfg="2", extreme=True),
         dict(M=65, N=47, K=2448, cfg="2", out="f16", mode=2), dict(M=1, N=33, K=16, cfg="3"), dict(M=65, N=70, K=400, cfg="3", out="f16"), dict(M=130, N=100, K=272, cfg="3", lda=288, ldw=304, ldc=101),
         dict(M=1, N=33, K=16, cfg="4"), dict(M=129, N=131, K=400, cfg="4", extreme=True), dict(M=140, N=264, K=272, cfg="4", out="f16", mode=2, ldc=272), dict(M=140, N=134, K=128, cfg="4", out="f16"),
-        dict(M=1, N=33, K=16, cfg="5"), dict(M=257, N=259, K=400, cfg="5", extreme=True), dict(M=300, N=264, K=272, cfg="5", out="f16", mode=2, ldc=272), dict(M=300, N=261, K=256, cfg="5", out="f16"),
-        dict(M=300, N=516, K=144, cfg="5", mode=1), dict(M=1, N=33, K=16, cfg="6"), dict(M=129, N=131, K=400, cfg="6", extreme=True), dict(M=140, N=264, K=656, cfg="6", out="f16", mode=2, ldc=272),
-        dict(M=257, N=131, K=400, cfg="7", extreme=True), dict(M=300, N=264, K=256, cfg="7", out="f16", mode=2, ldc=272), dict(M=193, N=259, K=400, cfg="8", extreme=True),
-        dict(M=200, N=264, K=272, cfg="8", out="f16"), dict(M=257, N=259, K=400, cfg="9", extreme=True), dict(M=300, N=264, K=272, cfg="9", out="f16", mode=2, ldc=272),
+        dict(M=1, N=33, K=16, cfg="5"), dict(M=129, N=131, K=400, cfg="5", extreme=True), dict(M=140, N=264, K=656, cfg="5", out="f16", mode=2, ldc=272), dict(M=128, N=128, K=768, cfg="5", out="f16"),
+        dict(M=1, N=33, K=16, cfg="6"), dict(M=193, N=259, K=400, cfg="6", extreme=True), dict(M=200, N=264, K=272, cfg="6", out="f16", mode=1), dict(M=1, N=33, K=16, cfg="7"),
+        dict(M=257, N=321, K=400, cfg="7", extreme=True), dict(M=260, N=328, K=272, cfg="7", out="f16", mode=2),
     ],
 }
 # Larger shapes, on the GPU alone: grids that stride, many chunks, tails.
