@@ -21,9 +21,10 @@ namespace mi {
 namespace {
 
 constexpr uint32_t kMaxGrid = 1u << 20;   // workgroups of a launch that strides over its units
-constexpr uint32_t kChunkMin = 16;        // rows of a chunk, at least (but for the last) ...
-constexpr uint32_t kChunkMax = 2048;      // ... and at most: the longest chain of fp32 additions
-constexpr uint32_t kChunks = 512;         // chunks of all images, about: two workgroups per CU
+constexpr uint32_t kChunkValues = 8192;   // values of a chunk, at least (but for the last), and ...
+constexpr uint32_t kChunkMax = 2048;      // ... rows at most: the longest chain of fp32 additions
+constexpr uint32_t kChunks = 256;         // chunks of all images, about: a workgroup per CU
+constexpr uint32_t kJoinParts = 4096;     // chunks times groups of an image that every workgroup joins by itself
 
 struct Stat {  // of one group of one image, 16 bytes: what `stats` holds
     float mean, low, inv, zero;
@@ -41,6 +42,8 @@ struct GnArgs {
     Part* part;
     uint32_t batch, pixels, C, groups, cg;
     uint32_t chunk, nchunk;  // rows of a chunk, chunks of an image
+    uint32_t cut, ncut;      // rows of a workgroup that stores y or dx, of such workgroups an image
+    uint32_t joined;         // stats hold the statistics; 0: they are joined from part
     float eps;
     uint64_t ldx, ldy, sx, sy;
 };
@@ -52,6 +55,7 @@ struct GnBwdArgs {
     float *dgamma, *dbeta;
     float* cpart;  // [batch][nchunk][2][C]: sums of w and of w xh
     float* gsum;   // [batch][groups][2]: mean(w gamma), mean(w gamma xh)
+    float* gpart;  // [batch][nchunk][groups][2]: a chunk's sums of w gamma and w gamma xh
     uint64_t lddy, ldres, lddx, sdy, sres, sdx;
 };
 
@@ -306,17 +310,467 @@ __global__ __launch_bounds__(256) void gn_bwd_apply_any_kernel(GnBwdArgs a) {
     }
 }
 
+// ---- rows of 16-byte vectors ---------------------------------------------------------
+//
+// C and the strides multiples of a vector (16 bytes of x: E values), 16-byte aligned tensors, C <= 4096, groups <= 256. A workgroup of T
+// threads takes a chunk: thread t holds the columns E (t % V) .. + E - 1 (V = C / E vectors a row) of the rows t / V, + T / V, ...,
+// with what it needs of its columns in registers.
+//
+// Statistics: a thread sums x - x0 and its square for each of its columns, x0 the column's first value of its own (at worst,
+// where x0 is the outlier that makes the variance, that costs a factor of the rows a thread takes, which is their
+// number and no more); the threads' sums are joined in 64 bits.
+// All of it is bound by memory: every pass reads x once (and dy), and one stores y or dx.
+constexpr uint32_t kFastChannels = 4096, kFastGroups = 256;
+constexpr int kRows = 4;  // rows a thread has in flight
+
+template <typename T>
+struct Vec {
+    static constexpr int E = 16 / static_cast<int>(sizeof(T));
+    typedef T type __attribute__((ext_vector_type(E)));
+};
+
+// A group's lanes: the largest power of two (at most 64) of threads that T threads have for each of G groups at once.
+__device__ __forceinline__ uint32_t lanes_of(uint32_t T, uint32_t G) {
+    uint32_t n = 1;
+    while (n < 64 && 2 * n * G <= T) n *= 2;
+    return n;
+}
+template <typename F>
+__device__ __forceinline__ F lanes_sum(F v, uint32_t n) {  // over n neighbouring lanes
+    for (uint32_t o = 1; o < n; o <<= 1) v += __shfl_xor(v, static_cast<int>(o));
+    return v;
+}
+
+// The statistics of image b's groups into st[G], by all threads: loaded, or joined from the chunks as gn_join_kernel does.
+__device__ __forceinline__ void image_stats(const GnArgs& a, uint64_t b, Stat* st) {
+    const uint32_t T = blockDim.x, tid = threadIdx.x;
+    if (a.joined) {
+        for (uint32_t g = tid; g < a.groups; g += T) st[g] = a.stats[b * a.groups + g];
+        __syncthreads();
+        return;
+    }
+    const uint32_t n = lanes_of(T, a.groups), lane = tid % n;
+    const double total = static_cast<double>(a.pixels) * a.cg;
+    const uint32_t per = T / n;
+    for (uint32_t g0 = 0; g0 < a.groups; g0 += per) {
+        const uint32_t g = min(g0 + tid / n, a.groups - 1);
+        const Part* p = a.part + b * a.nchunk * a.groups + g;
+        double s = 0.0;
+        for (uint32_t c = lane; c < a.nchunk; c += n) {
+            const Part q = p[static_cast<uint64_t>(c) * a.groups];
+            s += static_cast<double>(min(a.chunk, a.pixels - c * a.chunk)) * (static_cast<double>(q.shift) + static_cast<double>(q.rest));
+        }
+        const double mean = lanes_sum(s, n) / a.pixels;
+        s = 0.0;
+        for (uint32_t c = lane; c < a.nchunk; c += n) {
+            const Part q = p[static_cast<uint64_t>(c) * a.groups];
+            const double k = static_cast<double>(min(a.chunk, a.pixels - c * a.chunk)) * a.cg;
+            const double d = (static_cast<double>(q.shift) - mean) + static_cast<double>(q.rest);
+            s += static_cast<double>(q.m2) + k * d * d;
+        }
+        const double var = lanes_sum(s, n) / total;
+        if (lane == 0 && g0 + tid / n < a.groups) {
+            const float hi = static_cast<float>(mean);
+            st[g] = Stat{hi, static_cast<float>(mean - static_cast<double>(hi)), static_cast<float>(1.0 / sqrt(var + static_cast<double>(a.eps))), 0.0f};
+        }
+    }
+    __syncthreads();
+}
+
+// What a thread needs of E columns from c0 on.
+template <int E>
+struct Cols {
+    float mean[E], a[E], b[E];
+    __device__ __forceinline__ void set(const GnArgs& f, const Stat* st, uint32_t c0) {
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+            const uint32_t c = c0 + e;
+            const Coef k = coef(st[c / f.cg], f.gamma ? f.gamma[c] : 1.0f, f.beta ? f.beta[c] : 0.0f);
+            mean[e] = k.mean;
+            a[e] = k.a;
+            b[e] = k.b;
+        }
+    }
+};
+
+// Grid: batch * nchunk. LDS: 3 floats a thread's column.
+template <typename TX>
+__global__ __launch_bounds__(1024) void gn_part_kernel(GnArgs a) {
+    constexpr int E = Vec<TX>::E;
+    typedef typename Vec<TX>::type VT;
+    extern __shared__ __attribute__((aligned(16))) float red[];  // [3][T / V][C]: x0, sums of x - x0, of its square
+    const uint32_t T = blockDim.x, tid = threadIdx.x, V = a.C / E, rows_at = T / V;
+    const uint32_t ty = tid / V, tx = tid % V;
+    const uint64_t b = blockIdx.x / a.nchunk;
+    const uint32_t chunk = blockIdx.x % a.nchunk, r0 = chunk * a.chunk, rows = min(a.chunk, a.pixels - r0);
+    const TX* x = static_cast<const TX*>(a.x) + b * a.sx + static_cast<uint64_t>(r0) * a.ldx + tx * E;
+    float x0[E], s1[E], s2[E];
+#pragma unroll
+    for (int e = 0; e < E; ++e) x0[e] = s1[e] = s2[e] = 0.0f;
+    const bool in = ty < rows_at;
+    if (in && ty < rows) {
+        const VT v = *reinterpret_cast<const VT*>(x + ty * a.ldx);
+#pragma unroll
+        for (int e = 0; e < E; ++e) x0[e] = static_cast<float>(v[e]);
+        uint32_t r = ty + rows_at;
+        for (; r + (kRows - 1) * rows_at < rows; r += kRows * rows_at) {
+            VT w[kRows];
+#pragma unroll
+            for (int i = 0; i < kRows; ++i) w[i] = *reinterpret_cast<const VT*>(x + (r + i * rows_at) * a.ldx);
+#pragma unroll
+            for (int i = 0; i < kRows; ++i)
+#pragma unroll
+                for (int e = 0; e < E; ++e) {
+                    const float d = static_cast<float>(w[i][e]) - x0[e];
+                    s1[e] += d;
+                    s2[e] = __builtin_fmaf(d, d, s2[e]);
+                }
+        }
+        for (; r < rows; r += rows_at) {
+            const VT w = *reinterpret_cast<const VT*>(x + r * a.ldx);
+#pragma unroll
+            for (int e = 0; e < E; ++e) {
+                const float d = static_cast<float>(w[e]) - x0[e];
+                s1[e] += d;
+                s2[e] = __builtin_fmaf(d, d, s2[e]);
+            }
+        }
+    }
+    const uint32_t plane = rows_at * a.C;
+    if (in) {
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+            const uint32_t i = ty * a.C + tx * E + e;
+            red[i] = x0[e];
+            red[plane + i] = s1[e];
+            red[2 * plane + i] = s2[e];
+        }
+    }
+    __syncthreads();
+    // a group's sums about its first thread's first value, in 64 bits
+    const uint32_t n = lanes_of(T, a.groups), lane = tid % n, per = T / n;
+    const uint32_t used = min(rows_at, rows);
+    for (uint32_t g0 = 0; g0 < a.groups; g0 += per) {
+        const uint32_t g = min(g0 + tid / n, a.groups - 1);
+        const float ref = red[g * a.cg];
+        double t1 = 0.0, t2 = 0.0;
+        for (uint32_t y = 0; y < used; ++y) {
+            const double k = static_cast<double>((rows - y + rows_at - 1) / rows_at);  // rows of this thread
+            for (uint32_t c = lane; c < a.cg; c += n) {
+                const uint32_t i = y * a.C + g * a.cg + c;
+                const double d = static_cast<double>(red[i]) - static_cast<double>(ref), u = static_cast<double>(red[plane + i]);
+                t1 += u + k * d;
+                t2 += static_cast<double>(red[2 * plane + i]) + d * (2.0 * u + k * d);
+            }
+        }
+        t1 = lanes_sum(t1, n);
+        t2 = lanes_sum(t2, n);
+        if (lane == 0 && g0 + tid / n < a.groups) {
+            const double rest = t1 / (static_cast<double>(rows) * a.cg);
+            a.part[static_cast<uint64_t>(blockIdx.x) * a.groups + g] = Part{ref, static_cast<float>(rest), static_cast<float>(t2 - t1 * rest), 0.0f};
+        }
+    }
+}
+
+// Grid: batch * ncut, an image's workgroups from its last rows to its first: those that the statistics have read last are still
+// in the last-level cache. LDS: the statistics.
+template <typename TX, typename TY, int ACT>
+__global__ __launch_bounds__(1024) void gn_apply_kernel(GnArgs a) {
+    constexpr int E = Vec<TX>::E;
+    typedef typename Vec<TX>::type VT;
+    typedef TY YT __attribute__((ext_vector_type(E)));
+    extern __shared__ __attribute__((aligned(16))) Stat st[];
+    const uint32_t T = blockDim.x, tid = threadIdx.x, V = a.C / E, rows_at = T / V;
+    const uint32_t ty = tid / V, tx = tid % V;
+    const uint32_t wg = gridDim.x - 1 - blockIdx.x;
+    const uint64_t b = wg / a.ncut;
+    const uint32_t r0 = wg % a.ncut * a.cut, rows = min(a.cut, a.pixels - r0);
+    image_stats(a, b, st);
+    if (!a.joined && r0 == 0 && a.stats)
+        for (uint32_t g = tid; g < a.groups; g += T) a.stats[b * a.groups + g] = st[g];
+    if (ty >= rows_at) return;
+    Cols<E> k;
+    k.set(a, st, tx * E);
+    const TX* x = static_cast<const TX*>(a.x) + b * a.sx + static_cast<uint64_t>(r0) * a.ldx + tx * E;
+    TY* y = static_cast<TY*>(a.y) + b * a.sy + static_cast<uint64_t>(r0) * a.ldy + tx * E;
+    auto store = [&](uint32_t r, const VT& v) {
+        YT o;
+#pragma unroll
+        for (int e = 0; e < E; ++e) o[e] = static_cast<TY>(activate<ACT>(__builtin_fmaf(static_cast<float>(v[e]) - k.mean[e], k.a[e], k.b[e])));
+        *reinterpret_cast<YT*>(y + r * a.ldy) = o;
+    };
+    uint32_t r = ty;
+    for (; r + (kRows - 1) * rows_at < rows; r += kRows * rows_at) {
+        VT w[kRows];
+#pragma unroll
+        for (int i = 0; i < kRows; ++i) w[i] = *reinterpret_cast<const VT*>(x + (r + i * rows_at) * a.ldx);
+#pragma unroll
+        for (int i = 0; i < kRows; ++i) store(r + i * rows_at, w[i]);
+    }
+    for (; r < rows; r += rows_at) store(r, *reinterpret_cast<const VT*>(x + r * a.ldx));
+}
+
+// 8-bit rows: a wave takes a row at a time, four columns (lane + 64 i) each, so that a row's largest value is the wave's. Grid: batch *
+// ncut, T = 256.
+template <typename TX, int ACT, int NV>
+__global__ __launch_bounds__(256) void gn_apply_i8_kernel(GnArgs a) {
+    typedef TX VT __attribute__((ext_vector_type(4)));
+    extern __shared__ __attribute__((aligned(16))) Stat st[];
+    const uint32_t tid = threadIdx.x, lane = tid & 63, v4 = a.C / 4;
+    const uint32_t wg = gridDim.x - 1 - blockIdx.x;
+    const uint64_t b = wg / a.ncut;
+    const uint32_t r0 = wg % a.ncut * a.cut, rows = min(a.cut, a.pixels - r0);
+    image_stats(a, b, st);
+    if (!a.joined && r0 == 0 && a.stats)
+        for (uint32_t g = tid; g < a.groups; g += 256) a.stats[b * a.groups + g] = st[g];
+    Cols<4> k[NV];
+#pragma unroll
+    for (int i = 0; i < NV; ++i) k[i].set(a, st, min(lane + 64 * i, v4 - 1) * 4);
+    const TX* x = static_cast<const TX*>(a.x) + b * a.sx + static_cast<uint64_t>(r0) * a.ldx;
+    int8_t* y = static_cast<int8_t*>(a.y) + b * a.sy + static_cast<uint64_t>(r0) * a.ldy;
+    for (uint32_t r = tid >> 6; r < rows; r += 4) {
+        float z[NV][4];
+        uint32_t top = 0;
+        VT v[NV];
+#pragma unroll
+        for (int i = 0; i < NV; ++i) v[i] = *reinterpret_cast<const VT*>(x + r * a.ldx + min(lane + 64 * i, v4 - 1) * 4);
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                z[i][e] = activate<ACT>(__builtin_fmaf(static_cast<float>(v[i][e]) - k[i].mean[e], k[i].a[e], k[i].b[e]));
+                top = max(top, magnitude_bits(z[i][e]));  // (lanes past the row repeat its last columns)
+            }
+        const RowScale s = row_scale(wave_max(top));
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+            if (lane + 64 * i < v4) *reinterpret_cast<uint32_t*>(y + r * a.ldy + (lane + 64 * i) * 4) = quant_codes4(z[i], s);
+        if (lane == 0) a.y_scale[b * a.pixels + r0 + r] = s.scale;
+    }
+}
+
+// Sums of a chunk's w and w xh for each column, and of w gamma and w gamma xh for each group. Grid: batch * nchunk. LDS: the
+// statistics, then 2 floats a thread's column.
+template <typename TX, typename TD, int ACT>
+__global__ __launch_bounds__(1024) void gn_bwd_cols_kernel(GnBwdArgs a) {
+    constexpr int E = Vec<TX>::E;
+    typedef typename Vec<TX>::type VT;
+    typedef TD DT __attribute__((ext_vector_type(E)));
+    extern __shared__ __attribute__((aligned(16))) Stat st[];
+    const GnArgs& f = a.f;
+    float* const red = reinterpret_cast<float*>(st + f.groups);
+    const uint32_t T = blockDim.x, tid = threadIdx.x, V = f.C / E, rows_at = T / V;
+    const uint32_t ty = tid / V, tx = tid % V;
+    const uint64_t b = blockIdx.x / f.nchunk;
+    const uint32_t chunk = blockIdx.x % f.nchunk, r0 = chunk * f.chunk, rows = min(f.chunk, f.pixels - r0);
+    image_stats(f, b, st);
+    if (!f.joined && chunk == 0)
+        for (uint32_t g = tid; g < f.groups; g += T) f.stats[b * f.groups + g] = st[g];
+    const uint32_t plane = rows_at * f.C;
+    if (ty < rows_at) {
+        const TX* x = static_cast<const TX*>(f.x) + b * f.sx + static_cast<uint64_t>(r0) * f.ldx + tx * E;
+        const TD* dy = static_cast<const TD*>(a.dy) + b * a.sdy + static_cast<uint64_t>(r0) * a.lddy + tx * E;
+        float mean[E], inv[E], low[E], gamma[E], beta[E], s1[E], s2[E];
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+            const uint32_t c = tx * E + e;
+            const Coef one = coef(st[c / f.cg], 1.0f, 0.0f);
+            mean[e] = one.mean;
+            inv[e] = one.a;
+            low[e] = one.b;
+            gamma[e] = f.gamma ? f.gamma[c] : 1.0f;
+            beta[e] = f.beta ? f.beta[c] : 0.0f;
+            s1[e] = s2[e] = 0.0f;
+        }
+        auto add = [&](const VT& v, const DT& d) {
+#pragma unroll
+            for (int e = 0; e < E; ++e) {
+                const float xh = __builtin_fmaf(static_cast<float>(v[e]) - mean[e], inv[e], low[e]);
+                const float w = static_cast<float>(d[e]) * slope<ACT>(__builtin_fmaf(xh, gamma[e], beta[e]));
+                s1[e] += w;
+                s2[e] = __builtin_fmaf(w, xh, s2[e]);
+            }
+        };
+        uint32_t r = ty;
+        for (; r + rows_at < rows; r += 2 * rows_at) {
+            const VT v0 = *reinterpret_cast<const VT*>(x + r * f.ldx), v1 = *reinterpret_cast<const VT*>(x + (r + rows_at) * f.ldx);
+            const DT d0 = *reinterpret_cast<const DT*>(dy + r * a.lddy), d1 = *reinterpret_cast<const DT*>(dy + (r + rows_at) * a.lddy);
+            add(v0, d0);
+            add(v1, d1);
+        }
+        if (r < rows) add(*reinterpret_cast<const VT*>(x + r * f.ldx), *reinterpret_cast<const DT*>(dy + r * a.lddy));
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+            const uint32_t i = ty * f.C + tx * E + e;
+            red[i] = s1[e];
+            red[plane + i] = s2[e];
+        }
+    }
+    __syncthreads();
+    // each column over the threads that share it; the sums stay in the first row's places for the groups
+    float* const out = a.cpart + static_cast<uint64_t>(blockIdx.x) * 2 * f.C;
+    for (uint32_t c = tid; c < f.C; c += T) {
+        float u1 = red[c], u2 = red[plane + c];
+        for (uint32_t y = 1; y < rows_at; ++y) {
+            u1 += red[y * f.C + c];
+            u2 += red[plane + y * f.C + c];
+        }
+        out[c] = u1;
+        out[f.C + c] = u2;
+        const float gamma = f.gamma ? f.gamma[c] : 1.0f;
+        red[c] = u1 * gamma;
+        red[plane + c] = u2 * gamma;
+    }
+    __syncthreads();
+    const uint32_t n = lanes_of(T, f.groups), lane = tid % n, per = T / n;
+    for (uint32_t g0 = 0; g0 < f.groups; g0 += per) {
+        const uint32_t g = min(g0 + tid / n, f.groups - 1);
+        double t1 = 0.0, t2 = 0.0;
+        for (uint32_t c = lane; c < f.cg; c += n) {
+            t1 += static_cast<double>(red[g * f.cg + c]);
+            t2 += static_cast<double>(red[plane + g * f.cg + c]);
+        }
+        t1 = lanes_sum(t1, n);
+        t2 = lanes_sum(t2, n);
+        if (lane == 0 && g0 + tid / n < f.groups) {
+            float* const o = a.gpart + (static_cast<uint64_t>(blockIdx.x) * f.groups + g) * 2;
+            o[0] = static_cast<float>(t1);
+            o[1] = static_cast<float>(t2);
+        }
+    }
+}
+
+// dx. Grid: batch * ncut, then (with dgamma) the workgroups of the weights' gradients, 32 columns each. LDS: the statistics, the groups'
+// means (two floats each), or 32 doubles for each 32 threads.
+template <typename TX, typename TD, int ACT>
+__global__ __launch_bounds__(1024) void gn_bwd_apply_kernel(GnBwdArgs a) {
+    constexpr int E = Vec<TX>::E;
+    typedef typename Vec<TX>::type VT;
+    typedef TD DT __attribute__((ext_vector_type(E)));
+    extern __shared__ __attribute__((aligned(16))) Stat st[];
+    const GnArgs& f = a.f;
+    const uint32_t T = blockDim.x, tid = threadIdx.x;
+    const uint32_t images = f.batch * f.ncut;
+    if (blockIdx.x >= images) {
+        double* const sums = reinterpret_cast<double*>(st);
+        const uint32_t lane = tid & 31, grp = tid >> 5, groups = T >> 5, parts = f.batch * f.nchunk;
+        const uint32_t j = (blockIdx.x - images) * 32 + lane;
+        double s = 0.0;
+        if (j < 2 * f.C)
+            for (uint32_t p = grp; p < parts; p += groups) s += static_cast<double>(a.cpart[static_cast<uint64_t>(p) * 2 * f.C + j]);
+        sums[tid] = s;
+        __syncthreads();
+        if (grp == 0 && j < 2 * f.C) {
+            for (uint32_t i = 1; i < groups; ++i) s += sums[i * 32 + lane];
+            if (j < f.C) a.dbeta[j] = static_cast<float>(s);
+            else a.dgamma[j - f.C] = static_cast<float>(s);
+        }
+        return;
+    }
+    float* const gs = reinterpret_cast<float*>(st + f.groups);
+    const uint32_t V = f.C / E, rows_at = T / V, ty = tid / V, tx = tid % V;
+    const uint32_t wg = images - 1 - blockIdx.x;
+    const uint64_t b = wg / f.ncut;
+    const uint32_t r0 = wg % f.ncut * f.cut, rows = min(f.cut, f.pixels - r0);
+    for (uint32_t g = tid; g < f.groups; g += T) st[g] = f.stats[b * f.groups + g];
+    {
+        const uint32_t n = lanes_of(T, f.groups), lane = tid % n, per = T / n;
+        const double total = static_cast<double>(f.pixels) * f.cg;
+        for (uint32_t g0 = 0; g0 < f.groups; g0 += per) {
+            const uint32_t g = min(g0 + tid / n, f.groups - 1);
+            const float* p = a.gpart + (b * f.nchunk * f.groups + g) * 2;
+            double t1 = 0.0, t2 = 0.0;
+            for (uint32_t c = lane; c < f.nchunk; c += n) {
+                t1 += static_cast<double>(p[static_cast<uint64_t>(c) * f.groups * 2]);
+                t2 += static_cast<double>(p[static_cast<uint64_t>(c) * f.groups * 2 + 1]);
+            }
+            t1 = lanes_sum(t1, n);
+            t2 = lanes_sum(t2, n);
+            if (lane == 0 && g0 + tid / n < f.groups) {
+                gs[2 * g] = static_cast<float>(t1 / total);
+                gs[2 * g + 1] = static_cast<float>(t2 / total);
+            }
+        }
+    }
+    __syncthreads();
+    if (ty >= rows_at) return;
+    // dx = inv (w gamma - m1 - xh m2)
+    float mean[E], inv[E], low[E], gamma[E], beta[E], m1[E], m2[E];
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+        const uint32_t c = tx * E + e, g = c / f.cg;
+        const Coef one = coef(st[g], 1.0f, 0.0f);
+        mean[e] = one.mean;
+        inv[e] = one.a;
+        low[e] = one.b;
+        gamma[e] = f.gamma ? f.gamma[c] : 1.0f;
+        beta[e] = f.beta ? f.beta[c] : 0.0f;
+        m1[e] = gs[2 * g];
+        m2[e] = gs[2 * g + 1];
+    }
+    const TX* x = static_cast<const TX*>(f.x) + b * f.sx + static_cast<uint64_t>(r0) * f.ldx + tx * E;
+    const TD* dy = static_cast<const TD*>(a.dy) + b * a.sdy + static_cast<uint64_t>(r0) * a.lddy + tx * E;
+    const TX* res = a.res ? static_cast<const TX*>(a.res) + b * a.sres + static_cast<uint64_t>(r0) * a.ldres + tx * E : nullptr;
+    TX* dx = static_cast<TX*>(a.dx) + b * a.sdx + static_cast<uint64_t>(r0) * a.lddx + tx * E;
+    auto store = [&](uint32_t r, const VT& v, const DT& d, const VT& s) {
+        VT o;
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+            const float xh = __builtin_fmaf(static_cast<float>(v[e]) - mean[e], inv[e], low[e]);
+            const float w = static_cast<float>(d[e]) * slope<ACT>(__builtin_fmaf(xh, gamma[e], beta[e]));
+            const float q = inv[e] * __builtin_fmaf(-xh, m2[e], __builtin_fmaf(w, gamma[e], -m1[e]));
+            o[e] = static_cast<TX>(res ? q + static_cast<float>(s[e]) : q);
+        }
+        *reinterpret_cast<VT*>(dx + r * a.lddx) = o;
+    };
+    VT zero;
+#pragma unroll
+    for (int e = 0; e < E; ++e) zero[e] = static_cast<TX>(0.0f);
+    uint32_t r = ty;
+    for (; r + rows_at < rows; r += 2 * rows_at) {
+        const uint32_t q = r + rows_at;
+        const VT v0 = *reinterpret_cast<const VT*>(x + r * f.ldx), v1 = *reinterpret_cast<const VT*>(x + q * f.ldx);
+        const DT d0 = *reinterpret_cast<const DT*>(dy + r * a.lddy), d1 = *reinterpret_cast<const DT*>(dy + q * a.lddy);
+        const VT s0 = res ? *reinterpret_cast<const VT*>(res + r * a.ldres) : zero, s1 = res ? *reinterpret_cast<const VT*>(res + q * a.ldres) : zero;
+        store(r, v0, d0, s0);
+        store(q, v1, d1, s1);
+    }
+    if (r < rows)
+        store(r, *reinterpret_cast<const VT*>(x + r * f.ldx), *reinterpret_cast<const DT*>(dy + r * a.lddy),
+              res ? *reinterpret_cast<const VT*>(res + r * a.ldres) : zero);
+}
+
 // ---- host ------------------------------------------------------------------------------
 
 constexpr uint32_t kMaxBatch = 1u << 20, kMaxChannels = 1u << 20;
 constexpr uint64_t kMaxRows = 1ull << 31;
 
 void set_chunks(GnArgs& a) {
-    const uint64_t most = std::max<uint64_t>((static_cast<uint64_t>(a.pixels) + kChunkMin - 1) / kChunkMin, 1);
-    const uint64_t least = std::max<uint64_t>((static_cast<uint64_t>(a.pixels) + kChunkMax - 1) / kChunkMax, 1);
-    const uint64_t want = std::max<uint64_t>(std::min<uint64_t>(most, kChunks / std::max(a.batch, 1u)), least);
-    a.chunk = ceil_div(std::max(a.pixels, 1u), want);
-    a.nchunk = ceil_div(std::max(a.pixels, 1u), a.chunk);
+    const uint64_t pixels = std::max(a.pixels, 1u);
+    const uint64_t most = std::max<uint64_t>(pixels * a.C / kChunkValues, 1);
+    const uint64_t least = (pixels + kChunkMax - 1) / kChunkMax;
+    const uint64_t want = std::min(pixels, std::max<uint64_t>(std::min<uint64_t>(most, kChunks / std::max(a.batch, 1u)), least));
+    a.chunk = ceil_div(pixels, want);
+    a.nchunk = ceil_div(pixels, a.chunk);
+    // two workgroups store what one has summed
+    a.cut = ceil_div(a.chunk, 2);
+    a.ncut = ceil_div(pixels, a.cut);
+}
+
+// Threads of a workgroup whose threads take `vectors` columns: the smallest count from 256 on that leaves a tenth idle at most, or the
+// one that leaves fewest.
+uint32_t threads_for(uint32_t vectors, uint32_t most) {
+    uint32_t best = 256;
+    float use = 0.0f;
+    for (uint32_t t = 256; t <= most; t += 64) {
+        const float u = static_cast<float>(t / vectors * vectors) / static_cast<float>(t);
+        if (u > use + 0.001f) {
+            use = u;
+            best = t;
+        }
+        if (use >= 0.9f) break;
+    }
+    return best;
 }
 
 bool sizes_ok(uint32_t batch, uint32_t pixels, uint32_t channels, uint32_t groups) {
@@ -328,6 +782,7 @@ uint64_t up(uint64_t n) { return (n + 255) / 256 * 256; }
 uint64_t stat_bytes(const GnArgs& a) { return up(static_cast<uint64_t>(a.batch) * a.groups * sizeof(Stat)); }
 uint64_t part_bytes(const GnArgs& a) { return up(static_cast<uint64_t>(a.batch) * a.nchunk * a.groups * sizeof(Part)); }
 uint64_t cpart_bytes(const GnArgs& a) { return up(static_cast<uint64_t>(a.batch) * a.nchunk * 2 * a.C * 4); }
+uint64_t gpart_bytes(const GnArgs& a) { return up(static_cast<uint64_t>(a.batch) * a.nchunk * a.groups * 8); }
 uint64_t gsum_bytes(const GnArgs& a) { return up(static_cast<uint64_t>(a.batch) * a.groups * 8); }
 
 GnArgs sized(uint32_t batch, uint32_t pixels, uint32_t channels, uint32_t groups) {
@@ -426,31 +881,92 @@ int check_ws(const char* fn, const void* ws, uint64_t have, uint64_t need) {
     return MI_OK;
 }
 
+// Whether x's rows are whole 16-byte vectors, and so are the same columns of the other tensors (`e` values of `esz` bytes).
 template <typename TX>
-void launch_stats(const GnArgs& a, hipStream_t s) {
-    gn_part_any_kernel<TX><<<grid_of(static_cast<uint64_t>(a.batch) * a.nchunk * a.groups), 256, 0, s>>>(a);
+bool fast_x(const GnArgs& a) {
+    constexpr uint32_t E = Vec<TX>::E;
+    return a.C % E == 0 && a.C <= kFastChannels && a.groups <= kFastGroups && a.ldx % E == 0 && a.sx % E == 0 && aligned(a.x, 16);
+}
+bool fast_rows(const void* p, uint64_t ld, uint64_t s, uint32_t e, uint64_t esz) {
+    return !p || (ld % e == 0 && s % e == 0 && aligned(p, std::min<uint64_t>(16, e * esz)));
+}
+
+// The sums of the chunks. Returns whether they are joined into a.stats (else every workgroup that needs them joins them).
+template <typename TX>
+bool launch_stats(const GnArgs& a, bool fast, hipStream_t s) {
+    if (fast) {
+        constexpr uint32_t E = Vec<TX>::E;
+        const uint32_t T = threads_for(a.C / E, 4096 / E), rows_at = T / (a.C / E);
+        gn_part_kernel<TX><<<a.batch * a.nchunk, T, 3 * rows_at * a.C * sizeof(float), s>>>(a);
+        if (static_cast<uint64_t>(a.nchunk) * a.groups <= kJoinParts) return false;
+    } else {
+        gn_part_any_kernel<TX><<<grid_of(static_cast<uint64_t>(a.batch) * a.nchunk * a.groups), 256, 0, s>>>(a);
+    }
     gn_join_kernel<<<grid_of((static_cast<uint64_t>(a.batch) * a.groups + 3) / 4), 256, 0, s>>>(a);
+    return true;
+}
+
+template <typename TX, typename TY, int ACT>
+void launch_apply(const GnArgs& a, hipStream_t s) {
+    const uint32_t T = threads_for(a.C / Vec<TX>::E, 4096 / Vec<TX>::E);
+    gn_apply_kernel<TX, TY, ACT><<<a.batch * a.ncut, T, a.groups * sizeof(Stat), s>>>(a);
+}
+
+template <typename TX, int ACT>
+void launch_apply_i8(const GnArgs& a, hipStream_t s) {
+    const unsigned grid = a.batch * a.ncut, lds = a.groups * sizeof(Stat);
+    const uint32_t nv = ceil_div(a.C / 4, 64u);
+    if (nv <= 1) gn_apply_i8_kernel<TX, ACT, 1><<<grid, 256, lds, s>>>(a);
+    else if (nv <= 3) gn_apply_i8_kernel<TX, ACT, 3><<<grid, 256, lds, s>>>(a);
+    else if (nv <= 5) gn_apply_i8_kernel<TX, ACT, 5><<<grid, 256, lds, s>>>(a);
+    else if (nv <= 10) gn_apply_i8_kernel<TX, ACT, 10><<<grid, 256, lds, s>>>(a);
+    else gn_apply_i8_kernel<TX, ACT, 16><<<grid, 256, lds, s>>>(a);
+}
+
+template <typename TX, typename TY, int ACT>
+void launch_forward(GnArgs a, hipStream_t s) {
+    const bool fx = fast_x<TX>(a);
+    const bool fast = fx && fast_rows(a.y, a.ldy, a.sy, sizeof(TY) == 1 ? 4 : Vec<TX>::E, sizeof(TY));
+    a.joined = launch_stats<TX>(a, fx, s);
+    if (fast) {
+        if constexpr (sizeof(TY) == 1) launch_apply_i8<TX, ACT>(a, s);
+        else launch_apply<TX, TY, ACT>(a, s);
+        return;
+    }
+    if (!a.joined) gn_join_kernel<<<grid_of((static_cast<uint64_t>(a.batch) * a.groups + 3) / 4), 256, 0, s>>>(a);
+    gn_apply_any_kernel<TX, TY, ACT><<<grid_of((static_cast<uint64_t>(a.batch) * a.pixels + 3) / 4), 256, 0, s>>>(a);
 }
 
 template <typename TX, typename TY>
-void launch_apply(const GnArgs& a, int act, hipStream_t s) {
-    const unsigned grid = grid_of((static_cast<uint64_t>(a.batch) * a.pixels + 3) / 4);
-    if (act == MI_ACT_SILU) gn_apply_any_kernel<TX, TY, MI_ACT_SILU><<<grid, 256, 0, s>>>(a);
-    else gn_apply_any_kernel<TX, TY, MI_ACT_NONE><<<grid, 256, 0, s>>>(a);
+void launch_forward(const GnArgs& a, int act, hipStream_t s) {
+    if (act == MI_ACT_SILU) launch_forward<TX, TY, MI_ACT_SILU>(a, s);
+    else launch_forward<TX, TY, MI_ACT_NONE>(a, s);
 }
 
 template <typename TX>
 void launch_forward(const GnArgs& a, int y_dtype, int act, hipStream_t s) {
-    launch_stats<TX>(a, s);
-    if (y_dtype == MI_F32) launch_apply<TX, float>(a, act, s);
-    else if (y_dtype == MI_F16) launch_apply<TX, _Float16>(a, act, s);
-    else launch_apply<TX, int8_t>(a, act, s);
+    if (y_dtype == MI_F32) launch_forward<TX, float>(a, act, s);
+    else if (y_dtype == MI_F16) launch_forward<TX, _Float16>(a, act, s);
+    else launch_forward<TX, int8_t>(a, act, s);
 }
 
 template <typename TX, typename TD, int ACT>
-void launch_backward(const GnBwdArgs& a, bool stats, hipStream_t s) {
-    const GnArgs& f = a.f;
-    if (stats) launch_stats<TX>(f, s);
+void launch_backward(GnBwdArgs a, bool stats, hipStream_t s) {
+    GnArgs& f = a.f;
+    constexpr uint32_t E = Vec<TX>::E;
+    const bool fx = fast_x<TX>(f);
+    const bool fast = fx && fast_rows(a.dy, a.lddy, a.sdy, E, sizeof(TD)) && fast_rows(a.dx, a.lddx, a.sdx, E, sizeof(TX)) &&
+                      fast_rows(a.res, a.ldres, a.sres, E, sizeof(TX));
+    f.joined = stats ? launch_stats<TX>(f, fx, s) : 1;
+    if (fast) {
+        const uint32_t T = threads_for(f.C / E, 4096 / E), rows_at = T / (f.C / E);
+        const uint32_t lds = f.groups * sizeof(Stat);
+        gn_bwd_cols_kernel<TX, TD, ACT><<<f.batch * f.nchunk, T, lds + 2 * rows_at * f.C * sizeof(float), s>>>(a);
+        const uint32_t apply = f.batch * f.ncut + (a.dgamma ? ceil_div(2ull * f.C, 32) : 0);
+        gn_bwd_apply_kernel<TX, TD, ACT><<<apply, T, std::max<uint32_t>(lds + f.groups * 8, T * 8), s>>>(a);
+        return;
+    }
+    if (!f.joined) gn_join_kernel<<<grid_of((static_cast<uint64_t>(f.batch) * f.groups + 3) / 4), 256, 0, s>>>(f);
     gn_bwd_cols_any_kernel<TX, TD, ACT><<<grid_of(static_cast<uint64_t>(f.batch) * f.nchunk * ceil_div(f.C, 64)), 256, 0, s>>>(a);
     gn_bwd_groups_kernel<<<grid_of((static_cast<uint64_t>(f.batch) * f.groups + 3) / 4), 256, 0, s>>>(a);
     if (a.dgamma)
@@ -498,7 +1014,7 @@ extern "C" int mi_groupnorm(const mi_groupnorm_args* args, void* workspace, uint
 extern "C" uint64_t mi_groupnorm_bwd_ws_bytes(uint32_t batch, uint32_t pixels, uint32_t channels, uint32_t groups) {
     if (!sizes_ok(batch, pixels, channels, groups) || batch == 0 || pixels == 0) return 0;
     const GnArgs a = sized(batch, pixels, channels, groups);
-    return stat_bytes(a) + part_bytes(a) + gsum_bytes(a) + cpart_bytes(a);
+    return stat_bytes(a) + part_bytes(a) + gsum_bytes(a) + gpart_bytes(a) + cpart_bytes(a);
 }
 
 extern "C" int mi_groupnorm_bwd(const mi_groupnorm_bwd_args* args, void* workspace, uint64_t workspace_bytes, void* stream) {
@@ -552,7 +1068,8 @@ extern "C" int mi_groupnorm_bwd(const mi_groupnorm_bwd_args* args, void* workspa
     a.f.stats = g.stats ? reinterpret_cast<Stat*>(g.stats) : reinterpret_cast<Stat*>(ws);
     a.f.part = reinterpret_cast<Part*>(ws + stat_bytes(f));
     a.gsum = reinterpret_cast<float*>(ws + stat_bytes(f) + part_bytes(f));
-    a.cpart = reinterpret_cast<float*>(ws + stat_bytes(f) + part_bytes(f) + gsum_bytes(f));
+    a.gpart = reinterpret_cast<float*>(ws + stat_bytes(f) + part_bytes(f) + gsum_bytes(f));
+    a.cpart = reinterpret_cast<float*>(ws + stat_bytes(f) + part_bytes(f) + gsum_bytes(f) + gpart_bytes(f));
     const bool stats = !g.stats;
     if (g.x_dtype == MI_F32) {
         if (g.y_dtype == MI_F32) launch_backward<float, float>(a, g.act, stats, s);

@@ -43,4 +43,12 @@ __device__ __forceinline__ int quant_code(float v, const RowScale& s) {
     return static_cast<int>(q);
 }
 
+// Four codes as bytes.
+__device__ __forceinline__ uint32_t quant_codes4(const float (&v)[4], const RowScale& s) {
+    uint32_t r = 0;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) r |= (static_cast<uint32_t>(quant_code(v[e], s)) & 0xffu) << (8 * e);
+    return r;
+}
+
 }  // namespace mi

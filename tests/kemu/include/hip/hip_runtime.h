@@ -515,7 +515,8 @@ inline void wave_barrier() { wave_op("wave_barrier", nullptr, 0, nullptr, 0, nop
 
 // ---- launches ----------------------------------------------------------------------
 template <class... P, class... A>
-inline void launch(const char* name, void (*k)(P...), dim3 grid, dim3 block, size_t, hipStream_t, A&&... args) {
+inline void launch(const char* name, void (*k)(P...), dim3 grid, dim3 block, size_t shmem, hipStream_t, A&&... args) {
+    set_dynamic_lds(shmem);
     std::tuple<typename std::decay<P>::type...> t(static_cast<typename std::decay<P>::type>(args)...);
     auto f = [&]() { std::apply(k, t); };
     BodyOf<decltype(f)> body(std::move(f));

@@ -18,6 +18,23 @@
 #include <string>
 #include <vector>
 
+// LDS of the size that the running launch asks for, against a guard page
+static void* g_dynamic_lds = nullptr;
+static size_t g_dynamic_bytes = 0;
+extern "C" void* kemu_alloc(size_t bytes, int guard_front);
+extern "C" void kemu_free(void* p);
+namespace kemu {
+void set_dynamic_lds(size_t bytes) {
+    if (g_dynamic_lds) kemu_free(g_dynamic_lds);
+    g_dynamic_lds = bytes ? kemu_alloc(bytes, 0) : nullptr;
+    g_dynamic_bytes = bytes;
+}
+void* dynamic_lds() {
+    if (!g_dynamic_lds) die("a kernel with extern __shared__ was launched without dynamic LDS");
+    return g_dynamic_lds;
+}
+}  // namespace kemu
+
 extern "C" __attribute__((weak)) char __start_kemu_lds[];
 extern "C" __attribute__((weak)) char __stop_kemu_lds[];
 
@@ -171,6 +188,7 @@ void run_block(Block& b) {
     }
     if (__start_kemu_lds && __stop_kemu_lds > __start_kemu_lds)
         std::memset(__start_kemu_lds, 0xff, static_cast<size_t>(__stop_kemu_lds - __start_kemu_lds));
+    if (g_dynamic_lds) std::memset(g_dynamic_lds, 0xff, g_dynamic_bytes);
     const int nw = static_cast<int>(b.waves.size());
     auto run_thread = [&](Thread& t) {
         g_cur = &t;

@@ -77,6 +77,9 @@ struct Body {
     virtual void run() = 0;
     virtual ~Body() {}
 };
+// `extern __shared__` arrays: `bytes` of LDS for the launch that follows, filled with 0xFF before every workgroup
+void set_dynamic_lds(size_t bytes);
+void* dynamic_lds();
 void run_grid(const char* name, dim3v grid, dim3v block, Body& body);
 
 template <class F>

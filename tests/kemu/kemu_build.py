@@ -41,6 +41,9 @@ LAUNCH = re.compile(r"([A-Za-z_]\w*(?:<[^<>;()]*>)?)\s*<<<(.*?)>>>\s*\((.*?)\)\s
 # with no effect on values) have no host meaning
 PIN = re.compile(r'asm\s+volatile\(\s*""\s*:\s*"\+v"\([^;]*?\)\s*\)\s*;')
 
+# LDS of a size that the launch gives
+DYNAMIC = re.compile(r"extern\s+__shared__\s+__attribute__\(\(aligned\(16\)\)\)\s+(\w+)\s+(\w+)\[\];")
+
 
 def transform(text: str) -> str:
     """Rewrites every kernel launch into a call of the emulator's launcher."""
@@ -51,6 +54,7 @@ def transform(text: str) -> str:
         return f'::kemu::launch("{name}", {kernel}, {cfg}{sep}{args});'
 
     out = PIN.sub("(void)0;", LAUNCH.sub(repl, text))
+    out = DYNAMIC.sub(r"\1* const \2 = static_cast<\1*>(::kemu::dynamic_lds());", out)
     # LDS pointers are plain host pointers here
     out = out.replace("__attribute__((address_space(3)))", "")
     if "<<<" in out or re.search(r"\basm\b", out):

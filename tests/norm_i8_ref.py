@@ -375,6 +375,9 @@ CASES = {
         dict(P=200, C=64, G=8, offset=1000.0, act=1), dict(P=200, C=30, G=3, offset=-3e4), dict(P=200, C=64, G=8, outlier=1000.0), dict(P=100, C=30, G=3, outlier=300.0, typ="f16", out="f16"),
         dict(P=50, C=32, G=4, scale=1e15), dict(P=50, C=32, G=4, scale=1e-12, eps=1e-30), dict(P=50, C=32, G=4, eps=0.0), dict(P=50, C=32, G=4, constant=True), dict(P=50, C=33, G=3, constant=True),
         dict(P=64, C=32, G=4, act=1, affine="gamma", offset=0.0, scale=30.0, keep=False), dict(B=40, P=3, C=16, G=4, act=1),
+        # several chunks, joined by every workgroup or (many groups) by a launch of their own; some tensors off their 16-byte places
+        dict(P=300, C=320, G=32, act=1), dict(B=2, P=301, C=64, G=8, typ="f16", out="f16", offset=300.0), dict(P=700, C=256, G=256, typ="f16", out="f32", act=1), dict(P=300, C=320, G=32, yoff=1), dict(P=300, C=320, G=32, out="i8", yoff=1),
+        dict(P=301, C=320, G=32, typ="f16", out="i8"), dict(P=700, C=256, G=256, out="i8", keep=False), dict(P=600, C=37, G=1, outlier=500.0), dict(P=40, C=512, G=512), dict(P=3, C=4096, G=256, typ="f16", out="f16"),
         # 8-bit rows
         dict(P=1, C=1, G=1, out="i8"), dict(P=20, C=320, G=32, out="i8"), dict(B=2, P=33, C=640, G=32, typ="f16", out="i8"), dict(P=18, C=1280, G=32, typ="f16", out="i8", act=1),
         dict(P=11, C=37, G=1, out="i8", act=1), dict(B=2, P=19, C=64, G=8, ygap=16, gap=4, out="i8"), dict(B=3, P=9, C=64, G=8, order="rows", out="i8", ygap=1),
@@ -388,6 +391,8 @@ CASES = {
         dict(B=2, P=19, C=64, G=8, gap=3, dgap=1, act=1, res=True), dict(B=3, P=11, C=64, G=8, order="rows", act=1, kept=True), dict(P=30, C=64, G=8, off=1), dict(P=30, C=64, G=8, doff=1, act=1),
         dict(P=30, C=64, G=8, in_place=True), dict(P=31, C=33, G=3, in_place=True, typ="f16", dtyp="f16", act=1), dict(P=200, C=64, G=8, offset=1000.0), dict(P=200, C=64, G=8, offset=300.0, act=1, kept=True),
         dict(P=50, C=32, G=4, gstd=1e-20), dict(P=50, C=32, G=4, gstd=1e10, act=1), dict(B=40, P=3, C=16, G=4, act=1, res=True), dict(P=5, C=2600, G=1, act=1),
+        dict(P=300, C=320, G=32, act=1, res=True), dict(B=2, P=301, C=64, G=8, typ="f16", dtyp="f16", offset=30.0, kept=True), dict(P=700, C=256, G=256, typ="f16", dtyp="f32", act=1), dict(P=300, C=320, G=32, doff=1),
+        dict(P=600, C=37, G=1, act=1), dict(P=40, C=512, G=512), dict(P=3, C=4096, G=256, typ="f16", dtyp="f16", weights=False),
     ],
     "quantize": [
         dict(rows=1, cols=1), dict(rows=5, cols=320), dict(rows=9, cols=1280, typ="f16"), dict(rows=6, cols=37), dict(rows=7, cols=37, typ="f16"), dict(rows=3, cols=5120, typ="f16"),
