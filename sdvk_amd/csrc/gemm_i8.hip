@@ -502,6 +502,49 @@ __global__ __launch_bounds__(256) void quantize_rows_any_kernel(const T* x, int8
     }
 }
 
+// Rows of whole 16-byte vectors, cols <= 16 K (E values a lane, NV vectors): a wave takes a row, which stays in its registers from its
+// largest magnitude to its codes, so it is read once. Lanes past the row repeat its last vector and store nothing.
+template <typename T, int NV>
+__global__ __launch_bounds__(256) void quantize_rows_kernel(const T* x, int8_t* q, float* scale, uint32_t rows, uint32_t cols, uint64_t ldx,
+                                                            uint64_t ldq) {
+    constexpr int E = 16 / static_cast<int>(sizeof(T));
+    typedef T VT __attribute__((ext_vector_type(E)));
+    const uint32_t lane = threadIdx.x & 63, vecs = cols / E;
+    for (uint64_t r = blockIdx.x * 4ull + (threadIdx.x >> 6); r < rows; r += gridDim.x * 4ull) {
+        const T* xr = x + r * ldx;
+        VT v[NV];
+#pragma unroll
+        for (int i = 0; i < NV; ++i) v[i] = *reinterpret_cast<const VT*>(xr + min(lane + 64 * i, vecs - 1) * E);
+        uint32_t top = 0;
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+#pragma unroll
+            for (int e = 0; e < E; ++e) top = max(top, magnitude_bits(static_cast<float>(v[i][e])));
+        const RowScale s = row_scale(wave_max(top));
+        int8_t* qr = q + r * ldq;
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            uint32_t w[E / 4];
+#pragma unroll
+            for (int e = 0; e < E; e += 4) {
+                const float z[4] = {static_cast<float>(v[i][e]), static_cast<float>(v[i][e + 1]), static_cast<float>(v[i][e + 2]),
+                                    static_cast<float>(v[i][e + 3])};
+                w[e / 4] = quant_codes4(z, s);
+            }
+            if (lane + 64 * i < vecs) {
+                uint32_t* p = reinterpret_cast<uint32_t*>(qr + (lane + 64 * i) * E);
+                if constexpr (E == 8) {
+                    typedef uint32_t u2 __attribute__((ext_vector_type(2)));
+                    *reinterpret_cast<u2*>(p) = u2{w[0], w[1]};
+                } else {
+                    *p = w[0];
+                }
+            }
+        }
+        if (lane == 0) scale[r] = s.scale;
+    }
+}
+
 unsigned grid_of(uint64_t units) { return static_cast<unsigned>(std::min<uint64_t>(units, kMaxGrid)); }
 
 uint64_t span(uint64_t rows, uint64_t ld, uint64_t cols) { return rows ? (rows - 1) * ld + cols : 0; }
@@ -570,7 +613,17 @@ void launch_product(I8Args a, hipStream_t s) {
 
 template <typename T>
 void launch_quantize(const T* x, int8_t* q, float* scale, uint32_t rows, uint32_t cols, uint64_t ldx, uint64_t ldq, hipStream_t s) {
-    quantize_rows_any_kernel<T><<<grid_of((static_cast<uint64_t>(rows) + 3) / 4), 256, 0, s>>>(x, q, scale, rows, cols, ldx, ldq);
+    constexpr uint32_t E = 16 / sizeof(T);
+    const unsigned grid = grid_of((static_cast<uint64_t>(rows) + 3) / 4);
+    const uint32_t nv = ceil_div(cols, 64 * E);
+    if (cols % E != 0 || ldx % E != 0 || ldq % E != 0 || !aligned(x, 16) || !aligned(q, E) || nv > 32)
+        quantize_rows_any_kernel<T><<<grid, 256, 0, s>>>(x, q, scale, rows, cols, ldx, ldq);
+    else if (nv <= 2) quantize_rows_kernel<T, 2><<<grid, 256, 0, s>>>(x, q, scale, rows, cols, ldx, ldq);
+    else if (nv <= 3) quantize_rows_kernel<T, 3><<<grid, 256, 0, s>>>(x, q, scale, rows, cols, ldx, ldq);
+    else if (nv <= 5) quantize_rows_kernel<T, 5><<<grid, 256, 0, s>>>(x, q, scale, rows, cols, ldx, ldq);
+    else if (nv <= 10) quantize_rows_kernel<T, 10><<<grid, 256, 0, s>>>(x, q, scale, rows, cols, ldx, ldq);
+    else if (nv <= 20) quantize_rows_kernel<T, 20><<<grid, 256, 0, s>>>(x, q, scale, rows, cols, ldx, ldq);
+    else quantize_rows_kernel<T, 32><<<grid, 256, 0, s>>>(x, q, scale, rows, cols, ldx, ldq);
 }
 
 }  // namespace

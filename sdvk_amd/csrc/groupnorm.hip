@@ -24,7 +24,7 @@ constexpr uint32_t kMaxGrid = 1u << 20;   // workgroups of a launch that strides
 constexpr uint32_t kChunkValues = 8192;   // values of a chunk, at least (but for the last), and ...
 constexpr uint32_t kChunkMax = 2048;      // ... rows at most: the longest chain of fp32 additions
 constexpr uint32_t kChunks = 256;         // chunks of all images, about: a workgroup per CU
-constexpr uint32_t kJoinParts = 4096;     // chunks times groups of an image that every workgroup joins by itself
+constexpr uint32_t kJoinParts = 8192;     // chunks times groups of an image that every workgroup joins by itself
 
 struct Stat {  // of one group of one image, 16 bytes: what `stats` holds
     float mean, low, inv, zero;
@@ -64,6 +64,8 @@ __device__ __forceinline__ double wave_sum(double v) {
     for (int o = 1; o < 64; o <<= 1) v += __shfl_xor(v, o);
     return v;
 }
+
+__device__ __forceinline__ double not_below_zero(double v) { return v < 0.0 ? 0.0 : v; }  // (a NaN stays)
 
 // z = xh gamma + beta as one fma of x - mean: s.low inv gamma is far below beta's rounding unless the mean is large.
 struct Coef {
@@ -138,7 +140,7 @@ __global__ __launch_bounds__(256) void gn_part_any_kernel(GnArgs a) {
             d1 = (red[1][0] + red[1][1]) + (red[1][2] + red[1][3]);
             d2 = (red[2][0] + red[2][1]) + (red[2][2] + red[2][3]);
             const double rest = d1 / static_cast<double>(n);
-            a.part[bc * a.groups + g] = Part{shift, static_cast<float>(rest), static_cast<float>(d2 - d1 * rest), 0.0f};
+            a.part[bc * a.groups + g] = Part{shift, static_cast<float>(rest), static_cast<float>(not_below_zero(d2 - d1 * rest)), 0.0f};
         }
         __syncthreads();  // the sums are free for the next unit
     }
@@ -323,6 +325,7 @@ __global__ __launch_bounds__(256) void gn_bwd_apply_any_kernel(GnBwdArgs a) {
 constexpr uint32_t kFastChannels = 4096, kFastGroups = 256;
 constexpr int kRows = 4;  // rows a thread has in flight
 
+typedef float float2v __attribute__((ext_vector_type(2)));
 template <typename T>
 struct Vec {
     static constexpr int E = 16 / static_cast<int>(sizeof(T));
@@ -349,26 +352,34 @@ __device__ __forceinline__ void image_stats(const GnArgs& a, uint64_t b, Stat* s
         __syncthreads();
         return;
     }
-    const uint32_t n = lanes_of(T, a.groups), lane = tid % n;
+    const uint32_t n = lanes_of(T, a.groups), lane = tid % n, per = T / n;
     const double total = static_cast<double>(a.pixels) * a.cg;
-    const uint32_t per = T / n;
     for (uint32_t g0 = 0; g0 < a.groups; g0 += per) {
         const uint32_t g = min(g0 + tid / n, a.groups - 1);
         const Part* p = a.part + b * a.nchunk * a.groups + g;
-        double s = 0.0;
-        for (uint32_t c = lane; c < a.nchunk; c += n) {
-            const Part q = p[static_cast<uint64_t>(c) * a.groups];
-            s += static_cast<double>(min(a.chunk, a.pixels - c * a.chunk)) * (static_cast<double>(q.shift) + static_cast<double>(q.rest));
+        // sums about the first chunk's mean, in 64 bits; eight chunks' loads in flight (one after another they cost a round trip each:
+        // 2 x 16384 x 320, 128 chunks, 22 us for the kernel that stores y, 13 so)
+        const Part first = p[0];
+        const double ref = static_cast<double>(first.shift) + static_cast<double>(first.rest);
+        double s1 = 0.0, s2 = 0.0;
+        for (uint32_t c0 = lane; c0 < a.nchunk; c0 += 8 * n) {
+            Part q[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) q[i] = p[static_cast<uint64_t>(min(c0 + i * n, a.nchunk - 1)) * a.groups];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const uint32_t c = c0 + i * n;
+                if (c < a.nchunk) {
+                    const double k = static_cast<double>(min(a.chunk, a.pixels - c * a.chunk)) * a.cg;
+                    const double d = (static_cast<double>(q[i].shift) - ref) + static_cast<double>(q[i].rest);
+                    s1 += k * d;
+                    s2 += static_cast<double>(q[i].m2) + k * d * d;
+                }
+            }
         }
-        const double mean = lanes_sum(s, n) / a.pixels;
-        s = 0.0;
-        for (uint32_t c = lane; c < a.nchunk; c += n) {
-            const Part q = p[static_cast<uint64_t>(c) * a.groups];
-            const double k = static_cast<double>(min(a.chunk, a.pixels - c * a.chunk)) * a.cg;
-            const double d = (static_cast<double>(q.shift) - mean) + static_cast<double>(q.rest);
-            s += static_cast<double>(q.m2) + k * d * d;
-        }
-        const double var = lanes_sum(s, n) / total;
+        s1 = lanes_sum(s1, n);
+        s2 = lanes_sum(s2, n);
+        const double off = s1 / total, mean = ref + off, var = not_below_zero(s2 - s1 * off) / total;
         if (lane == 0 && g0 + tid / n < a.groups) {
             const float hi = static_cast<float>(mean);
             st[g] = Stat{hi, static_cast<float>(mean - static_cast<double>(hi)), static_cast<float>(1.0 / sqrt(var + static_cast<double>(a.eps))), 0.0f};
@@ -377,15 +388,41 @@ __device__ __forceinline__ void image_stats(const GnArgs& a, uint64_t b, Stat* s
     __syncthreads();
 }
 
+// The E values of gamma or beta from column c0 on (`other` without them).
+template <int E>
+__device__ __forceinline__ void column_values(const float* p, uint32_t c0, float other, float (&v)[E]) {
+#pragma unroll
+    for (int e = 0; e < E; ++e) v[e] = p ? p[c0 + e] : other;
+}
+// The groups of columns c0 .. c0 + E - 1, by one division.
+template <int E>
+__device__ __forceinline__ void column_groups(uint32_t c0, uint32_t cg, uint32_t (&g)[E]) {
+    uint32_t q = c0 / cg, r = c0 - q * cg;
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+        g[e] = q;
+        if (++r == cg) {
+            r = 0;
+            ++q;
+        }
+    }
+}
+
 // What a thread needs of E columns from c0 on.
 template <int E>
 struct Cols {
     float mean[E], a[E], b[E];
+    // before the statistics are there: gamma and beta
+    __device__ __forceinline__ void load(const GnArgs& f, uint32_t c0) {
+        column_values(f.gamma, c0, 1.0f, a);
+        column_values(f.beta, c0, 0.0f, b);
+    }
     __device__ __forceinline__ void set(const GnArgs& f, const Stat* st, uint32_t c0) {
+        uint32_t g[E];
+        column_groups(c0, f.cg, g);
 #pragma unroll
         for (int e = 0; e < E; ++e) {
-            const uint32_t c = c0 + e;
-            const Coef k = coef(st[c / f.cg], f.gamma ? f.gamma[c] : 1.0f, f.beta ? f.beta[c] : 0.0f);
+            const Coef k = coef(st[g[e]], a[e], b[e]);
             mean[e] = k.mean;
             a[e] = k.a;
             b[e] = k.b;
@@ -467,7 +504,7 @@ __global__ __launch_bounds__(1024) void gn_part_kernel(GnArgs a) {
         t2 = lanes_sum(t2, n);
         if (lane == 0 && g0 + tid / n < a.groups) {
             const double rest = t1 / (static_cast<double>(rows) * a.cg);
-            a.part[static_cast<uint64_t>(blockIdx.x) * a.groups + g] = Part{ref, static_cast<float>(rest), static_cast<float>(t2 - t1 * rest), 0.0f};
+            a.part[static_cast<uint64_t>(blockIdx.x) * a.groups + g] = Part{ref, static_cast<float>(rest), static_cast<float>(not_below_zero(t2 - t1 * rest)), 0.0f};
         }
     }
 }
@@ -485,11 +522,12 @@ __global__ __launch_bounds__(1024) void gn_apply_kernel(GnArgs a) {
     const uint32_t wg = gridDim.x - 1 - blockIdx.x;
     const uint64_t b = wg / a.ncut;
     const uint32_t r0 = wg % a.ncut * a.cut, rows = min(a.cut, a.pixels - r0);
+    Cols<E> k;
+    k.load(a, tx * E);
     image_stats(a, b, st);
     if (!a.joined && r0 == 0 && a.stats)
         for (uint32_t g = tid; g < a.groups; g += T) a.stats[b * a.groups + g] = st[g];
     if (ty >= rows_at) return;
-    Cols<E> k;
     k.set(a, st, tx * E);
     const TX* x = static_cast<const TX*>(a.x) + b * a.sx + static_cast<uint64_t>(r0) * a.ldx + tx * E;
     TY* y = static_cast<TY*>(a.y) + b * a.sy + static_cast<uint64_t>(r0) * a.ldy + tx * E;
@@ -520,10 +558,12 @@ __global__ __launch_bounds__(256) void gn_apply_i8_kernel(GnArgs a) {
     const uint32_t wg = gridDim.x - 1 - blockIdx.x;
     const uint64_t b = wg / a.ncut;
     const uint32_t r0 = wg % a.ncut * a.cut, rows = min(a.cut, a.pixels - r0);
+    Cols<4> k[NV];
+#pragma unroll
+    for (int i = 0; i < NV; ++i) k[i].load(a, min(lane + 64 * i, v4 - 1) * 4);
     image_stats(a, b, st);
     if (!a.joined && r0 == 0 && a.stats)
         for (uint32_t g = tid; g < a.groups; g += 256) a.stats[b * a.groups + g] = st[g];
-    Cols<4> k[NV];
 #pragma unroll
     for (int i = 0; i < NV; ++i) k[i].set(a, st, min(lane + 64 * i, v4 - 1) * 4);
     const TX* x = static_cast<const TX*>(a.x) + b * a.sx + static_cast<uint64_t>(r0) * a.ldx;
@@ -563,6 +603,9 @@ __global__ __launch_bounds__(1024) void gn_bwd_cols_kernel(GnBwdArgs a) {
     const uint32_t ty = tid / V, tx = tid % V;
     const uint64_t b = blockIdx.x / f.nchunk;
     const uint32_t chunk = blockIdx.x % f.nchunk, r0 = chunk * f.chunk, rows = min(f.chunk, f.pixels - r0);
+    float mean[E], inv[E], low[E], gamma[E], beta[E], s1[E], s2[E];
+    column_values(f.gamma, tx * E, 1.0f, gamma);
+    column_values(f.beta, tx * E, 0.0f, beta);
     image_stats(f, b, st);
     if (!f.joined && chunk == 0)
         for (uint32_t g = tid; g < f.groups; g += T) f.stats[b * f.groups + g] = st[g];
@@ -570,16 +613,14 @@ __global__ __launch_bounds__(1024) void gn_bwd_cols_kernel(GnBwdArgs a) {
     if (ty < rows_at) {
         const TX* x = static_cast<const TX*>(f.x) + b * f.sx + static_cast<uint64_t>(r0) * f.ldx + tx * E;
         const TD* dy = static_cast<const TD*>(a.dy) + b * a.sdy + static_cast<uint64_t>(r0) * a.lddy + tx * E;
-        float mean[E], inv[E], low[E], gamma[E], beta[E], s1[E], s2[E];
+        uint32_t g[E];
+        column_groups(tx * E, f.cg, g);
 #pragma unroll
         for (int e = 0; e < E; ++e) {
-            const uint32_t c = tx * E + e;
-            const Coef one = coef(st[c / f.cg], 1.0f, 0.0f);
+            const Coef one = coef(st[g[e]], 1.0f, 0.0f);
             mean[e] = one.mean;
             inv[e] = one.a;
             low[e] = one.b;
-            gamma[e] = f.gamma ? f.gamma[c] : 1.0f;
-            beta[e] = f.beta ? f.beta[c] : 0.0f;
             s1[e] = s2[e] = 0.0f;
         }
         auto add = [&](const VT& v, const DT& d) {
@@ -656,8 +697,16 @@ __global__ __launch_bounds__(1024) void gn_bwd_apply_kernel(GnBwdArgs a) {
         const uint32_t lane = tid & 31, grp = tid >> 5, groups = T >> 5, parts = f.batch * f.nchunk;
         const uint32_t j = (blockIdx.x - images) * 32 + lane;
         double s = 0.0;
-        if (j < 2 * f.C)
-            for (uint32_t p = grp; p < parts; p += groups) s += static_cast<double>(a.cpart[static_cast<uint64_t>(p) * 2 * f.C + j]);
+        if (j < 2 * f.C) {
+            const float* q = a.cpart + j;
+            const uint64_t w = 2ull * f.C;
+            uint32_t p = grp;
+            for (; p + 3 * groups < parts; p += 4 * groups) {
+                const float v0 = q[p * w], v1 = q[(p + groups) * w], v2 = q[(p + 2 * groups) * w], v3 = q[(p + 3 * groups) * w];
+                s += (static_cast<double>(v0) + static_cast<double>(v1)) + (static_cast<double>(v2) + static_cast<double>(v3));
+            }
+            for (; p < parts; p += groups) s += static_cast<double>(q[p * w]);
+        }
         sums[tid] = s;
         __syncthreads();
         if (grp == 0 && j < 2 * f.C) {
@@ -672,17 +721,27 @@ __global__ __launch_bounds__(1024) void gn_bwd_apply_kernel(GnBwdArgs a) {
     const uint32_t wg = images - 1 - blockIdx.x;
     const uint64_t b = wg / f.ncut;
     const uint32_t r0 = wg % f.ncut * f.cut, rows = min(f.cut, f.pixels - r0);
+    float mean[E], inv[E], low[E], gamma[E], beta[E], m1[E], m2[E];
+    column_values(f.gamma, tx * E, 1.0f, gamma);
+    column_values(f.beta, tx * E, 0.0f, beta);
     for (uint32_t g = tid; g < f.groups; g += T) st[g] = f.stats[b * f.groups + g];
     {
         const uint32_t n = lanes_of(T, f.groups), lane = tid % n, per = T / n;
         const double total = static_cast<double>(f.pixels) * f.cg;
         for (uint32_t g0 = 0; g0 < f.groups; g0 += per) {
             const uint32_t g = min(g0 + tid / n, f.groups - 1);
-            const float* p = a.gpart + (b * f.nchunk * f.groups + g) * 2;
+            const float2v* p = reinterpret_cast<const float2v*>(a.gpart) + b * f.nchunk * f.groups + g;
             double t1 = 0.0, t2 = 0.0;
-            for (uint32_t c = lane; c < f.nchunk; c += n) {
-                t1 += static_cast<double>(p[static_cast<uint64_t>(c) * f.groups * 2]);
-                t2 += static_cast<double>(p[static_cast<uint64_t>(c) * f.groups * 2 + 1]);
+            for (uint32_t c0 = lane; c0 < f.nchunk; c0 += 8 * n) {
+                float2v q[8];
+#pragma unroll
+                for (int i = 0; i < 8; ++i) q[i] = p[static_cast<uint64_t>(min(c0 + i * n, f.nchunk - 1)) * f.groups];
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+                    if (c0 + i * n < f.nchunk) {
+                        t1 += static_cast<double>(q[i][0]);
+                        t2 += static_cast<double>(q[i][1]);
+                    }
             }
             t1 = lanes_sum(t1, n);
             t2 = lanes_sum(t2, n);
@@ -695,18 +754,16 @@ __global__ __launch_bounds__(1024) void gn_bwd_apply_kernel(GnBwdArgs a) {
     __syncthreads();
     if (ty >= rows_at) return;
     // dx = inv (w gamma - m1 - xh m2)
-    float mean[E], inv[E], low[E], gamma[E], beta[E], m1[E], m2[E];
+    uint32_t g[E];
+    column_groups(tx * E, f.cg, g);
 #pragma unroll
     for (int e = 0; e < E; ++e) {
-        const uint32_t c = tx * E + e, g = c / f.cg;
-        const Coef one = coef(st[g], 1.0f, 0.0f);
+        const Coef one = coef(st[g[e]], 1.0f, 0.0f);
         mean[e] = one.mean;
         inv[e] = one.a;
         low[e] = one.b;
-        gamma[e] = f.gamma ? f.gamma[c] : 1.0f;
-        beta[e] = f.beta ? f.beta[c] : 0.0f;
-        m1[e] = gs[2 * g];
-        m2[e] = gs[2 * g + 1];
+        m1[e] = gs[2 * g[e]];
+        m2[e] = gs[2 * g[e] + 1];
     }
     const TX* x = static_cast<const TX*>(f.x) + b * f.sx + static_cast<uint64_t>(r0) * f.ldx + tx * E;
     const TD* dy = static_cast<const TD*>(a.dy) + b * a.sdy + static_cast<uint64_t>(r0) * a.lddy + tx * E;
