@@ -516,10 +516,22 @@ __global__ __launch_bounds__(256) void quantize_rows_kernel(const T* x, int8_t* 
 #pragma unroll
         for (int i = 0; i < NV; ++i) v[i] = *reinterpret_cast<const VT*>(xr + min(lane + 64 * i, vecs - 1) * E);
         uint32_t top = 0;
+        if constexpr (E == 8) {
+            // fp16 magnitudes order as 16-bit integers, two at a time
+            typedef uint16_t U8 __attribute__((ext_vector_type(8)));
+            U8 m = __builtin_bit_cast(U8, v[0]) & static_cast<uint16_t>(0x7fff);
 #pragma unroll
-        for (int i = 0; i < NV; ++i)
+            for (int i = 1; i < NV; ++i) m = __builtin_elementwise_max(m, __builtin_bit_cast(U8, v[i]) & static_cast<uint16_t>(0x7fff));
+            uint16_t t = 0;
 #pragma unroll
-            for (int e = 0; e < E; ++e) top = max(top, magnitude_bits(static_cast<float>(v[i][e])));
+            for (int e = 0; e < 8; ++e) t = t > m[e] ? t : m[e];
+            top = magnitude_bits(static_cast<float>(__builtin_bit_cast(_Float16, t)));
+        } else {
+#pragma unroll
+            for (int i = 0; i < NV; ++i)
+#pragma unroll
+                for (int e = 0; e < E; ++e) top = max(top, magnitude_bits(static_cast<float>(v[i][e])));
+        }
         const RowScale s = row_scale(wave_max(top));
         int8_t* qr = q + r * ldq;
 #pragma unroll

@@ -146,34 +146,47 @@ __global__ __launch_bounds__(256) void gn_part_any_kernel(GnArgs a) {
     }
 }
 
-// Joins the chunks of a group (a wave each): the mean of the means, then each chunk's deviations about it.
+// Sums of the chunks' means and deviations about `ref`, in 64 bits, over the chunks first, first + n, ... of a group whose parts begin at
+// p: (sum of values - ref, sum of squares about ref). Eight chunks' loads are in flight: one after another they would cost a
+// round trip each.
+__device__ __forceinline__ void join(const GnArgs& a, const Part* p, uint32_t first, uint32_t n, double ref, double& s1, double& s2) {
+    s1 = s2 = 0.0;
+    for (uint32_t c0 = first; c0 < a.nchunk; c0 += 8 * n) {
+        Part q[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) q[i] = p[static_cast<uint64_t>(min(c0 + i * n, a.nchunk - 1)) * a.groups];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const uint32_t c = c0 + i * n;
+            if (c < a.nchunk) {
+                const double k = static_cast<double>(min(a.chunk, a.pixels - c * a.chunk)) * a.cg;
+                const double d = (static_cast<double>(q[i].shift) - ref) + static_cast<double>(q[i].rest);
+                s1 += k * d;
+                s2 += static_cast<double>(q[i].m2) + k * d * d;
+            }
+        }
+    }
+}
+__device__ __forceinline__ Stat stat_of(const GnArgs& a, double ref, double s1, double s2) {
+    const double total = static_cast<double>(a.pixels) * a.cg, off = s1 / total, mean = ref + off;
+    const double var = not_below_zero(s2 - s1 * off) / total;
+    const float hi = static_cast<float>(mean);
+    return Stat{hi, static_cast<float>(mean - static_cast<double>(hi)), static_cast<float>(1.0 / sqrt(var + static_cast<double>(a.eps))), 0.0f};
+}
+
+// Joins the chunks of a group, a wave each.
 __global__ __launch_bounds__(256) void gn_join_kernel(GnArgs a) {
     const uint32_t lane = threadIdx.x & 63;
     const uint64_t units = static_cast<uint64_t>(a.batch) * a.groups;
     for (uint64_t u = blockIdx.x * 4ull + (threadIdx.x >> 6); u < units; u += gridDim.x * 4ull) {
-        const uint64_t b = u / a.groups, g = u % a.groups;
-        const Part* p = a.part + b * a.nchunk * a.groups + g;
-        const double total = static_cast<double>(a.pixels) * a.cg;
-        double s = 0.0;
-        for (uint32_t c = lane; c < a.nchunk; c += 64) {
-            const Part q = p[static_cast<uint64_t>(c) * a.groups];
-            const double n = static_cast<double>(min(a.chunk, a.pixels - c * a.chunk)) * a.cg;
-            s += n * (static_cast<double>(q.shift) + static_cast<double>(q.rest));
-        }
-        const double mean = wave_sum(s) / total;
-        s = 0.0;
-        for (uint32_t c = lane; c < a.nchunk; c += 64) {
-            const Part q = p[static_cast<uint64_t>(c) * a.groups];
-            const double n = static_cast<double>(min(a.chunk, a.pixels - c * a.chunk)) * a.cg;
-            const double d = (static_cast<double>(q.shift) - mean) + static_cast<double>(q.rest);
-            s += static_cast<double>(q.m2) + n * d * d;
-        }
-        const double var = wave_sum(s) / total;
-        if (lane == 0) {
-            const float hi = static_cast<float>(mean);
-            a.stats[u] = Stat{hi, static_cast<float>(mean - static_cast<double>(hi)),
-                              static_cast<float>(1.0 / sqrt(var + static_cast<double>(a.eps))), 0.0f};
-        }
+        const Part* p = a.part + u / a.groups * a.nchunk * a.groups + u % a.groups;
+        const Part first = p[0];
+        const double ref = static_cast<double>(first.shift) + static_cast<double>(first.rest);
+        double s1, s2;
+        join(a, p, lane, 64, ref, s1, s2);
+        s1 = wave_sum(s1);
+        s2 = wave_sum(s2);
+        if (lane == 0) a.stats[u] = stat_of(a, ref, s1, s2);
     }
 }
 
@@ -353,37 +366,16 @@ __device__ __forceinline__ void image_stats(const GnArgs& a, uint64_t b, Stat* s
         return;
     }
     const uint32_t n = lanes_of(T, a.groups), lane = tid % n, per = T / n;
-    const double total = static_cast<double>(a.pixels) * a.cg;
     for (uint32_t g0 = 0; g0 < a.groups; g0 += per) {
         const uint32_t g = min(g0 + tid / n, a.groups - 1);
         const Part* p = a.part + b * a.nchunk * a.groups + g;
-        // sums about the first chunk's mean, in 64 bits; eight chunks' loads in flight (one after another they cost a round trip each:
-        // 2 x 16384 x 320, 128 chunks, 22 us for the kernel that stores y, 13 so)
         const Part first = p[0];
         const double ref = static_cast<double>(first.shift) + static_cast<double>(first.rest);
-        double s1 = 0.0, s2 = 0.0;
-        for (uint32_t c0 = lane; c0 < a.nchunk; c0 += 8 * n) {
-            Part q[8];
-#pragma unroll
-            for (int i = 0; i < 8; ++i) q[i] = p[static_cast<uint64_t>(min(c0 + i * n, a.nchunk - 1)) * a.groups];
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const uint32_t c = c0 + i * n;
-                if (c < a.nchunk) {
-                    const double k = static_cast<double>(min(a.chunk, a.pixels - c * a.chunk)) * a.cg;
-                    const double d = (static_cast<double>(q[i].shift) - ref) + static_cast<double>(q[i].rest);
-                    s1 += k * d;
-                    s2 += static_cast<double>(q[i].m2) + k * d * d;
-                }
-            }
-        }
+        double s1, s2;
+        join(a, p, lane, n, ref, s1, s2);
         s1 = lanes_sum(s1, n);
         s2 = lanes_sum(s2, n);
-        const double off = s1 / total, mean = ref + off, var = not_below_zero(s2 - s1 * off) / total;
-        if (lane == 0 && g0 + tid / n < a.groups) {
-            const float hi = static_cast<float>(mean);
-            st[g] = Stat{hi, static_cast<float>(mean - static_cast<double>(hi)), static_cast<float>(1.0 / sqrt(var + static_cast<double>(a.eps))), 0.0f};
-        }
+        if (lane == 0 && g0 + tid / n < a.groups) st[g] = stat_of(a, ref, s1, s2);
     }
     __syncthreads();
 }
@@ -449,27 +441,20 @@ __global__ __launch_bounds__(1024) void gn_part_kernel(GnArgs a) {
         const VT v = *reinterpret_cast<const VT*>(x + ty * a.ldx);
 #pragma unroll
         for (int e = 0; e < E; ++e) x0[e] = static_cast<float>(v[e]);
-        uint32_t r = ty + rows_at;
-        for (; r + (kRows - 1) * rows_at < rows; r += kRows * rows_at) {
+        // (a batch's rows past the chunk repeat its last row and add nothing: one by one they would cost a round trip each)
+        for (uint32_t r = ty + rows_at; r < rows; r += kRows * rows_at) {
             VT w[kRows];
 #pragma unroll
-            for (int i = 0; i < kRows; ++i) w[i] = *reinterpret_cast<const VT*>(x + (r + i * rows_at) * a.ldx);
+            for (int i = 0; i < kRows; ++i) w[i] = *reinterpret_cast<const VT*>(x + min(r + i * rows_at, rows - 1) * a.ldx);
 #pragma unroll
-            for (int i = 0; i < kRows; ++i)
+            for (int i = 0; i < kRows; ++i) {
+                const bool whole = r + i * rows_at < rows;
 #pragma unroll
                 for (int e = 0; e < E; ++e) {
-                    const float d = static_cast<float>(w[i][e]) - x0[e];
+                    const float d = whole ? static_cast<float>(w[i][e]) - x0[e] : 0.0f;
                     s1[e] += d;
                     s2[e] = __builtin_fmaf(d, d, s2[e]);
                 }
-        }
-        for (; r < rows; r += rows_at) {
-            const VT w = *reinterpret_cast<const VT*>(x + r * a.ldx);
-#pragma unroll
-            for (int e = 0; e < E; ++e) {
-                const float d = static_cast<float>(w[e]) - x0[e];
-                s1[e] += d;
-                s2[e] = __builtin_fmaf(d, d, s2[e]);
             }
         }
     }
@@ -537,21 +522,20 @@ __global__ __launch_bounds__(1024) void gn_apply_kernel(GnArgs a) {
         for (int e = 0; e < E; ++e) o[e] = static_cast<TY>(activate<ACT>(__builtin_fmaf(static_cast<float>(v[e]) - k.mean[e], k.a[e], k.b[e])));
         *reinterpret_cast<YT*>(y + r * a.ldy) = o;
     };
-    uint32_t r = ty;
-    for (; r + (kRows - 1) * rows_at < rows; r += kRows * rows_at) {
+    for (uint32_t r = ty; r < rows; r += kRows * rows_at) {
         VT w[kRows];
 #pragma unroll
-        for (int i = 0; i < kRows; ++i) w[i] = *reinterpret_cast<const VT*>(x + (r + i * rows_at) * a.ldx);
+        for (int i = 0; i < kRows; ++i) w[i] = *reinterpret_cast<const VT*>(x + min(r + i * rows_at, rows - 1) * a.ldx);
 #pragma unroll
-        for (int i = 0; i < kRows; ++i) store(r + i * rows_at, w[i]);
+        for (int i = 0; i < kRows; ++i)
+            if (r + i * rows_at < rows) store(r + i * rows_at, w[i]);
     }
-    for (; r < rows; r += rows_at) store(r, *reinterpret_cast<const VT*>(x + r * a.ldx));
 }
 
-// 8-bit rows: a wave takes a row at a time, four columns (lane + 64 i) each, so that a row's largest value is the wave's. Grid: batch *
-// ncut, T = 256.
-template <typename TX, int ACT, int NV>
-__global__ __launch_bounds__(256) void gn_apply_i8_kernel(GnArgs a) {
+// 8-bit rows: a wave takes two rows at a time, four columns (lane + 64 i) each, so that a row's largest value is the wave's. Grid: batch *
+// ncut, T threads.
+template <typename TX, int ACT, int NV, int T>
+__global__ __launch_bounds__(T) void gn_apply_i8_kernel(GnArgs a) {
     typedef TX VT __attribute__((ext_vector_type(4)));
     extern __shared__ __attribute__((aligned(16))) Stat st[];
     const uint32_t tid = threadIdx.x, lane = tid & 63, v4 = a.C / 4;
@@ -563,29 +547,39 @@ __global__ __launch_bounds__(256) void gn_apply_i8_kernel(GnArgs a) {
     for (int i = 0; i < NV; ++i) k[i].load(a, min(lane + 64 * i, v4 - 1) * 4);
     image_stats(a, b, st);
     if (!a.joined && r0 == 0 && a.stats)
-        for (uint32_t g = tid; g < a.groups; g += 256) a.stats[b * a.groups + g] = st[g];
+        for (uint32_t g = tid; g < a.groups; g += T) a.stats[b * a.groups + g] = st[g];
 #pragma unroll
     for (int i = 0; i < NV; ++i) k[i].set(a, st, min(lane + 64 * i, v4 - 1) * 4);
     const TX* x = static_cast<const TX*>(a.x) + b * a.sx + static_cast<uint64_t>(r0) * a.ldx;
     int8_t* y = static_cast<int8_t*>(a.y) + b * a.sy + static_cast<uint64_t>(r0) * a.ldy;
-    for (uint32_t r = tid >> 6; r < rows; r += 4) {
-        float z[NV][4];
-        uint32_t top = 0;
-        VT v[NV];
+    constexpr int kPair = NV > 10 ? 1 : 2;  // (16 vectors leave registers for one row)
+    constexpr uint32_t kWaves = T / 64;
+    for (uint32_t r = tid >> 6; r < rows; r += kPair * kWaves) {
+        VT v[kPair][NV];
 #pragma unroll
-        for (int i = 0; i < NV; ++i) v[i] = *reinterpret_cast<const VT*>(x + r * a.ldx + min(lane + 64 * i, v4 - 1) * 4);
+        for (int u = 0; u < kPair; ++u)
 #pragma unroll
-        for (int i = 0; i < NV; ++i)
+            for (int i = 0; i < NV; ++i)
+                v[u][i] = *reinterpret_cast<const VT*>(x + min(r + u * kWaves, rows - 1) * a.ldx + min(lane + 64 * i, v4 - 1) * 4);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                z[i][e] = activate<ACT>(__builtin_fmaf(static_cast<float>(v[i][e]) - k[i].mean[e], k[i].a[e], k[i].b[e]));
-                top = max(top, magnitude_bits(z[i][e]));  // (lanes past the row repeat its last columns)
-            }
-        const RowScale s = row_scale(wave_max(top));
+        for (int u = 0; u < kPair; ++u) {
+            const uint32_t row = r + u * kWaves;
+            if (row >= rows) break;  // (the wave's: every lane agrees)
+            float z[NV][4];
+            uint32_t top = 0;
 #pragma unroll
-        for (int i = 0; i < NV; ++i)
-            if (lane + 64 * i < v4) *reinterpret_cast<uint32_t*>(y + r * a.ldy + (lane + 64 * i) * 4) = quant_codes4(z[i], s);
-        if (lane == 0) a.y_scale[b * a.pixels + r0 + r] = s.scale;
+            for (int i = 0; i < NV; ++i)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    z[i][e] = activate<ACT>(__builtin_fmaf(static_cast<float>(v[u][i][e]) - k[i].mean[e], k[i].a[e], k[i].b[e]));
+                    top = max(top, magnitude_bits(z[i][e]));  // (lanes past the row repeat its last columns)
+                }
+            const RowScale s = row_scale(wave_max(top));
+#pragma unroll
+            for (int i = 0; i < NV; ++i)
+                if (lane + 64 * i < v4) *reinterpret_cast<uint32_t*>(y + row * a.ldy + (lane + 64 * i) * 4) = quant_codes4(z[i], s);
+            if (lane == 0) a.y_scale[b * a.pixels + r0 + row] = s.scale;
+        }
     }
 }
 
@@ -623,23 +617,22 @@ __global__ __launch_bounds__(1024) void gn_bwd_cols_kernel(GnBwdArgs a) {
             low[e] = one.b;
             s1[e] = s2[e] = 0.0f;
         }
-        auto add = [&](const VT& v, const DT& d) {
+        auto add = [&](const VT& v, const DT& d, bool whole) {
 #pragma unroll
             for (int e = 0; e < E; ++e) {
                 const float xh = __builtin_fmaf(static_cast<float>(v[e]) - mean[e], inv[e], low[e]);
                 const float w = static_cast<float>(d[e]) * slope<ACT>(__builtin_fmaf(xh, gamma[e], beta[e]));
-                s1[e] += w;
-                s2[e] = __builtin_fmaf(w, xh, s2[e]);
+                s1[e] += whole ? w : 0.0f;
+                s2[e] = whole ? __builtin_fmaf(w, xh, s2[e]) : s2[e];
             }
         };
-        uint32_t r = ty;
-        for (; r + rows_at < rows; r += 2 * rows_at) {
-            const VT v0 = *reinterpret_cast<const VT*>(x + r * f.ldx), v1 = *reinterpret_cast<const VT*>(x + (r + rows_at) * f.ldx);
-            const DT d0 = *reinterpret_cast<const DT*>(dy + r * a.lddy), d1 = *reinterpret_cast<const DT*>(dy + (r + rows_at) * a.lddy);
-            add(v0, d0);
-            add(v1, d1);
+        for (uint32_t r = ty; r < rows; r += 2 * rows_at) {
+            const uint32_t q = min(r + rows_at, rows - 1);
+            const VT v0 = *reinterpret_cast<const VT*>(x + r * f.ldx), v1 = *reinterpret_cast<const VT*>(x + q * f.ldx);
+            const DT d0 = *reinterpret_cast<const DT*>(dy + r * a.lddy), d1 = *reinterpret_cast<const DT*>(dy + q * a.lddy);
+            add(v0, d0, true);
+            add(v1, d1, r + rows_at < rows);
         }
-        if (r < rows) add(*reinterpret_cast<const VT*>(x + r * f.ldx), *reinterpret_cast<const DT*>(dy + r * a.lddy));
 #pragma unroll
         for (int e = 0; e < E; ++e) {
             const uint32_t i = ty * f.C + tx * E + e;
@@ -783,18 +776,127 @@ __global__ __launch_bounds__(1024) void gn_bwd_apply_kernel(GnBwdArgs a) {
     VT zero;
 #pragma unroll
     for (int e = 0; e < E; ++e) zero[e] = static_cast<TX>(0.0f);
-    uint32_t r = ty;
-    for (; r + rows_at < rows; r += 2 * rows_at) {
-        const uint32_t q = r + rows_at;
+    for (uint32_t r = ty; r < rows; r += 2 * rows_at) {
+        const uint32_t q = min(r + rows_at, rows - 1);
         const VT v0 = *reinterpret_cast<const VT*>(x + r * f.ldx), v1 = *reinterpret_cast<const VT*>(x + q * f.ldx);
         const DT d0 = *reinterpret_cast<const DT*>(dy + r * a.lddy), d1 = *reinterpret_cast<const DT*>(dy + q * a.lddy);
-        const VT s0 = res ? *reinterpret_cast<const VT*>(res + r * a.ldres) : zero, s1 = res ? *reinterpret_cast<const VT*>(res + q * a.ldres) : zero;
+        const VT s0 = res ? *reinterpret_cast<const VT*>(res + r * a.ldres) : zero;
+        VT s1 = zero;
+        if (res && r + rows_at < rows) s1 = *reinterpret_cast<const VT*>(res + q * a.ldres);  // (dx may be res: not after its store)
         store(r, v0, d0, s0);
-        store(q, v1, d1, s1);
+        if (r + rows_at < rows) store(q, v1, d1, s1);
     }
-    if (r < rows)
-        store(r, *reinterpret_cast<const VT*>(x + r * f.ldx), *reinterpret_cast<const DT*>(dy + r * a.lddy),
-              res ? *reinterpret_cast<const VT*>(res + r * a.ldres) : zero);
+}
+
+// ---- a group in a workgroup's registers --------------------------------------------------
+//
+// Images of few pixels: a workgroup holds one group of one image, loads it once and stores y: one launch instead of two, whose second
+// would wait for the first (256 x 1280 fp32 9.7 us with two). A thread's unit is VE neighbouring values, NU units at
+// most. The sums are taken about the mean that a first sum gives.
+constexpr uint32_t kSlabThreads = 512, kSlabChannels = 1024, kSlabGroups = 1u << 20;
+
+template <int CTRL>
+__device__ __forceinline__ float dpp_add(float v) {
+    return v + __builtin_bit_cast(float, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, v), CTRL, 0xf, 0xf, false));
+}
+__device__ __forceinline__ float wave_sum32(float v) {
+    v = dpp_add<0xb1>(v);   // quad_perm [1, 0, 3, 2]
+    v = dpp_add<0x4e>(v);   // quad_perm [2, 3, 0, 1]
+    v = dpp_add<0x141>(v);  // row_half_mirror
+    v = dpp_add<0x140>(v);  // row_mirror
+    v += __shfl_xor(v, 16);
+    v += __shfl_xor(v, 32);
+    return v;
+}
+
+template <typename TX, typename TY, int ACT, int VE, int NU>
+__global__ __launch_bounds__(512) void gn_slab_kernel(GnArgs a) {
+    constexpr uint32_t T = kSlabThreads;
+    typedef TX VT __attribute__((ext_vector_type(VE)));
+    typedef TY YT __attribute__((ext_vector_type(VE)));
+    __shared__ float sums[3][T / 64];
+    __shared__ float ca[kSlabChannels], cb[kSlabChannels];
+    const uint32_t tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const uint32_t b = blockIdx.x / a.groups, g = blockIdx.x % a.groups;
+    const uint32_t upr = a.cg / VE, units = a.pixels * upr, step_r = T / upr, step_c = T % upr;
+    const uint32_t row0 = tid / upr, col0 = tid % upr;
+    const TX* x = static_cast<const TX*>(a.x) + b * a.sx + static_cast<uint64_t>(g) * a.cg;
+    TY* y = static_cast<TY*>(a.y) + b * a.sy + static_cast<uint64_t>(g) * a.cg;
+    for (uint32_t c = tid; c < a.cg; c += T) {
+        ca[c] = a.gamma ? a.gamma[g * a.cg + c] : 1.0f;
+        cb[c] = a.beta ? a.beta[g * a.cg + c] : 0.0f;
+    }
+    VT v[NU];
+    uint32_t row = row0, col = col0;
+    auto next = [&]() {
+        row += step_r;
+        col += step_c;
+        if (col >= upr) {
+            col -= upr;
+            ++row;
+        }
+    };
+#pragma unroll
+    for (int i = 0; i < NU; ++i) {
+        const bool in = tid + i * T < units;
+        v[i] = *reinterpret_cast<const VT*>(x + (in ? row : 0u) * a.ldx + (in ? col : 0u) * VE);
+        next();
+    }
+    float s = 0.0f;
+#pragma unroll
+    for (int i = 0; i < NU; ++i)
+#pragma unroll
+        for (int e = 0; e < VE; ++e) s += tid + i * T < units ? static_cast<float>(v[i][e]) : 0.0f;
+    s = wave_sum32(s);
+    if (lane == 0) sums[0][wave] = s;
+    __syncthreads();
+    double t = 0.0;
+#pragma unroll
+    for (uint32_t w = 0; w < T / 64; ++w) t += static_cast<double>(sums[0][w]);
+    const float ref = static_cast<float>(t / (static_cast<double>(a.pixels) * a.cg));
+    float s1 = 0.0f, s2 = 0.0f;
+#pragma unroll
+    for (int i = 0; i < NU; ++i)
+#pragma unroll
+        for (int e = 0; e < VE; ++e) {
+            const float d = tid + i * T < units ? static_cast<float>(v[i][e]) - ref : 0.0f;
+            s1 += d;
+            s2 = __builtin_fmaf(d, d, s2);
+        }
+    s1 = wave_sum32(s1);
+    s2 = wave_sum32(s2);
+    if (lane == 0) {
+        sums[1][wave] = s1;
+        sums[2][wave] = s2;
+    }
+    __syncthreads();
+    double d1 = 0.0, d2 = 0.0;
+#pragma unroll
+    for (uint32_t w = 0; w < T / 64; ++w) {
+        d1 += static_cast<double>(sums[1][w]);
+        d2 += static_cast<double>(sums[2][w]);
+    }
+    const Stat st = stat_of(a, static_cast<double>(ref), d1, d2);
+    for (uint32_t c = tid; c < a.cg; c += T) {
+        const Coef k = coef(st, ca[c], cb[c]);
+        ca[c] = k.a;
+        cb[c] = k.b;
+    }
+    if (tid == 0) a.stats[blockIdx.x] = st;
+    __syncthreads();
+    row = row0;
+    col = col0;
+#pragma unroll
+    for (int i = 0; i < NU; ++i) {
+        if (tid + i * T < units) {
+            YT o;
+#pragma unroll
+            for (int e = 0; e < VE; ++e)
+                o[e] = static_cast<TY>(activate<ACT>(__builtin_fmaf(static_cast<float>(v[i][e]) - st.mean, ca[col * VE + e], cb[col * VE + e])));
+            *reinterpret_cast<YT*>(y + row * a.ldy + col * VE) = o;
+        }
+        next();
+    }
 }
 
 // ---- host ------------------------------------------------------------------------------
@@ -814,12 +916,12 @@ void set_chunks(GnArgs& a) {
     a.ncut = ceil_div(pixels, a.cut);
 }
 
-// Threads of a workgroup whose threads take `vectors` columns: the smallest count from 256 on that leaves a tenth idle at most, or the
+// Threads of a workgroup whose threads take `vectors` columns: the smallest count from 512 on that leaves a tenth idle at most, or the
 // one that leaves fewest.
 uint32_t threads_for(uint32_t vectors, uint32_t most) {
-    uint32_t best = 256;
+    uint32_t best = 512;
     float use = 0.0f;
-    for (uint32_t t = 256; t <= most; t += 64) {
+    for (uint32_t t = 512; t <= most; t += 64) {
         const float u = static_cast<float>(t / vectors * vectors) / static_cast<float>(t);
         if (u > use + 0.001f) {
             use = u;
@@ -944,7 +1046,7 @@ bool fast_x(const GnArgs& a) {
     constexpr uint32_t E = Vec<TX>::E;
     return a.C % E == 0 && a.C <= kFastChannels && a.groups <= kFastGroups && a.ldx % E == 0 && a.sx % E == 0 && aligned(a.x, 16);
 }
-bool fast_rows(const void* p, uint64_t ld, uint64_t s, uint32_t e, uint64_t esz) {
+bool fast_rows(const void* p, uint64_t ld, uint64_t s, uint32_t e, uint64_t esz) {  // (esz e is a power of two)
     return !p || (ld % e == 0 && s % e == 0 && aligned(p, std::min<uint64_t>(16, e * esz)));
 }
 
@@ -973,15 +1075,32 @@ template <typename TX, int ACT>
 void launch_apply_i8(const GnArgs& a, hipStream_t s) {
     const unsigned grid = a.batch * a.ncut, lds = a.groups * sizeof(Stat);
     const uint32_t nv = ceil_div(a.C / 4, 64u);
-    if (nv <= 1) gn_apply_i8_kernel<TX, ACT, 1><<<grid, 256, lds, s>>>(a);
-    else if (nv <= 3) gn_apply_i8_kernel<TX, ACT, 3><<<grid, 256, lds, s>>>(a);
-    else if (nv <= 5) gn_apply_i8_kernel<TX, ACT, 5><<<grid, 256, lds, s>>>(a);
-    else if (nv <= 10) gn_apply_i8_kernel<TX, ACT, 10><<<grid, 256, lds, s>>>(a);
-    else gn_apply_i8_kernel<TX, ACT, 16><<<grid, 256, lds, s>>>(a);
+    if (nv <= 1) gn_apply_i8_kernel<TX, ACT, 1, 512><<<grid, 512, lds, s>>>(a);
+    else if (nv <= 3) gn_apply_i8_kernel<TX, ACT, 3, 512><<<grid, 512, lds, s>>>(a);
+    else if (nv <= 5) gn_apply_i8_kernel<TX, ACT, 5, 512><<<grid, 512, lds, s>>>(a);
+    else if (nv <= 10) gn_apply_i8_kernel<TX, ACT, 10, 256><<<grid, 256, lds, s>>>(a);
+    else gn_apply_i8_kernel<TX, ACT, 16, 256><<<grid, 256, lds, s>>>(a);
+}
+
+// Launches gn_slab_kernel for units of VE values where a group fits and its rows allow them.
+template <typename TX, typename TY, int ACT, int VE>
+bool launch_slab(const GnArgs& a, hipStream_t s) {
+    const uint64_t units = static_cast<uint64_t>(a.pixels) * a.cg / VE;
+    if (a.cg % VE != 0 || a.cg > kSlabChannels || units > 16 * kSlabThreads || !fast_rows(a.x, a.ldx, a.sx, VE, sizeof(TX)) ||
+        !fast_rows(a.y, a.ldy, a.sy, VE, sizeof(TY)))
+        return false;
+    const unsigned grid = a.batch * a.groups;
+    if (units <= 8 * kSlabThreads) gn_slab_kernel<TX, TY, ACT, VE, 8><<<grid, kSlabThreads, 0, s>>>(a);
+    else gn_slab_kernel<TX, TY, ACT, VE, 16><<<grid, kSlabThreads, 0, s>>>(a);
+    return true;
 }
 
 template <typename TX, typename TY, int ACT>
 void launch_forward(GnArgs a, hipStream_t s) {
+    if constexpr (sizeof(TY) != 1) {
+        // (a row's scale needs all groups)
+        if (static_cast<uint64_t>(a.batch) * a.groups <= kSlabGroups && (launch_slab<TX, TY, ACT, 4>(a, s) || launch_slab<TX, TY, ACT, 2>(a, s))) return;
+    }
     const bool fx = fast_x<TX>(a);
     const bool fast = fx && fast_rows(a.y, a.ldy, a.sy, sizeof(TY) == 1 ? 4 : Vec<TX>::E, sizeof(TY));
     a.joined = launch_stats<TX>(a, fx, s);

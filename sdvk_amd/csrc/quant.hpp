@@ -43,12 +43,26 @@ __device__ __forceinline__ int quant_code(float v, const RowScale& s) {
     return static_cast<int>(q);
 }
 
-// Four codes as bytes.
+// Four codes as bytes. Adding 1.5 * 2^23 rounds the product v / scale to an integer in the sum's low bits, whose low byte is the code;
+// where what is left of every value is less than half a step the codes are the nearest integers, and a lane that holds a tie
+// or a quotient that rounded over one (one value in 2^16) takes quant_code.
 __device__ __forceinline__ uint32_t quant_codes4(const float (&v)[4], const RowScale& s) {
-    uint32_t r = 0;
+    constexpr float kMagic = 12582912.0f;
+    float t[4], rest = 0.0f;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) r |= (static_cast<uint32_t>(quant_code(v[e], s)) & 0xffu) << (8 * e);
-    return r;
+    for (int e = 0; e < 4; ++e) {
+        t[e] = __builtin_fmaf(v[e], s.inv, kMagic);
+        rest = fmaxf(rest, fabsf(__builtin_fmaf(kMagic - t[e], s.scale, v[e])));
+    }
+    if (!(rest < 0.5f * s.scale)) {
+        uint32_t r = 0;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) r |= (static_cast<uint32_t>(quant_code(v[e], s)) & 0xffu) << (8 * e);
+        return r;
+    }
+    const uint32_t lo = __builtin_amdgcn_perm(__float_as_uint(t[1]), __float_as_uint(t[0]), 0x0c0c0400u);
+    const uint32_t hi = __builtin_amdgcn_perm(__float_as_uint(t[3]), __float_as_uint(t[2]), 0x04000c0cu);
+    return lo | hi;
 }
 
 }  // namespace mi
