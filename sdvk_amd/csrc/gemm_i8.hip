@@ -14,6 +14,7 @@ namespace mi {
 namespace {
 
 constexpr uint32_t kMaxGrid = 1u << 20;  // workgroups of a launch that strides over its units
+constexpr uint32_t kMaxFastCols = 8192;  // columns of a row that a wave holds
 constexpr uint32_t kMaxK = 131071;       // 2^31 / 2^14
 constexpr uint64_t kMaxLd = 1u << 22;    // row strides that 256 rows address in 31 bits
 
@@ -534,25 +535,19 @@ __global__ __launch_bounds__(256) void quantize_rows_kernel(const T* x, int8_t* 
         }
         const RowScale s = row_scale(wave_max(top));
         int8_t* qr = q + r * ldq;
+        uint32_t w[NV * E / 4];
+        quant_codes<NV * E>([&](int i) { return static_cast<float>(v[i / E][i % E]); }, s, w);
 #pragma unroll
-        for (int i = 0; i < NV; ++i) {
-            uint32_t w[E / 4];
-#pragma unroll
-            for (int e = 0; e < E; e += 4) {
-                const float z[4] = {static_cast<float>(v[i][e]), static_cast<float>(v[i][e + 1]), static_cast<float>(v[i][e + 2]),
-                                    static_cast<float>(v[i][e + 3])};
-                w[e / 4] = quant_codes4(z, s);
-            }
+        for (int i = 0; i < NV; ++i)
             if (lane + 64 * i < vecs) {
                 uint32_t* p = reinterpret_cast<uint32_t*>(qr + (lane + 64 * i) * E);
                 if constexpr (E == 8) {
                     typedef uint32_t u2 __attribute__((ext_vector_type(2)));
-                    *reinterpret_cast<u2*>(p) = u2{w[0], w[1]};
+                    *reinterpret_cast<u2*>(p) = u2{w[2 * i], w[2 * i + 1]};
                 } else {
-                    *p = w[0];
+                    *p = w[i];
                 }
             }
-        }
         if (lane == 0) scale[r] = s.scale;
     }
 }
@@ -628,14 +623,14 @@ void launch_quantize(const T* x, int8_t* q, float* scale, uint32_t rows, uint32_
     constexpr uint32_t E = 16 / sizeof(T);
     const unsigned grid = grid_of((static_cast<uint64_t>(rows) + 3) / 4);
     const uint32_t nv = ceil_div(cols, 64 * E);
-    if (cols % E != 0 || ldx % E != 0 || ldq % E != 0 || !aligned(x, 16) || !aligned(q, E) || nv > 32)
+    if (cols % E != 0 || ldx % E != 0 || ldq % E != 0 || !aligned(x, 16) || !aligned(q, E) || cols > kMaxFastCols)
         quantize_rows_any_kernel<T><<<grid, 256, 0, s>>>(x, q, scale, rows, cols, ldx, ldq);
     else if (nv <= 2) quantize_rows_kernel<T, 2><<<grid, 256, 0, s>>>(x, q, scale, rows, cols, ldx, ldq);
     else if (nv <= 3) quantize_rows_kernel<T, 3><<<grid, 256, 0, s>>>(x, q, scale, rows, cols, ldx, ldq);
     else if (nv <= 5) quantize_rows_kernel<T, 5><<<grid, 256, 0, s>>>(x, q, scale, rows, cols, ldx, ldq);
     else if (nv <= 10) quantize_rows_kernel<T, 10><<<grid, 256, 0, s>>>(x, q, scale, rows, cols, ldx, ldq);
-    else if (nv <= 20) quantize_rows_kernel<T, 20><<<grid, 256, 0, s>>>(x, q, scale, rows, cols, ldx, ldq);
-    else quantize_rows_kernel<T, 32><<<grid, 256, 0, s>>>(x, q, scale, rows, cols, ldx, ldq);
+    else if (sizeof(T) == 2 || nv <= 16) quantize_rows_kernel<T, 16><<<grid, 256, 0, s>>>(x, q, scale, rows, cols, ldx, ldq);
+    else if constexpr (sizeof(T) == 4) quantize_rows_kernel<T, 32><<<grid, 256, 0, s>>>(x, q, scale, rows, cols, ldx, ldq);
 }
 
 }  // namespace

@@ -79,14 +79,14 @@ __device__ __forceinline__ float apply(float x, const Coef& k) { return __builti
 
 constexpr float kLog2e = 1.44269504088896340736f;
 // z sigma(z). The exponential and the reciprocal are the hardware's (1 ulp each); the exponent's argument is off by 2^-24 of
-// itself, which is |z| 2^-24 of the result: no more than z's own rounding does to it. Below z = -87.3 e is held at 2^126: what
-// is left, |z| 2^-126 at most, stands for results below 1e-36.
+// itself, which is |z| 2^-24 of the result: no more than z's own rounding does to it. Where the exponential overflows (z < -88) or
+// its reciprocal is no normal number the result is zero for one below 1e-36.
 template <int ACT>
 __device__ __forceinline__ float activate(float z) {
     if constexpr (ACT == MI_ACT_NONE) return z;
-    return z * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(fminf(-kLog2e * z, 126.0f)));
+    return z * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-kLog2e * z));
 }
-// act'(z) = sigma(z) (1 + z sigma(-z)), sigma(-z) = e sigma(z)
+// act'(z) = sigma(z) (1 + z sigma(-z)), sigma(-z) = e sigma(z); e is held at 2^126, so that e sigma stays 1
 template <int ACT>
 __device__ __forceinline__ float slope(float z) {
     if constexpr (ACT == MI_ACT_NONE) return 1.0f;
@@ -507,6 +507,14 @@ __global__ __launch_bounds__(1024) void gn_apply_kernel(GnArgs a) {
     const uint32_t wg = gridDim.x - 1 - blockIdx.x;
     const uint64_t b = wg / a.ncut;
     const uint32_t r0 = wg % a.ncut * a.cut, rows = min(a.cut, a.pixels - r0);
+    const TX* x = static_cast<const TX*>(a.x) + b * a.sx + static_cast<uint64_t>(r0) * a.ldx + tx * E;
+    // the first rows are on their way while the statistics are joined
+    VT w[kRows];
+    auto load = [&](uint32_t r) {
+#pragma unroll
+        for (int i = 0; i < kRows; ++i) w[i] = *reinterpret_cast<const VT*>(x + min(r + i * rows_at, rows - 1) * a.ldx);
+    };
+    load(ty);
     Cols<E> k;
     k.load(a, tx * E);
     image_stats(a, b, st);
@@ -514,7 +522,6 @@ __global__ __launch_bounds__(1024) void gn_apply_kernel(GnArgs a) {
         for (uint32_t g = tid; g < a.groups; g += T) a.stats[b * a.groups + g] = st[g];
     if (ty >= rows_at) return;
     k.set(a, st, tx * E);
-    const TX* x = static_cast<const TX*>(a.x) + b * a.sx + static_cast<uint64_t>(r0) * a.ldx + tx * E;
     TY* y = static_cast<TY*>(a.y) + b * a.sy + static_cast<uint64_t>(r0) * a.ldy + tx * E;
     auto store = [&](uint32_t r, const VT& v) {
         YT o;
@@ -523,9 +530,7 @@ __global__ __launch_bounds__(1024) void gn_apply_kernel(GnArgs a) {
         *reinterpret_cast<YT*>(y + r * a.ldy) = o;
     };
     for (uint32_t r = ty; r < rows; r += kRows * rows_at) {
-        VT w[kRows];
-#pragma unroll
-        for (int i = 0; i < kRows; ++i) w[i] = *reinterpret_cast<const VT*>(x + min(r + i * rows_at, rows - 1) * a.ldx);
+        if (r != ty) load(r);
 #pragma unroll
         for (int i = 0; i < kRows; ++i)
             if (r + i * rows_at < rows) store(r + i * rows_at, w[i]);
@@ -542,6 +547,19 @@ __global__ __launch_bounds__(T) void gn_apply_i8_kernel(GnArgs a) {
     const uint32_t wg = gridDim.x - 1 - blockIdx.x;
     const uint64_t b = wg / a.ncut;
     const uint32_t r0 = wg % a.ncut * a.cut, rows = min(a.cut, a.pixels - r0);
+    const TX* x = static_cast<const TX*>(a.x) + b * a.sx + static_cast<uint64_t>(r0) * a.ldx;
+    int8_t* y = static_cast<int8_t*>(a.y) + b * a.sy + static_cast<uint64_t>(r0) * a.ldy;
+    constexpr int kPair = NV > 10 ? 1 : 2;  // (16 vectors leave registers for one row)
+    constexpr uint32_t kWaves = T / 64;
+    VT v[kPair][NV];
+    auto load = [&](uint32_t r) {
+#pragma unroll
+        for (int u = 0; u < kPair; ++u)
+#pragma unroll
+            for (int i = 0; i < NV; ++i)
+                v[u][i] = *reinterpret_cast<const VT*>(x + min(r + u * kWaves, rows - 1) * a.ldx + min(lane + 64 * i, v4 - 1) * 4);
+    };
+    load(tid >> 6);  // on their way while the statistics are joined
     Cols<4> k[NV];
 #pragma unroll
     for (int i = 0; i < NV; ++i) k[i].load(a, min(lane + 64 * i, v4 - 1) * 4);
@@ -550,17 +568,8 @@ __global__ __launch_bounds__(T) void gn_apply_i8_kernel(GnArgs a) {
         for (uint32_t g = tid; g < a.groups; g += T) a.stats[b * a.groups + g] = st[g];
 #pragma unroll
     for (int i = 0; i < NV; ++i) k[i].set(a, st, min(lane + 64 * i, v4 - 1) * 4);
-    const TX* x = static_cast<const TX*>(a.x) + b * a.sx + static_cast<uint64_t>(r0) * a.ldx;
-    int8_t* y = static_cast<int8_t*>(a.y) + b * a.sy + static_cast<uint64_t>(r0) * a.ldy;
-    constexpr int kPair = NV > 10 ? 1 : 2;  // (16 vectors leave registers for one row)
-    constexpr uint32_t kWaves = T / 64;
     for (uint32_t r = tid >> 6; r < rows; r += kPair * kWaves) {
-        VT v[kPair][NV];
-#pragma unroll
-        for (int u = 0; u < kPair; ++u)
-#pragma unroll
-            for (int i = 0; i < NV; ++i)
-                v[u][i] = *reinterpret_cast<const VT*>(x + min(r + u * kWaves, rows - 1) * a.ldx + min(lane + 64 * i, v4 - 1) * 4);
+        if (r != tid >> 6) load(r);
 #pragma unroll
         for (int u = 0; u < kPair; ++u) {
             const uint32_t row = r + u * kWaves;
@@ -575,9 +584,11 @@ __global__ __launch_bounds__(T) void gn_apply_i8_kernel(GnArgs a) {
                     top = max(top, magnitude_bits(z[i][e]));  // (lanes past the row repeat its last columns)
                 }
             const RowScale s = row_scale(wave_max(top));
+            uint32_t w[NV];
+            quant_codes<NV * 4>([&](int i) { return z[i / 4][i % 4]; }, s, w);
 #pragma unroll
             for (int i = 0; i < NV; ++i)
-                if (lane + 64 * i < v4) *reinterpret_cast<uint32_t*>(y + row * a.ldy + (lane + 64 * i) * 4) = quant_codes4(z[i], s);
+                if (lane + 64 * i < v4) *reinterpret_cast<uint32_t*>(y + row * a.ldy + (lane + 64 * i) * 4) = w[i];
             if (lane == 0) a.y_scale[b * a.pixels + r0 + row] = s.scale;
         }
     }
@@ -597,6 +608,19 @@ __global__ __launch_bounds__(1024) void gn_bwd_cols_kernel(GnBwdArgs a) {
     const uint32_t ty = tid / V, tx = tid % V;
     const uint64_t b = blockIdx.x / f.nchunk;
     const uint32_t chunk = blockIdx.x % f.nchunk, r0 = chunk * f.chunk, rows = min(f.chunk, f.pixels - r0);
+    const TX* x = static_cast<const TX*>(f.x) + b * f.sx + static_cast<uint64_t>(r0) * f.ldx + tx * E;
+    const TD* dy = static_cast<const TD*>(a.dy) + b * a.sdy + static_cast<uint64_t>(r0) * a.lddy + tx * E;
+    VT v[2];
+    DT d[2];
+    auto load = [&](uint32_t r) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const uint32_t q = min(r + i * rows_at, rows - 1);
+            v[i] = *reinterpret_cast<const VT*>(x + q * f.ldx);
+            d[i] = *reinterpret_cast<const DT*>(dy + q * a.lddy);
+        }
+    };
+    load(ty);  // on their way while the statistics are joined
     float mean[E], inv[E], low[E], gamma[E], beta[E], s1[E], s2[E];
     column_values(f.gamma, tx * E, 1.0f, gamma);
     column_values(f.beta, tx * E, 0.0f, beta);
@@ -605,8 +629,6 @@ __global__ __launch_bounds__(1024) void gn_bwd_cols_kernel(GnBwdArgs a) {
         for (uint32_t g = tid; g < f.groups; g += T) f.stats[b * f.groups + g] = st[g];
     const uint32_t plane = rows_at * f.C;
     if (ty < rows_at) {
-        const TX* x = static_cast<const TX*>(f.x) + b * f.sx + static_cast<uint64_t>(r0) * f.ldx + tx * E;
-        const TD* dy = static_cast<const TD*>(a.dy) + b * a.sdy + static_cast<uint64_t>(r0) * a.lddy + tx * E;
         uint32_t g[E];
         column_groups(tx * E, f.cg, g);
 #pragma unroll
@@ -617,21 +639,19 @@ __global__ __launch_bounds__(1024) void gn_bwd_cols_kernel(GnBwdArgs a) {
             low[e] = one.b;
             s1[e] = s2[e] = 0.0f;
         }
-        auto add = [&](const VT& v, const DT& d, bool whole) {
+        auto add = [&](const VT& vr, const DT& dr, bool whole) {
 #pragma unroll
             for (int e = 0; e < E; ++e) {
-                const float xh = __builtin_fmaf(static_cast<float>(v[e]) - mean[e], inv[e], low[e]);
-                const float w = static_cast<float>(d[e]) * slope<ACT>(__builtin_fmaf(xh, gamma[e], beta[e]));
+                const float xh = __builtin_fmaf(static_cast<float>(vr[e]) - mean[e], inv[e], low[e]);
+                const float w = static_cast<float>(dr[e]) * slope<ACT>(__builtin_fmaf(xh, gamma[e], beta[e]));
                 s1[e] += whole ? w : 0.0f;
                 s2[e] = whole ? __builtin_fmaf(w, xh, s2[e]) : s2[e];
             }
         };
         for (uint32_t r = ty; r < rows; r += 2 * rows_at) {
-            const uint32_t q = min(r + rows_at, rows - 1);
-            const VT v0 = *reinterpret_cast<const VT*>(x + r * f.ldx), v1 = *reinterpret_cast<const VT*>(x + q * f.ldx);
-            const DT d0 = *reinterpret_cast<const DT*>(dy + r * a.lddy), d1 = *reinterpret_cast<const DT*>(dy + q * a.lddy);
-            add(v0, d0, true);
-            add(v1, d1, r + rows_at < rows);
+            if (r != ty) load(r);
+            add(v[0], d[0], true);
+            add(v[1], d[1], r + rows_at < rows);
         }
 #pragma unroll
         for (int e = 0; e < E; ++e) {
@@ -714,6 +734,27 @@ __global__ __launch_bounds__(1024) void gn_bwd_apply_kernel(GnBwdArgs a) {
     const uint32_t wg = images - 1 - blockIdx.x;
     const uint64_t b = wg / f.ncut;
     const uint32_t r0 = wg % f.ncut * f.cut, rows = min(f.cut, f.pixels - r0);
+    const TX* x = static_cast<const TX*>(f.x) + b * f.sx + static_cast<uint64_t>(r0) * f.ldx + tx * E;
+    const TD* dy = static_cast<const TD*>(a.dy) + b * a.sdy + static_cast<uint64_t>(r0) * a.lddy + tx * E;
+    const TX* res = a.res ? static_cast<const TX*>(a.res) + b * a.sres + static_cast<uint64_t>(r0) * a.ldres + tx * E : nullptr;
+    TX* dx = static_cast<TX*>(a.dx) + b * a.sdx + static_cast<uint64_t>(r0) * a.lddx + tx * E;
+    VT v[2], s[2];
+    DT d[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int e = 0; e < E; ++e) s[i][e] = static_cast<TX>(0.0f);
+    auto load = [&](uint32_t r) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const uint32_t q = min(r + i * rows_at, rows - 1);
+            v[i] = *reinterpret_cast<const VT*>(x + q * f.ldx);
+            d[i] = *reinterpret_cast<const DT*>(dy + q * a.lddy);
+            // (a thread's own rows alone: dx may be res, and another thread stores them)
+            if (res && r + i * rows_at < rows && ty < rows_at) s[i] = *reinterpret_cast<const VT*>(res + q * a.ldres);
+        }
+    };
+    load(ty);  // on their way while the sums are joined
     float mean[E], inv[E], low[E], gamma[E], beta[E], m1[E], m2[E];
     column_values(f.gamma, tx * E, 1.0f, gamma);
     column_values(f.beta, tx * E, 0.0f, beta);
@@ -758,33 +799,21 @@ __global__ __launch_bounds__(1024) void gn_bwd_apply_kernel(GnBwdArgs a) {
         m1[e] = gs[2 * g[e]];
         m2[e] = gs[2 * g[e] + 1];
     }
-    const TX* x = static_cast<const TX*>(f.x) + b * f.sx + static_cast<uint64_t>(r0) * f.ldx + tx * E;
-    const TD* dy = static_cast<const TD*>(a.dy) + b * a.sdy + static_cast<uint64_t>(r0) * a.lddy + tx * E;
-    const TX* res = a.res ? static_cast<const TX*>(a.res) + b * a.sres + static_cast<uint64_t>(r0) * a.ldres + tx * E : nullptr;
-    TX* dx = static_cast<TX*>(a.dx) + b * a.sdx + static_cast<uint64_t>(r0) * a.lddx + tx * E;
-    auto store = [&](uint32_t r, const VT& v, const DT& d, const VT& s) {
+    auto store = [&](uint32_t r, const VT& vr, const DT& dr, const VT& sr) {
         VT o;
 #pragma unroll
         for (int e = 0; e < E; ++e) {
-            const float xh = __builtin_fmaf(static_cast<float>(v[e]) - mean[e], inv[e], low[e]);
-            const float w = static_cast<float>(d[e]) * slope<ACT>(__builtin_fmaf(xh, gamma[e], beta[e]));
+            const float xh = __builtin_fmaf(static_cast<float>(vr[e]) - mean[e], inv[e], low[e]);
+            const float w = static_cast<float>(dr[e]) * slope<ACT>(__builtin_fmaf(xh, gamma[e], beta[e]));
             const float q = inv[e] * __builtin_fmaf(-xh, m2[e], __builtin_fmaf(w, gamma[e], -m1[e]));
-            o[e] = static_cast<TX>(res ? q + static_cast<float>(s[e]) : q);
+            o[e] = static_cast<TX>(res ? q + static_cast<float>(sr[e]) : q);
         }
         *reinterpret_cast<VT*>(dx + r * a.lddx) = o;
     };
-    VT zero;
-#pragma unroll
-    for (int e = 0; e < E; ++e) zero[e] = static_cast<TX>(0.0f);
     for (uint32_t r = ty; r < rows; r += 2 * rows_at) {
-        const uint32_t q = min(r + rows_at, rows - 1);
-        const VT v0 = *reinterpret_cast<const VT*>(x + r * f.ldx), v1 = *reinterpret_cast<const VT*>(x + q * f.ldx);
-        const DT d0 = *reinterpret_cast<const DT*>(dy + r * a.lddy), d1 = *reinterpret_cast<const DT*>(dy + q * a.lddy);
-        const VT s0 = res ? *reinterpret_cast<const VT*>(res + r * a.ldres) : zero;
-        VT s1 = zero;
-        if (res && r + rows_at < rows) s1 = *reinterpret_cast<const VT*>(res + q * a.ldres);  // (dx may be res: not after its store)
-        store(r, v0, d0, s0);
-        if (r + rows_at < rows) store(q, v1, d1, s1);
+        if (r != ty) load(r);
+        store(r, v[0], d[0], s[0]);
+        if (r + rows_at < rows) store(r + rows_at, v[1], d[1], s[1]);
     }
 }
 

@@ -32,37 +32,45 @@ __device__ __forceinline__ RowScale row_scale(uint32_t top) {
     return RowScale{s, 1.0f / s};
 }
 
+constexpr float kQuantMagic = 12582912.0f;  // 1.5 * 2^23: a sum of it and a code holds the code in its low bits
+
+// v / scale rounded, as kQuantMagic + code: the fma's rounding is that of v * inv, which is off by 2^-17 at most, so where
+// the exact rest is under half a step the code is the nearest integer. rest: the largest of those seen.
+__device__ __forceinline__ float quant_fast(float v, const RowScale& s, float& rest) {
+    const float t = __builtin_fmaf(v, s.inv, kQuantMagic);
+    rest = fmaxf(rest, fabsf(__builtin_fmaf(kQuantMagic - t, s.scale, v)));
+    return t;
+}
+// ... put right where it is a tie or went one too far (t's last place is one code).
+__device__ __forceinline__ float quant_right(float v, float t, const RowScale& s) {
+    if (s.inv == 0.0f) return kQuantMagic;
+    const float r = __builtin_fmaf(kQuantMagic - t, s.scale, v);
+    const uint32_t bits = __float_as_uint(t);
+    // over half a step, or half a step and an odd code: magnitudes order as integers
+    const bool wrong = magnitude_bits(r) + (bits & 1u) > __float_as_uint(0.5f * s.scale);
+    return wrong ? __uint_as_float(r > 0.0f ? bits + 1 : bits - 1) : t;
+}
 __device__ __forceinline__ int quant_code(float v, const RowScale& s) {
-    if (s.inv == 0.0f) return 0;
-    // within 2^-15 of the quotient: off by one at most, near a tie
-    float q = rintf(v * s.inv);
-    const float rest = __builtin_fmaf(-q, s.scale, v), half = 0.5f * s.scale;  // exact
-    const bool odd = (static_cast<int>(q) & 1) != 0;
-    if (rest > half || (rest == half && odd)) q += 1.0f;
-    else if (rest < -half || (rest == -half && odd)) q -= 1.0f;
-    return static_cast<int>(q);
+    float rest = 0.0f;
+    const float t = quant_right(v, quant_fast(v, s, rest), s);
+    return static_cast<int8_t>(__float_as_uint(t) & 0xffu);
 }
 
-// Four codes as bytes. Adding 1.5 * 2^23 rounds the product v / scale to an integer in the sum's low bits, whose low byte is the code;
-// where what is left of every value is less than half a step the codes are the nearest integers, and a lane that holds a tie
-// or a quotient that rounded over one (one value in 2^16) takes quant_code.
-__device__ __forceinline__ uint32_t quant_codes4(const float (&v)[4], const RowScale& s) {
-    constexpr float kMagic = 12582912.0f;
-    float t[4], rest = 0.0f;
+// N codes of value(0) .. value(N - 1), four a dword. One value in 2^18 or a tie sends its lane through quant_right (code of its own for
+// every value, or branches among them, made the kernels wait for instructions: 2048 x 5120 fp16 14 us).
+template <int N, typename F>
+__device__ __forceinline__ void quant_codes(const F& value, const RowScale& s, uint32_t (&out)[N / 4]) {
+    float t[N], rest = 0.0f;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-        t[e] = __builtin_fmaf(v[e], s.inv, kMagic);
-        rest = fmaxf(rest, fabsf(__builtin_fmaf(kMagic - t[e], s.scale, v[e])));
-    }
+    for (int i = 0; i < N; ++i) t[i] = quant_fast(value(i), s, rest);
     if (!(rest < 0.5f * s.scale)) {
-        uint32_t r = 0;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) r |= (static_cast<uint32_t>(quant_code(v[e], s)) & 0xffu) << (8 * e);
-        return r;
+        for (int i = 0; i < N; ++i) t[i] = quant_right(value(i), t[i], s);
     }
-    const uint32_t lo = __builtin_amdgcn_perm(__float_as_uint(t[1]), __float_as_uint(t[0]), 0x0c0c0400u);
-    const uint32_t hi = __builtin_amdgcn_perm(__float_as_uint(t[3]), __float_as_uint(t[2]), 0x04000c0cu);
-    return lo | hi;
+#pragma unroll
+    for (int i = 0; i < N; i += 4)
+        out[i / 4] = __builtin_amdgcn_perm(__float_as_uint(t[i + 1]), __float_as_uint(t[i]), 0x0c0c0400u) |
+                     __builtin_amdgcn_perm(__float_as_uint(t[i + 3]), __float_as_uint(t[i + 2]), 0x04000c0cu);
 }
 
 }  // namespace mi
