@@ -24,7 +24,9 @@ constexpr uint32_t kMaxGrid = 1u << 20;   // workgroups of a launch that strides
 constexpr uint32_t kChunkValues = 8192;   // values of a chunk, at least (but for the last), and ...
 constexpr uint32_t kChunkMax = 2048;      // ... rows at most: the longest chain of fp32 additions
 constexpr uint32_t kChunks = 256;         // chunks of all images, about: a workgroup per CU
-constexpr uint32_t kJoinParts = 8192;     // chunks times groups of an image that every workgroup joins by itself
+// Parts (of 16 bytes) that all workgroups together read where each joins an image's statistics by itself; more are joined by a launch of
+// its own. us by themselves / by a launch: 2 x 16384 x 320 (2^21 parts) 23.2 / 21.8, 2 x 1024 x 2560 18.5 / 16.6, 576 x 1280 in 8 bits (2^19) 20.0 / 20.9.
+constexpr uint64_t kJoinParts = 1u << 19;
 
 struct Stat {  // of one group of one image, 16 bytes: what `stats` holds
     float mean, low, inv, zero;
@@ -424,7 +426,7 @@ struct Cols {
 
 // Grid: batch * nchunk. LDS: 3 floats a thread's column.
 template <typename TX>
-__global__ __launch_bounds__(1024) void gn_part_kernel(GnArgs a) {
+__global__ __launch_bounds__(4096 / Vec<TX>::E) void gn_part_kernel(GnArgs a) {
     constexpr int E = Vec<TX>::E;
     typedef typename Vec<TX>::type VT;
     extern __shared__ __attribute__((aligned(16))) float red[];  // [3][T / V][C]: x0, sums of x - x0, of its square
@@ -497,7 +499,7 @@ __global__ __launch_bounds__(1024) void gn_part_kernel(GnArgs a) {
 // Grid: batch * ncut, an image's workgroups from its last rows to its first: those that the statistics have read last are still
 // in the last-level cache. LDS: the statistics.
 template <typename TX, typename TY, int ACT>
-__global__ __launch_bounds__(1024) void gn_apply_kernel(GnArgs a) {
+__global__ __launch_bounds__(4096 / Vec<TX>::E) void gn_apply_kernel(GnArgs a) {
     constexpr int E = Vec<TX>::E;
     typedef typename Vec<TX>::type VT;
     typedef TY YT __attribute__((ext_vector_type(E)));
@@ -597,7 +599,7 @@ __global__ __launch_bounds__(T) void gn_apply_i8_kernel(GnArgs a) {
 // Sums of a chunk's w and w xh for each column, and of w gamma and w gamma xh for each group. Grid: batch * nchunk. LDS: the
 // statistics, then 2 floats a thread's column.
 template <typename TX, typename TD, int ACT>
-__global__ __launch_bounds__(1024) void gn_bwd_cols_kernel(GnBwdArgs a) {
+__global__ __launch_bounds__(4096 / Vec<TX>::E) void gn_bwd_cols_kernel(GnBwdArgs a) {
     constexpr int E = Vec<TX>::E;
     typedef typename Vec<TX>::type VT;
     typedef TD DT __attribute__((ext_vector_type(E)));
@@ -650,8 +652,8 @@ __global__ __launch_bounds__(1024) void gn_bwd_cols_kernel(GnBwdArgs a) {
         };
         for (uint32_t r = ty; r < rows; r += 2 * rows_at) {
             if (r != ty) load(r);
-            add(v[0], d[0], true);
-            add(v[1], d[1], r + rows_at < rows);
+#pragma unroll
+            for (int i = 0; i < 2; ++i) add(v[i], d[i], r + i * rows_at < rows);
         }
 #pragma unroll
         for (int e = 0; e < E; ++e) {
@@ -697,7 +699,7 @@ __global__ __launch_bounds__(1024) void gn_bwd_cols_kernel(GnBwdArgs a) {
 // dx. Grid: batch * ncut, then (with dgamma) the workgroups of the weights' gradients, 32 columns each. LDS: the statistics, the groups'
 // means (two floats each), or 32 doubles for each 32 threads.
 template <typename TX, typename TD, int ACT>
-__global__ __launch_bounds__(1024) void gn_bwd_apply_kernel(GnBwdArgs a) {
+__global__ __launch_bounds__(4096 / Vec<TX>::E) void gn_bwd_apply_kernel(GnBwdArgs a) {
     constexpr int E = Vec<TX>::E;
     typedef typename Vec<TX>::type VT;
     typedef TD DT __attribute__((ext_vector_type(E)));
@@ -1086,7 +1088,7 @@ bool launch_stats(const GnArgs& a, bool fast, hipStream_t s) {
         constexpr uint32_t E = Vec<TX>::E;
         const uint32_t T = threads_for(a.C / E, 4096 / E), rows_at = T / (a.C / E);
         gn_part_kernel<TX><<<a.batch * a.nchunk, T, 3 * rows_at * a.C * sizeof(float), s>>>(a);
-        if (static_cast<uint64_t>(a.nchunk) * a.groups <= kJoinParts) return false;
+        if (static_cast<uint64_t>(a.nchunk) * a.groups * a.batch * a.ncut <= kJoinParts) return false;
     } else {
         gn_part_any_kernel<TX><<<grid_of(static_cast<uint64_t>(a.batch) * a.nchunk * a.groups), 256, 0, s>>>(a);
     }
