@@ -34,7 +34,7 @@ int check_launch(const char* what);
 // rows (their own kernel does not round the weights, the tiles do).
 constexpr int kGemmBuilds = 7;  // tile builds of gemm_q8.hip (kNumCfg)
 constexpr int kGemmBwdBuilds = 4;  // tile builds of gemm_q8_bwd.hip
-constexpr int kGemmI8Builds = 8;   // builds of gemm_i8.hip
+constexpr int kGemmI8Builds = 9;   // builds of gemm_i8.hip
 struct Tuning {
     std::atomic<int> gemm_cfg{-1};          // tile build, or -1
     std::atomic<int> gemm_splits{1};        // K splits with gemm_cfg (workspace entries)

@@ -123,7 +123,7 @@ __global__ __launch_bounds__(256) void gemm_i8_any_kernel(I8Args a) {
 // ---- tiles ---------------------------------------------------------------------------
 //
 // A workgroup computes a BM x BN tile of C in steps of 128 codes. A step's rows go from memory straight into LDS
-// (buffer loads with an LDS destination: 8 rows of 128 bytes an instruction), two stages deep. An LDS row is 128 bytes, its
+// (buffer loads with an LDS destination: 8 rows of 128 bytes an instruction), a ring of NS stages deep. An LDS row is 128 bytes, its
 // eight 16-byte slots in the order slot ^ (row / 2) % 8, so that the 16 rows that a fragment read takes at a time lie in
 // different banks; the loads' lanes permute their addresses accordingly (the 128 bytes of a row stay one segment).
 // The product is transposed (W is the MFMA's A operand): a lane holds one row m of C and runs of four columns.
@@ -132,8 +132,23 @@ typedef int intx4 __attribute__((ext_vector_type(4)));
 typedef int intx16 __attribute__((ext_vector_type(16)));
 
 __device__ __forceinline__ uint32_t swz(uint32_t row) { return (row >> 1) & 7u; }
-__device__ __forceinline__ void wait_loads() { __builtin_amdgcn_s_waitcnt(0x0F70); }  // vmcnt(0)
 __device__ __forceinline__ void wait_lds() { __builtin_amdgcn_s_waitcnt(0xC07F); }    // lgkmcnt(0)
+// Waits until at most N of the wave's loads are on their way.
+template <int N>
+__device__ __forceinline__ void wait_loads() {
+    static_assert(N < 64, "vmcnt has six bits");
+    __builtin_amdgcn_s_waitcnt(0x0F70 | (N & 15) | ((N >> 4) << 14));
+}
+// A barrier that waits for nothing else: __syncthreads() would wait for every load on its way. A wave has the fragments of the step
+// before when it gets here (its products have taken them).
+__device__ __forceinline__ void barrier() {
+    __atomic_signal_fence(__ATOMIC_SEQ_CST);
+    __builtin_amdgcn_sched_barrier(0);
+    wait_lds();
+    __builtin_amdgcn_s_barrier();
+    __builtin_amdgcn_sched_barrier(0);
+    __atomic_signal_fence(__ATOMIC_SEQ_CST);
+}
 
 // 16 bytes a lane from `off` of the `bytes` at base (zeros past them) to LDS: lane l's to dst + 16 l.
 __device__ __forceinline__ void load_lds(const int8_t* base, int bytes, int8_t* dst, uint32_t off) {
@@ -181,23 +196,27 @@ struct Out {
     static constexpr int V = 16 / static_cast<int>(sizeof(TC)), LPR = TN / V, RPI = 64 / LPR;  // columns a lane, lanes a row, rows at a time
 };
 
-// KG groups of WM x WN waves take the steps in turn; with two, each hands the other the sums of half its rows at the end.
-template <typename TC, int BM, int BN, int WM, int WN, int KG>
-__global__ __launch_bounds__(KG * WM * WN * 64) void gemm_i8_tile_kernel(I8Args a) {
+template <typename TC, int BM, int BN, int WM, int WN, int NS>
+__global__ __launch_bounds__(WM * WN * 64) void gemm_i8_tile_kernel(I8Args a) {
     constexpr int NW = WM * WN, TM = BM / WM, TN = BN / WN, FM = TM / 32, FN = TN / 32;
-    constexpr int A_IT = BM / 8 / NW, W_IT = BN / 8 / NW, FO = FM / KG;  // FO: 32-row blocks of a wave's own at the end
-    typedef Out<TC, TN, (TN > 128 ? 16 : 32)> O;
-    static_assert(BM % (8 * NW) == 0 && BN % (8 * NW) == 0 && FM % KG == 0, "loads and rows divide evenly");
-    constexpr int P = KG * 128 * (BM > BN ? BM : BN) / (O::kInts * 4), Q = KG * 128 * (BM > BN ? BN : BM) / (O::kInts * 4);
-    static_assert(2 * (P + Q) >= KG * NW, "the epilogue's regions fit the stages");
-    static_assert(KG == 1 || (KG == 2 && FO * FN * 4096 * ((NW + 1) / 2) <= KG * 128 * (BM < BN ? BM : BN)), "the exchanged sums fit the stages");
+    constexpr int A_IT = BM / 8 / NW, W_IT = BN / 8 / NW, T = NW * 64;
+    // the epilogue's regions: P waves' in each of the two larger stage arrays, Q in each of the others, 32 rows each where they fit
+    constexpr int kBig = 128 * (BM > BN ? BM : BN), kSmall = 128 * (BM > BN ? BN : BM), kRow = (TN + 4) * 4;
+    constexpr int R = 2 * (kBig / (32 * kRow) + kSmall / (32 * kRow)) >= NW ? 32 : 16;
+    typedef Out<TC, TN, R> O;
+    static_assert(BM % (8 * NW) == 0 && BN % (8 * NW) == 0, "loads divide evenly");
+    constexpr int P = kBig / (O::kInts * 4), Q = kSmall / (O::kInts * 4);
+    static_assert(2 * (P + Q) >= NW, "the epilogue's regions fit the stages");
     // arrays of their own: the compiler then knows that reads of one stage do not wait for the loads into the other
-    __shared__ __attribute__((aligned(16))) int8_t as0[KG * BM * 128], as1[KG * BM * 128], ws0[KG * BN * 128], ws1[KG * BN * 128];
+    __shared__ __attribute__((aligned(16))) int8_t as0[BM * 128], as1[BM * 128], ws0[BN * 128], ws1[BN * 128];
+    __shared__ __attribute__((aligned(16))) int8_t as2[NS > 2 ? BM * 128 : 16], ws2[NS > 2 ? BN * 128 : 16];
+    __shared__ __attribute__((aligned(16))) int8_t as3[NS > 3 ? BM * 128 : 16], ws3[NS > 3 ? BN * 128 : 16];
+    static_assert(NS >= 2 && NS <= 4, "two to four stages");
     // the tile's scales and biases, read while the first codes are on their way: from memory in the epilogue each would cost a
     // round trip
     __shared__ __attribute__((aligned(16))) float sas[BM], sws[BN], biases[BN];
     const int tid = threadIdx.x, lane = tid & 63;
-    const int wv = __builtin_amdgcn_readfirstlane(tid >> 6), kg = wv / NW, wave = wv % NW;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int l32 = lane & 31, g = lane >> 5, wm = wave % WM, wn = wave / WM;
     uint32_t tm, tn;
     tile_of(a, blockIdx.x, tm, tn);
@@ -216,8 +235,8 @@ __global__ __launch_bounds__(KG * WM * WN * 64) void gemm_i8_tile_kernel(I8Args 
             for (int r = 0; r < 16; ++r) acc[i][j][r] = 0;
     // the fragments of the next 32 codes are read ahead of the products of these
     auto compute = [&](const int8_t* as, const int8_t* ws) {
-        const int8_t* ap = as + kg * BM * 128 + wm * TM * 128;
-        const int8_t* wp = ws + kg * BN * 128 + wn * TN * 128;
+        const int8_t* ap = as + wm * TM * 128;
+        const int8_t* wp = ws + wn * TN * 128;
         intx4 x[2][FM], w[2][FN];
         auto read = [&](auto S) {
             constexpr int s = decltype(S)::value;
@@ -247,74 +266,70 @@ __global__ __launch_bounds__(KG * WM * WN * 64) void gemm_i8_tile_kernel(I8Args 
         multiply(std::integral_constant<int, 3>{});
     };
     auto load = [&](int8_t* as, int8_t* ws, uint32_t k) {  // past K: zeros
-        ra.load(as + kg * BM * 128, k);
-        rw.load(ws + kg * BN * 128, k);
+        ra.load(as, k);
+        rw.load(ws, k);
     };
-    constexpr uint32_t kStep = 128 * KG;
-    const uint32_t kk = 128 * kg;
-    load(as0, ws0, kk);
-    for (int i = tid; i < BM; i += KG * NW * 64) sas[i] = a.sa[min(m0 + i, a.M - 1)];
-    for (int i = tid; i < BN; i += KG * NW * 64) {
-        sws[i] = a.sw[min(n0 + i, a.N - 1)];
-        biases[i] = a.bias ? a.bias[min(n0 + i, a.N - 1)] : 0.0f;
-    }
-    wait_loads();
-    __syncthreads();
-    // two steps a trip, an odd last one behind them (leaving the loop in its middle would copy every sum)
-    const uint32_t steps = (a.K + kStep - 1) / kStep;
-    uint32_t k = kk;
-    for (uint32_t p = steps / 2; p > 0; --p, k += 2 * kStep) {
-        load(as1, ws1, k + kStep);
-        compute(as0, ws0);
-        wait_loads();
-        __syncthreads();
-        load(as0, ws0, k + 2 * kStep);
-        compute(as1, ws1);
-        wait_loads();
-        __syncthreads();
-    }
-    if (steps & 1) {
-        compute(as0, ws0);
-        __syncthreads();
-    }
-    // (every wave has read its last step, no load is in flight: the stages are free)
-    if constexpr (KG == 2) {
-        // slots of (wave, group) in turn over the four arrays, the partner's rows in register order
-        auto slot = [&](int i) {
-            int8_t* const p = (i & 3) == 0 ? as0 : (i & 3) == 1 ? as1 : (i & 3) == 2 ? ws0 : ws1;
-            return reinterpret_cast<intx4*>(p) + (i >> 2) * (FO * FN * 4 * 64) + lane;
-        };
-        intx4* const out = slot(2 * wave + kg);
+    const uint32_t steps = (a.K + 127) / 128;
+    uint32_t k = 0;  // of the next step to compute
+    // (their loads first: what waits for them then waits for no codes)
+    float sa_[(BM + T - 1) / T], sw_[(BN + T - 1) / T], bias_[(BN + T - 1) / T];
 #pragma unroll
-        for (int i = 0; i < FO; ++i)
+    for (int i = 0; i < (BM + T - 1) / T; ++i) sa_[i] = a.sa[min(m0 + min(tid + i * T, BM - 1), a.M - 1)];
 #pragma unroll
-            for (int j = 0; j < FN; ++j)
+    for (int i = 0; i < (BN + T - 1) / T; ++i) {
+        const uint32_t c = min(n0 + min(tid + i * T, BN - 1), a.N - 1);
+        sw_[i] = a.sw[c];
+        bias_[i] = a.bias ? a.bias[c] : 0.0f;
+    }
+    __builtin_amdgcn_sched_barrier(0);
+    load(as0, ws0, k);
+    if constexpr (NS > 2) load(as1, ws1, k + 128);
+    if constexpr (NS > 3) load(as2, ws2, k + 256);
+    __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-                for (int q = 0; q < 4; ++q) {
-                    const intx16 v = kg ? acc[i][j] : acc[FO + i][j];
-                    out[((i * FN + j) * 4 + q) * 64] = intx4{v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]};
+    for (int i = 0; i < (BM + T - 1) / T; ++i)
+        if (tid + i * T < BM) sas[tid + i * T] = sa_[i];
+#pragma unroll
+    for (int i = 0; i < (BN + T - 1) / T; ++i)
+        if (tid + i * T < BN) {
+            sws[tid + i * T] = sw_[i];
+            biases[tid + i * T] = bias_[i];
+        }
+    // One step: its loads have landed (a wave's own, then with the barrier everybody's, and everybody has read the step before), the
+    // loads of the step NS - 1 ahead go where that one was, and its products run.
+    auto step = [&](auto S) {
+        constexpr int s = decltype(S)::value, f = (s + NS - 1) % NS;
+        wait_loads<(NS - 2) * (A_IT + W_IT)>();
+        barrier();
+        load(f == 0 ? as0 : f == 1 ? as1 : f == 2 ? as2 : as3, f == 0 ? ws0 : f == 1 ? ws1 : f == 2 ? ws2 : ws3, k + (NS - 1) * 128);
+        compute(s == 0 ? as0 : s == 1 ? as1 : s == 2 ? as2 : as3, s == 0 ? ws0 : s == 1 ? ws1 : s == 2 ? ws2 : ws3);
+        k += 128;
+    };
+    // NS steps a trip, the last ones behind them (leaving the loop in its middle would copy every sum)
+    for (uint32_t p = steps / NS; p > 0; --p) {
+        step(std::integral_constant<int, 0>{});
+        step(std::integral_constant<int, 1>{});
+        if constexpr (NS > 2) step(std::integral_constant<int, 2>{});
+        if constexpr (NS > 3) step(std::integral_constant<int, 3>{});
+    }
+    const uint32_t rest = steps % NS;
+    if (rest > 0) {
+        step(std::integral_constant<int, 0>{});
+        if constexpr (NS > 2) {
+            if (rest > 1) {
+                step(std::integral_constant<int, 1>{});
+                if constexpr (NS > 3) {
+                    if (rest > 2) step(std::integral_constant<int, 2>{});
                 }
-        __syncthreads();
-        const intx4* const in = slot(2 * wave + 1 - kg);
-#pragma unroll
-        for (int i = 0; i < FO; ++i)
-#pragma unroll
-            for (int j = 0; j < FN; ++j) {
-                intx16 v = kg ? acc[FO + i][j] : acc[i][j];
-#pragma unroll
-                for (int q = 0; q < 4; ++q) {
-                    const intx4 y = in[((i * FN + j) * 4 + q) * 64];
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) v[4 * q + e] += y[e];
-                }
-                acc[i][j] = v;
             }
-        __syncthreads();
+        }
     }
-    // P waves' regions in each of the two larger arrays, Q in each of the others
-    int8_t* const big = (BM > BN ? wv < P ? as0 : as1 : wv < P ? ws0 : ws1) + wv % P * O::kInts * 4;
-    int8_t* const small = (BM > BN ? wv - 2 * P < Q ? ws0 : ws1 : wv - 2 * P < Q ? as0 : as1) + (wv - 2 * P + 2 * P * Q) % Q * O::kInts * 4;
-    int* const stage = reinterpret_cast<int*>(wv < 2 * P ? big : small);
+    wait_loads<0>();
+    __syncthreads();
+    // (every wave has read its last step, no load is on its way: the stages are free)
+    int8_t* const big = (BM > BN ? wave < P ? as0 : as1 : wave < P ? ws0 : ws1) + wave % P * O::kInts * 4;
+    int8_t* const small = (BM > BN ? wave - 2 * P < Q ? ws0 : ws1 : wave - 2 * P < Q ? as0 : as1) + (wave < 2 * P ? 0 : (wave - 2 * P) % (Q ? Q : 1)) * O::kInts * 4;
+    int* const stage = reinterpret_cast<int*>(wave < 2 * P ? big : small);
     const int lrow = lane / O::LPR, lcol = lane % O::LPR * O::V;
     const bool busy = lane < O::LPR * O::RPI;
     const uint32_t n = n0 + wn * TN + lcol;
@@ -327,7 +342,7 @@ __global__ __launch_bounds__(KG * WM * WN * 64) void gemm_i8_tile_kernel(I8Args 
     auto rows = [&](int i, auto WHOLE) {
 #pragma unroll
         for (int h = 0; h < 32; h += O::R) {
-            const int r0 = wm * TM + 32 * (kg * FO + i) + h;
+            const int r0 = wm * TM + 32 * i + h;
             if (O::R == 32 || (l32 & 16) == h) {
 #pragma unroll
                 for (int j = 0; j < FN; ++j)
@@ -358,10 +373,10 @@ __global__ __launch_bounds__(KG * WM * WN * 64) void gemm_i8_tile_kernel(I8Args 
     };
     if (a.wide && m0 + BM <= a.M && n0 + BN <= a.N) {
 #pragma unroll
-        for (int i = 0; i < FO; ++i) rows(i, std::true_type{});
+        for (int i = 0; i < FM; ++i) rows(i, std::true_type{});
     } else {
 #pragma unroll
-        for (int i = 0; i < FO; ++i) rows(i, std::false_type{});
+        for (int i = 0; i < FM; ++i) rows(i, std::false_type{});
     }
 }
 
@@ -405,18 +420,18 @@ __global__ __launch_bounds__(512) void gemm_i8_split_kernel(I8Args a) {
     while (k < a.K) {
         if (k + 1024 < a.K) {
             load(s1, k + 1024);
-            __builtin_amdgcn_s_waitcnt(0x0F78);  // vmcnt(8): the other stage's loads
+            wait_loads<8>();  // (the other stage's)
         } else {
-            wait_loads();
+            wait_loads<0>();
         }
         compute(s0);
         k += 1024;
         if (k >= a.K) break;
         if (k + 1024 < a.K) {
             load(s0, k + 1024);
-            __builtin_amdgcn_s_waitcnt(0x0F78);
+            wait_loads<8>();
         } else {
-            wait_loads();
+            wait_loads<0>();
         }
         compute(s1);
         k += 1024;
@@ -556,22 +571,22 @@ unsigned grid_of(uint64_t units) { return static_cast<unsigned>(std::min<uint64_
 
 uint64_t span(uint64_t rows, uint64_t ld, uint64_t cols) { return rows ? (rows - 1) * ld + cols : 0; }
 
-// Builds: 0 any shape, 1 few rows, 2 waves split K (32 x 32), the others tiles; 5 is 4 with two groups of waves, which take the
-// steps in turn.
+// Builds: 0 any shape, 1 few rows, 2 waves split K (32 x 32), the others tiles: 8 is 3 with three stages, 5 is 4 with four (and eight
+// waves: one workgroup a CU, whose loads alone have to hide their latency).
 //
-// us of a tile build = 3 + n (tile + steps step), n tiles on the fullest of 256 CUs, fitted to a sweep (MI355X). A step is bound by LDS:
-// 8.7 cycles a fragment read and 18.6 a KB loaded into it predict all of them but 64 x 64's. Sweep, us, fp16 C, the five tiles in
-// order: 1024x1280x1280 6.6 / 10.8 / 9.8 / 15.1 / 23.5, 2048x1280x5120 26.9 / 31.5 / 25.4 / 44.1 / 66.0, 8192x640x2560 27.7 / 21.6 / 30.3 / 27.1 / 38.9,
-// 2048x10240x1280 48.9 / 37.0 / 43.8 / 36.1 / 32.4, 8192x5120x640 60.2 / 43.7 / 63.6 / 47.3 / 43.2. 256 x 256 and 256 x 128 tiles were
-// between their neighbours everywhere.
+// us of a tile build = 3 + n (tile + steps step), n tiles on the fullest of 256 CUs, fitted to a sweep (MI355X, fp16 C, us of builds 3, 8, 4, 5, 6, 7):
+//   576x1280x1280     6.7   5.7   8.9   6.9  15.3  24.8      2048x1280x1280   8.8   9.7  10.7   9.2  16.1  25.8
+//   2048x1280x5120   25.6  26.7  30.9  21.8  45.9  69.9      8192x640x2560   26.7  24.3  21.3  25.9  27.3  41.2
+//   8192x640x640     10.0  10.7   9.5  12.4  11.9  18.7      2048x10240x1280 47.6  51.7  36.8  43.3  35.8  32.3
+// (128 x 128 with two groups of waves that take the steps in turn: 24.8 for 2048x1280x5120; 256 x 256, 256 x 128, 128 x 64, 128 x 192 and
+// 64 x 128 tiles were between their neighbours.)
 struct Build {
-    uint32_t bm, bn, step;   // codes of a step
+    uint32_t bm, bn;
     float tile_us, step_us;
 };
-constexpr Build kBuilds[kGemmI8Builds] = {{64, 64, 32, 0, 0}, {16, 16, 0, 0, 0}, {32, 32, 0, 0, 0}, {64, 64, 128, 0.2f, 0.22f}, {128, 128, 128, 1.6f, 0.42f},
-                                          {128, 128, 256, 2.2f, 1.05f}, {192, 256, 128, 3.4f, 0.94f}, {256, 320, 128, 7.7f, 1.38f}};
-enum { kAny = 0, kFew = 1, kSplitK = 2, k64 = 3, k128 = 4, k128x2 = 5, k192 = 6, k256 = 7 };
-constexpr float kAlone128 = 0.68f;  // us a step of 128 x 128 with no second tile on the CU to fill its waits
+constexpr Build kBuilds[kGemmI8Builds] = {{64, 64, 0, 0},          {16, 16, 0, 0},           {32, 32, 0, 0},           {64, 64, 0.2f, 0.23f},  {128, 128, 1.2f, 0.42f},
+                                          {128, 128, 2.05f, 0.42f}, {192, 256, 3.4f, 0.94f}, {256, 320, 7.7f, 1.38f}, {64, 64, 0.2f, 0.15f}};
+enum { kAny = 0, kFew = 1, kSplitK = 2, k64 = 3, k128 = 4, k128x4 = 5, k192 = 6, k256 = 7, k64x3 = 8 };
 
 int choose(const I8Args& a) {
     const bool vec = a.K % 16 == 0 && a.lda % 16 == 0 && a.ldw % 16 == 0 && aligned(a.A, 16) && aligned(a.W, 16) &&
@@ -583,10 +598,12 @@ int choose(const I8Args& a) {
     if (static_cast<uint64_t>(ceil_div(a.M, 64)) * ceil_div(a.N, 64) <= 128) return kSplitK;
     int best = k64;
     float least = 0.0f;
-    for (int b = k64; b <= k256; ++b) {
-        const uint64_t tiles = static_cast<uint64_t>(ceil_div(a.M, kBuilds[b].bm)) * ceil_div(a.N, kBuilds[b].bn);
-        const float n = static_cast<float>((tiles + 255) / 256);
-        const float us = n * (kBuilds[b].tile_us + ceil_div(a.K, kBuilds[b].step) * (b == k128 && tiles <= 256 ? kAlone128 : kBuilds[b].step_us));
+    for (int b = k64; b <= k64x3; ++b) {
+        const uint64_t n = (static_cast<uint64_t>(ceil_div(a.M, kBuilds[b].bm)) * ceil_div(a.N, kBuilds[b].bn) + 255) / 256;
+        if (b == k64x3 && n > 2) continue;  // three workgroups a CU; with more tiles four are faster
+        if (b == k128 && n < 2) continue;   // two workgroups a CU hide each other's latency; one needs four stages
+        const float step = b == k64 && n == 3 ? 0.183f : kBuilds[b].step_us;
+        const float us = static_cast<float>(n) * (kBuilds[b].tile_us + ceil_div(a.K, 128) * step);
         if (b == k64 || us < least) {
             best = b;
             least = us;
@@ -610,11 +627,12 @@ void launch_product(I8Args a, hipStream_t s) {
     switch (build) {
         case kFew: gemm_i8_few_kernel<TC><<<grid, 512, 0, s>>>(a); break;
         case kSplitK: gemm_i8_split_kernel<TC><<<grid, 512, 0, s>>>(a); break;
-        case k64: gemm_i8_tile_kernel<TC, 64, 64, 2, 2, 1><<<grid, 256, 0, s>>>(a); break;
-        case k128: gemm_i8_tile_kernel<TC, 128, 128, 2, 2, 1><<<grid, 256, 0, s>>>(a); break;
-        case k128x2: gemm_i8_tile_kernel<TC, 128, 128, 2, 2, 2><<<grid, 512, 0, s>>>(a); break;
-        case k192: gemm_i8_tile_kernel<TC, 192, 256, 2, 4, 1><<<grid, 512, 0, s>>>(a); break;
-        default: gemm_i8_tile_kernel<TC, 256, 320, 4, 2, 1><<<grid, 512, 0, s>>>(a); break;
+        case k64: gemm_i8_tile_kernel<TC, 64, 64, 2, 2, 2><<<grid, 256, 0, s>>>(a); break;
+        case k128: gemm_i8_tile_kernel<TC, 128, 128, 2, 2, 2><<<grid, 256, 0, s>>>(a); break;
+        case k128x4: gemm_i8_tile_kernel<TC, 128, 128, 4, 2, 4><<<grid, 512, 0, s>>>(a); break;
+        case k192: gemm_i8_tile_kernel<TC, 192, 256, 2, 4, 2><<<grid, 512, 0, s>>>(a); break;
+        case k256: gemm_i8_tile_kernel<TC, 256, 320, 4, 2, 2><<<grid, 512, 0, s>>>(a); break;
+        default: gemm_i8_tile_kernel<TC, 64, 64, 2, 2, 3><<<grid, 256, 0, s>>>(a); break;
     }
 }
 

@@ -546,6 +546,7 @@ inline T __shfl_xor(T v, int mask, int width = 64) {
 #define __builtin_amdgcn_readfirstlane ::kemu::readfirstlane
 #define __builtin_amdgcn_mbcnt_lo ::kemu::mbcnt_lo
 #define __builtin_amdgcn_mbcnt_hi ::kemu::mbcnt_hi
+#define __builtin_amdgcn_s_barrier ::kemu::syncthreads
 #define __builtin_amdgcn_wave_barrier ::kemu::wave_barrier
 #define __builtin_amdgcn_perm ::kemu::perm
 #define __builtin_amdgcn_alignbit ::kemu::alignbit

@@ -416,6 +416,7 @@ CASES = {
         dict(M=1, N=33, K=16, cfg="4"), dict(M=129, N=131, K=400, cfg="4", extreme=True), dict(M=140, N=264, K=272, cfg="4", out="f16", mode=2, ldc=272), dict(M=140, N=134, K=128, cfg="4", out="f16"),
         dict(M=1, N=33, K=16, cfg="5"), dict(M=129, N=131, K=400, cfg="5", extreme=True), dict(M=140, N=264, K=656, cfg="5", out="f16", mode=2, ldc=272), dict(M=128, N=128, K=768, cfg="5", out="f16"),
         dict(M=1, N=33, K=16, cfg="6"), dict(M=193, N=259, K=400, cfg="6", extreme=True), dict(M=200, N=264, K=272, cfg="6", out="f16", mode=1), dict(M=1, N=33, K=16, cfg="7"),
+        *(dict(M=m + 1, N=n + 1, K=k, cfg=c, extreme=True, **o) for c, m, n in (("3", 64, 64), ("5", 128, 128), ("8", 64, 64)) for k, o in ((16, {}), (128, dict(out="f16")), (400, {}), (528, dict(mode=2, out="f16")), (768, dict(mode=1)))),
         dict(M=257, N=321, K=400, cfg="7", extreme=True), dict(M=260, N=328, K=272, cfg="7", out="f16", mode=2),
     ],
 }
