@@ -21,7 +21,7 @@ namespace mi {
 namespace {
 
 constexpr uint32_t kMaxGrid = 1u << 20;   // workgroups of a launch that strides over its units
-constexpr uint32_t kChunkValues = 8192;   // values of a chunk, at least (but for the last), and ...
+constexpr uint32_t kChunkValues = 16384;  // values of a chunk, at least (but for the last), and ...
 constexpr uint32_t kChunkMax = 2048;      // ... rows at most: the longest chain of fp32 additions
 constexpr uint32_t kChunks = 256;         // chunks of all images, about: a workgroup per CU
 // Parts (of 16 bytes) that all workgroups together read where each joins an image's statistics by itself; more are joined by a launch of
@@ -821,10 +821,12 @@ __global__ __launch_bounds__(4096 / Vec<TX>::E) void gn_bwd_apply_kernel(GnBwdAr
 
 // ---- a group in a workgroup's registers --------------------------------------------------
 //
-// Images of few pixels: a workgroup holds one group of one image, loads it once and stores y: one launch instead of two, whose second
-// would wait for the first (256 x 1280 fp32 9.7 us with two). A thread's unit is VE neighbouring values, NU units at
-// most. The sums are taken about the mean that a first sum gives.
-constexpr uint32_t kSlabThreads = 512, kSlabChannels = 1024, kSlabGroups = 1u << 20;
+// Images of few pixels: a workgroup holds one group of one image, loads it once and stores y: one launch instead of two or three, which
+// wait for each other. A thread's unit is VE neighbouring values, NU units at most. The sums are taken about the mean
+// that a first sum gives. us this way / in launches: 256 x 1280 fp32 6.2 / 9.7, 2 x 1024 x 1280 fp16 13.2 / 14.8, but 1024 x 1920 fp32 15.5 / 13.6:
+// a CU takes 256 bytes of x a thread at most. Backward 256 x 1280 fp32 8.8 / 12.4, 2 x 576 x 1280 fp16 20.4 / 17.0: eight units.
+constexpr uint32_t kSlabThreads = 512, kSlabChannels = 1024, kSlabGroups = 1u << 20, kSlabBytes = 256;
+constexpr int kBwdSlabUnits = 8;
 
 template <int CTRL>
 __device__ __forceinline__ float dpp_add(float v) {
@@ -927,6 +929,139 @@ __global__ __launch_bounds__(512) void gn_slab_kernel(GnArgs a) {
             *reinterpret_cast<YT*>(y + row * a.ldy + col * VE) = o;
         }
         next();
+    }
+}
+
+// The gradients of one group of one image: x and dy are loaded once. The threads in use are a multiple of a row's units, so that a thread's
+// columns are the same in all of its rows and their sums stay in registers. part: [batch][2][C] of the weights' gradients, to
+// be summed over the images, or NULL; with one image they are stored as they are.
+template <typename TX, typename TD, int ACT, int VE, int NU>
+__global__ __launch_bounds__(512) void gn_bwd_slab_kernel(GnBwdArgs a, uint32_t recompute) {
+    constexpr uint32_t T = kSlabThreads;
+    typedef TX VT __attribute__((ext_vector_type(VE)));
+    typedef TD DT __attribute__((ext_vector_type(VE)));
+    __shared__ float sums[4][T / 64];
+    __shared__ float red[2][T * VE];
+    const GnArgs& f = a.f;
+    const uint32_t tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const uint32_t b = blockIdx.x / f.groups, g = blockIdx.x % f.groups;
+    const uint32_t upr = f.cg / VE, rows_at = T / upr, row0 = tid / upr, col = tid % upr * VE, c0 = g * f.cg + col;
+    const bool use = row0 < rows_at;
+    const TX* x = static_cast<const TX*>(f.x) + b * f.sx + c0;
+    const TD* dy = static_cast<const TD*>(a.dy) + b * a.sdy + c0;
+    auto in = [&](int i) { return use && row0 + i * rows_at < f.pixels; };
+    VT v[NU];
+    DT d[NU];
+#pragma unroll
+    for (int i = 0; i < NU; ++i) v[i] = *reinterpret_cast<const VT*>(x + (in(i) ? row0 + i * rows_at : 0u) * f.ldx);
+#pragma unroll
+    for (int i = 0; i < NU; ++i) d[i] = *reinterpret_cast<const DT*>(dy + (in(i) ? row0 + i * rows_at : 0u) * a.lddy);
+    float gamma[VE], beta[VE];
+    column_values(f.gamma, c0, 1.0f, gamma);
+    column_values(f.beta, c0, 0.0f, beta);
+    auto total = [&](int k, float s) {  // over the workgroup, in 64 bits over the waves
+        s = wave_sum32(s);
+        if (lane == 0) sums[k][wave] = s;
+    };
+    auto read = [&](int k) {
+        double t = 0.0;
+#pragma unroll
+        for (uint32_t w = 0; w < T / 64; ++w) t += static_cast<double>(sums[k][w]);
+        return t;
+    };
+    const double n = static_cast<double>(f.pixels) * f.cg;
+    Stat st;
+    if (recompute) {
+        float s = 0.0f;
+#pragma unroll
+        for (int i = 0; i < NU; ++i)
+#pragma unroll
+            for (int e = 0; e < VE; ++e) s += in(i) ? static_cast<float>(v[i][e]) : 0.0f;
+        total(0, s);
+        __syncthreads();
+        const float ref = static_cast<float>(read(0) / n);
+        float s1 = 0.0f, s2 = 0.0f;
+#pragma unroll
+        for (int i = 0; i < NU; ++i)
+#pragma unroll
+            for (int e = 0; e < VE; ++e) {
+                const float q = in(i) ? static_cast<float>(v[i][e]) - ref : 0.0f;
+                s1 += q;
+                s2 = __builtin_fmaf(q, q, s2);
+            }
+        total(1, s1);
+        total(2, s2);
+        __syncthreads();
+        st = stat_of(f, static_cast<double>(ref), read(1), read(2));
+        __syncthreads();  // the sums are free
+    } else {
+        st = f.stats[blockIdx.x];
+    }
+#pragma unroll
+    for (int i = 0; i < NU; ++i) asm volatile("" : "+v"(v[i]));
+    const Coef one = coef(st, 1.0f, 0.0f);
+    float u1[VE], u2[VE];
+#pragma unroll
+    for (int e = 0; e < VE; ++e) u1[e] = u2[e] = 0.0f;
+    auto xhat = [&](int i, int e) { return __builtin_fmaf(static_cast<float>(v[i][e]) - one.mean, one.a, one.b); };
+#pragma unroll
+    for (int i = 0; i < NU; ++i)
+#pragma unroll
+        for (int e = 0; e < VE; ++e) {
+            const float xh = xhat(i, e), w = static_cast<float>(d[i][e]) * slope<ACT>(__builtin_fmaf(xh, gamma[e], beta[e]));
+            u1[e] += in(i) ? w : 0.0f;
+            u2[e] = in(i) ? __builtin_fmaf(w, xh, u2[e]) : u2[e];
+        }
+    float t1 = 0.0f, t2 = 0.0f;
+#pragma unroll
+    for (int e = 0; e < VE; ++e) {
+        t1 += u1[e] * gamma[e];
+        t2 += u2[e] * gamma[e];
+        red[0][tid * VE + e] = u1[e];
+        red[1][tid * VE + e] = u2[e];
+    }
+    total(0, t1);
+    total(3, t2);
+    __syncthreads();
+    const float m1 = static_cast<float>(read(0) / n), m2 = static_cast<float>(read(3) / n);
+    if (a.dgamma) {
+        // a column's sums: eight threads, rows r, r + 8, ... each (a row of threads is cg values)
+        for (uint32_t j0 = 0; j0 < 2 * f.cg; j0 += T / 8) {
+            const uint32_t j = min(j0 + tid / 8, 2 * f.cg - 1), c = j % f.cg;
+            const float* q = red[j / f.cg] + c;
+            float s = 0.0f;
+            for (uint32_t r = tid % 8; r < rows_at; r += 8) s += q[r * f.cg];
+            s = lanes_sum(s, 8);
+            if (tid % 8 == 0 && j0 + tid / 8 < 2 * f.cg) {
+                if (f.batch > 1) a.cpart[(static_cast<uint64_t>(b) * 2 + j / f.cg) * f.C + g * f.cg + c] = s;
+                else (j < f.cg ? a.dbeta : a.dgamma)[g * f.cg + c] = s;
+            }
+        }
+    }
+    if (!use) return;
+    // what the sums took of x and dy is computed again: kept, it would not fit the registers
+#pragma unroll
+    for (int i = 0; i < NU; ++i) {
+        asm volatile("" : "+v"(v[i]));
+        asm volatile("" : "+v"(d[i]));
+    }
+    TX* dx = static_cast<TX*>(a.dx) + b * a.sdx + c0;
+    const TX* res = a.res ? static_cast<const TX*>(a.res) + b * a.sres + c0 : nullptr;
+#pragma unroll
+    for (int i = 0; i < NU; ++i) {
+        if (!in(i)) continue;
+        const uint64_t r = row0 + i * rows_at;
+        VT o, q;
+#pragma unroll
+        for (int e = 0; e < VE; ++e) q[e] = static_cast<TX>(0.0f);
+        if (res) q = *reinterpret_cast<const VT*>(res + r * a.ldres);
+#pragma unroll
+        for (int e = 0; e < VE; ++e) {
+            const float xh = xhat(i, e), w = static_cast<float>(d[i][e]) * slope<ACT>(__builtin_fmaf(xh, gamma[e], beta[e]));
+            const float t = st.inv * __builtin_fmaf(-xh, m2, __builtin_fmaf(w, gamma[e], -m1));
+            o[e] = static_cast<TX>(res ? t + static_cast<float>(q[e]) : t);
+        }
+        *reinterpret_cast<VT*>(dx + r * a.lddx) = o;
     }
 }
 
@@ -1117,12 +1252,14 @@ void launch_apply_i8(const GnArgs& a, hipStream_t s) {
 template <typename TX, typename TY, int ACT, int VE>
 bool launch_slab(const GnArgs& a, hipStream_t s) {
     const uint64_t units = static_cast<uint64_t>(a.pixels) * a.cg / VE;
-    if (a.cg % VE != 0 || a.cg > kSlabChannels || units > 16 * kSlabThreads || !fast_rows(a.x, a.ldx, a.sx, VE, sizeof(TX)) ||
+    if (a.cg % VE != 0 || a.cg > kSlabChannels || units > 32 * kSlabThreads || units * VE * sizeof(TX) > kSlabBytes * kSlabThreads || !fast_rows(a.x, a.ldx, a.sx, VE, sizeof(TX)) ||
         !fast_rows(a.y, a.ldy, a.sy, VE, sizeof(TY)))
         return false;
     const unsigned grid = a.batch * a.groups;
+    constexpr int kMost = kSlabBytes / (VE * sizeof(TX));
     if (units <= 8 * kSlabThreads) gn_slab_kernel<TX, TY, ACT, VE, 8><<<grid, kSlabThreads, 0, s>>>(a);
-    else gn_slab_kernel<TX, TY, ACT, VE, 16><<<grid, kSlabThreads, 0, s>>>(a);
+    else if (units <= 16 * kSlabThreads) gn_slab_kernel<TX, TY, ACT, VE, 16><<<grid, kSlabThreads, 0, s>>>(a);
+    else if constexpr (kMost > 16) gn_slab_kernel<TX, TY, ACT, VE, 32><<<grid, kSlabThreads, 0, s>>>(a);
     return true;
 }
 
@@ -1157,10 +1294,29 @@ void launch_forward(const GnArgs& a, int y_dtype, int act, hipStream_t s) {
     else launch_forward<TX, int8_t>(a, act, s);
 }
 
+// Launches gn_bwd_slab_kernel for units of VE values where a group fits and its rows allow them.
+template <typename TX, typename TD, int ACT, int VE>
+bool launch_bwd_slab(const GnBwdArgs& a, bool stats, hipStream_t s) {
+    const GnArgs& f = a.f;
+    if (f.cg % VE != 0 || f.cg / VE > kSlabThreads) return false;
+    const uint32_t rows_at = kSlabThreads / (f.cg / VE);
+    const uint64_t units = (static_cast<uint64_t>(f.pixels) + rows_at - 1) / rows_at;  // a thread's
+    if (units > kBwdSlabUnits || !fast_rows(f.x, f.ldx, f.sx, VE, sizeof(TX)) || !fast_rows(a.dy, a.lddy, a.sdy, VE, sizeof(TD)) ||
+        !fast_rows(a.dx, a.lddx, a.sdx, VE, sizeof(TX)) || !fast_rows(a.res, a.ldres, a.sres, VE, sizeof(TX)))
+        return false;
+    const unsigned grid = f.batch * f.groups;
+    gn_bwd_slab_kernel<TX, TD, ACT, VE, kBwdSlabUnits><<<grid, kSlabThreads, 0, s>>>(a, stats);
+    if (a.dgamma && f.batch > 1) gn_bwd_params_kernel<<<grid_of(ceil_div(f.C, 64)), 256, 0, s>>>(a.cpart, a.dgamma, a.dbeta, f.batch, f.C);
+    return true;
+}
+
 template <typename TX, typename TD, int ACT>
 void launch_backward(GnBwdArgs a, bool stats, hipStream_t s) {
     GnArgs& f = a.f;
     constexpr uint32_t E = Vec<TX>::E;
+    if (static_cast<uint64_t>(f.batch) * f.groups <= kSlabGroups &&
+        (launch_bwd_slab<TX, TD, ACT, 4>(a, stats, s) || launch_bwd_slab<TX, TD, ACT, 2>(a, stats, s)))
+        return;
     const bool fx = fast_x<TX>(f);
     const bool fast = fx && fast_rows(a.dy, a.lddy, a.sdy, E, sizeof(TD)) && fast_rows(a.dx, a.lddx, a.sdx, E, sizeof(TX)) &&
                       fast_rows(a.res, a.ldres, a.sres, E, sizeof(TX));

@@ -380,7 +380,7 @@ CASES = {
         dict(P=301, C=320, G=32, typ="f16", out="i8"), dict(P=700, C=256, G=256, out="i8", keep=False), dict(P=600, C=37, G=1, outlier=500.0), dict(P=40, C=512, G=512), dict(P=3, C=4096, G=256, typ="f16", out="f16"),
         # a group in a workgroup's registers, at its border and past it; units of two values
         dict(P=256, C=256, G=2, act=1), dict(P=257, C=128, G=1), dict(P=128, C=256, G=1, typ="f16", out="f32"), dict(B=2, P=819, C=20, G=2, typ="f16", out="f16", act=1), dict(P=1639, C=20, G=2),
-        dict(P=16, C=2048, G=2), dict(P=15, C=2052, G=2, act=1), dict(P=100, C=60, G=10, offset=-1000.0, gap=2, ygap=4), dict(P=90, C=64, G=4, off=2, yoff=2, typ="f16", out="f16"),
+        dict(P=512, C=64, G=1, act=1), dict(P=513, C=64, G=1), dict(P=1024, C=64, G=1, typ="f16", out="f16", act=1), dict(P=1025, C=64, G=1, typ="f16", out="f16"), dict(P=1300, C=50, G=2, typ="f16", out="f32", offset=200.0), dict(P=16, C=2048, G=2), dict(P=15, C=2052, G=2, act=1), dict(P=100, C=60, G=10, offset=-1000.0, gap=2, ygap=4), dict(P=90, C=64, G=4, off=2, yoff=2, typ="f16", out="f16"),
         # 8-bit rows
         dict(P=1, C=1, G=1, out="i8"), dict(P=20, C=320, G=32, out="i8"), dict(B=2, P=33, C=640, G=32, typ="f16", out="i8"), dict(P=18, C=1280, G=32, typ="f16", out="i8", act=1),
         dict(P=11, C=37, G=1, out="i8", act=1), dict(B=2, P=19, C=64, G=8, ygap=16, gap=4, out="i8"), dict(B=3, P=9, C=64, G=8, order="rows", out="i8", ygap=1),
@@ -395,6 +395,9 @@ CASES = {
         dict(P=30, C=64, G=8, in_place=True), dict(P=31, C=33, G=3, in_place=True, typ="f16", dtyp="f16", act=1), dict(P=200, C=64, G=8, offset=1000.0), dict(P=200, C=64, G=8, offset=300.0, act=1, kept=True),
         dict(P=50, C=32, G=4, gstd=1e-20), dict(P=50, C=32, G=4, gstd=1e10, act=1), dict(B=40, P=3, C=16, G=4, act=1, res=True), dict(P=5, C=2600, G=1, act=1),
         dict(P=300, C=320, G=32, act=1, res=True), dict(B=2, P=301, C=64, G=8, typ="f16", dtyp="f16", offset=30.0, kept=True), dict(P=700, C=256, G=256, typ="f16", dtyp="f32", act=1), dict(P=300, C=320, G=32, doff=1),
+        dict(P=408, C=40, G=1, act=1, res=True), dict(P=409, C=40, G=1, act=1), dict(P=408, C=80, G=2, typ="f16", dtyp="f16", act=1, kept=True), dict(P=409, C=80, G=2, typ="f16", dtyp="f32"), dict(B=3, P=816, C=10, G=1),
+        dict(B=2, P=300, C=20, G=2, typ="f16", dtyp="f16", act=1, res=True, gap=2, dgap=2), dict(B=2, P=2, C=2048, G=1, act=1), dict(P=2, C=2052, G=1), dict(P=16, C=2048, G=2, weights=False, kept=True),
+        dict(P=400, C=40, G=1, offset=1000.0), dict(B=2, P=520, C=64, G=2, act=1, in_place=True), dict(P=8, C=4096, G=2, typ="f16", dtyp="f32", act=1),
         dict(P=600, C=37, G=1, act=1), dict(P=40, C=512, G=512), dict(P=3, C=4096, G=256, typ="f16", dtyp="f16", weights=False),
     ],
     "quantize": [
