@@ -12,6 +12,7 @@ from pathlib import Path
 HERE = Path(__file__).resolve().parent
 sys.path[:0] = [str(HERE.parent.parent), str(HERE.parent), str(HERE)]
 
+import norm_i8_chain  # noqa: E402
 import norm_i8_ref  # noqa: E402
 from bwd_cases import Backend  # noqa: E402
 
@@ -24,7 +25,7 @@ def main(argv):
     _lib.load = lambda: be.E.lib  # sdvk_amd.ops on the emulated library
     for o in orders:
         be.E.order(o, bool(o))
-        norm_i8_ref.OPS[op](be, **spec)
+        {**norm_i8_ref.OPS, **norm_i8_chain.OPS}[op](be, **spec)
         print(f"OK order {o}", flush=True)
 
 

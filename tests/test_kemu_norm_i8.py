@@ -12,6 +12,7 @@ from pathlib import Path
 
 import pytest
 
+import norm_i8_chain
 import norm_i8_ref
 
 KEMU = Path(__file__).resolve().parent / "kemu"
@@ -43,3 +44,8 @@ def check(specs):
 @pytest.mark.parametrize("op", list(norm_i8_ref.CASES))
 def test_kernels_on_emulator(emulator, op):
     check([dict(op=op, orders=ORDERS, **c) for c in norm_i8_ref.CASES[op]])
+
+
+def test_chain_on_emulator(emulator):
+    """The operators run together, around each other and the existing ones."""
+    check([dict(op=op, orders=ORDERS) for op in norm_i8_chain.OPS])
