@@ -86,6 +86,8 @@ int mi_version(void);
  *   "gemm_bwd_cfg"      "<build 0..3>[:<N parts>]" (input-gradient GEMM tile
  *                       build; 3 is fp32 only and runs as 0 for fp16; the
  *                       parts apply to calls with a workspace)
+ *   "gemm_i8_cfg"       "<build 0..8>" (8-bit product's build; one that cannot
+ *                       serve a call leaves it to the rules)
  * MI_ERR_INVALID_ARG for an unknown name or a malformed value. Not
  * synchronised with calls in flight on other threads.                      */
 int mi_tuning_set(const char* name, const char* value);
@@ -639,7 +641,8 @@ int mi_groupnorm_bwd(const mi_groupnorm_bwd_args* args, void* workspace, uint64_
  * 127). A row with an infinity or a NaN gets the scale NaN and codes 0. x MI_F32 or MI_F16
  * (dtype); row strides ldx, ldq in elements (0 -> cols). For weights, one scale a channel:
  * mi_q8_0_dequant, then this. Tensors aligned to their element; cols % 16 == 0 with 16-byte
- * aligned rows and cols <= 8192 is the fast path. q and scale overlap nothing.               */
+ * aligned rows and cols <= 8192 is the fast path. rows <= 2^31, cols <= 2^30. q and scale
+ * overlap nothing.                                                                  */
 int mi_quantize_rows_i8(const void* x, int dtype, int8_t* q, float* scale, uint32_t rows, uint32_t cols, uint32_t ldx,
                         uint32_t ldq, void* stream);
 
@@ -649,8 +652,8 @@ int mi_quantize_rows_i8(const void* x, int dtype, int8_t* q, float* scale, uint3
  * fma(float(sum) a_scale, w_scale, bias), so a call's bits do not depend on the sizes around it.
  * C MI_F32 or MI_F16 (c_dtype, rounded once); mode 0 stores, 1 adds without the bias, 2 adds
  * with it (the residual). Row strides lda, ldw (0 -> K) and ldc (0 -> N). bias fp32 or NULL.
- * Fast: K % 16 == 0, A and W 16-byte aligned with strides of 16, A's and W's rows within
- * 4 GiB. C overlaps no input.                                                       */
+ * Fast: K % 16 == 0, A and W 16-byte aligned, their strides multiples of 16 and at most 2^22.
+ * M, N <= 2^31. C overlaps no input. K == 0 is unsupported.                          */
 int mi_gemm_nt_i8(const int8_t* A, const float* a_scale, const int8_t* W, const float* w_scale, const float* bias, void* C,
                   int c_dtype, uint32_t M, uint32_t N, uint32_t K, uint32_t mode, uint32_t lda, uint32_t ldw, uint32_t ldc,
                   void* stream);

@@ -15,6 +15,8 @@ namespace {
 
 constexpr uint32_t kMaxGrid = 1u << 20;  // workgroups of a launch that strides over its units
 constexpr uint32_t kMaxFastCols = 8192;  // columns of a row that a wave holds
+constexpr uint32_t kMaxSize = 1u << 31;  // rows and columns of a product, rows of the quantiser ...
+constexpr uint32_t kMaxCols = 1u << 30;  // ... and its columns: counted in 32 bits with a tile or a wave past the end
 constexpr uint32_t kMaxK = 131071;       // 2^31 / 2^14
 constexpr uint64_t kMaxLd = 1u << 22;    // row strides that 256 rows address in 31 bits
 
@@ -77,10 +79,10 @@ __device__ __forceinline__ void store_run(const I8Args& a, uint32_t m, uint32_t 
 // Any K, any alignment: a 64 x 64 tile in steps of 32 codes, 4 x 4 outputs a thread.
 template <typename TC>
 __global__ __launch_bounds__(256) void gemm_i8_any_kernel(I8Args a) {
-    __shared__ int8_t at[64][36], wt[64][36];
+    __shared__ __attribute__((aligned(4))) int8_t at[64][36], wt[64][36];
     const uint32_t tid = threadIdx.x, tx = tid & 15, ty = tid >> 4;
     const uint32_t tiles_n = (a.N + 63) / 64;
-    const uint64_t tiles = static_cast<uint64_t>((a.M + 63) / 64) * tiles_n;
+    const uint64_t tiles = static_cast<uint64_t>((a.M + 63) / 64) * tiles_n;  // (M, N <= 2^31)
     for (uint64_t t = blockIdx.x; t < tiles; t += gridDim.x) {
         const uint32_t m0 = static_cast<uint32_t>(t / tiles_n) * 64, n0 = static_cast<uint32_t>(t % tiles_n) * 64;
         int acc[4][4] = {};
@@ -92,17 +94,17 @@ __global__ __launch_bounds__(256) void gemm_i8_any_kernel(I8Args a) {
                 wt[r][k] = in && n0 + r < a.N ? a.W[(n0 + r) * a.ldw + k0 + k] : static_cast<int8_t>(0);
             }
             __syncthreads();
-            for (int k = 0; k < 32; ++k) {
+            for (int k = 0; k < 32; k += 4) {
                 int x[4], w[4];
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    x[i] = at[ty + 16 * i][k];
-                    w[i] = wt[tx + 16 * i][k];
+                    x[i] = *reinterpret_cast<const int*>(&at[ty + 16 * i][k]);
+                    w[i] = *reinterpret_cast<const int*>(&wt[tx + 16 * i][k]);
                 }
 #pragma unroll
                 for (int i = 0; i < 4; ++i)
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) acc[i][j] += x[i] * w[j];
+                    for (int j = 0; j < 4; ++j) acc[i][j] = __builtin_amdgcn_sdot4(x[i], w[j], acc[i][j], false);
             }
             __syncthreads();
         }
@@ -592,19 +594,23 @@ int choose(const I8Args& a) {
     const bool vec = a.K % 16 == 0 && a.lda % 16 == 0 && a.ldw % 16 == 0 && aligned(a.A, 16) && aligned(a.W, 16) &&
                      a.lda <= kMaxLd && a.ldw <= kMaxLd;
     if (!vec) return kAny;
+    // (a launch has fewer than 2^32 threads)
+    auto tiles = [&](int b) { return static_cast<uint64_t>(ceil_div(a.M, kBuilds[b].bm)) * ceil_div(a.N, kBuilds[b].bn); };
+    auto fits = [&](int b) { return tiles(b) < (1u << 23) && (b != kFew || a.M <= kFewRows); };
     const int cfg = tuning().gemm_i8_cfg.load();
-    if (cfg >= 0 && (cfg != kFew || a.M <= kFewRows)) return cfg;
-    if (a.M <= kFewRows) return kFew;
+    if (cfg >= 0 && fits(cfg)) return cfg;
+    if (fits(kFew)) return kFew;
     if (static_cast<uint64_t>(ceil_div(a.M, 64)) * ceil_div(a.N, 64) <= 128) return kSplitK;
-    int best = k64;
+    int best = kAny;
     float least = 0.0f;
     for (int b = k64; b <= k64x3; ++b) {
-        const uint64_t n = (static_cast<uint64_t>(ceil_div(a.M, kBuilds[b].bm)) * ceil_div(a.N, kBuilds[b].bn) + 255) / 256;
+        if (!fits(b)) continue;
+        const uint64_t n = (tiles(b) + 255) / 256;
         if (b == k64x3 && n > 2) continue;  // three workgroups a CU; with more tiles four are faster
         if (b == k128 && n < 2) continue;   // two workgroups a CU hide each other's latency; one needs four stages
         const float step = b == k64 && n == 3 ? 0.183f : kBuilds[b].step_us;
         const float us = static_cast<float>(n) * (kBuilds[b].tile_us + ceil_div(a.K, 128) * step);
-        if (b == k64 || us < least) {
+        if (best == kAny || us < least) {
             best = b;
             least = us;
         }
@@ -661,6 +667,7 @@ extern "C" int mi_quantize_rows_i8(const void* x, int dtype, int8_t* q, float* s
     const char* fn = "mi_quantize_rows_i8";
     if (dtype != MI_F32 && dtype != MI_F16) return fail(MI_ERR_INVALID_ARG, "%s: dtype %d", fn, dtype);
     if (rows == 0 || cols == 0) return MI_OK;
+    if (rows > kMaxSize || cols > kMaxCols) return fail(MI_ERR_UNSUPPORTED, "%s: rows %u > 2^31 or columns %u > 2^30", fn, rows, cols);
     if (!x || !q || !scale) return fail(MI_ERR_INVALID_ARG, "%s: null pointer", fn);
     const uint64_t lx = ldx ? ldx : cols, lq = ldq ? ldq : cols, e = dtype == MI_F16 ? 2 : 4;
     if (lx < cols || lq < cols) return fail(MI_ERR_INVALID_ARG, "%s: a row stride below %u columns", fn, cols);
@@ -681,6 +688,7 @@ extern "C" int mi_gemm_nt_i8(const int8_t* A, const float* a_scale, const int8_t
     if (c_dtype != MI_F32 && c_dtype != MI_F16) return fail(MI_ERR_INVALID_ARG, "%s: c_dtype %d", fn, c_dtype);
     if (mode > 2) return fail(MI_ERR_INVALID_ARG, "%s: mode %u", fn, mode);
     if (M == 0 || N == 0) return MI_OK;
+    if (M > kMaxSize || N > kMaxSize) return fail(MI_ERR_UNSUPPORTED, "%s: M %u or N %u > 2^31", fn, M, N);
     if (K == 0 || K > kMaxK) return fail(MI_ERR_UNSUPPORTED, "%s: K %u (1 .. %u: the sum is held in 32 bits)", fn, K, kMaxK);
     if (!A || !a_scale || !W || !w_scale || !C) return fail(MI_ERR_INVALID_ARG, "%s: null pointer", fn);
     I8Args a{A, W, a_scale, w_scale, mode == 1 ? nullptr : bias, C, M, N, K, mode, lda ? lda : K, ldw ? ldw : K, ldc ? ldc : N, 0, 0, 0, 0};

@@ -346,6 +346,11 @@ struct Vec {
     static constexpr int E = 16 / static_cast<int>(sizeof(T));
     typedef T type __attribute__((ext_vector_type(E)));
 };
+// E neighbouring values of T, 16-byte aligned at most (eight floats are two vectors).
+template <typename T, int E>
+struct Run {
+    typedef T type __attribute__((ext_vector_type(E), aligned(E * sizeof(T) > 16 ? 16 : E * sizeof(T))));
+};
 
 // A group's lanes: the largest power of two (at most 64) of threads that T threads have for each of G groups at once.
 __device__ __forceinline__ uint32_t lanes_of(uint32_t T, uint32_t G) {
@@ -502,7 +507,7 @@ template <typename TX, typename TY, int ACT>
 __global__ __launch_bounds__(4096 / Vec<TX>::E) void gn_apply_kernel(GnArgs a) {
     constexpr int E = Vec<TX>::E;
     typedef typename Vec<TX>::type VT;
-    typedef TY YT __attribute__((ext_vector_type(E)));
+    typedef typename Run<TY, E>::type YT;
     extern __shared__ __attribute__((aligned(16))) Stat st[];
     const uint32_t T = blockDim.x, tid = threadIdx.x, V = a.C / E, rows_at = T / V;
     const uint32_t ty = tid / V, tx = tid % V;
@@ -602,7 +607,7 @@ template <typename TX, typename TD, int ACT>
 __global__ __launch_bounds__(4096 / Vec<TX>::E) void gn_bwd_cols_kernel(GnBwdArgs a) {
     constexpr int E = Vec<TX>::E;
     typedef typename Vec<TX>::type VT;
-    typedef TD DT __attribute__((ext_vector_type(E)));
+    typedef typename Run<TD, E>::type DT;
     extern __shared__ __attribute__((aligned(16))) Stat st[];
     const GnArgs& f = a.f;
     float* const red = reinterpret_cast<float*>(st + f.groups);
@@ -702,7 +707,7 @@ template <typename TX, typename TD, int ACT>
 __global__ __launch_bounds__(4096 / Vec<TX>::E) void gn_bwd_apply_kernel(GnBwdArgs a) {
     constexpr int E = Vec<TX>::E;
     typedef typename Vec<TX>::type VT;
-    typedef TD DT __attribute__((ext_vector_type(E)));
+    typedef typename Run<TD, E>::type DT;
     extern __shared__ __attribute__((aligned(16))) Stat st[];
     const GnArgs& f = a.f;
     const uint32_t T = blockDim.x, tid = threadIdx.x;

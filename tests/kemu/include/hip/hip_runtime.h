@@ -510,6 +510,13 @@ inline float fdot2(kemu_h2 a, kemu_h2 b, float c, bool clamp) {
     return static_cast<float>(r);
 }
 
+// v_dot4_i32_i8: c + the sum of four products of signed bytes.
+inline int sdot4(int a, int b, int c, bool clamp) {
+    if (clamp) die("sdot4: clamp not emulated");
+    for (int i = 0; i < 4; ++i) c += static_cast<int8_t>(a >> (8 * i)) * static_cast<int8_t>(b >> (8 * i));
+    return c;
+}
+
 inline void nop_fn(const unsigned char (*)[256], unsigned char (*)[256], const void*) {}
 inline void wave_barrier() { wave_op("wave_barrier", nullptr, 0, nullptr, 0, nop_fn, nullptr); }
 
@@ -554,6 +561,7 @@ inline T __shfl_xor(T v, int mask, int width = 64) {
 #define __builtin_amdgcn_rcpf(x) (1.0f / (x))
 #define __builtin_amdgcn_ds_read_tr16_b64_v4f16 ::kemu::ds_read_tr16_b64
 #define __builtin_amdgcn_permlane32_swap ::kemu::permlane32_swap
+#define __builtin_amdgcn_sdot4 ::kemu::sdot4
 #define __builtin_amdgcn_fdot2 ::kemu::fdot2
 #define __builtin_amdgcn_raw_ptr_buffer_load_lds ::kemu::buffer_load_lds
 #define __builtin_amdgcn_sched_barrier(...) ((void)0)

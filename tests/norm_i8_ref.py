@@ -358,13 +358,53 @@ def product(be, *, M, N, K, out="f32", mode=0, bias=True, lda=0, ldw=0, ldc=0, o
         assert np.array_equal(be.get(bc, dt, nc).view(np.uint8), flat.view(np.uint8)), "a second call gave other bits"
 
 
-OPS = {"groupnorm": groupnorm, "groupnorm_bwd": groupnorm_bwd, "quantize": quantize, "product": product}
+def broken(be, *, B=2, P, C, G, typ="f32", out="f32", act=1, value="nan", seed=6):
+    """A NaN or an infinity in one group of one image leaves NaN in that group, forward and backward (in an 8-bit row's scale), and every
+    other group as it is without it."""
+    rng = rng_of(seed)
+    x = pixels_of(rng, B, P, C, 0.2, 0.0).astype(DT[typ])
+    dy = rng.standard_normal((B, P, C)).astype(DT[typ])
+    gamma, beta = affine_of(rng, C, "both")
+    odt = {"f32": np.float32, "f16": np.float16, "i8": np.int8}[out]
+    cg, g, im = C // G, G // 2, B - 1
+    hit = np.zeros((B, P, C), bool)
+    hit[im, :, g * cg:(g + 1) * cg] = True
+    got = []
+    for bad in (False, True):
+        xx = x.copy()
+        if bad:
+            xx[im, P // 2, g * cg] = float(value)
+        bx, bg, bb, bd = (be.buf(np.ascontiguousarray(t).reshape(-1)) for t in (xx, gamma, beta, dy))
+        by, bs = be.buf(np.zeros(B * P * C, odt)), be.buf(np.zeros(B * P, np.float32))
+        bo, bdg, bdb = be.buf(np.zeros(B * P * C, DT[typ])), be.buf(np.zeros(C, np.float32)), be.buf(np.zeros(C, np.float32))
+        need = be.value("mi_groupnorm_bwd_ws_bytes", B, P, C, G)
+        ws = be.buf(np.full(need, 0xff, np.uint8))
+        a = MiGroupnormArgs(bx.ptr, bg.ptr, bb.ptr, by.ptr, bs.ptr if out == "i8" else None, None, B, P, C, G, CODE[typ], {"f32": 0, "f16": 1, "i8": I8}[out], act, 1e-5, 0, 0, 0, 0)
+        be.call("mi_groupnorm", ctypes.byref(a), ws.ptr, need, None)
+        a.y_dtype = CODE[typ]
+        q = MiGroupnormBwdArgs(a, bd.ptr, None, bo.ptr, bdg.ptr, bdb.ptr, 0, 0, 0, 0, 0, 0)
+        be.call("mi_groupnorm_bwd", ctypes.byref(q), ws.ptr, need, None)
+        got.append([f64(be.get(by, odt, B * P * C)).reshape(B, P, C), be.get(bs, np.float32, B * P).reshape(B, P), f64(be.get(bo, DT[typ], B * P * C)).reshape(B, P, C),
+                    be.get(bdg, np.float32, C), be.get(bdb, np.float32, C)])
+    (y0, s0, d0, g0, b0), (y1, s1, d1, g1, b1) = got
+    assert np.array_equal(d1[~hit], d0[~hit]) and np.all(np.isnan(d1[hit]))
+    cols = hit[im, 0]
+    assert np.array_equal(g1[~cols], g0[~cols]) and np.all(np.isnan(g1[cols])) and np.array_equal(b1[~cols], b0[~cols])
+    if out == "i8":
+        assert np.array_equal(y1[:im], y0[:im]) and np.array_equal(s1[:im], s0[:im]) and np.all(np.isnan(s1[im])) and np.all(y1[im] == 0)
+    else:
+        assert np.array_equal(y1[~hit], y0[~hit]) and np.all(np.isnan(y1[hit]))
+
+
+OPS = {"broken": broken, "groupnorm": groupnorm, "groupnorm_bwd": groupnorm_bwd, "quantize": quantize, "product": product}
 
 # Small shapes where the operators can go wrong, on the emulator and on the GPU.
 CASES = {
+    "broken": [dict(P=p, C=c, G=g, out=o, value=v, act=a) for p, c, g in ((20, 64, 8), (300, 128, 8), (40, 33, 3), (7, 1024, 512)) for o in ("f32", "i8") for v, a in (("nan", 1), ("inf", 0))]
+    + [dict(P=600, C=64, G=2, typ="f16", out="f16", value="-inf")],
     "groupnorm": [
         dict(P=1, C=1, G=1), dict(P=1, C=4, G=4), dict(P=1, C=320, G=32, typ="f16", out="f16", act=1), dict(P=7, C=6, G=2), dict(P=300, C=3, G=1, act=1),
-        dict(P=40, C=64, G=8, typ="f16", out="f16", act=1), dict(B=2, P=37, C=320, G=32, act=1), dict(B=3, P=70, C=40, G=4, typ="f16", out="f32"),
+        dict(P=40, C=64, G=8, typ="f16", out="f16", act=1), dict(B=2, P=37, C=320, G=32, act=1), dict(B=3, P=70, C=40, G=4, typ="f16", out="f32"), dict(P=300, C=320, G=32, typ="f16", out="f32", yoff=4), dict(P=1100, C=64, G=2, typ="f16", out="f32", yoff=4, act=1),
         dict(B=2, P=33, C=96, G=32, typ="f32", out="f16", act=1), dict(P=20, C=640, G=32, typ="f16", out="f16"), dict(P=17, C=1000, G=2), dict(P=5, C=2600, G=1),
         dict(P=9, C=1280, G=32, affine="none"), dict(P=9, C=64, G=32, affine="gamma", act=1), dict(P=9, C=64, G=1, affine="beta"),
         # strides, alignment, the images' rows in turn
@@ -394,7 +434,7 @@ CASES = {
         dict(B=2, P=19, C=64, G=8, gap=3, dgap=1, act=1, res=True), dict(B=3, P=11, C=64, G=8, order="rows", act=1, kept=True), dict(P=30, C=64, G=8, off=1), dict(P=30, C=64, G=8, doff=1, act=1),
         dict(P=30, C=64, G=8, in_place=True), dict(P=31, C=33, G=3, in_place=True, typ="f16", dtyp="f16", act=1), dict(P=200, C=64, G=8, offset=1000.0), dict(P=200, C=64, G=8, offset=300.0, act=1, kept=True),
         dict(P=50, C=32, G=4, gstd=1e-20), dict(P=50, C=32, G=4, gstd=1e10, act=1), dict(B=40, P=3, C=16, G=4, act=1, res=True), dict(P=5, C=2600, G=1, act=1),
-        dict(P=300, C=320, G=32, act=1, res=True), dict(B=2, P=301, C=64, G=8, typ="f16", dtyp="f16", offset=30.0, kept=True), dict(P=700, C=256, G=256, typ="f16", dtyp="f32", act=1), dict(P=300, C=320, G=32, doff=1),
+        dict(P=300, C=320, G=32, act=1, res=True), dict(B=2, P=301, C=64, G=8, typ="f16", dtyp="f16", offset=30.0, kept=True), dict(P=700, C=256, G=256, typ="f16", dtyp="f32", act=1), dict(P=300, C=320, G=32, doff=1), dict(P=1100, C=64, G=2, typ="f16", dtyp="f32", off=8, doff=8, act=1), dict(P=1100, C=64, G=2, typ="f16", dtyp="f32", doff=4),
         dict(P=408, C=40, G=1, act=1, res=True), dict(P=409, C=40, G=1, act=1), dict(P=408, C=80, G=2, typ="f16", dtyp="f16", act=1, kept=True), dict(P=409, C=80, G=2, typ="f16", dtyp="f32"), dict(B=3, P=816, C=10, G=1),
         dict(B=2, P=300, C=20, G=2, typ="f16", dtyp="f16", act=1, res=True, gap=2, dgap=2), dict(B=2, P=2, C=2048, G=1, act=1), dict(P=2, C=2052, G=1), dict(P=16, C=2048, G=2, weights=False, kept=True),
         dict(P=400, C=40, G=1, offset=1000.0), dict(B=2, P=520, C=64, G=2, act=1, in_place=True), dict(P=8, C=4096, G=2, typ="f16", dtyp="f32", act=1),

@@ -89,6 +89,8 @@ def test_quantize(lib):
     assert call(rows=0, x=None) == _lib.MI_OK and call(cols=0, q=None) == _lib.MI_OK
     for bad in (dict(x=None), dict(q=None), dict(scale=None), dict(dtype=2), dict(dtype=-1), dict(ldx=63), dict(ldq=63)):
         assert call(**bad) == INVALID, bad
+    for bad in (dict(rows=(1 << 31) + 1, cols=1), dict(rows=1, cols=(1 << 30) + 1)):
+        assert call(**bad) == UNSUPPORTED, bad
     for bad in (dict(x=addr(0) + 2), dict(x=addr(0) + 1, dtype=1), dict(scale=addr(2) + 2)):
         assert call(**bad) == ALIGN, bad
     for bad in (dict(q=addr(0)), dict(q=addr(0) + 5 * 64 * 4 - 1), dict(scale=addr(0) + 4), dict(scale=addr(1) + 4)):
@@ -102,9 +104,17 @@ def test_product(lib):
     assert call(M=0, A=None) == _lib.MI_OK and call(N=0, K=0) == _lib.MI_OK
     for bad in (dict(A=None), dict(sa=None), dict(W=None), dict(sw=None), dict(C=None), dict(dt=2), dict(mode=3), dict(lda=63), dict(ldw=63), dict(ldc=7)):
         assert call(**bad) == INVALID, bad
-    for bad in (dict(K=0), dict(K=131072)):
+    for bad in (dict(K=0), dict(K=131072), dict(M=(1 << 31) + 1), dict(N=(1 << 31) + 1)):
         assert call(**bad) == UNSUPPORTED, bad
     for bad in (dict(sa=addr(1) + 2), dict(sw=addr(3) + 1), dict(bias=addr(4) + 2), dict(C=addr(5) + 2), dict(C=addr(5) + 1, dt=1)):
         assert call(**bad) == ALIGN, bad
     for bad in (dict(C=addr(0)), dict(C=addr(1)), dict(C=addr(2) + 64), dict(C=addr(3)), dict(C=addr(4) + 28)):
         assert call(**bad) == ALIAS, bad
+
+
+def test_plan_override(lib):
+    assert lib.mi_tuning_set(b"gemm_i8_cfg", b"8") == _lib.MI_OK
+    for bad in (b"9", b"-1", b"x", b"1:2"):
+        assert lib.mi_tuning_set(b"gemm_i8_cfg", bad) == INVALID, bad
+    assert lib.mi_tuning_set(b"gemm_i8_cfg", None) == _lib.MI_OK
+    lib.mi_tuning_reset()
