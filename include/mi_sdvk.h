@@ -593,8 +593,8 @@ int mi_layernorm_bwd(const float* x, const float* gamma, const void* dy, int dy_
  * Means and variances keep their accuracy whatever the mean's size (values below 1e18 in
  * magnitude: squares are summed in fp32). groups divides channels; batch and channels <=
  * 2^20, batch * pixels <= 2^31. Tensors aligned to their element. Fast: channels and strides
- * multiples of 16 bytes (MI_I8: of 16 codes), 16-byte aligned tensors, channels <= 4096. y, y_scale,
- * stats and workspace overlap no input and not each other. workspace:
+ * multiples of x's 16-byte vectors (8 fp16 or 4 fp32 values), 16-byte aligned tensors (MI_I8
+ * rows: of 4 bytes), channels <= 4096, groups <= 256. y, y_scale, stats and workspace overlap no input and not each other. workspace:
  * mi_groupnorm_ws_bytes(...) bytes, 16-byte aligned. batch or pixels 0: nothing is written. */
 enum { MI_ACT_NONE = 0, MI_ACT_SILU = 1 };
 

@@ -18,7 +18,7 @@ constexpr uint32_t kMaxFastCols = 8192;  // columns of a row that a wave holds
 constexpr uint32_t kMaxSize = 1u << 31;  // rows and columns of a product, rows of the quantiser ...
 constexpr uint32_t kMaxCols = 1u << 30;  // ... and its columns: counted in 32 bits with a tile or a wave past the end
 constexpr uint32_t kMaxK = 131071;       // 2^31 / 2^14
-constexpr uint64_t kMaxLd = 1u << 22;    // row strides that 256 rows address in 31 bits
+constexpr uint64_t kMaxLd = 1u << 22;    // row strides that a tile's 320 rows address in 31 bits
 
 struct I8Args {
     const int8_t *A, *W;
@@ -134,12 +134,16 @@ typedef int intx4 __attribute__((ext_vector_type(4)));
 typedef int intx16 __attribute__((ext_vector_type(16)));
 
 __device__ __forceinline__ uint32_t swz(uint32_t row) { return (row >> 1) & 7u; }
-__device__ __forceinline__ void wait_lds() { __builtin_amdgcn_s_waitcnt(0xC07F); }    // lgkmcnt(0)
+__device__ __forceinline__ void wait_lds() {  // lgkmcnt(0)
+    __builtin_amdgcn_s_waitcnt(0xC07F);
+    __atomic_signal_fence(__ATOMIC_SEQ_CST);  // no access that follows moves before the wait
+}
 // Waits until at most N of the wave's loads are on their way.
 template <int N>
 __device__ __forceinline__ void wait_loads() {
     static_assert(N < 64, "vmcnt has six bits");
     __builtin_amdgcn_s_waitcnt(0x0F70 | (N & 15) | ((N >> 4) << 14));
+    __atomic_signal_fence(__ATOMIC_SEQ_CST);
 }
 // A barrier that waits for nothing else: __syncthreads() would wait for every load on its way. A wave has the fragments of the step
 // before when it gets here (its products have taken them).
