@@ -157,9 +157,9 @@ __device__ __forceinline__ void barrier() {
 }
 
 // 16 bytes a lane from `off` of the `bytes` at base (zeros past them) to LDS: lane l's to dst + 16 l.
-__device__ __forceinline__ void load_lds(const int8_t* base, int bytes, int8_t* dst, uint32_t off) {
+__device__ __forceinline__ void load_lds(const int8_t* base, int bytes, int8_t* dst, uint32_t off, int at = 0) {
     const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(const_cast<int8_t*>(base), 0, bytes, 0x00020000);
-    __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (__attribute__((address_space(3))) void*)(dst), 16, off, 0, 0, 0);
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (__attribute__((address_space(3))) void*)(dst), 16, off, at, 0, 0);
 }
 
 // Rows of one operand: IT load instructions a wave brings into LDS (rows 8 (IT wave + i) .. + 7).
@@ -179,9 +179,14 @@ struct Rows {
 #pragma unroll
         for (int i = 0; i < IT; ++i) off[i] = (8 * (wave * IT + i) + (lane >> 3)) * static_cast<uint32_t>(ld) + col[i & 1];
     }
-    __device__ __forceinline__ void load(int8_t* stage, uint32_t k0) const {
+    // (steps in turn: a lane whose codes are past K once stays there)
+    __device__ __forceinline__ void load(int8_t* stage, uint32_t k0) {
+        if (k0 + 128 > K) {
 #pragma unroll
-        for (int i = 0; i < IT; ++i) load_lds(base, bytes, stage + at + i * 1024, k0 + col[i & 1] < K ? off[i] + k0 : kPast);
+            for (int i = 0; i < IT; ++i) off[i] = k0 + col[i & 1] < K ? off[i] : kPast;
+        }
+#pragma unroll
+        for (int i = 0; i < IT; ++i) load_lds(base, bytes, stage + at + i * 1024, off[i], static_cast<int>(k0));
     }
 };
 
@@ -227,8 +232,8 @@ __global__ __launch_bounds__(WM * WN * 64) void gemm_i8_tile_kernel(I8Args a) {
     uint32_t tm, tn;
     tile_of(a, blockIdx.x, tm, tn);
     const uint32_t m0 = tm * BM, n0 = tn * BN;
-    const Rows<A_IT> ra(a.A, a.lda, m0, min(static_cast<uint32_t>(BM), a.M - m0), a.K, wave, lane);
-    const Rows<W_IT> rw(a.W, a.ldw, n0, min(static_cast<uint32_t>(BN), a.N - n0), a.K, wave, lane);
+    Rows<A_IT> ra(a.A, a.lda, m0, min(static_cast<uint32_t>(BM), a.M - m0), a.K, wave, lane);
+    Rows<W_IT> rw(a.W, a.ldw, n0, min(static_cast<uint32_t>(BN), a.N - n0), a.K, wave, lane);
     int at[4];  // the lane's piece of a 32-row block, for each 32 codes of a step
 #pragma unroll
     for (int s = 0; s < 4; ++s) at[s] = l32 * 128 + (((2 * s + g) ^ swz(l32)) * 16);
@@ -401,7 +406,7 @@ __global__ __launch_bounds__(512) void gemm_i8_split_kernel(I8Args a) {
     uint32_t tm, tn;
     tile_of(a, blockIdx.x, tm, tn);
     const uint32_t m0 = tm * 32, n0 = tn * 32;
-    const Rows<4> ra(a.A, a.lda, m0, min(32u, a.M - m0), a.K, 0, lane), rw(a.W, a.ldw, n0, min(32u, a.N - n0), a.K, 0, lane);
+    Rows<4> ra(a.A, a.lda, m0, min(32u, a.M - m0), a.K, 0, lane), rw(a.W, a.ldw, n0, min(32u, a.N - n0), a.K, 0, lane);
     int8_t* const s0 = st0 + wave * kWave;
     int8_t* const s1 = st1 + wave * kWave;
     intx16 acc;
@@ -584,7 +589,8 @@ uint64_t span(uint64_t rows, uint64_t ld, uint64_t cols) { return rows ? (rows -
 //   576x1280x1280     6.7   5.7   8.9   6.9  15.3  24.8      2048x1280x1280   8.8   9.7  10.7   9.2  16.1  25.8
 //   2048x1280x5120   25.6  26.7  30.9  21.8  45.9  69.9      8192x640x2560   26.7  24.3  21.3  25.9  27.3  41.2
 //   8192x640x640     10.0  10.7   9.5  12.4  11.9  18.7      2048x10240x1280 47.6  51.7  36.8  43.3  35.8  32.3
-// (128 x 128 with two groups of waves that take the steps in turn: 24.8 for 2048x1280x5120; 256 x 256, 256 x 128, 128 x 64, 128 x 192 and
+// (128 x 128 with two groups of waves that take the steps in turn: 24.8 for 2048x1280x5120; 128 x 80 in 256 workgroups of four waves of 64 x 80,
+// half of each step's codes each, with the next step's fragments read ahead: 21.8; 256 x 256, 256 x 128, 128 x 64, 128 x 192 and
 // 64 x 128 tiles were between their neighbours.)
 struct Build {
     uint32_t bm, bn;
