@@ -76,7 +76,8 @@ __device__ __forceinline__ void store_run(const I8Args& a, uint32_t m, uint32_t 
         }
 }
 
-// Any K, any alignment: a 64 x 64 tile in steps of 32 codes, 4 x 4 outputs a thread.
+// Any K, any alignment: a 64 x 64 tile in steps of 32 codes, 4 x 4 outputs a thread, four products an instruction; bound by its
+// byte loads: 2048x10240x1280 493 us, tiles 32.
 template <typename TC>
 __global__ __launch_bounds__(256) void gemm_i8_any_kernel(I8Args a) {
     __shared__ __attribute__((aligned(4))) int8_t at[64][36], wt[64][36];
@@ -130,6 +131,9 @@ __global__ __launch_bounds__(256) void gemm_i8_any_kernel(I8Args a) {
 // different banks; the loads' lanes permute their addresses accordingly (the 128 bytes of a row stay one segment).
 // The product is transposed (W is the MFMA's A operand): a lane holds one row m of C and runs of four columns.
 // Codes past K are zeros in both operands, rows past M or N are out of the resources' range.
+// What bounds it: a CU is fed about 75 bytes a ns (128 x 128 and four stages 0.42 us a step, 256 x 320 1.38), so tiles as large as the
+// registers allow where there are enough of them: 256 x 320 reads 72 KB for 10.5 M products and has its MFMAs busy for 89% of a step
+// (2048x10240x1280: 1670 TOP/s over the call, whose first loads and 42 MB of C no product hides), 128 x 128 32 KB for 2.1 M.
 typedef int intx4 __attribute__((ext_vector_type(4)));
 typedef int intx16 __attribute__((ext_vector_type(16)));
 
@@ -394,7 +398,8 @@ __global__ __launch_bounds__(WM * WN * 64) void gemm_i8_tile_kernel(I8Args a) {
 // ---- small grids: a workgroup's waves split K ---------------------------------------------
 //
 // Eight waves compute the same 32 x 32 tile, each from the 128-code steps wave, wave + 8, ... through LDS stages of its own
-// (no barrier: a wave waits for its own loads alone), and add their sums through LDS. One launch, no workspace.
+// (no barrier: a wave waits for its own loads alone), and add their sums through LDS. One launch, no workspace. Bound by the launch and two
+// round trips of loads: 154x1280x2048 4.7 us, tiles of 64 x 64 6.4.
 template <typename TC>
 __global__ __launch_bounds__(512) void gemm_i8_split_kernel(I8Args a) {
     constexpr int kWave = 64 * 128;  // bytes of a wave's stage: 32 rows of A, 32 of W
@@ -476,7 +481,8 @@ __global__ __launch_bounds__(512) void gemm_i8_split_kernel(I8Args a) {
 // ---- few rows ------------------------------------------------------------------------------
 //
 // Up to 16 rows (single tokens): a workgroup takes 16 columns and its eight waves the 256-code pieces of K in turn, the
-// weights straight from memory into MFMA operands (16 rows x 64 bytes an instruction); the sums are added through LDS.
+// weights straight from memory into MFMA operands (16 rows x 64 bytes an instruction); the sums are added through LDS. 2x1280x1280 3.0 us
+// (an empty launch 2.0 by the same clock).
 constexpr uint32_t kFewRows = 16;
 
 template <typename TC>
@@ -529,19 +535,24 @@ __global__ __launch_bounds__(256) void quantize_rows_any_kernel(const T* x, int8
     }
 }
 
-// Rows of whole 16-byte vectors, cols <= 16 K (E values a lane, NV vectors): a wave takes a row, which stays in its registers from its
-// largest magnitude to its codes, so it is read once. Lanes past the row repeat its last vector and store nothing.
-template <typename T, int NV>
+// Rows of whole 16-byte vectors, cols <= 8192 (E values a lane, NV vectors): a wave takes a row, or the W = 4 waves of a workgroup do, and it
+// stays in their registers from its largest magnitude to its codes, so it is read once. Lanes past the row repeat its last vector and
+// store nothing. Bound by memory and, for few rows, by the launch: 2048 x 5120 fp16 (31 MB) 8.3 us with four waves a row, 10.2 with one,
+// whose registers leave two waves a SIMD; 4096 x 8192 fp16 17.9 / 35, 64 x 4096 fp16 4.2 / 5.8; but 8192 x 640 fp16 8.8 / 5.2: up to three
+// vectors a lane are one wave's.
+template <typename T, int NV, int W>
 __global__ __launch_bounds__(256) void quantize_rows_kernel(const T* x, int8_t* q, float* scale, uint32_t rows, uint32_t cols, uint64_t ldx,
                                                             uint64_t ldq) {
     constexpr int E = 16 / static_cast<int>(sizeof(T));
     typedef T VT __attribute__((ext_vector_type(E)));
-    const uint32_t lane = threadIdx.x & 63, vecs = cols / E;
-    for (uint64_t r = blockIdx.x * 4ull + (threadIdx.x >> 6); r < rows; r += gridDim.x * 4ull) {
+    __shared__ uint32_t tops[2][4];  // (a row's, and the next one's: one barrier a row)
+    const uint32_t wave = threadIdx.x >> 6, at = threadIdx.x % (64 * W), vecs = cols / E;
+    uint32_t turn = 0;
+    for (uint64_t r = blockIdx.x * (4ull / W) + wave / W; r < rows; r += gridDim.x * (4ull / W), turn ^= 1) {
         const T* xr = x + r * ldx;
         VT v[NV];
 #pragma unroll
-        for (int i = 0; i < NV; ++i) v[i] = *reinterpret_cast<const VT*>(xr + min(lane + 64 * i, vecs - 1) * E);
+        for (int i = 0; i < NV; ++i) v[i] = *reinterpret_cast<const VT*>(xr + min(at + 64 * W * i, vecs - 1) * E);
         uint32_t top = 0;
         if constexpr (E == 8) {
             // fp16 magnitudes order as 16-bit integers, two at a time
@@ -559,14 +570,20 @@ __global__ __launch_bounds__(256) void quantize_rows_kernel(const T* x, int8_t* 
 #pragma unroll
                 for (int e = 0; e < E; ++e) top = max(top, magnitude_bits(static_cast<float>(v[i][e])));
         }
-        const RowScale s = row_scale(wave_max(top));
+        top = wave_max(top);
+        if constexpr (W > 1) {  // (every wave of the workgroup has this row)
+            if ((threadIdx.x & 63) == 0) tops[turn][wave] = top;
+            __syncthreads();
+            top = max(max(tops[turn][0], tops[turn][1]), max(tops[turn][2], tops[turn][3]));
+        }
+        const RowScale s = row_scale(top);
         int8_t* qr = q + r * ldq;
         uint32_t w[NV * E / 4];
         quant_codes<NV * E>([&](int i) { return static_cast<float>(v[i / E][i % E]); }, s, w);
 #pragma unroll
         for (int i = 0; i < NV; ++i)
-            if (lane + 64 * i < vecs) {
-                uint32_t* p = reinterpret_cast<uint32_t*>(qr + (lane + 64 * i) * E);
+            if (at + 64 * W * i < vecs) {
+                uint32_t* p = reinterpret_cast<uint32_t*>(qr + (at + 64 * W * i) * E);
                 if constexpr (E == 8) {
                     typedef uint32_t u2 __attribute__((ext_vector_type(2)));
                     *reinterpret_cast<u2*>(p) = u2{w[2 * i], w[2 * i + 1]};
@@ -574,7 +591,7 @@ __global__ __launch_bounds__(256) void quantize_rows_kernel(const T* x, int8_t* 
                     *p = w[i];
                 }
             }
-        if (lane == 0) scale[r] = s.scale;
+        if (at == 0) scale[r] = s.scale;
     }
 }
 
@@ -655,16 +672,16 @@ void launch_product(I8Args a, hipStream_t s) {
 template <typename T>
 void launch_quantize(const T* x, int8_t* q, float* scale, uint32_t rows, uint32_t cols, uint64_t ldx, uint64_t ldq, hipStream_t s) {
     constexpr uint32_t E = 16 / sizeof(T);
-    const unsigned grid = grid_of((static_cast<uint64_t>(rows) + 3) / 4);
     const uint32_t nv = ceil_div(cols, 64 * E);
+    const unsigned grid = grid_of((static_cast<uint64_t>(rows) + 3) / 4), wide = grid_of(rows);
     if (cols % E != 0 || ldx % E != 0 || ldq % E != 0 || !aligned(x, 16) || !aligned(q, E) || cols > kMaxFastCols)
         quantize_rows_any_kernel<T><<<grid, 256, 0, s>>>(x, q, scale, rows, cols, ldx, ldq);
-    else if (nv <= 2) quantize_rows_kernel<T, 2><<<grid, 256, 0, s>>>(x, q, scale, rows, cols, ldx, ldq);
-    else if (nv <= 3) quantize_rows_kernel<T, 3><<<grid, 256, 0, s>>>(x, q, scale, rows, cols, ldx, ldq);
-    else if (nv <= 5) quantize_rows_kernel<T, 5><<<grid, 256, 0, s>>>(x, q, scale, rows, cols, ldx, ldq);
-    else if (nv <= 10) quantize_rows_kernel<T, 10><<<grid, 256, 0, s>>>(x, q, scale, rows, cols, ldx, ldq);
-    else if (sizeof(T) == 2 || nv <= 16) quantize_rows_kernel<T, 16><<<grid, 256, 0, s>>>(x, q, scale, rows, cols, ldx, ldq);
-    else if constexpr (sizeof(T) == 4) quantize_rows_kernel<T, 32><<<grid, 256, 0, s>>>(x, q, scale, rows, cols, ldx, ldq);
+    else if (nv <= 2) quantize_rows_kernel<T, 2, 1><<<grid, 256, 0, s>>>(x, q, scale, rows, cols, ldx, ldq);
+    else if (nv <= 3) quantize_rows_kernel<T, 3, 1><<<grid, 256, 0, s>>>(x, q, scale, rows, cols, ldx, ldq);
+    else if (nv <= 8) quantize_rows_kernel<T, 2, 4><<<wide, 256, 0, s>>>(x, q, scale, rows, cols, ldx, ldq);
+    else if (nv <= 12) quantize_rows_kernel<T, 3, 4><<<wide, 256, 0, s>>>(x, q, scale, rows, cols, ldx, ldq);
+    else if (sizeof(T) == 2 || nv <= 16) quantize_rows_kernel<T, 4, 4><<<wide, 256, 0, s>>>(x, q, scale, rows, cols, ldx, ldq);
+    else if constexpr (sizeof(T) == 4) quantize_rows_kernel<T, 8, 4><<<wide, 256, 0, s>>>(x, q, scale, rows, cols, ldx, ldq);
 }
 
 }  // namespace

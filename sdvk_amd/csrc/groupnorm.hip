@@ -98,6 +98,8 @@ __device__ __forceinline__ float slope(float z) {
 }
 
 // ---- any shape and alignment -------------------------------------------------------
+//
+// Element by element, four or five launches; bound by the loads' latency (2 x 4096 x 640 fp16 backward 202 us, by vectors 23).
 
 // One group of one chunk per workgroup; two passes over its values, sums in 64 bits.
 template <typename TX>
@@ -336,7 +338,9 @@ __global__ __launch_bounds__(256) void gn_bwd_apply_any_kernel(GnBwdArgs a) {
 // Statistics: a thread sums x - x0 and its square for each of its columns, x0 the column's first value of its own (at worst,
 // where x0 is the outlier that makes the variance, that costs a factor of the rows a thread takes, which is their
 // number and no more); the threads' sums are joined in 64 bits.
-// All of it is bound by memory: every pass reads x once (and dy), and one stores y or dx.
+// All of it is bound by memory: every pass reads x once (and dy), and one stores y or dx. One 2^20 x 128 image, fp16 (268 MB): sums 76 us (3.5
+// TB/s), join 5, store 85 (6.3 TB/s, part of x from the last-level cache). 2 x 16384 x 320 fp16 (21 MB): 8.4, 3.1 and 9.4 us, of which 2 are
+// the launch. Backward 2 x 4096 x 640 fp16 (10 MB a tensor): sums 9.8 us, dx and the weights' gradients 12.7.
 constexpr uint32_t kFastChannels = 4096, kFastGroups = 256;
 constexpr int kRows = 4;  // rows a thread has in flight
 
@@ -545,7 +549,7 @@ __global__ __launch_bounds__(4096 / Vec<TX>::E) void gn_apply_kernel(GnArgs a) {
 }
 
 // 8-bit rows: a wave takes two rows at a time, four columns (lane + 64 i) each, so that a row's largest value is the wave's. Grid: batch *
-// ncut, T threads.
+// ncut, T threads. 2 x 4096 x 640 fp16 6.5 us (16 MB), bound by the instructions of the quantiser and of the statistics' use.
 template <typename TX, int ACT, int NV, int T>
 __global__ __launch_bounds__(T) void gn_apply_i8_kernel(GnArgs a) {
     typedef TX VT __attribute__((ext_vector_type(4)));
