@@ -446,6 +446,9 @@ CASES = {
         dict(rows=5, cols=64, off=2, typ="f16"), dict(rows=12, cols=96, kind="ties"), dict(rows=12, cols=97, kind="ties"), dict(rows=12, cols=96, kind="ties", typ="f16"), dict(rows=12, cols=512, kind="near"),
         dict(rows=12, cols=33, kind="near"), dict(rows=16, cols=64, kind="sizes"), dict(rows=16, cols=65, kind="sizes"), dict(rows=7, cols=64, kind="broken"), dict(rows=7, cols=51, kind="broken", typ="f16"),
         dict(rows=16, cols=64, kind="sizes", typ="f16"),
+        # rows that four waves share
+        dict(rows=7, cols=784, kind="broken"), dict(rows=7, cols=1552, kind="broken", typ="f16"), dict(rows=12, cols=2048, kind="ties"), dict(rows=4, cols=2816, kind="near", ldx=2832, ldq=2820),
+        dict(rows=5, cols=4096, typ="f16"), dict(rows=5, cols=8192, typ="f16", kind="ties"), dict(rows=6, cols=4080, kind="sizes"), dict(rows=3, cols=8192, kind="near"),
     ],
     "product": [
         dict(M=1, N=1, K=1), dict(M=1, N=1, K=16), dict(M=2, N=40, K=64), dict(M=16, N=48, K=320), dict(M=17, N=33, K=48), dict(M=70, N=65, K=144, out="f16"), dict(M=5, N=130, K=37, bias=False),
