@@ -14,7 +14,7 @@ namespace mi {
 namespace {
 
 constexpr uint32_t kMaxGrid = 1u << 20;  // workgroups of a launch that strides over its units
-constexpr uint32_t kMaxFastCols = 8192;  // columns of a row that a wave holds
+constexpr uint32_t kMaxFastCols = 8192;  // columns of a row that stays in registers
 constexpr uint32_t kMaxSize = 1u << 31;  // rows and columns of a product, rows of the quantiser ...
 constexpr uint32_t kMaxCols = 1u << 30;  // ... and its columns: counted in 32 bits with a tile or a wave past the end
 constexpr uint32_t kMaxK = 131071;       // 2^31 / 2^14
