@@ -122,3 +122,24 @@ def test_wide_results(gpu):
     for m in (0, rows // 2, rows - 1):
         assert np.array_equal(q.download(np.int8, cols, offset=m * cols), want[0])
     assert not np.any(q.download(np.int8, cols, offset=(rows - 2) * cols))
+
+
+def test_many_columns(gpu):
+    """Two rows and 2^27 columns: more of the few-row kernel's tiles than a launch has workgroups."""
+    print("[case] product of 2 x (2^27 + 21)", flush=True)
+    M, N, K = 2, (1 << 27) + 21, 16
+    r = ref.rng_of(54)
+    a, w = (r.integers(-127, 128, (n, K)).astype(np.int8) for n in (M, 3))
+    sa = r.uniform(0.5, 2, M).astype(np.float32)
+    W, C = DeviceBuffer(N * K), DeviceBuffer(M * N * 2)
+    W.fill_zero()
+    at = (0, N // 2, N - 1)
+    for n, row in zip(at, w):
+        W.upload(row, offset=n * K)
+    ops.gemm_nt_i8(DeviceBuffer.from_array(a), DeviceBuffer.from_array(sa), W, DeviceBuffer.from_array(np.full(N, 0.0625, np.float32)), C, M, N, K, c_dtype=ops.MI_F16)
+    synchronize()
+    for m in range(M):
+        for n, row in zip(at, w):
+            part = (a[m].astype(np.float64) @ row.astype(np.float64)) * np.float64(sa[m]) * 0.0625
+            assert abs(float(C.download(H, 1, offset=(m * N + n) * 2)[0]) - part) <= 2.0 ** -11 * abs(part) * 1.001, (m, n)
+        assert not np.any(C.download(H, 1000, offset=(m * N + N // 2 + 1) * 2)) and not np.any(C.download(H, 1000, offset=(m * N + N - 1001) * 2))
