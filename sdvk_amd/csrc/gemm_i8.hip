@@ -183,14 +183,15 @@ struct Rows {
 #pragma unroll
         for (int i = 0; i < IT; ++i) off[i] = (8 * (wave * IT + i) + (lane >> 3)) * static_cast<uint32_t>(ld) + col[i & 1];
     }
-    // (steps in turn: a lane whose codes are past K once stays there)
+    // (steps in turn: a lane whose codes are past K once stays there. The scalar offset stays within K, so within `bytes`: the range
+    // check subtracts it from them in 32 bits, and a larger one would wrap and let kPast through)
     __device__ __forceinline__ void load(int8_t* stage, uint32_t k0) {
         if (k0 + 128 > K) {
 #pragma unroll
             for (int i = 0; i < IT; ++i) off[i] = k0 + col[i & 1] < K ? off[i] : kPast;
         }
 #pragma unroll
-        for (int i = 0; i < IT; ++i) load_lds(base, bytes, stage + at + i * 1024, off[i], static_cast<int>(k0));
+        for (int i = 0; i < IT; ++i) load_lds(base, bytes, stage + at + i * 1024, off[i], static_cast<int>(min(k0, K)));
     }
 };
 

@@ -160,6 +160,8 @@ inline Rsrc make_rsrc(const void* p, int stride, int num, int) {
     return Rsrc{static_cast<unsigned char*>(const_cast<void*>(p)), static_cast<uint32_t>(num)};
 }
 inline bool in_range(const Rsrc& r, uint32_t voff, uint32_t soff, uint32_t at, uint32_t size, const char* what) {
+    // (the hardware compares voffset with num_records - soffset, in 32 bits: past num_records that would wrap)
+    if (soff > r.num) die("%s: soffset %u past num_records %u", what, soff, r.num);
     const uint64_t o = static_cast<uint64_t>(voff) + soff + at;
     const uint64_t ov = static_cast<uint64_t>(voff) + at;
     const bool in = o + size <= r.num;
