@@ -638,7 +638,9 @@ int mi_groupnorm_bwd(const mi_groupnorm_bwd_args* args, void* workspace, uint64_
 
 /* Rows of 8-bit codes: scale[r] = max(max|x[r]|, 127 * 2^-126) / 127 in fp32, q[r, c] = x[r, c] /
  * scale[r] rounded to the nearest integer, ties to even (of the exact quotient: -127 ..
- * 127). A row with an infinity or a NaN gets the scale NaN and codes 0. x MI_F32 or MI_F16
+ * 127). The scale is the rounded quotient: max|x| * (1 / 127) is another number for one row in
+ * twenty, and values at a tie then have other codes. A row with an infinity or a NaN gets the
+ * scale NaN and codes 0. x MI_F32 or MI_F16
  * (dtype); row strides ldx, ldq in elements (0 -> cols). For weights, one scale a channel:
  * mi_q8_0_dequant, then this. Tensors aligned to their element; cols % 16 == 0 with 16-byte
  * aligned rows and cols <= 8192 is the fast path. rows <= 2^31, cols <= 2^30. q and scale

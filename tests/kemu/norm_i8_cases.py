@@ -1,4 +1,4 @@
-"""One case of tests/norm_i8_ref.py or tests/norm_i8_chain.py on the kernel emulator, in a process of its own (a fault in an emulated
+"""One case of tests/norm_i8_ref.py, norm_i8_limits.py or norm_i8_chain.py on the kernel emulator, in a process of its own (a fault in an emulated
 kernel ends that process with the emulator's report):
 
     python tests/kemu/norm_i8_cases.py '<json: {"op": name, "orders": [...], ...parameters}>'
@@ -13,6 +13,7 @@ HERE = Path(__file__).resolve().parent
 sys.path[:0] = [str(HERE.parent.parent), str(HERE.parent), str(HERE)]
 
 import norm_i8_chain  # noqa: E402
+import norm_i8_limits  # noqa: E402
 import norm_i8_ref  # noqa: E402
 from bwd_cases import Backend  # noqa: E402
 
@@ -25,7 +26,7 @@ def main(argv):
     _lib.load = lambda: be.E.lib  # sdvk_amd.ops on the emulated library
     for o in orders:
         be.E.order(o, bool(o))
-        {**norm_i8_ref.OPS, **norm_i8_chain.OPS}[op](be, **spec)
+        {**norm_i8_ref.OPS, **norm_i8_limits.OPS, **norm_i8_chain.OPS}[op](be, **spec)
         print(f"OK order {o}", flush=True)
 
 

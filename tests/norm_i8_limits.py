@@ -1,0 +1,91 @@
+"""GroupNorm, the token quantiser and the 8-bit product at the edges of what their documentation promises, against plain 64-bit formulas:
+cases that run on any backend with the C-ABI (the GPU, or the CPU emulator of tests/kemu), with the bounds of tests/norm_i8_ref.py.
+"""
+from __future__ import annotations
+
+import numpy as np
+
+from bwd_ref import CODE, DT, SENTINEL, U, Arena, check, f64, rng_of
+from norm_i8_ref import codes_of
+
+F127, R127 = np.float32(127), np.float32(1) / np.float32(127)
+
+
+def reciprocal_codes(x):
+    """What a scale of max|x| * (1 / 127) gives in place of the rounded quotient max|x| / 127."""
+    scale = np.abs(x).max(1) * R127
+    return np.rint(f64(x) / f64(scale)[:, None]).astype(np.int8), scale
+
+
+def rows_reciprocal(rng, rows, cols, typ):
+    """Rows whose maximum gives another scale by a product with 1 / 127, of values at the ties of the quotient's."""
+    if typ == "f16":
+        every = np.arange(1, 0x7c00, dtype=np.uint16).view(np.float16)
+        every = every[every > 1e-3]
+        tops = every[every > 1].astype(np.float32)
+        tops = tops[tops / F127 != tops * R127]
+        found = []
+        for t in rng.permutation(tops):
+            v = every[every.astype(np.float32) < t].astype(np.float32)
+            q = [np.rint(f64(v) / float(s)) for s in (t / F127, t * R127)]
+            if np.any(q[0] != q[1]):
+                found.append((t, v[q[0] != q[1]]))
+            if len(found) == rows:
+                break
+    else:
+        tops = (2.0 ** rng.uniform(-10, 10, 64 * rows)).astype(np.float32)
+        tops = tops[tops / F127 != tops * R127][:rows]
+        found = []
+        for t in tops:
+            s = t / F127
+            v = ((rng.integers(0, 127, 4 * cols) + 0.5) * float(s)).astype(np.float32)
+            v = np.concatenate([v, np.nextafter(v, np.float32(0)), np.nextafter(v, t)])
+            q = [np.rint(f64(v) / float(c)) for c in (s, t * R127)]
+            found.append((t, v[q[0] != q[1]]))
+    assert len(found) == rows and all(len(v) for _, v in found)
+    x = np.stack([np.resize(v, cols) for _, v in found]) * rng.choice([-1, 1], (rows, cols))
+    x[:, cols // 3] = [t for t, _ in found]
+    return x
+
+
+ROWS = {"reciprocal": (rows_reciprocal, reciprocal_codes)}
+
+
+def rows_of(rng, rows, cols, typ, kind):
+    """(x, codes and scales by the definition): the mistake that the rows are made for has other codes in each of them."""
+    make, mistake = ROWS[kind]
+    x = make(rng, rows, cols, typ).astype(DT[typ])
+    right, wrong = codes_of(x.astype(np.float32)), mistake(x.astype(np.float32))
+    assert np.all((right[0] != wrong[0]).any(1))
+    return x, right
+
+
+def codes(be, *, rows, cols, kind, typ="f32", N=24, seed=11):
+    """The quantiser's codes and scales, and the product of them, of rows at a rounding's edge."""
+    rng = rng_of(seed)
+    x, (q, s) = rows_of(rng, rows, cols, typ, kind)
+    A = Arena(be)
+    bx = A.put(x.reshape(-1))
+    bq, bs = A.out(rows * cols, np.int8), A.out(rows, np.float32)
+    be.call("mi_quantize_rows_i8", bx.ptr, CODE[typ], bq.ptr, bs.ptr, rows, cols, 0, 0, None)
+    got, gs = be.get(bq, np.int8, rows * cols).reshape(rows, cols), be.get(bs, np.float32, rows)
+    assert np.array_equal(gs, s), np.flatnonzero(gs != s)[:5]
+    assert np.array_equal(got, q), [(i, x[tuple(i)], s[i[0]], got[tuple(i)], q[tuple(i)]) for i in np.argwhere(got != q)[:5]]
+    w = rng.integers(-127, 128, (N, cols)).astype(np.int8)
+    sw = rng.uniform(0.5, 2, N).astype(np.float32)
+    bw, bsw, bc = A.put(w.reshape(-1)), A.put(sw), A.out(rows * N, np.float32)
+    be.call("mi_gemm_nt_i8", bq.ptr, bs.ptr, bw.ptr, bsw.ptr, None, bc.ptr, 0, rows, N, cols, 0, 0, 0, 0, None)
+    want = f64(q) @ f64(w).T * f64(s)[:, None] * f64(sw)
+    # float(sum), its product with the row's scale, the fma
+    check(be.get(bc, np.float32, rows * N).reshape(rows, N), want, 4.01 * U * np.abs(want) + 1e-44, "linear")
+    A.unchanged()
+
+
+OPS = {"codes": codes}
+
+CASES = {
+    "codes": [dict(rows=9, cols=64, kind="reciprocal"), dict(rows=20, cols=77, kind="reciprocal"), dict(rows=5, cols=2048, kind="reciprocal"), dict(rows=3, cols=1280, kind="reciprocal", typ="f16")],
+}
+GPU_CASES = {
+    "codes": [dict(rows=154, cols=2048, kind="reciprocal", N=1280), dict(rows=16, cols=5120, kind="reciprocal", typ="f16", N=640)],
+}
