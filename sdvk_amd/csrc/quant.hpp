@@ -3,7 +3,8 @@
 //   scale = max(max|x|, 127 * 2^-126) / 127 in fp32,  code = x / scale rounded to the nearest integer, ties to even
 //
 // The quotient is exact: which of two integers is nearest is decided by x - code * scale, which fp32 holds without rounding (a
-// multiple of the smaller operand's last place, no larger than the scale). The floor keeps 1 / scale finite: rows smaller
+// multiple of the smaller operand's last place, no larger than the scale); twice it is held against the scale (half a scale below
+// 2^-125 is no fp32 number if its last place is odd). The floor keeps 1 / scale finite: rows smaller
 // than it (zeros among them) get codes in steps of 2^-126. A row that holds an infinity or a NaN gets the scale NaN
 // and codes 0, so that everything computed from it is NaN.
 #pragma once
@@ -47,7 +48,7 @@ __device__ __forceinline__ float quant_right(float v, float t, const RowScale& s
     const float r = __builtin_fmaf(kQuantMagic - t, s.scale, v);
     const uint32_t bits = __float_as_uint(t);
     // over half a step, or half a step and an odd code: magnitudes order as integers
-    const bool wrong = magnitude_bits(r) + (bits & 1u) > __float_as_uint(0.5f * s.scale);
+    const bool wrong = magnitude_bits(r + r) + (bits & 1u) > __float_as_uint(s.scale);
     return wrong ? __uint_as_float(r > 0.0f ? bits + 1 : bits - 1) : t;
 }
 __device__ __forceinline__ int quant_code(float v, const RowScale& s) {
@@ -63,7 +64,7 @@ __device__ __forceinline__ void quant_codes(const F& value, const RowScale& s, u
     float t[N], rest = 0.0f;
 #pragma unroll
     for (int i = 0; i < N; ++i) t[i] = quant_fast(value(i), s, rest);
-    if (!(rest < 0.5f * s.scale)) {
+    if (!(rest + rest < s.scale)) {
 #pragma unroll
         for (int i = 0; i < N; ++i) t[i] = quant_right(value(i), t[i], s);
     }

@@ -48,7 +48,39 @@ def rows_reciprocal(rng, rows, cols, typ):
     return x
 
 
-ROWS = {"reciprocal": (rows_reciprocal, reciprocal_codes)}
+def rounded_half_codes(x):
+    """The nearest codes where the rest of a product with 1 / scale is held against half a scale in fp32: of a scale below 2^-125 with an
+    odd last place that half is no fp32 number, and rounds."""
+    scale = np.abs(x).max(1) / F127
+    inv, half = np.float32(1) / scale, np.float32(0.5) * scale
+    t = np.rint(f64(x) * f64(inv)[:, None])
+    r = (f64(x) - t * f64(scale)[:, None]).astype(np.float32)
+    off = np.abs(r).view(np.uint32) + (t % 2 != 0) > half.view(np.uint32)[:, None]
+    return (t + np.where(off, np.sign(r), 0)).astype(np.int8), scale
+
+
+def rows_half(rng, rows, cols, typ):
+    """Rows of the smallest scales above the floor (maxima of 1.5e-36 to 3e-36), of values a step of fp32 from a tie."""
+    found = []
+    while len(found) < rows:
+        m = 2 * int(rng.integers(2 ** 22, 2 ** 23)) + 1  # the scale in steps of 2^-149
+        t = np.float32(127 * m * 2.0 ** -149)
+        s = t / F127
+        if s != m * 2.0 ** -149:
+            continue
+        n = np.array([k * m + (m + o) // 2 for k in range(8) for o in (-1, 1)], np.float64)
+        v = (n * 2.0 ** -149).astype(np.float32)
+        v = v[f64(v) == n * 2.0 ** -149]
+        x = np.concatenate([[t], v])[None].astype(np.float32)
+        q = [c[0, 1:] for c, _ in (codes_of(x), rounded_half_codes(x))]
+        if np.any(q[0] != q[1]):
+            found.append((t, v[q[0] != q[1]]))
+    x = np.stack([np.resize(v, cols) for _, v in found]) * rng.choice([-1, 1], (rows, cols))
+    x[:, cols // 3] = [t for t, _ in found]
+    return x
+
+
+ROWS = {"reciprocal": (rows_reciprocal, reciprocal_codes), "half": (rows_half, rounded_half_codes)}
 
 
 def rows_of(rng, rows, cols, typ, kind):
@@ -84,8 +116,9 @@ def codes(be, *, rows, cols, kind, typ="f32", N=24, seed=11):
 OPS = {"codes": codes}
 
 CASES = {
-    "codes": [dict(rows=9, cols=64, kind="reciprocal"), dict(rows=20, cols=77, kind="reciprocal"), dict(rows=5, cols=2048, kind="reciprocal"), dict(rows=3, cols=1280, kind="reciprocal", typ="f16")],
+    "codes": [dict(rows=9, cols=64, kind="reciprocal"), dict(rows=20, cols=77, kind="reciprocal"), dict(rows=5, cols=2048, kind="reciprocal"), dict(rows=3, cols=1280, kind="reciprocal", typ="f16"),
+              dict(rows=40, cols=64, kind="half"), dict(rows=9, cols=75, kind="half"), dict(rows=5, cols=2048, kind="half")],
 }
 GPU_CASES = {
-    "codes": [dict(rows=154, cols=2048, kind="reciprocal", N=1280), dict(rows=16, cols=5120, kind="reciprocal", typ="f16", N=640)],
+    "codes": [dict(rows=154, cols=2048, kind="reciprocal", N=1280), dict(rows=16, cols=5120, kind="reciprocal", typ="f16", N=640), dict(rows=300, cols=1280, kind="half")],
 }
