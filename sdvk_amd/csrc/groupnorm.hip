@@ -31,9 +31,22 @@ constexpr uint64_t kJoinParts = 1u << 19;
 struct Stat {  // of one group of one image, 16 bytes: what `stats` holds
     float mean, low, inv, zero;
 };
-struct Part {  // of one group of one chunk: mean = shift + rest, m2 = sum of (x - mean)^2
-    float shift, rest, m2, zero;
+struct Part {  // of one group of one chunk: mean = shift + rest, var = mean of (x - mean)^2 (their sum could pass fp32's range)
+    float shift, rest, var, zero;
 };
+
+// Squares are summed in fp32, of differences times a power of two: fp32 values below 1e18 differ by 2e18 at most, and the longest sums
+// are 2048 of a column and 4096 of a wave's lanes, 4096 (2e18 / 16)^2 = 6.4e37 in all. (fp16 values stay below 2^17.)
+template <typename TX>
+constexpr float kDown = sizeof(TX) == 4 ? 0.0625f : 1.0f;
+template <typename TX>
+constexpr double kUp = 1.0 / kDown<TX>;
+// (x - shift) kDown of a shift that is held times kDown: exactly that multiple of the rounded difference
+template <typename TX>
+__device__ __forceinline__ float down(float x, float shift) {
+    if constexpr (sizeof(TX) == 4) return __builtin_fmaf(x, kDown<TX>, -shift);
+    return x - shift;
+}
 
 struct GnArgs {
     const void* x;
@@ -144,7 +157,7 @@ __global__ __launch_bounds__(256) void gn_part_any_kernel(GnArgs a) {
             d1 = (red[1][0] + red[1][1]) + (red[1][2] + red[1][3]);
             d2 = (red[2][0] + red[2][1]) + (red[2][2] + red[2][3]);
             const double rest = d1 / static_cast<double>(n);
-            a.part[bc * a.groups + g] = Part{shift, static_cast<float>(rest), static_cast<float>(not_below_zero(d2 - d1 * rest)), 0.0f};
+            a.part[bc * a.groups + g] = Part{shift, static_cast<float>(rest), static_cast<float>(not_below_zero(d2 - d1 * rest) / static_cast<double>(n)), 0.0f};
         }
         __syncthreads();  // the sums are free for the next unit
     }
@@ -166,7 +179,7 @@ __device__ __forceinline__ void join(const GnArgs& a, const Part* p, uint32_t fi
                 const double k = static_cast<double>(min(a.chunk, a.pixels - c * a.chunk)) * a.cg;
                 const double d = (static_cast<double>(q[i].shift) - ref) + static_cast<double>(q[i].rest);
                 s1 += k * d;
-                s2 += static_cast<double>(q[i].m2) + k * d * d;
+                s2 += k * (static_cast<double>(q[i].var) + d * d);
             }
         }
     }
@@ -438,7 +451,7 @@ template <typename TX>
 __global__ __launch_bounds__(4096 / Vec<TX>::E) void gn_part_kernel(GnArgs a) {
     constexpr int E = Vec<TX>::E;
     typedef typename Vec<TX>::type VT;
-    extern __shared__ __attribute__((aligned(16))) float red[];  // [3][T / V][C]: x0, sums of x - x0, of its square
+    extern __shared__ __attribute__((aligned(16))) float red[];  // [3][T / V][C]: x0, sums of x - x0, of its square, of values times kDown
     const uint32_t T = blockDim.x, tid = threadIdx.x, V = a.C / E, rows_at = T / V;
     const uint32_t ty = tid / V, tx = tid % V;
     const uint64_t b = blockIdx.x / a.nchunk;
@@ -451,7 +464,7 @@ __global__ __launch_bounds__(4096 / Vec<TX>::E) void gn_part_kernel(GnArgs a) {
     if (in && ty < rows) {
         const VT v = *reinterpret_cast<const VT*>(x + ty * a.ldx);
 #pragma unroll
-        for (int e = 0; e < E; ++e) x0[e] = static_cast<float>(v[e]);
+        for (int e = 0; e < E; ++e) x0[e] = static_cast<float>(v[e]) * kDown<TX>;
         // (a batch's rows past the chunk repeat its last row and add nothing: one by one they would cost a round trip each)
         for (uint32_t r = ty + rows_at; r < rows; r += kRows * rows_at) {
             VT w[kRows];
@@ -462,7 +475,7 @@ __global__ __launch_bounds__(4096 / Vec<TX>::E) void gn_part_kernel(GnArgs a) {
                 const bool whole = r + i * rows_at < rows;
 #pragma unroll
                 for (int e = 0; e < E; ++e) {
-                    const float d = whole ? static_cast<float>(w[i][e]) - x0[e] : 0.0f;
+                    const float d = whole ? down<TX>(static_cast<float>(w[i][e]), x0[e]) : 0.0f;
                     s1[e] += d;
                     s2[e] = __builtin_fmaf(d, d, s2[e]);
                 }
@@ -499,8 +512,10 @@ __global__ __launch_bounds__(4096 / Vec<TX>::E) void gn_part_kernel(GnArgs a) {
         t1 = lanes_sum(t1, n);
         t2 = lanes_sum(t2, n);
         if (lane == 0 && g0 + tid / n < a.groups) {
-            const double rest = t1 / (static_cast<double>(rows) * a.cg);
-            a.part[static_cast<uint64_t>(blockIdx.x) * a.groups + g] = Part{ref, static_cast<float>(rest), static_cast<float>(not_below_zero(t2 - t1 * rest)), 0.0f};
+            const double total = static_cast<double>(rows) * a.cg, rest = t1 / total;
+            a.part[static_cast<uint64_t>(blockIdx.x) * a.groups + g] =
+                Part{static_cast<float>(ref * kUp<TX>), static_cast<float>(rest * kUp<TX>),
+                     static_cast<float>(not_below_zero(t2 - t1 * rest) / total * (kUp<TX> * kUp<TX>)), 0.0f};
         }
     }
 }
@@ -895,13 +910,13 @@ __global__ __launch_bounds__(512) void gn_slab_kernel(GnArgs a) {
     double t = 0.0;
 #pragma unroll
     for (uint32_t w = 0; w < T / 64; ++w) t += static_cast<double>(sums[0][w]);
-    const float ref = static_cast<float>(t / (static_cast<double>(a.pixels) * a.cg));
+    const float ref = static_cast<float>(t / (static_cast<double>(a.pixels) * a.cg)) * kDown<TX>;
     float s1 = 0.0f, s2 = 0.0f;
 #pragma unroll
     for (int i = 0; i < NU; ++i)
 #pragma unroll
         for (int e = 0; e < VE; ++e) {
-            const float d = tid + i * T < units ? static_cast<float>(v[i][e]) - ref : 0.0f;
+            const float d = tid + i * T < units ? down<TX>(static_cast<float>(v[i][e]), ref) : 0.0f;
             s1 += d;
             s2 = __builtin_fmaf(d, d, s2);
         }
@@ -918,7 +933,7 @@ __global__ __launch_bounds__(512) void gn_slab_kernel(GnArgs a) {
         d1 += static_cast<double>(sums[1][w]);
         d2 += static_cast<double>(sums[2][w]);
     }
-    const Stat st = stat_of(a, static_cast<double>(ref), d1, d2);
+    const Stat st = stat_of(a, ref * kUp<TX>, d1 * kUp<TX>, d2 * (kUp<TX> * kUp<TX>));
     for (uint32_t c = tid; c < a.cg; c += T) {
         const Coef k = coef(st, ca[c], cb[c]);
         ca[c] = k.a;
@@ -988,20 +1003,20 @@ __global__ __launch_bounds__(512) void gn_bwd_slab_kernel(GnBwdArgs a, uint32_t 
             for (int e = 0; e < VE; ++e) s += in(i) ? static_cast<float>(v[i][e]) : 0.0f;
         total(0, s);
         __syncthreads();
-        const float ref = static_cast<float>(read(0) / n);
+        const float ref = static_cast<float>(read(0) / n) * kDown<TX>;
         float s1 = 0.0f, s2 = 0.0f;
 #pragma unroll
         for (int i = 0; i < NU; ++i)
 #pragma unroll
             for (int e = 0; e < VE; ++e) {
-                const float q = in(i) ? static_cast<float>(v[i][e]) - ref : 0.0f;
+                const float q = in(i) ? down<TX>(static_cast<float>(v[i][e]), ref) : 0.0f;
                 s1 += q;
                 s2 = __builtin_fmaf(q, q, s2);
             }
         total(1, s1);
         total(2, s2);
         __syncthreads();
-        st = stat_of(f, static_cast<double>(ref), read(1), read(2));
+        st = stat_of(f, ref * kUp<TX>, read(1) * kUp<TX>, read(2) * (kUp<TX> * kUp<TX>));
         __syncthreads();  // the sums are free
     } else {
         st = f.stats[blockIdx.x];

@@ -3,8 +3,11 @@ cases that run on any backend with the C-ABI (the GPU, or the CPU emulator of te
 """
 from __future__ import annotations
 
+from unittest import mock
+
 import numpy as np
 
+import norm_i8_ref
 from bwd_ref import CODE, DT, SENTINEL, U, Arena, check, f64, rng_of
 from norm_i8_ref import codes_of
 
@@ -113,12 +116,48 @@ def codes(be, *, rows, cols, kind, typ="f32", N=24, seed=11):
     A.unchanged()
 
 
-OPS = {"codes": codes}
+# ---------------------------------------------------------------- GroupNorm --
+
+def pixels_of(kind):
+    """Pixels in the place of norm_i8_ref.pixels_of's."""
+    def make(rng, B, P, C, offset, outlier):
+        if kind == "signs":  # magnitudes just below the documented 1e18
+            return rng.choice([-9.99e17, 9.99e17], (B, P, C))
+        if kind == "range":
+            return rng.uniform(-9.99e17, 9.99e17, (B, P, C))
+        if kind == "halves":  # the first row of a chunk and of a thread on one side, the rest on the other
+            x = np.full((B, P, C), 9.99e17)
+            x[:, ::2] = -9.99e17
+            x[:, 0] = -9.99e17
+            return x
+        assert kind == "single"  # one value of a group
+        x = np.zeros((B, P, C))
+        x[:, 0, ::7] = 9.99e17
+        return x
+    return make
+
+
+def norm(be, *, pixels, **case):
+    """norm_i8_ref.groupnorm, or groupnorm_bwd (dtyp given), of other pixels."""
+    with mock.patch.object(norm_i8_ref, "pixels_of", pixels_of(pixels)):
+        (norm_i8_ref.groupnorm_bwd if "dtyp" in case else norm_i8_ref.groupnorm)(be, **case)
+
+
+OPS = {"codes": codes, "norm": norm}
+
+# what takes a group in registers (units of four and two values, whole and part full), chunks, and element by element
+NORM_SIZES = [dict(P=50, C=32, G=4), dict(P=256, C=64, G=1), dict(P=100, C=60, G=10, gap=2), dict(P=300, C=40, G=1), dict(P=600, C=320, G=32), dict(P=600, C=128, G=2), dict(P=300, C=33, G=1)]
 
 CASES = {
+    "norm": [dict(pixels=k, **c) for k in ("signs", "range", "halves", "single") for c in NORM_SIZES]
+    + [dict(pixels="signs", P=40, C=320, G=32, out="i8"), dict(pixels="halves", P=300, C=64, G=2, out="i8", act=1), dict(pixels="signs", P=30, C=33, G=3, out="i8"), dict(pixels="range", B=2, P=513, C=64, G=1, out="f16", act=1)]
+    + [dict(pixels=k, dtyp="f32", act=a, **c) for k, a in (("signs", 0), ("halves", 1)) for c in NORM_SIZES],
     "codes": [dict(rows=9, cols=64, kind="reciprocal"), dict(rows=20, cols=77, kind="reciprocal"), dict(rows=5, cols=2048, kind="reciprocal"), dict(rows=3, cols=1280, kind="reciprocal", typ="f16"),
               dict(rows=40, cols=64, kind="half"), dict(rows=9, cols=75, kind="half"), dict(rows=5, cols=2048, kind="half")],
 }
 GPU_CASES = {
+    # chunks of 2048 rows; a workgroup's registers full
+    "norm": [dict(pixels=k, **c) for k in ("signs", "halves") for c in (dict(B=256, P=2048, C=64, G=2), dict(P=20000, C=256, G=2, act=1), dict(P=1024, C=1280, G=32, out="i8"), dict(P=32768, C=4, G=4))]
+    + [dict(pixels="signs", P=1024, C=1280, G=32, dtyp="f32"), dict(pixels="halves", B=256, P=2048, C=64, G=2, dtyp="f32")],
     "codes": [dict(rows=154, cols=2048, kind="reciprocal", N=1280), dict(rows=16, cols=5120, kind="reciprocal", typ="f16", N=640), dict(rows=300, cols=1280, kind="half")],
 }
