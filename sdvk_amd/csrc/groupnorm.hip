@@ -348,9 +348,9 @@ __global__ __launch_bounds__(256) void gn_bwd_apply_any_kernel(GnBwdArgs a) {
 // threads takes a chunk: thread t holds the columns E (t % V) .. + E - 1 (V = C / E vectors a row) of the rows t / V, + T / V, ...,
 // with what it needs of its columns in registers.
 //
-// Statistics: a thread sums x - x0 and its square for each of its columns, x0 the column's first value of its own (at worst,
-// where x0 is the outlier that makes the variance, that costs a factor of the rows a thread takes, which is their
-// number and no more); the threads' sums are joined in 64 bits.
+// Statistics: a thread sums x - x0 and its square for each of its columns, x0 the column's first value of its own, and after 17, 65,
+// 257 and 1025 rows the mean of those (about the first value alone, an outlier there that makes the variance multiplies the sums' rounding
+// by the rows of a thread: of 2048 the variance was 8% off); the threads' sums are joined in 64 bits.
 // All of it is bound by memory: every pass reads x once (and dy), and one stores y or dx. One 2^20 x 128 image, fp16 (268 MB): sums 76 us (3.5
 // TB/s), join 5, store 85 (6.3 TB/s, part of x from the last-level cache). 2 x 16384 x 320 fp16 (21 MB): 8.4, 3.1 and 9.4 us, of which 2 are
 // the launch. Backward 2 x 4096 x 640 fp16 (10 MB a tensor): sums 9.8 us, dx and the weights' gradients 12.7.
@@ -446,8 +446,10 @@ struct Cols {
     }
 };
 
-// Grid: batch * nchunk. LDS: 3 floats a thread's column.
-template <typename TX>
+// Grid: batch * nchunk. LDS: 3 floats a thread's column. LONG: a thread may take more than kShort rows (the code for them costs 2 x 16384 x
+// 320 fp16, eleven rows a thread, 0.1 us of 21.8, 1024 x 1280 fp32 backward 0.2 of 21.7).
+constexpr uint32_t kShort = 1 + 4 * kRows;
+template <typename TX, bool LONG>
 __global__ __launch_bounds__(4096 / Vec<TX>::E) void gn_part_kernel(GnArgs a) {
     constexpr int E = Vec<TX>::E;
     typedef typename Vec<TX>::type VT;
@@ -466,6 +468,7 @@ __global__ __launch_bounds__(4096 / Vec<TX>::E) void gn_part_kernel(GnArgs a) {
 #pragma unroll
         for (int e = 0; e < E; ++e) x0[e] = static_cast<float>(v[e]) * kDown<TX>;
         // (a batch's rows past the chunk repeat its last row and add nothing: one by one they would cost a round trip each)
+        uint32_t batch = 0, next = 4;
         for (uint32_t r = ty + rows_at; r < rows; r += kRows * rows_at) {
             VT w[kRows];
 #pragma unroll
@@ -478,6 +481,19 @@ __global__ __launch_bounds__(4096 / Vec<TX>::E) void gn_part_kernel(GnArgs a) {
                     const float d = whole ? down<TX>(static_cast<float>(w[i][e]), x0[e]) : 0.0f;
                     s1[e] += d;
                     s2[e] = __builtin_fmaf(d, d, s2[e]);
+                }
+            }
+            // the sums so far, about their mean
+            if (LONG && ++batch == next && r + kRows * rows_at < rows) {
+                next *= 4;
+                const float k = static_cast<float>(1 + kRows * batch);
+#pragma unroll
+                for (int e = 0; e < E; ++e) {
+                    const float mean = x0[e] + s1[e] / k;
+                    const double t = static_cast<double>(mean) - static_cast<double>(x0[e]), u = static_cast<double>(s1[e]);
+                    s2[e] = static_cast<float>(static_cast<double>(s2[e]) + t * (k * t - 2.0 * u));
+                    s1[e] = static_cast<float>(u - k * t);
+                    x0[e] = mean;
                 }
             }
         }
@@ -512,10 +528,10 @@ __global__ __launch_bounds__(4096 / Vec<TX>::E) void gn_part_kernel(GnArgs a) {
         t1 = lanes_sum(t1, n);
         t2 = lanes_sum(t2, n);
         if (lane == 0 && g0 + tid / n < a.groups) {
-            const double total = static_cast<double>(rows) * a.cg, rest = t1 / total;
+            const double each = 1.0 / (static_cast<double>(rows) * a.cg), rest = t1 * each;
             a.part[static_cast<uint64_t>(blockIdx.x) * a.groups + g] =
                 Part{static_cast<float>(ref * kUp<TX>), static_cast<float>(rest * kUp<TX>),
-                     static_cast<float>(not_below_zero(t2 - t1 * rest) / total * (kUp<TX> * kUp<TX>)), 0.0f};
+                     static_cast<float>(not_below_zero(t2 - t1 * rest) * each * (kUp<TX> * kUp<TX>)), 0.0f};
         }
     }
 }
@@ -1246,7 +1262,9 @@ bool launch_stats(const GnArgs& a, bool fast, hipStream_t s) {
     if (fast) {
         constexpr uint32_t E = Vec<TX>::E;
         const uint32_t T = threads_for(a.C / E, 4096 / E), rows_at = T / (a.C / E);
-        gn_part_kernel<TX><<<a.batch * a.nchunk, T, 3 * rows_at * a.C * sizeof(float), s>>>(a);
+        const uint32_t lds = 3 * rows_at * a.C * sizeof(float);
+        if (a.chunk > kShort * rows_at) gn_part_kernel<TX, true><<<a.batch * a.nchunk, T, lds, s>>>(a);
+        else gn_part_kernel<TX, false><<<a.batch * a.nchunk, T, lds, s>>>(a);
         if (static_cast<uint64_t>(a.nchunk) * a.groups * a.batch * a.ncut <= kJoinParts) return false;
     } else {
         gn_part_any_kernel<TX><<<grid_of(static_cast<uint64_t>(a.batch) * a.nchunk * a.groups), 256, 0, s>>>(a);

@@ -3,6 +3,7 @@ cases that run on any backend with the C-ABI (the GPU, or the CPU emulator of te
 """
 from __future__ import annotations
 
+import ctypes
 from unittest import mock
 
 import numpy as np
@@ -10,6 +11,7 @@ import numpy as np
 import norm_i8_ref
 from bwd_ref import CODE, DT, SENTINEL, U, Arena, check, f64, rng_of
 from norm_i8_ref import codes_of
+from sdvk_amd._lib import MiGroupnormArgs
 
 F127, R127 = np.float32(127), np.float32(1) / np.float32(127)
 
@@ -143,12 +145,45 @@ def norm(be, *, pixels, **case):
         (norm_i8_ref.groupnorm_bwd if "dtyp" in case else norm_i8_ref.groupnorm)(be, **case)
 
 
-OPS = {"codes": codes, "norm": norm}
+def outliers(be, *, C, G, typ, B=256, P=2048, first=1, every=3, seed=13):
+    """The statistics of the first image of a batch whose images are a chunk each: a thread takes up to 2048 rows of its columns. The first
+    rows of every third column are 1000 times the others' spread and more. (Images overlap in x, a row apart; on the emulator the first alone runs.)"""
+    rng = rng_of(seed)
+    x = rng.standard_normal((P + B - 1, C)) * 0.01
+    size = 500.0 * 8 ** rng.random(G)
+    x[:first, ::every] = np.repeat(size, C // G)[::every]
+    x = x.astype(DT[typ])
+    A = Arena(be)
+    bx = A.put(x.reshape(-1))
+    emulated = hasattr(be, "E")
+    by = be.E.buf(nbytes=B * P * C * 2) if emulated else be.buf(np.zeros(B * P * C, np.float16))
+    bst = A.out(B * G * 4, np.float32)
+    need = be.value("mi_groupnorm_ws_bytes", B, P, C, G)
+    ws = be.buf(np.full(need, 0xff, np.uint8))
+    a = MiGroupnormArgs(bx.ptr, None, None, by.ptr, None, bst.ptr, B, P, C, G, CODE[typ], CODE["f16"], 0, 1e-5, C, C, C, P * C)
+    if emulated:
+        be.E.sample("gn_part_kernel|0|*|*;gn_apply_kernel|-1|*|*")
+    be.call("mi_groupnorm", ctypes.byref(a), ws.ptr, need, None)
+    if emulated:
+        be.E.sample("")
+    q = norm_i8_ref.Group(x[None, :P], G, 1e-5)
+    st = f64(be.get(bst, np.float32, G * 4)).reshape(G, 4)
+    # additions of up to 2048 squares to a sum that the outlier's makes up, and of 16 rows about the outlier itself (a sum 16 times as large)
+    e_var = (P + 16 * 16 + 40) * U * q.var.reshape(G)
+    e_mean = (P + 16 * 16 + 40) * U * np.sqrt(q.var.reshape(G))
+    inv = q.inv.reshape(G)
+    check(st[:, 0] + st[:, 1], q.mean.reshape(G), e_mean, "mean")
+    check(st[:, 2], inv, inv * (0.5 * e_var / (q.var.reshape(G) + 1e-5) + 4 * U), "inv")
+    A.unchanged()
+
+
+OPS = {"codes": codes, "norm": norm, "outliers": outliers}
 
 # what takes a group in registers (units of four and two values, whole and part full), chunks, and element by element
 NORM_SIZES = [dict(P=50, C=32, G=4), dict(P=256, C=64, G=1), dict(P=100, C=60, G=10, gap=2), dict(P=300, C=40, G=1), dict(P=600, C=320, G=32), dict(P=600, C=128, G=2), dict(P=300, C=33, G=1)]
 
 CASES = {
+    "outliers": [dict(C=2048, G=16, typ="f32"), dict(C=2048, G=32, typ="f16"), dict(C=2048, G=16, typ="f32", first=5), dict(C=1024, G=8, typ="f16", first=64, every=1)],
     "norm": [dict(pixels=k, **c) for k in ("signs", "range", "halves", "single") for c in NORM_SIZES]
     + [dict(pixels="signs", P=40, C=320, G=32, out="i8"), dict(pixels="halves", P=300, C=64, G=2, out="i8", act=1), dict(pixels="signs", P=30, C=33, G=3, out="i8"), dict(pixels="range", B=2, P=513, C=64, G=1, out="f16", act=1)]
     + [dict(pixels=k, dtyp="f32", act=a, **c) for k, a in (("signs", 0), ("halves", 1)) for c in NORM_SIZES],
