@@ -31,6 +31,7 @@ struct I8Args {
 };
 
 constexpr uint32_t kPast = 0x80000000u;  // a buffer offset past every record: the load returns zeros
+constexpr int kAll = 0x7fffffff;         // bytes of a resource that kPast alone is past
 
 // C from a sum: mode 0 stores, mode 1 adds, mode 2 adds with the bias (NULL for mode 1).
 __device__ __forceinline__ float result(int acc, float sa, float sw, float bias) {
@@ -130,7 +131,7 @@ __global__ __launch_bounds__(256) void gemm_i8_any_kernel(I8Args a) {
 // eight 16-byte slots in the order slot ^ (row / 2) % 8, so that the 16 rows that a fragment read takes at a time lie in
 // different banks; the loads' lanes permute their addresses accordingly (the 128 bytes of a row stay one segment).
 // The product is transposed (W is the MFMA's A operand): a lane holds one row m of C and runs of four columns.
-// Codes past K are zeros in both operands, rows past M or N are out of the resources' range.
+// Codes past K and rows past M or N are zeros: their lanes' offsets are out of the resources' range.
 // What bounds it: a CU is fed about 75 bytes a ns (128 x 128 and four stages 0.42 us a step, 256 x 320 1.38), so tiles as large as the
 // registers allow where there are enough of them: 256 x 320 reads 72 KB for 10.5 M products and has its MFMAs busy for 89% of a step
 // (2048x10240x1280: 1670 TOP/s over the call, whose first loads and 42 MB of C no product hides), 128 x 128 32 KB for 2.1 M.
@@ -160,9 +161,10 @@ __device__ __forceinline__ void barrier() {
     __atomic_signal_fence(__ATOMIC_SEQ_CST);
 }
 
-// 16 bytes a lane from `off` of the `bytes` at base (zeros past them) to LDS: lane l's to dst + 16 l.
-__device__ __forceinline__ void load_lds(const int8_t* base, int bytes, int8_t* dst, uint32_t off, int at = 0) {
-    const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(const_cast<int8_t*>(base), 0, bytes, 0x00020000);
+// 16 bytes a lane from base + off + at (zeros for off = kPast) to LDS: lane l's to dst + 16 l. The range check subtracts `at` from the
+// resource's bytes in 32 bits: those are more than any `at`, so that the difference cannot wrap.
+__device__ __forceinline__ void load_lds(const int8_t* base, int8_t* dst, uint32_t off, int at) {
+    const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(const_cast<int8_t*>(base), 0, kAll, 0x00020000);
     __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (__attribute__((address_space(3))) void*)(dst), 16, off, at, 0, 0);
 }
 
@@ -170,28 +172,28 @@ __device__ __forceinline__ void load_lds(const int8_t* base, int bytes, int8_t* 
 template <int IT>
 struct Rows {
     const int8_t* base;
-    int bytes;                    // that the rows span
     uint32_t off[IT], col[2], K;  // col: the lane's place in 128 codes, by the parity of its eight rows
     int at;                       // bytes into a stage
-    // rows r0 .. r0 + count - 1 of X at stride ld
+    // rows r0 .. r0 + count - 1 of X at stride ld; further ones are zeros
     __device__ __forceinline__ Rows(const int8_t* X, uint64_t ld, uint32_t r0, uint32_t count, uint32_t K_, int wave, int lane) : K(K_) {
         base = X + r0 * ld;
-        bytes = static_cast<int>((count - 1) * ld + K);
         at = wave * IT * 1024;
 #pragma unroll
         for (int i = 0; i < 2; ++i) col[i] = ((lane & 7) ^ swz(8 * (wave * IT + i) + (lane >> 3))) * 16;
 #pragma unroll
-        for (int i = 0; i < IT; ++i) off[i] = (8 * (wave * IT + i) + (lane >> 3)) * static_cast<uint32_t>(ld) + col[i & 1];
+        for (int i = 0; i < IT; ++i) {
+            const uint32_t r = 8 * (wave * IT + i) + (lane >> 3);
+            off[i] = r < count ? r * static_cast<uint32_t>(ld) + col[i & 1] : kPast;
+        }
     }
-    // (steps in turn: a lane whose codes are past K once stays there. The scalar offset stays within K, so within `bytes`: the range
-    // check subtracts it from them in 32 bits, and a larger one would wrap and let kPast through)
+    // (steps in turn: a lane whose codes are past K once stays there)
     __device__ __forceinline__ void load(int8_t* stage, uint32_t k0) {
         if (k0 + 128 > K) {
 #pragma unroll
             for (int i = 0; i < IT; ++i) off[i] = k0 + col[i & 1] < K ? off[i] : kPast;
         }
 #pragma unroll
-        for (int i = 0; i < IT; ++i) load_lds(base, bytes, stage + at + i * 1024, off[i], static_cast<int>(min(k0, K)));
+        for (int i = 0; i < IT; ++i) load_lds(base, stage + at + i * 1024, off[i], static_cast<int>(k0));
     }
 };
 
