@@ -177,7 +177,7 @@ def outliers(be, *, C, G, typ, B=256, P=2048, first=1, every=3, seed=13):
     A.unchanged()
 
 
-OPS = {"codes": codes, "norm": norm, "outliers": outliers}
+OPS = {"codes": codes, "norm": norm, "outliers": outliers, "strided": lambda be, *, op, **case: norm_i8_ref.OPS[op](be, **case)}
 
 # what takes a group in registers (units of four and two values, whole and part full), chunks, and element by element
 NORM_SIZES = [dict(P=50, C=32, G=4), dict(P=256, C=64, G=1), dict(P=100, C=60, G=10, gap=2), dict(P=300, C=40, G=1), dict(P=600, C=320, G=32), dict(P=600, C=128, G=2), dict(P=300, C=33, G=1)]
@@ -191,6 +191,9 @@ CASES = {
               dict(rows=40, cols=64, kind="half"), dict(rows=9, cols=75, kind="half"), dict(rows=5, cols=2048, kind="half")],
 }
 GPU_CASES = {
+    # more than 2^20 units of the kernels that stride
+    "strided": [dict(op="groupnorm", B=32769, P=1, C=96, G=32, gap=1), dict(op="groupnorm", P=4194305, C=3, G=1), dict(op="groupnorm_bwd", B=32769, P=1, C=96, G=32, gap=1, act=1),
+                dict(op="groupnorm_bwd", P=4194305, C=3, G=1), dict(op="quantize", rows=4194305, cols=3), dict(op="product", M=(1 << 26) + 1, N=1, K=1)],
     # chunks of 2048 rows; a workgroup's registers full
     "norm": [dict(pixels=k, **c) for k in ("signs", "halves") for c in (dict(B=256, P=2048, C=64, G=2), dict(P=20000, C=256, G=2, act=1), dict(P=1024, C=1280, G=32, out="i8"), dict(P=32768, C=4, G=4))]
     + [dict(pixels="signs", P=1024, C=1280, G=32, dtyp="f32"), dict(pixels="halves", B=256, P=2048, C=64, G=2, dtyp="f32")],

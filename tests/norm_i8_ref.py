@@ -466,7 +466,7 @@ CASES = {
         dict(M=257, N=321, K=400, cfg="7", extreme=True), dict(M=260, N=328, K=272, cfg="7", out="f16", mode=2),
     ],
 }
-# Larger shapes, on the GPU alone: grids that stride, many chunks, tails.
+# Larger shapes, on the GPU alone: many chunks, tails.
 GPU_CASES = {
     "groupnorm": [
         dict(B=2, P=4096, C=640, G=32, typ="f16", out="f16", act=1), dict(P=16385, C=320, G=32, act=1), dict(P=65536, C=128, G=32, typ="f16", out="f16", act=1), dict(B=2, P=1024, C=2560, G=32, typ="f16", out="f16", act=1),

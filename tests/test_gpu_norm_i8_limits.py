@@ -16,7 +16,7 @@ def backend(gpu):
     return Backend(gpu)
 
 
-ALL = [(op, c) for op in norm_i8_limits.CASES for c in norm_i8_limits.CASES[op] + norm_i8_limits.GPU_CASES.get(op, [])]
+ALL = [(op, c) for op in norm_i8_limits.OPS for c in norm_i8_limits.CASES.get(op, []) + norm_i8_limits.GPU_CASES.get(op, [])]
 
 
 @pytest.mark.parametrize("op,case", ALL, ids=[f"{op}-{json.dumps(c)}" for op, c in ALL])
