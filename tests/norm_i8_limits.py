@@ -132,6 +132,8 @@ def pixels_of(kind):
             x[:, ::2] = -9.99e17
             x[:, 0] = -9.99e17
             return x
+        if kind == "ratio":  # a mean 1e5 times the spread
+            return 1000 + 0.01 * rng.standard_normal((B, P, C))
         assert kind == "single"  # one value of a group
         x = np.zeros((B, P, C))
         x[:, 0, ::7] = 9.99e17
@@ -186,7 +188,8 @@ CASES = {
     "outliers": [dict(C=2048, G=16, typ="f32"), dict(C=2048, G=32, typ="f16"), dict(C=2048, G=16, typ="f32", first=5), dict(C=1024, G=8, typ="f16", first=64, every=1)],
     "norm": [dict(pixels=k, **c) for k in ("signs", "range", "halves", "single") for c in NORM_SIZES]
     + [dict(pixels="signs", P=40, C=320, G=32, out="i8"), dict(pixels="halves", P=300, C=64, G=2, out="i8", act=1), dict(pixels="signs", P=30, C=33, G=3, out="i8"), dict(pixels="range", B=2, P=513, C=64, G=1, out="f16", act=1)]
-    + [dict(pixels=k, dtyp="f32", act=a, **c) for k, a in (("signs", 0), ("halves", 1)) for c in NORM_SIZES],
+    + [dict(pixels=k, dtyp="f32", act=a, **c) for k, a in (("signs", 0), ("halves", 1)) for c in NORM_SIZES]
+    + [dict(pixels="ratio", **o, **c) for o in (dict(act=1), dict(dtyp="f32")) for c in NORM_SIZES] + [dict(pixels="ratio", P=300, C=64, G=8, out="i8"), dict(pixels="ratio", P=50, C=64, G=8, out="i8", act=1)],
     "codes": [dict(rows=9, cols=64, kind="reciprocal"), dict(rows=20, cols=77, kind="reciprocal"), dict(rows=5, cols=2048, kind="reciprocal"), dict(rows=3, cols=1280, kind="reciprocal", typ="f16"),
               dict(rows=40, cols=64, kind="half"), dict(rows=9, cols=75, kind="half"), dict(rows=5, cols=2048, kind="half")],
 }
@@ -196,6 +199,7 @@ GPU_CASES = {
                 dict(op="groupnorm_bwd", P=4194305, C=3, G=1), dict(op="quantize", rows=4194305, cols=3), dict(op="product", M=(1 << 26) + 1, N=1, K=1)],
     # chunks of 2048 rows; a workgroup's registers full
     "norm": [dict(pixels=k, **c) for k in ("signs", "halves") for c in (dict(B=256, P=2048, C=64, G=2), dict(P=20000, C=256, G=2, act=1), dict(P=1024, C=1280, G=32, out="i8"), dict(P=32768, C=4, G=4))]
+    + [dict(pixels="ratio", P=20000, C=256, G=32), dict(pixels="ratio", P=1024, C=1280, G=32, dtyp="f32", act=1)]
     + [dict(pixels="signs", P=1024, C=1280, G=32, dtyp="f32"), dict(pixels="halves", B=256, P=2048, C=64, G=2, dtyp="f32")],
     "codes": [dict(rows=154, cols=2048, kind="reciprocal", N=1280), dict(rows=16, cols=5120, kind="reciprocal", typ="f16", N=640), dict(rows=300, cols=1280, kind="half")],
 }
