@@ -78,7 +78,7 @@ __device__ __forceinline__ void store_run(const I8Args& a, uint32_t m, uint32_t 
 }
 
 // Any K, any alignment: a 64 x 64 tile in steps of 32 codes, 4 x 4 outputs a thread, four products an instruction; bound by its
-// byte loads: 2048x10240x1280 493 us, tiles 32.
+// byte loads: 2048x10240x1280 489 us, tiles 32; 154x1280x2048 154, waves that split K 5.
 template <typename TC>
 __global__ __launch_bounds__(256) void gemm_i8_any_kernel(I8Args a) {
     __shared__ __attribute__((aligned(4))) int8_t at[64][36], wt[64][36];
@@ -132,9 +132,11 @@ __global__ __launch_bounds__(256) void gemm_i8_any_kernel(I8Args a) {
 // different banks; the loads' lanes permute their addresses accordingly (the 128 bytes of a row stay one segment).
 // The product is transposed (W is the MFMA's A operand): a lane holds one row m of C and runs of four columns.
 // Codes past K and rows past M or N are zeros: their lanes' offsets are out of the resources' range.
-// What bounds it: a CU is fed about 75 bytes a ns (128 x 128 and four stages 0.42 us a step, 256 x 320 1.38), so tiles as large as the
-// registers allow where there are enough of them: 256 x 320 reads 72 KB for 10.5 M products and has its MFMAs busy for 89% of a step
-// (2048x10240x1280: 1670 TOP/s over the call, whose first loads and 42 MB of C no product hides), 128 x 128 32 KB for 2.1 M.
+// What bounds it: a CU is fed about 75 bytes a ns (128 x 128 and four stages 0.42 us a step), so tiles as large as the registers allow where
+// there are enough of them: 256 x 320 reads 72 KB for 10.5 M products, 128 x 128 32 KB for 2.1 M. 2048x10240x1280 fp16 (256 x 320, a tile a
+// CU, 1670 TOP/s over the call) takes 15.2 us with K = 128, 31.7 with 1280, 51.2 with 2560: a step is 1.95 us in a long run (its MFMAs at
+// 80% of their rate at the 1.67 GHz that the card then holds), and some 12 us are the launch, the first loads and 42 MB of C that all CUs
+// store at once, with no product beside them.
 typedef int intx4 __attribute__((ext_vector_type(4)));
 typedef int intx16 __attribute__((ext_vector_type(16)));
 
@@ -485,7 +487,7 @@ __global__ __launch_bounds__(512) void gemm_i8_split_kernel(I8Args a) {
 //
 // Up to 16 rows (single tokens): a workgroup takes 16 columns and its eight waves the 256-code pieces of K in turn, the
 // weights straight from memory into MFMA operands (16 rows x 64 bytes an instruction); the sums are added through LDS. 2x1280x1280 3.0 us
-// (an empty launch 2.0 by the same clock).
+// (an empty launch 2.0 by the same clock); K below 2048 leaves waves idle (1280 three of the eight).
 constexpr uint32_t kFewRows = 16;
 
 template <typename TC>
@@ -605,10 +607,16 @@ uint64_t span(uint64_t rows, uint64_t ld, uint64_t cols) { return rows ? (rows -
 // Builds: 0 any shape, 1 few rows, 2 waves split K (32 x 32), the others tiles: 8 is 3 with three stages, 5 is 4 with four (and eight
 // waves: one workgroup a CU, whose loads alone have to hide their latency).
 //
-// us of a tile build = 3 + n (tile + steps step), n tiles on the fullest of 256 CUs, fitted to a sweep (MI355X, fp16 C, us of builds 3, 8, 4, 5, 6, 7):
-//   576x1280x1280     6.7   5.7   8.9   6.9  15.3  24.8      2048x1280x1280   8.8   9.7  10.7   9.2  16.1  25.8
-//   2048x1280x5120   25.6  26.7  30.9  21.8  45.9  69.9      8192x640x2560   26.7  24.3  21.3  25.9  27.3  41.2
-//   8192x640x640     10.0  10.7   9.5  12.4  11.9  18.7      2048x10240x1280 47.6  51.7  36.8  43.3  35.8  32.3
+// The cost of a tile build, n tiles on the fullest of 256 CUs: 3 + n (tile + steps step). It is there to rank builds: what a call's C
+// costs beyond its tiles' share is the same for all and is not in it, nor is C's type, nor the lower clock of long runs of products.
+// us (MI355X, fp16 C) of builds 3, 8, 4, 5, 6, 7, and by the cost where a rule does not keep the build out:
+//   576x1280x1280     5.3  5.3  8.7  7.9 15.0 24.4   (5.5  4.7   -   9.2 15.8 24.5)
+//   2048x1280x1280    8.3  9.2  9.4  8.7 15.6 24.9   (9.1   -    -   9.2 15.8 24.5)
+//   2048x1280x5120   24.9 25.7 30.1 21.5 45.5 67.0  (25.6   -    -  21.9 44.0 65.9)
+//   8192x640x2560    25.3 23.7 20.8 24.4 27.0 40.2  (27.0   -  22.2 23.9 25.2 38.3)
+//   8192x640x640      9.4  9.9  9.3 12.0 11.6 18.8   (9.8   -   9.6 11.3 11.1 17.6)
+//   2048x10240x1280  48.3 49.9 35.2 40.3 35.2 32.3  (53.0   -  30.0 34.2 28.6 24.5)
+// The fastest is chosen in each, and so it is with fp32 C (2048x1280x5120 21.7, 8192x640x2560 22.2, 2048x10240x1280 35.7: 4 us more for C).
 // (128 x 128 with two groups of waves that take the steps in turn: 24.8 for 2048x1280x5120; 128 x 80 in 256 workgroups of four waves of 64 x 80,
 // half of each step's codes each, with the next step's fragments read ahead: 21.8; 256 x 256, 256 x 128, 128 x 64, 128 x 192 and
 // 64 x 128 tiles were between their neighbours.)
@@ -638,6 +646,8 @@ int choose(const I8Args& a) {
         const uint64_t n = (tiles(b) + 255) / 256;
         if (b == k64x3 && n > 2) continue;  // three workgroups a CU; with more tiles four are faster
         if (b == k128 && n < 2) continue;   // two workgroups a CU hide each other's latency; one needs four stages
+        // (three of its four places on a CU taken: 0.19 us a tile and step with 40 steps, 0.16 with 10, where two take 0.23 and 0.14, four 0.20
+        // and 0.18, six 0.21 and 0.20; 2048x1280x1280 has three)
         const float step = b == k64 && n == 3 ? 0.183f : kBuilds[b].step_us;
         const float us = static_cast<float>(n) * (kBuilds[b].tile_us + ceil_div(a.K, 128) * step);
         if (best == kAny || us < least) {

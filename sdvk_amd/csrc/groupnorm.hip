@@ -23,9 +23,12 @@ namespace {
 constexpr uint32_t kMaxGrid = 1u << 20;   // workgroups of a launch that strides over its units
 constexpr uint32_t kChunkValues = 16384;  // values of a chunk, at least (but for the last), and ...
 constexpr uint32_t kChunkMax = 2048;      // ... rows at most: the longest chain of fp32 additions
-constexpr uint32_t kChunks = 256;         // chunks of all images, about: a workgroup per CU
+constexpr uint32_t kChunks = 256;         // chunks of all images, about: a workgroup per CU (images of 4 M values and more; kChunkValues
+                                          // binds the others: 576 x 1280 has 45 chunks)
 // Parts (of 16 bytes) that all workgroups together read where each joins an image's statistics by itself; more are joined by a launch of
-// its own. us by themselves / by a launch: 2 x 16384 x 320 (2^21 parts) 23.2 / 21.8, 2 x 1024 x 2560 18.5 / 16.6, 576 x 1280 in 8 bits (2^19) 20.0 / 20.9.
+// its own. us of a call by themselves / by a launch: 576 x 1280 in 8 bits (2^16.9 parts) 13.2 / 14.6, 2304 x 640 in 8 bits (2^18.95) 12.9 /
+// 14.8, 2 x 1024 x 1280 in 8 bits (2^19.5) 19.6 / 19.0, 1024 x 2560 fp16 (2^20.2) 14.2 / 14.9, 4096 x 640 fp32 (2^20.6) 16.9 / 15.6,
+// 2 x 16384 x 320 fp16 (2^21) 23.3 / 22.5, 16384 x 320 fp16 (2^22) 21.3 / 17.8: equal somewhere from 2^19.5 to 2^20.5.
 constexpr uint64_t kJoinParts = 1u << 19;
 
 struct Stat {  // of one group of one image, 16 bytes: what `stats` holds
@@ -112,7 +115,8 @@ __device__ __forceinline__ float slope(float z) {
 
 // ---- any shape and alignment -------------------------------------------------------
 //
-// Element by element, four or five launches; bound by the loads' latency (2 x 4096 x 640 fp16 backward 202 us, by vectors 23).
+// Element by element, four or five launches; bound by the loads' latency (2 x 4096 x 640 fp16 backward with the statistics 110 us, by
+// vectors 33).
 
 // One group of one chunk per workgroup; two passes over its values, sums in 64 bits.
 template <typename TX>
@@ -351,9 +355,9 @@ __global__ __launch_bounds__(256) void gn_bwd_apply_any_kernel(GnBwdArgs a) {
 // Statistics: a thread sums x - x0 and its square for each of its columns, x0 the column's first value of its own, and after 17, 65,
 // 257 and 1025 rows the mean of those (about the first value alone, an outlier there that makes the variance multiplies the sums' rounding
 // by the rows of a thread: of 2048 the variance was 8% off); the threads' sums are joined in 64 bits.
-// All of it is bound by memory: every pass reads x once (and dy), and one stores y or dx. One 2^20 x 128 image, fp16 (268 MB): sums 76 us (3.5
-// TB/s), join 5, store 85 (6.3 TB/s, part of x from the last-level cache). 2 x 16384 x 320 fp16 (21 MB): 8.4, 3.1 and 9.4 us, of which 2 are
-// the launch. Backward 2 x 4096 x 640 fp16 (10 MB a tensor): sums 9.8 us, dx and the weights' gradients 12.7.
+// All of it is bound by memory: every pass reads x once (and dy), and one stores y or dx. One 2^20 x 128 image, fp16 (268 MB): sums 75 us (3.6
+// TB/s), join 5, store 85 (6.3 TB/s, part of x from the last-level cache). 2 x 16384 x 320 fp16 (21 MB): 9.5, 3.3 and 9.0 us, of which 2 are
+// the launch. Backward 2 x 4096 x 640 fp16 (10 MB a tensor): sums 10.0 us, dx and the weights' gradients 13.0.
 constexpr uint32_t kFastChannels = 4096, kFastGroups = 256;
 constexpr int kRows = 4;  // rows a thread has in flight
 
@@ -580,7 +584,7 @@ __global__ __launch_bounds__(4096 / Vec<TX>::E) void gn_apply_kernel(GnArgs a) {
 }
 
 // 8-bit rows: a wave takes two rows at a time, four columns (lane + 64 i) each, so that a row's largest value is the wave's. Grid: batch *
-// ncut, T threads. 2 x 4096 x 640 fp16 6.5 us (16 MB), bound by the instructions of the quantiser and of the statistics' use.
+// ncut, T threads. 2 x 4096 x 640 fp16 7.1 us (16 MB), bound by the instructions of the quantiser and of the statistics' use.
 template <typename TX, int ACT, int NV, int T>
 __global__ __launch_bounds__(T) void gn_apply_i8_kernel(GnArgs a) {
     typedef TX VT __attribute__((ext_vector_type(4)));
