@@ -39,7 +39,7 @@ def few(emulator, tmp_path_factory):  # noqa: F811
         yield
 
 
-@pytest.mark.parametrize("op", list(norm_i8_ref.CASES))
+@pytest.mark.parametrize("op", ["groupnorm", "groupnorm_bwd", "quantize", "product"])
 def test_strided_on_emulator(few, op):
     check([dict(op=op, orders=ORDERS, **c) for c in norm_i8_ref.CASES[op]])
 
