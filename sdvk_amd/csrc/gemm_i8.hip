@@ -33,13 +33,17 @@ struct I8Args {
 constexpr uint32_t kPast = 0x80000000u;  // a buffer offset past every record: the load returns zeros
 constexpr int kAll = 0x7fffffff;         // bytes of a resource that kPast alone is past
 
-// C from a sum: mode 0 stores, mode 1 adds, mode 2 adds with the bias (NULL for mode 1).
+// C from a sum: mode 0 stores, mode 1 adds, mode 2 adds with the bias (NULL for mode 1). An fp32 number also where fp16 is stored: as one
+// instruction with that rounding, which the compiler would make of some results and not of others, one in 10^5 had other bits.
+template <typename TC>
 __device__ __forceinline__ float result(int acc, float sa, float sw, float bias) {
-    return __builtin_fmaf(static_cast<float>(acc) * sa, sw, bias);
+    float r = __builtin_fmaf(static_cast<float>(acc) * sa, sw, bias);
+    if constexpr (sizeof(TC) == 2) asm volatile("" : "+v"(r));
+    return r;
 }
 template <typename TC>
 __device__ __forceinline__ void store_one(const I8Args& a, uint32_t m, uint32_t n, int acc, float sa) {
-    float v = result(acc, sa, a.sw[n], a.bias ? a.bias[n] : 0.0f);
+    float v = result<TC>(acc, sa, a.sw[n], a.bias ? a.bias[n] : 0.0f);
     TC* p = static_cast<TC*>(a.C) + m * a.ldc + n;
     if (a.mode) v += static_cast<float>(*p);
     *p = static_cast<TC>(v);
@@ -60,10 +64,10 @@ __device__ __forceinline__ void store_run(const I8Args& a, uint32_t m, uint32_t 
         if (a.mode) {
             const Run old = *reinterpret_cast<const Run*>(p);
 #pragma unroll
-            for (int e = 0; e < V; ++e) r[e] = static_cast<TC>(result(acc[e], sa, c.sw[e], c.bias[e]) + static_cast<float>(old[e]));
+            for (int e = 0; e < V; ++e) r[e] = static_cast<TC>(result<TC>(acc[e], sa, c.sw[e], c.bias[e]) + static_cast<float>(old[e]));
         } else {
 #pragma unroll
-            for (int e = 0; e < V; ++e) r[e] = static_cast<TC>(result(acc[e], sa, c.sw[e], c.bias[e]));
+            for (int e = 0; e < V; ++e) r[e] = static_cast<TC>(result<TC>(acc[e], sa, c.sw[e], c.bias[e]));
         }
         *reinterpret_cast<Run*>(p) = r;
         return;
@@ -71,7 +75,7 @@ __device__ __forceinline__ void store_run(const I8Args& a, uint32_t m, uint32_t 
 #pragma unroll
     for (int e = 0; e < V; ++e)
         if (n + e < a.N) {
-            float v = result(acc[e], sa, c.sw[e], c.bias[e]);
+            float v = result<TC>(acc[e], sa, c.sw[e], c.bias[e]);
             if (a.mode) v += static_cast<float>(p[e]);
             p[e] = static_cast<TC>(v);
         }

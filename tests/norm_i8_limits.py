@@ -179,12 +179,38 @@ def outliers(be, *, C, G, typ, B=256, P=2048, first=1, every=3, seed=13):
     A.unchanged()
 
 
-OPS = {"codes": codes, "norm": norm, "outliers": outliers, "strided": lambda be, *, op, **case: norm_i8_ref.OPS[op](be, **case)}
+def builds(be, *, M, N, K, out, mode=0, seed=14):
+    """Every build of the product, storing whole runs or element by element, gives the same bits."""
+    rng = rng_of(seed)
+    a, w = (rng.integers(-127, 128, (r, K)).astype(np.int8) for r in (M, N))
+    sa, sw = (rng.uniform(0.5, 2, M) / 128).astype(np.float32), (rng.uniform(0.5, 2, N) / 256).astype(np.float32)
+    bias, dt = rng.standard_normal(N).astype(np.float32), DT[out]
+    old = rng.standard_normal((M, N)).astype(dt)
+    A = Arena(be)
+    ba, bw, bsa, bsw, bb = (A.put(np.ascontiguousarray(t).reshape(-1)) for t in (a, w, sa, sw, bias))
+    first = None
+    for cfg in ("0", "2", "3", "4", "5", "6", "7", "8", None):
+        for ldc in (N, N + 1):
+            c = np.zeros((M, ldc), dt)
+            c[:, :N] = old
+            bc = A.out(0, dt, c.reshape(-1))
+            be.tune("gemm_i8_cfg", cfg)
+            be.call("mi_gemm_nt_i8", ba.ptr, bsa.ptr, bw.ptr, bsw.ptr, bb.ptr, bc.ptr, CODE[out], M, N, K, mode, 0, 0, ldc, None)
+            be.tune("gemm_i8_cfg", None)
+            got = be.get(bc, dt, M * ldc).reshape(M, ldc)[:, :N]
+            first = got if first is None else first
+            bad = np.argwhere(got != first)
+            assert not len(bad), (cfg, ldc, len(bad), [(tuple(map(int, i)), got[tuple(i)], first[tuple(i)]) for i in bad[:3]])
+    A.unchanged()
+
+
+OPS = {"codes": codes, "builds": builds, "norm": norm, "outliers": outliers, "strided": lambda be, *, op, **case: norm_i8_ref.OPS[op](be, **case)}
 
 # what takes a group in registers (units of four and two values, whole and part full), chunks, and element by element
 NORM_SIZES = [dict(P=50, C=32, G=4), dict(P=256, C=64, G=1), dict(P=100, C=60, G=10, gap=2), dict(P=300, C=40, G=1), dict(P=600, C=320, G=32), dict(P=600, C=128, G=2), dict(P=300, C=33, G=1)]
 
 CASES = {
+    "builds": [dict(M=70, N=64, K=48, out="f16"), dict(M=70, N=64, K=48, out="f16", mode=2), dict(M=33, N=136, K=16, out="f32")],
     "outliers": [dict(C=2048, G=16, typ="f32"), dict(C=2048, G=32, typ="f16"), dict(C=2048, G=16, typ="f32", first=5), dict(C=1024, G=8, typ="f16", first=64, every=1)],
     "norm": [dict(pixels=k, **c) for k in ("signs", "range", "halves", "single") for c in NORM_SIZES]
     + [dict(pixels="signs", P=40, C=320, G=32, out="i8"), dict(pixels="halves", P=300, C=64, G=2, out="i8", act=1), dict(pixels="signs", P=30, C=33, G=3, out="i8"), dict(pixels="range", B=2, P=513, C=64, G=1, out="f16", act=1)]
@@ -194,6 +220,7 @@ CASES = {
               dict(rows=40, cols=64, kind="half"), dict(rows=9, cols=75, kind="half"), dict(rows=5, cols=2048, kind="half")],
 }
 GPU_CASES = {
+    "builds": [dict(M=1024, N=1000, K=64, out="f16"), dict(M=1024, N=1000, K=64, out="f16", mode=2), dict(M=1024, N=1000, K=64, out="f16", mode=1), dict(M=1024, N=1000, K=64, out="f32", mode=2)],
     # more than 2^20 units of the kernels that stride
     "strided": [dict(op="groupnorm", B=32769, P=1, C=96, G=32, gap=1), dict(op="groupnorm", P=4194305, C=3, G=1), dict(op="groupnorm_bwd", B=32769, P=1, C=96, G=32, gap=1, act=1),
                 dict(op="groupnorm_bwd", P=4194305, C=3, G=1), dict(op="quantize", rows=4194305, cols=3), dict(op="product", M=(1 << 26) + 1, N=1, K=1)],
