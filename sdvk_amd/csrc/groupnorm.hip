@@ -9,9 +9,9 @@
 //
 // Statistics: an image's rows are cut into chunks. A chunk's sums are taken about a shift, the mean of some of its own values,
 // so that neither a large common mean nor an outlier cancels the variance (the shift lies within sqrt(n / m) standard
-// deviations of the chunk's mean, m the values that made it); the chunks' means and squared deviations are then joined in
-// 64 bits. A mean is held as two floats: with the first alone x - m would be off by 2^-24 m, which a large mean over a
-// small spread shows.
+// deviations of the chunk's mean, m the values that made it); the chunks' means and variances are then joined in 64 bits.
+// A mean is held as two floats, a chunk's and a group's: with the first alone x - m would be off by 2^-24 m, which a large mean over
+// a small spread shows.
 #include "common.hpp"
 #include "quant.hpp"
 
@@ -34,9 +34,13 @@ constexpr uint64_t kJoinParts = 1u << 19;
 struct Stat {  // of one group of one image, 16 bytes: what `stats` holds
     float mean, low, inv, zero;
 };
-struct Part {  // of one group of one chunk: mean = shift + rest, var = mean of (x - mean)^2 (their sum could pass fp32's range)
-    float shift, rest, var, zero;
+struct Part {  // of one group of one chunk: its mean as two floats, var = mean of (x - mean)^2 (their sum could pass fp32's range)
+    float mean, low, var, zero;
 };
+__device__ __forceinline__ Part part_of(double mean, double var) {
+    const float hi = static_cast<float>(mean);
+    return Part{hi, static_cast<float>(mean - static_cast<double>(hi)), static_cast<float>(var), 0.0f};
+}
 
 // Squares are summed in fp32, of differences times a power of two: fp32 values below 1e18 differ by 2e18 at most, and the longest sums
 // are 2048 of a column and 4096 of a wave's lanes, 4096 (2e18 / 16)^2 = 6.4e37 in all. (fp16 values stay below 2^17.)
@@ -161,7 +165,7 @@ __global__ __launch_bounds__(256) void gn_part_any_kernel(GnArgs a) {
             d1 = (red[1][0] + red[1][1]) + (red[1][2] + red[1][3]);
             d2 = (red[2][0] + red[2][1]) + (red[2][2] + red[2][3]);
             const double rest = d1 / static_cast<double>(n);
-            a.part[bc * a.groups + g] = Part{shift, static_cast<float>(rest), static_cast<float>(not_below_zero(d2 - d1 * rest) / static_cast<double>(n)), 0.0f};
+            a.part[bc * a.groups + g] = part_of(static_cast<double>(shift) + rest, not_below_zero(d2 - d1 * rest) / static_cast<double>(n));
         }
         __syncthreads();  // the sums are free for the next unit
     }
@@ -181,7 +185,7 @@ __device__ __forceinline__ void join(const GnArgs& a, const Part* p, uint32_t fi
             const uint32_t c = c0 + i * n;
             if (c < a.nchunk) {
                 const double k = static_cast<double>(min(a.chunk, a.pixels - c * a.chunk)) * a.cg;
-                const double d = (static_cast<double>(q[i].shift) - ref) + static_cast<double>(q[i].rest);
+                const double d = (static_cast<double>(q[i].mean) - ref) + static_cast<double>(q[i].low);
                 s1 += k * d;
                 s2 += k * (static_cast<double>(q[i].var) + d * d);
             }
@@ -202,7 +206,7 @@ __global__ __launch_bounds__(256) void gn_join_kernel(GnArgs a) {
     for (uint64_t u = blockIdx.x * 4ull + (threadIdx.x >> 6); u < units; u += gridDim.x * 4ull) {
         const Part* p = a.part + u / a.groups * a.nchunk * a.groups + u % a.groups;
         const Part first = p[0];
-        const double ref = static_cast<double>(first.shift) + static_cast<double>(first.rest);
+        const double ref = static_cast<double>(first.mean) + static_cast<double>(first.low);
         double s1, s2;
         join(a, p, lane, 64, ref, s1, s2);
         s1 = wave_sum(s1);
@@ -398,7 +402,7 @@ __device__ __forceinline__ void image_stats(const GnArgs& a, uint64_t b, Stat* s
         const uint32_t g = min(g0 + tid / n, a.groups - 1);
         const Part* p = a.part + b * a.nchunk * a.groups + g;
         const Part first = p[0];
-        const double ref = static_cast<double>(first.shift) + static_cast<double>(first.rest);
+        const double ref = static_cast<double>(first.mean) + static_cast<double>(first.low);
         double s1, s2;
         join(a, p, lane, n, ref, s1, s2);
         s1 = lanes_sum(s1, n);
@@ -534,8 +538,7 @@ __global__ __launch_bounds__(4096 / Vec<TX>::E) void gn_part_kernel(GnArgs a) {
         if (lane == 0 && g0 + tid / n < a.groups) {
             const double each = 1.0 / (static_cast<double>(rows) * a.cg), rest = t1 * each;
             a.part[static_cast<uint64_t>(blockIdx.x) * a.groups + g] =
-                Part{static_cast<float>(ref * kUp<TX>), static_cast<float>(rest * kUp<TX>),
-                     static_cast<float>(not_below_zero(t2 - t1 * rest) * each * (kUp<TX> * kUp<TX>)), 0.0f};
+                part_of((static_cast<double>(ref) + rest) * kUp<TX>, not_below_zero(t2 - t1 * rest) * each * (kUp<TX> * kUp<TX>));
         }
     }
 }

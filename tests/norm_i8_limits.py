@@ -204,12 +204,19 @@ def builds(be, *, M, N, K, out, mode=0, seed=14):
     A.unchanged()
 
 
-OPS = {"codes": codes, "builds": builds, "norm": norm, "outliers": outliers, "strided": lambda be, *, op, **case: norm_i8_ref.OPS[op](be, **case)}
+def plain(be, *, of, **case):
+    norm_i8_ref.OPS[of](be, **case)
+
+
+OPS = {"codes": codes, "builds": builds, "norm": norm, "outliers": outliers, "plain": plain, "strided": plain}
 
 # what takes a group in registers (units of four and two values, whole and part full), chunks, and element by element
 NORM_SIZES = [dict(P=50, C=32, G=4), dict(P=256, C=64, G=1), dict(P=100, C=60, G=10, gap=2), dict(P=300, C=40, G=1), dict(P=600, C=320, G=32), dict(P=600, C=128, G=2), dict(P=300, C=33, G=1)]
 
 CASES = {
+    # a chunk's first value far from its mean, which many values make
+    "plain": [dict(of="groupnorm", B=9, P=3, C=4096, G=1, offset=-20.0, outlier=300.0), dict(of="groupnorm", B=9, P=4, C=4096, G=1, outlier=5000.0, out="f16"), dict(of="groupnorm", B=2, P=14, C=2048, G=2, offset=-20.0, outlier=1000.0), dict(of="groupnorm", P=250, C=128, G=1, offset=3.0, outlier=3e4),
+              dict(of="groupnorm", P=60, C=4096, G=1, offset=-20.0, outlier=300.0, out="f16"), dict(of="groupnorm", P=700, C=33, G=1, offset=-20.0, outlier=300.0), dict(of="groupnorm_bwd", P=3, C=4096, G=1, offset=-20.0)],
     "builds": [dict(M=70, N=64, K=48, out="f16"), dict(M=70, N=64, K=48, out="f16", mode=2), dict(M=33, N=136, K=16, out="f32")],
     "outliers": [dict(C=2048, G=16, typ="f32"), dict(C=2048, G=32, typ="f16"), dict(C=2048, G=16, typ="f32", first=5), dict(C=1024, G=8, typ="f16", first=64, every=1)],
     "norm": [dict(pixels=k, **c) for k in ("signs", "range", "halves", "single") for c in NORM_SIZES]
@@ -222,8 +229,8 @@ CASES = {
 GPU_CASES = {
     "builds": [dict(M=1024, N=1000, K=64, out="f16"), dict(M=1024, N=1000, K=64, out="f16", mode=2), dict(M=1024, N=1000, K=64, out="f16", mode=1), dict(M=1024, N=1000, K=64, out="f32", mode=2)],
     # more than 2^20 units of the kernels that stride
-    "strided": [dict(op="groupnorm", B=32769, P=1, C=96, G=32, gap=1), dict(op="groupnorm", P=4194305, C=3, G=1), dict(op="groupnorm_bwd", B=32769, P=1, C=96, G=32, gap=1, act=1),
-                dict(op="groupnorm_bwd", P=4194305, C=3, G=1), dict(op="quantize", rows=4194305, cols=3), dict(op="product", M=(1 << 26) + 1, N=1, K=1)],
+    "strided": [dict(of="groupnorm", B=32769, P=1, C=96, G=32, gap=1), dict(of="groupnorm", P=4194305, C=3, G=1), dict(of="groupnorm_bwd", B=32769, P=1, C=96, G=32, gap=1, act=1),
+                dict(of="groupnorm_bwd", P=4194305, C=3, G=1), dict(of="quantize", rows=4194305, cols=3), dict(of="product", M=(1 << 26) + 1, N=1, K=1)],
     # chunks of 2048 rows; a workgroup's registers full
     "norm": [dict(pixels=k, **c) for k in ("signs", "halves") for c in (dict(B=256, P=2048, C=64, G=2), dict(P=20000, C=256, G=2, act=1), dict(P=1024, C=1280, G=32, out="i8"), dict(P=32768, C=4, G=4))]
     + [dict(pixels="ratio", P=20000, C=256, G=32), dict(pixels="ratio", P=1024, C=1280, G=32, dtyp="f32", act=1)]
