@@ -139,7 +139,7 @@ __global__ __launch_bounds__(256) void gemm_i8_any_kernel(I8Args a) {
 // What bounds it: a CU is fed about 75 bytes a ns (128 x 128 and four stages 0.42 us a step), so tiles as large as the registers allow where
 // there are enough of them: 256 x 320 reads 72 KB for 10.5 M products, 128 x 128 32 KB for 2.1 M. 2048x10240x1280 fp16 (256 x 320, a tile a
 // CU, 1670 TOP/s over the call) takes 15.2 us with K = 128, 31.7 with 1280, 51.2 with 2560: a step is 1.95 us in a long run (its MFMAs at
-// 80% of their rate at the 1.67 GHz that the card then holds), and some 12 us are the launch, the first loads and 42 MB of C that all CUs
+// 80% of their rate at the 1.67 GHz that the card then holds), and 11 to 12 us are the launch, the first loads and 42 MB of C that all CUs
 // store at once, with no product beside them.
 typedef int intx4 __attribute__((ext_vector_type(4)));
 typedef int intx16 __attribute__((ext_vector_type(16)));
